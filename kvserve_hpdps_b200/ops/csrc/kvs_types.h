@@ -98,4 +98,55 @@ struct LayerLaunch {
 };
 constexpr int kTraceCtas = 8;
 
+// One append: rows of keys, values and (optionally) queries of `tokens` new
+// tokens; strides in elements of the 16-bit inputs (multiples of 8).
+struct AppendLaunch {
+  const void* key;
+  const void* value;
+  const void* query;   // nullptr: none
+  void* query_out;
+  const void* slots;   // [tokens] block * block_size + offset, < 0: not appended
+  const void* pos;     // [tokens] rows of `table`; nullptr: no rotation
+  const void* table;   // [max_pos][rotary]: cosines, then sines
+  void* cache;
+  uint32_t* err;
+  long long key_ts, key_hs, val_ts, val_hs, q_ts, q_hs, qo_ts, qo_hs;  // token, head
+  // 16-bit cache: element strides of (block, plane, slot, head).  4-bit cache:
+  // block_stride and head_stride are the bytes between records.
+  long long block_stride, kv_stride, slot_stride, head_stride;
+  long long num_slots, max_pos, table_stride;
+  int tokens, heads, q_heads, block_size, rotary, interleaved;
+  int fp16;        // 0: bf16, 1: fp16
+  int slots64, pos64, table32;  // index widths; fp32 table (else the 16-bit type)
+  int groups;      // 4-bit cache: channel groups a row (1, 2, 4); 0: 16-bit cache
+  int pad_;
+};
+
+// Rows of a 4-bit cache read as 16-bit values: out [2][tokens][heads][128].
+struct Read4Launch {
+  const void* cache;
+  const void* slots;
+  void* out;
+  uint32_t* err;
+  long long block_stride, head_stride, num_slots;
+  int tokens, heads, block_size, groups, fp16, slots64;
+};
+
+// Attention of `tokens` query rows over a 4-bit cache.
+struct Attn4Launch {
+  const void* q;
+  void* out;
+  float* lse;              // [tokens][q_heads] or nullptr
+  const void* cache;
+  const int32_t* table;    // [seqs][table_cols] block ids
+  const int32_t* lens;     // [seqs] cached tokens, the queries' own among them
+  const int32_t* start;    // [seqs+1] first query row of each sequence; nullptr: row r
+  void* scratch;
+  uint32_t* err;
+  long long q_ts, q_hs, o_ts, o_hs, block_stride, head_stride, table_stride;
+  int seqs, tokens, table_cols, num_blocks, q_heads, heads, block_size, groups, fp16, max_q;
+  float scale;
+  int pad_;
+};
+
 }  // namespace kvs
