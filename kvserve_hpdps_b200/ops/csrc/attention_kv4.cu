@@ -2,18 +2,38 @@
 //
 // With n query rows of a sequence whose cache holds `len` tokens, row i sees
 // keys j < len - n + i + 1.  Over a group g of channels,
-//   q . k_j = sum_g [ step_jg * (sum_d q_d code_jd - 8 Q_g) + mid_jg * Q_g ],
-// Q_g = sum of q over the group; likewise the output is
-//   o_d = (sum_j p_j (mid_jg + (code_jd - 8) step_jg)) / sum_j p_j.
-// A row that sees no key returns zeros and lse = -inf.
+//   q . k_j = sum_g [ step_jg * sum_d q_d code_jd + (mid_jg - 8 step_jg) * Q_g ],
+// Q_g = sum of q over the group, and the output is
+//   o_d = [ sum_j w_jg code_jd - 8 sum_j w_jg + sum_j p_j mid_jg ] / sum_j p_j,
+// w_jg = p_j step_jg.  A row that sees no key returns zeros and lse = -inf.
 //
-// k_attn4_simple: one warp a (row, head), four channels a lane, one pass over
-// the keys with the running maximum and sum.
+// Codes never become 16-bit values of their own: a code in bits 4..7 of an
+// fp16 is the subnormal code * 2^-20, which the matrix instructions take
+// exactly.  One AND, and a shift for three of four, makes two operands out
+// of a packed word, and products with the (power-of-two scaled) query are
+// exact.  The place matters: sums are aligned to the operands' exponent
+// fields, 2^-14 for every subnormal, so a code at 2^-24 loses 4 bits more of
+// the 24 (measured: 2^-16 of the largest product against 2^-20).  For the
+// output the one rounding is that of w to fp16, relative 2^-11; the -8 is
+// taken off with the same rounded w.
+//
+// Why mma.sync and not tcgen05 for few query rows: tcgen05 reads its operands
+// from shared or tensor memory, so every code would be written there as 16
+// bits and read again, 4 + 4 bytes for each byte that HBM delivers.  At HBM's
+// rate (23 bytes a clock and SM) that is above what shared memory moves.
+// mma.sync takes the operands from the registers that unpack them.
 #include "kv4.cuh"
 
 namespace kvs {
 
 namespace {
+
+constexpr int kWarps = 4;             // a CTA
+constexpr int kStep = 32;             // tokens a warp takes at a time
+constexpr int kUnit = kWarps * kStep; // tokens a CTA takes at a time: the unit of work
+constexpr float kLowest = -1e30f;     // running maximum of a row that has seen nothing
+constexpr int kLowestExp = -100;      // smallest exponent that values are scaled by
+constexpr float kLazy = 8.f;          // log2 by which a score may pass its running maximum
 
 struct Seq {
   int row0, n, len;  // first query row, query rows, cached tokens
@@ -42,75 +62,718 @@ KVS_DEV Seq sequence(const Attn4Launch& L, int r, bool report) {
   return s;
 }
 
-template <bool FP16>
-__global__ void __launch_bounds__(128) k_attn4_simple(const __grid_constant__ Attn4Launch L) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r = blockIdx.y, i = blockIdx.x / L.q_heads, hq = blockIdx.x % L.q_heads;
-  const int group = L.q_heads / L.heads, h = hq / group;
-  const Seq s = sequence(L, r, threadIdx.x == 0);
-  if (i >= s.n) return;
-  const long long t = s.row0 + i;
-  const Kv4Record R{L.groups, L.block_size};
-  const int q = lane >> 3, j = lane & 7, ch = 32 * q + 4 * j;  // the lane's four channels
-  const int grp = ch / (128 / L.groups);
-  const uint16_t* qp = static_cast<const uint16_t*>(L.q) + t * L.q_ts + hq * L.q_hs + ch;
-  float qv[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, sum = 0.f;
+KVS_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+KVS_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                      uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transposes an 8x8 matrix of 16-bit elements held two to a lane.
+KVS_DEV uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+// Two codes as fp16 operands, code * 2^-20, out of bits 4..7 of both halves.
+KVS_DEV uint32_t code2(uint32_t w) { return w & 0x00F000F0u; }
+KVS_DEV uint32_t half2_bits(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+KVS_DEV void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+KVS_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+KVS_DEV void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+KVS_DEV uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a));
+  return v;
+}
+KVS_DEV uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+KVS_DEV uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+template <int NG>
+KVS_DEV void lds_meta(uint32_t a, uint32_t (&m)[NG]) {
+  if constexpr (NG == 4) {
+    const uint4 v = lds128(a);
+    m[0] = v.x;
+    m[1] = v.y;
+    m[2] = v.z;
+    m[3] = v.w;
+  } else if constexpr (NG == 2) {
+    const uint2 v = lds64(a);
+    m[0] = v.x;
+    m[1] = v.y;
+  } else {
+    m[0] = lds32(a);
+  }
+}
+
+// ------------------------------------------------------------- work split
+// The work is cut at the granularity of kUnit tokens and dealt out evenly:
+// item (sequence, kv head, row tile) has ceil(len / kUnit) units (at least one, so that rows
+// that see nothing are written), all items' units form one line, and CTA b
+// of B <= U takes [U b / B, U (b + 1) / B) of it.  Ragged batches load every CTA
+// alike and one long sequence is spread over all of them.  A CTA that holds
+// an item whole writes its output; else it leaves a partial result (at most
+// two: one for an item that began before its share, one for an item that
+// goes on behind it) and k_attn4_combine joins an item's parts in order, so
+// results do not depend on timing.
+struct Parts {
+  int4* desc;   // [B] item that begins in CTA b and goes on: (r, h, tile, parts) or r < 0
+  float2* ml;   // [2 B][rows] running maximum and sum
+  float* o;     // [2 B][rows][128]
+};
+KVS_DEV Parts parts(void* scratch, int B, int rows) {
+  Parts p;
+  p.desc = static_cast<int4*>(scratch);
+  p.ml = reinterpret_cast<float2*>(p.desc + B);
+  p.o = reinterpret_cast<float*>(p.ml + 2ll * B * rows);
+  return p;
+}
+
+struct Work {
+  long long units;  // a sequence's units
+  int tiles, per;   // row tiles a head, units an item
+};
+KVS_DEV Work work_of(const Attn4Launch& L, const Seq& s, int rows, int group) {
+  Work w;
+  w.tiles = (s.n * group + rows - 1) / rows;
+  w.per = s.len > 0 ? (s.len + kUnit - 1) / kUnit : 1;
+  w.units = static_cast<long long>(w.tiles) * L.heads * w.per;
+  return w;
+}
+
+template <int NG>
+constexpr int half_bytes() {  // 16 tokens in shared memory: K, V codes, K, V meta
+  return 2048 + 128 * NG;
+}
+
+// NT * 8 query rows a tile.  Fragments (lane = 4 g + c): scores are computed
+// transposed, tokens x rows, so that the 8 rows of a kv head's group fill the
+// narrow side of the instruction and none of the 16 is padding; K is the A
+// operand as loaded.  Their transposed fragments (movmatrix) are the B
+// operand of V^T P^T, whose A operand is V with two tokens' words joined.
+// Row m of a 16-token tile is token (m / 2) + 4 (m % 2) (+ 8): with the
+// swizzle below both kinds of fragment loads are free of bank conflicts.
+template <bool FP16, int NG, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
+    k_attn4(const __grid_constant__ Attn4Launch L) {
+  constexpr int ROWS = 8 * NT;
+  constexpr int HALF = half_bytes<NG>();
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long s_scan[kWarps];
+  __shared__ long long s_begin;
+  __shared__ int s_seq;
+  __shared__ float2 s_ml[kWarps][ROWS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+  const int group = L.q_heads / L.heads;
+  const int B = gridDim.x, b = blockIdx.x;
+  const Parts P = parts(L.scratch, B, ROWS);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---- this CTA's share [pos, end) and the sequence that it begins in
+  long long mine = 0;
+  for (int r = tid; r < L.seqs; r += kWarps * 32)
+    mine += work_of(L, sequence(L, r, b == 0), ROWS, group).units;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) qv[k] = h2f<FP16>(qp[k]) * L.scale;
-  const int seen = s.len - s.n + i + 1;
-  for (int tok = warp; tok < seen; tok += 4) {
-    const int blk = L.table[r * L.table_stride + tok / L.block_size];
-    if (blk < 0 || blk >= L.num_blocks) {
-      if (lane == 0) record_error(L.err, ERR_BOUNDS);
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, o);
+  if (lane == 0) s_scan[warp] = mine;
+  __syncthreads();
+  long long U = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) U += s_scan[w];
+  const long long used = U < B ? U : B;  // no CTA in the line has an empty share
+  if (tid == 0) P.desc[b] = make_int4(-1, 0, 0, 0);
+  if (b >= used) return;
+  long long pos = U * b / used;
+  const long long end = U * (b + 1) / used;
+  long long base = 0;
+  for (int r0 = 0; r0 < L.seqs; r0 += kWarps * 32) {
+    const int r = r0 + tid;
+    const long long v =
+        r < L.seqs ? work_of(L, sequence(L, r, false), ROWS, group).units : 0;
+    long long inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    __syncthreads();
+    if (lane == 31) s_scan[warp] = inc;
+    __syncthreads();
+    long long before = base;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += s_scan[w];
+      base += s_scan[w];
+    }
+    if (before + inc - v <= pos && pos < before + inc) {
+      s_seq = r;
+      s_begin = before + inc - v;
+    }
+    if (pos < base) break;  // the same for every thread
+  }
+  __syncthreads();
+  int r = s_seq;
+  long long begin = s_begin;  // of sequence r on the line
+
+  const uint32_t ring = smem_u32(smem) + warp * (4 * HALF);  // two stages of two halves
+  float* const s_o = reinterpret_cast<float*>(smem + warp * (4 * HALF));  // later: [ROWS][128]
+  const int granules = L.block_size / 16;
+  const int sg = (g >> 1) + 4 * (g & 1);  // the token of fragment row g
+  // fragment addresses inside a half
+  const uint32_t k_at = (sg >> 1) * 128 + (((((sg & 1) << 2) | c) ^ (sg & 4)) << 4);
+  const uint32_t v_at = 1024 + (c >> 1) * 128 + (c & 1) * 64 +
+                        ((((g >> 1) ^ (c & 2)) << 4) | ((g & 1) << 3));
+  const uint32_t m_at = 2048 + sg * 4 * NG;
+  // copy addresses inside a half: chunk `lane` of K, of V (chunk lane + 32 is
+  // 512 bytes on in both places: eight rows further, the same swizzle)
+  const int crow = lane >> 2, cc = lane & 3;
+  const uint32_t ck_dst = (crow >> 1) * 128 + (((((crow & 1) << 2) | cc) ^ (crow & 4)) << 4);
+  const uint32_t cv_dst = 1024 + (crow >> 1) * 128 + (crow & 1) * 64 + ((cc ^ (crow & 2)) << 4);
+
+  while (pos < end) {
+    const Seq s = sequence(L, r, false);
+    const Work wk = work_of(L, s, ROWS, group);
+    if (pos >= begin + wk.units) {  // on to the next sequence that has work
+      begin += wk.units;
+      ++r;
       continue;
     }
-    const int off = tok % L.block_size;
-    const uint8_t* rec = static_cast<const uint8_t*>(L.cache) + blk * L.block_stride +
-                         h * L.head_stride;
-    const uint32_t kc = *reinterpret_cast<const uint16_t*>(rec + R.codes(0, off) + 16 * (j >> 1) +
-                                                           4 * q + 2 * (j & 1));
-    const uint32_t vc = *reinterpret_cast<const uint16_t*>(rec + R.codes(1, off) + 8 * j + 2 * q);
-    const uint32_t km = reinterpret_cast<const uint32_t*>(rec + R.meta(0, off))[grp];
-    const uint32_t vm = reinterpret_cast<const uint32_t*>(rec + R.meta(1, off))[grp];
-    float dot = 0.f;
+    const long long rem = pos - begin;
+    const int item = static_cast<int>(rem / wk.per);
+    const int unit0 = static_cast<int>(rem - static_cast<long long>(item) * wk.per);
+    const long long left = end - pos;
+    const int units = static_cast<int>(left < wk.per - unit0 ? left : wk.per - unit0);
+    const int h = item / wk.tiles, ti = item - h * wk.tiles;
+    // low and high tiles in turn: with causal limits, neighbours add up to alike work
+    const int tile = (ti & 1) ? wk.tiles - 1 - (ti >> 1) : ti >> 1;
+    const int nrows = s.n * group;
+    const int last_row = min(nrows, (tile + 1) * ROWS) - 1;
+    const int min_seen = max(0, s.len - s.n + tile * ROWS / group + 1);
+    const int limit = max(0, s.len - s.n + last_row / group + 1);
+
+    // ---- query fragments: fp16, each row scaled by a power of two so that its largest
+    // element is in [2^14, 2^15); exact unless 2^-31 of the largest
+    uint32_t qf[NT][4][2][2];
+    float f[NT][2], qs[NG][NT][2];  // of this lane's columns 2c, 2c + 1
+    int seen[NT][2];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      dot += qv[k] * (h2f<FP16>(km >> 16) +
-                      (static_cast<float>((kc >> (4 * k)) & 15u) - 8.f) * h2f<FP16>(km & 0xFFFFu));
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = tile * ROWS + nt * 8 + g;
+      uint4 raw[4] = {};
+      if (row < nrows) {
+        const uint16_t* qp = static_cast<const uint16_t*>(L.q) +
+                             (s.row0 + row / group) * L.q_ts +
+                             (h * group + row % group) * L.q_hs + 8 * c;
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, x);
-    const float mn = fmaxf(m, dot), p = __expf(dot - mn), f = __expf(m - mn);
-    m = mn;
-    sum = sum * f + p;
+        for (int q = 0; q < 4; ++q) raw[q] = *reinterpret_cast<const uint4*>(qp + 32 * q);
+      }
+      float x[4][8], top = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      o[k] = o[k] * f +
-             p * (h2f<FP16>(vm >> 16) +
-                  (static_cast<float>((vc >> (4 * k)) & 15u) - 8.f) * h2f<FP16>(vm & 0xFFFFu));
-  }
-  __shared__ float sm[4], ss[4], so[4][128];
-  if (lane == 0) {
-    sm[warp] = m;
-    ss[warp] = sum;
-  }
+      for (int q = 0; q < 4; ++q) {
+        unpack8<FP16>(raw[q], x[q]);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) so[warp][ch + k] = o[k];
-  __syncthreads();
-  const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float total = 0.f, acc = 0.f;
-  if (!(top == -INFINITY)) {
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[q][i]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+      int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+      e = top == 0.f ? 0 : max(kLowestExp, min(e, 100));
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23) *
+                       (L.scale < 0.f ? -1.f : 1.f);
+      const float fr = fabsf(L.scale) * 1.4426950408889634f *
+                       __uint_as_float(static_cast<uint32_t>(127 + 6 + e) << 23);
+      float sum[4];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = sm[w] == -INFINITY ? 0.f : __expf(sm[w] - top);
-      total += ss[w] * f;
-      acc += so[w][threadIdx.x] * f;
+      for (int q = 0; q < 4; ++q) {
+        sum[q] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[q][i] *= up;
+          sum[q] += x[q][i];
+        }
+        sum[q] += __shfl_xor_sync(0xFFFFFFFFu, sum[q], 1);
+        sum[q] += __shfl_xor_sync(0xFFFFFFFFu, sum[q], 2);
+        sum[q] *= 9.5367431640625e-7f;  // 2^-20, the codes' unit
+        qf[nt][q][0][0] = half2_bits(x[q][0], x[q][4]);
+        qf[nt][q][0][1] = half2_bits(x[q][2], x[q][6]);
+        qf[nt][q][1][0] = half2_bits(x[q][1], x[q][5]);
+        qf[nt][q][1][1] = half2_bits(x[q][3], x[q][7]);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int from = (2 * c + j) * 4;
+        f[nt][j] = __shfl_sync(0xFFFFFFFFu, fr, from);
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) qs[gr][nt][j] = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          qs[q * NG / 4][nt][j] += __shfl_sync(0xFFFFFFFFu, sum[q], from);
+        const int cr = tile * ROWS + nt * 8 + 2 * c + j;
+        seen[nt][j] = cr < nrows ? s.len - s.n + cr / group + 1 : 0x7FFFFFFF;
+      }
     }
-    acc /= total;
+
+    float acc[8][NT][4], wsum[NT][4], msum[NG][NT][2], l[NT][2], M[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][nt][i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) wsum[nt][i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        l[nt][j] = 0.f;
+        M[nt][j] = kLowest;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) msum[gr][nt][j] = 0.f;
+      }
+    }
+    int E = kLowestExp;
+
+    // ---- this warp's steps: tokens first + kUnit k + [0, 32)
+    const int first = unit0 * kUnit + warp * kStep;
+    const int stop = min(limit, (unit0 + units) * kUnit);
+    const int steps = first < stop ? (stop - first + kUnit - 1) / kUnit : 0;
+    const uint8_t* const head = static_cast<const uint8_t*>(L.cache) + h * L.head_stride;
+    const int32_t* const table = L.table + r * L.table_stride;
+    int ids = -1, offs = 0;      // of step k % 16 = lane / 2, half lane % 2
+    uint32_t have = 0;           // bit 2 (k % 2) + half: that half was copied
+    auto copy_step = [&](int k) {
+      if ((k & 15) == 0) {
+        const int tok = first + (k + (lane >> 1)) * kUnit + 16 * (lane & 1);
+        ids = -1;
+        if (tok < stop) {
+          const int page = tok / 16 / granules;
+          offs = tok - page * L.block_size;
+          ids = table[page];
+          if (ids < 0 || ids >= L.num_blocks) {
+            record_error(L.err, ERR_BOUNDS);
+            ids = -1;
+          }
+        }
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int from = 2 * (k & 15) + hf;
+        const int id = __shfl_sync(0xFFFFFFFFu, ids, from);
+        const int off = __shfl_sync(0xFFFFFFFFu, offs, from);
+        const uint32_t bit = 1u << (2 * (k & 1) + hf);
+        have &= ~bit;
+        if (id >= 0) {
+          have |= bit;
+          const uint8_t* rec = head + id * L.block_stride;
+          const uint32_t dst = ring + ((k & 1) * 2 + hf) * HALF;
+          const uint8_t* kc = rec + off * 64 + lane * 16;
+          const uint8_t* vc = kc + L.block_size * 64;
+          cp_async16(dst + ck_dst, kc);
+          cp_async16(dst + ck_dst + 512, kc + 512);
+          cp_async16(dst + cv_dst, vc);
+          cp_async16(dst + cv_dst + 512, vc + 512);
+          if (lane < 8 * NG) {
+            const int value = lane >= 4 * NG;
+            cp_async16(dst + 2048 + lane * 16,
+                       rec + L.block_size * (128 + value * 4 * NG) + off * 4 * NG +
+                           (lane - value * 4 * NG) * 16);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+    if (steps > 0) copy_step(0);
+    for (int k = 0; k < steps; ++k) {
+      const uint32_t had = have >> (2 * (k & 1));
+      if (k + 1 < steps) {
+        copy_step(k + 1);
+        cp_async_wait<1>();
+      } else {
+        cp_async_wait<0>();
+      }
+      __syncwarp();
+      const int t0 = first + k * kUnit;
+      const bool masked = (had & 3u) != 3u || t0 + kStep > min_seen;
+      const uint32_t st = ring + (k & 1) * 2 * HALF;
+
+      float sc[2][NT][4];
+      uint32_t vm[2][2][NG];  // [half][row g, g + 8] (step, mid) of the values
+      uint32_t big = 0;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const uint32_t at = st + hf * HALF;
+        const uint4 ka = lds128(at + k_at), kb = lds128(at + k_at + 512);
+        const uint32_t kw0[4] = {ka.x, ka.y, ka.z, ka.w}, kw1[4] = {kb.x, kb.y, kb.z, kb.w};
+        uint32_t km0[NG], km1[NG];
+        lds_meta<NG>(at + m_at, km0);
+        lds_meta<NG>(at + m_at + 32 * NG, km1);
+        lds_meta<NG>(at + m_at + 64 * NG, vm[hf][0]);
+        lds_meta<NG>(at + m_at + 96 * NG, vm[hf][1]);
+        if (masked) {  // what no row of the tile sees counts as zeros, whatever its bytes are
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (!(had >> hf & 1u) || t0 + 16 * hf + sg + 8 * i >= limit) {
+#pragma unroll
+              for (int gr = 0; gr < NG; ++gr) vm[hf][i][gr] = 0;
+            }
+        }
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          float a[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[nt][i] = 0.f;
+#pragma unroll
+          for (int q = gr * 4 / NG; q < (gr + 1) * 4 / NG; ++q) {
+            const uint32_t w0 = kw0[q], w1 = kw1[q];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816(a[nt], code2(w0 << 4), code2(w1 << 4), code2(w0 >> 4), code2(w1 >> 4),
+                       qf[nt][q][0][0], qf[nt][q][0][1]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816(a[nt], code2(w0), code2(w1), code2(w0 >> 8), code2(w1 >> 8),
+                       qf[nt][q][1][0], qf[nt][q][1][1]);
+          }
+          const float s0 = h2f<FP16>(km0[gr] & 0xFFFFu), s1 = h2f<FP16>(km1[gr] & 0xFFFFu);
+          const float z0 = fmaf(-8.f, s0, h2f<FP16>(km0[gr] >> 16));
+          const float z1 = fmaf(-8.f, s1, h2f<FP16>(km1[gr] >> 16));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float zq = (i < 2 ? z0 : z1) * qs[gr][nt][i & 1];
+              const float add = fmaf(i < 2 ? s0 : s1, a[nt][i], zq);
+              sc[hf][nt][i] = gr == 0 ? add : sc[hf][nt][i] + add;
+            }
+          big = __vmaxu2(big, __vmaxu2(vm[hf][0][gr] & 0x7FFF7FFFu, vm[hf][1][gr] & 0x7FFF7FFFu));
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int tok = t0 + 16 * hf + sg + (i < 2 ? 0 : 8);
+              if (!(had >> hf & 1u) || tok >= seen[nt][i & 1]) sc[hf][nt][i] = -INFINITY;
+            }
+      }
+      // ---- reference M of the exponentials: a row's running maximum, passed by up to
+      // 2^kLazy before it is moved, plus the exponent E of the largest step or
+      // mid seen (moved when passed by 2^4): w then stays inside fp16's range
+      // whatever the values' scale, and sums keep one scale.
+      float t[2][NT][4];
+      const float most = fmaxf(h2f<FP16>(big & 0xFFFFu), h2f<FP16>(big >> 16));
+      bool move = most > __uint_as_float(static_cast<uint32_t>(127 + 4 + E) << 23);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            t[hf][nt][i] = fmaf(sc[hf][nt][i], f[nt][i & 1], -M[nt][i & 1]);
+            move |= t[hf][nt][i] > kLazy - E;
+          }
+      if (__any_sync(0xFFFFFFFFu, move)) {
+        const uint32_t all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
+        const int e = min(max(static_cast<int>(all >> 23) - 127, E), 100);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float top = fmaxf(fmaxf(sc[0][nt][j], sc[0][nt][j + 2]),
+                              fmaxf(sc[1][nt][j], sc[1][nt][j + 2])) * f[nt][j];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1)
+              top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            const float old = M[nt][j];
+            const float m = fmaxf(fmaxf(old - E, top) + e, kLowest);
+            M[nt][j] = m;
+            const float k2 = ex2(old - m);
+            l[nt][j] *= k2;
+            wsum[nt][j] *= k2;
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) msum[gr][nt][j] *= k2;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+              acc[d][nt][j] *= k2;
+              acc[d][nt][j + 2] *= k2;
+            }
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              t[hf][nt][j] = fmaf(sc[hf][nt][j], f[nt][j], -m);
+              t[hf][nt][j + 2] = fmaf(sc[hf][nt][j + 2], f[nt][j], -m);
+            }
+          }
+        E = e;
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const uint32_t at = st + hf * HALF;
+        float p[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[nt][i] = ex2(t[hf][nt][i]);
+            l[nt][i & 1] += p[nt][i];
+          }
+        const uint2 v0 = lds64(at + v_at), v1 = lds64(at + v_at + 256),
+                    v2 = lds64(at + v_at + 512), v3 = lds64(at + v_at + 768);
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          const float s0 = h2f<FP16>(vm[hf][0][gr] & 0xFFFFu), z0 = h2f<FP16>(vm[hf][0][gr] >> 16);
+          const float s1 = h2f<FP16>(vm[hf][1][gr] & 0xFFFFu), z1 = h2f<FP16>(vm[hf][1][gr] >> 16);
+          uint32_t b0[NT], b1[NT];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float w[4], y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              w[i] = p[nt][i] * (i < 2 ? s0 : s1);
+              y[i] = p[nt][i] * (i < 2 ? z0 : z1);
+              // a row that does not see the token takes nothing of it, NaN or not
+              if (masked && t[hf][nt][i] == -INFINITY) w[i] = y[i] = 0.f;
+            }
+            msum[gr][nt][0] += y[0] + y[2];
+            msum[gr][nt][1] += y[1] + y[3];
+            b0[nt] = transpose8(half2_bits(w[0], w[1]));
+            b1[nt] = transpose8(half2_bits(w[2], w[3]));
+            // row gr of this product is the sum of the rounded weights
+            const uint32_t one = g == gr ? 0x3C003C00u : 0u;
+            mma16816(wsum[nt], one, 0u, one, 0u, b0[nt], b1[nt]);
+          }
+#pragma unroll
+          for (int q = gr * 4 / NG; q < (gr + 1) * 4 / NG; ++q) {
+            const uint32_t pick = (q & 1) ? 0x7632u : 0x5410u;
+            const uint32_t x01 = __byte_perm(q < 2 ? v0.x : v0.y, q < 2 ? v1.x : v1.y, pick);
+            const uint32_t x23 = __byte_perm(q < 2 ? v2.x : v2.y, q < 2 ? v3.x : v3.y, pick);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816(acc[2 * q][nt], code2(x01 << 4), code2(x01 >> 4), code2(x23 << 4),
+                       code2(x23 >> 4), b0[nt], b1[nt]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816(acc[2 * q + 1][nt], code2(x01), code2(x01 >> 8), code2(x23),
+                       code2(x23 >> 8), b0[nt], b1[nt]);
+          }
+        }
+      }
+      __syncwarp();  // the stage may be overwritten
+    }
+
+    // ---- join the warps' results
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = nt * 8 + 2 * c + j;
+        float ls = l[nt][j], corr[NG];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) ls += __shfl_xor_sync(0xFFFFFFFFu, ls, o);
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          float ms = msum[gr][nt][j];
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) ms += __shfl_xor_sync(0xFFFFFFFFu, ms, o);
+          corr[gr] = ms - 8.f * __shfl_sync(0xFFFFFFFFu, wsum[nt][j], 4 * gr + c);
+        }
+        if (g == 0) s_ml[warp][row] = make_float2(M[nt][j], ls);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float z = corr[q * NG / 4];
+          float4 o4;  // channels 32 q + 4 g + 0..3
+          o4.x = fmaf(acc[2 * q][nt][j], 1048576.f, z);
+          o4.y = fmaf(acc[2 * q + 1][nt][j], 1048576.f, z);
+          o4.z = fmaf(acc[2 * q][nt][j + 2], 1048576.f, z);
+          o4.w = fmaf(acc[2 * q + 1][nt][j + 2], 1048576.f, z);
+          *reinterpret_cast<float4*>(s_o + row * 128 + 32 * q + 4 * g) = o4;
+        }
+      }
+    __syncthreads();
+    const bool whole = unit0 == 0 && units == wk.per;
+    const int slot = 2 * b + (unit0 == 0 ? 1 : 0);
+    for (int row = 0; row < ROWS; ++row) {
+      const int rr = tile * ROWS + row;
+      if (rr >= nrows) break;
+      float m = kLowest;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ml[w][row].x);
+      float ls = 0.f, o = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float k2 = ex2(s_ml[w][row].x - m);
+        ls += s_ml[w][row].y * k2;
+        o += reinterpret_cast<const float*>(smem + w * (4 * HALF))[row * 128 + tid] * k2;
+      }
+      if (whole) {
+        const long long tq = s.row0 + rr / group;
+        const int hq = h * group + rr % group;
+        static_cast<uint16_t*>(L.out)[tq * L.o_ts + hq * L.o_hs + tid] =
+            static_cast<uint16_t>(f2h<FP16>(ls == 0.f ? 0.f : o / ls));
+        if (L.lse != nullptr && tid == 0)
+          L.lse[tq * L.q_heads + hq] =
+              ls == 0.f ? -INFINITY : (m + log2f(ls)) * 0.69314718055994531f;
+      } else {
+        P.o[(static_cast<long long>(slot) * ROWS + row) * 128 + tid] = o;
+        if (tid == 0) P.ml[slot * ROWS + row] = make_float2(m, ls);
+      }
+    }
+    if (!whole && unit0 == 0 && tid == 0) {
+      // the CTA that holds the item's last unit x: the smallest b' whose share ends behind it
+      const long long x = pos + wk.per - 1;
+      const long long last = ((x + 1) * used + U - 1) / U - 1;
+      P.desc[b] = make_int4(r, h, tile, static_cast<int>(last - b) + 1);
+    }
+    __syncthreads();
+    pos += units;
   }
-  static_cast<uint16_t*>(L.out)[t * L.o_ts + hq * L.o_hs + threadIdx.x] =
-      static_cast<uint16_t>(f2h<FP16>(acc));
-  if (L.lse != nullptr && threadIdx.x == 0)
-    L.lse[t * L.q_heads + hq] = top == -INFINITY ? -INFINITY : top + logf(total);
+}
+
+// Joins the parts of the item that begins in CTA blockIdx.x and goes on in
+// the next ones: 8 rows a CTA, four groups of parts at a time.
+template <bool FP16, int NT>
+__global__ void __launch_bounds__(1024) k_attn4_combine(const __grid_constant__ Attn4Launch L) {
+  constexpr int ROWS = 8 * NT;
+  extern __shared__ float s_f[];  // [parts][8] factors
+  __shared__ float s_m[32], s_l[32], s_acc[4][8][128];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int B = gridDim.x, b = blockIdx.x;
+  const Parts P = parts(L.scratch, B, ROWS);
+  const int4 d = P.desc[b];
+  if (d.x < 0) return;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = warp & 7, quarter = warp >> 3;
+  const int np = d.w, in_tile = blockIdx.y * 8 + row;
+  // slot of part i: the item's beginning is CTA b's second slot, the rest the first ones of the next
+  auto slot = [&](int i) { return i == 0 ? 2 * b + 1 : 2 * (b + i); };
+  float m = kLowest;
+  for (int i = quarter * 32 + lane; i < np; i += 128) m = fmaxf(m, P.ml[slot(i) * ROWS + in_tile].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  if (lane == 0) s_m[warp] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_m[row], s_m[row + 8]), fmaxf(s_m[row + 16], s_m[row + 24]));
+  float ls = 0.f;
+  for (int i = quarter * 32 + lane; i < np; i += 128) {
+    const float2 ml = P.ml[slot(i) * ROWS + in_tile];
+    const float k2 = ex2(ml.x - m);
+    s_f[i * 8 + row] = k2;
+    ls += ml.y * k2;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xFFFFFFFFu, ls, o);
+  if (lane == 0) s_l[warp] = ls;
+  __syncthreads();
+  ls = (s_l[row] + s_l[row + 8]) + (s_l[row + 16] + s_l[row + 24]);
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int i = quarter; i < np; i += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(
+        P.o + (static_cast<long long>(slot(i)) * ROWS + in_tile) * 128 + lane * 4);
+    const float k2 = s_f[i * 8 + row];
+    a.x = fmaf(x.x, k2, a.x);
+    a.y = fmaf(x.y, k2, a.y);
+    a.z = fmaf(x.z, k2, a.z);
+    a.w = fmaf(x.w, k2, a.w);
+  }
+  *reinterpret_cast<float4*>(&s_acc[quarter][row][lane * 4]) = a;
+  __syncthreads();
+  if (quarter != 0) return;
+  const int group = L.q_heads / L.heads;
+  const Seq s = sequence(L, d.x, false);
+  const int rr = d.z * ROWS + in_tile;
+  if (rr >= s.n * group) return;
+  const long long tq = s.row0 + rr / group;
+  const int hq = d.y * group + rr % group;
+  float o4[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float o = (s_acc[0][row][lane * 4 + k] + s_acc[1][row][lane * 4 + k]) +
+                    (s_acc[2][row][lane * 4 + k] + s_acc[3][row][lane * 4 + k]);
+    o4[k] = ls == 0.f ? 0.f : o / ls;
+  }
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + tq * L.o_ts + hq * L.o_hs + lane * 4) =
+      make_uint2(f2h2<FP16>(o4[0], o4[1]), f2h2<FP16>(o4[2], o4[3]));
+  if (L.lse != nullptr && lane == 0)
+    L.lse[tq * L.q_heads + hq] = ls == 0.f ? -INFINITY : (m + log2f(ls)) * 0.69314718055994531f;
+}
+
+struct Grid {
+  int ctas, rows;
+  bool split;  // whether an item can have more than one unit
+};
+
+// Rows a tile: 8 hold a decode step's query heads of one kv head (up to 8);
+// more rows take 16, which unpack each code once for twice the rows.
+Grid grid_of(const Attn4Launch* L) {
+  Grid g;
+  const int group = L->q_heads / L->heads;
+  const long long rows = static_cast<long long>(L->max_q) * group;
+  g.rows = rows <= 8 ? 8 : 16;
+  const long long per = (static_cast<long long>(L->table_cols) * L->block_size + kUnit - 1) / kUnit;
+  const long long units = static_cast<long long>(L->seqs) * L->heads *
+                          ((rows + g.rows - 1) / g.rows) * (per > 0 ? per : 1);
+  const long long most = 148ll * (g.rows == 8 ? 4 : 3);  // resident at once
+  g.ctas = static_cast<int>(units < most ? units : most);
+  g.split = per > 1;
+  return g;
+}
+
+template <bool FP16, int NG, int NT>
+cudaError_t launch(const Attn4Launch& L, const Grid& g, cudaStream_t s) {
+  const int smem = kWarps * 4 * half_bytes<NG>();
+  cudaError_t e = cudaFuncSetAttribute(k_attn4<FP16, NG, NT>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  k_attn4<FP16, NG, NT><<<g.ctas, kWarps * 32, smem, s>>>(L);
+  if ((e = cudaGetLastError()) != cudaSuccess || !g.split) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(g.ctas, NT);
+  cfg.blockDim = dim3(1024);
+  cfg.dynamicSmemBytes = static_cast<size_t>(g.ctas) * 8 * sizeof(float);
+  cfg.stream = s;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_attn4_combine<FP16, NT>, L);
+}
+
+template <bool FP16, int NG>
+cudaError_t launch_rows(const Attn4Launch& L, const Grid& g, cudaStream_t s) {
+  return g.rows == 8 ? launch<FP16, NG, 1>(L, g, s) : launch<FP16, NG, 2>(L, g, s);
+}
+template <bool FP16>
+cudaError_t launch_groups(const Attn4Launch& L, const Grid& g, cudaStream_t s) {
+  return L.groups == 1   ? launch_rows<FP16, 1>(L, g, s)
+         : L.groups == 2 ? launch_rows<FP16, 2>(L, g, s)
+                         : launch_rows<FP16, 4>(L, g, s);
 }
 
 }  // namespace
@@ -122,18 +785,18 @@ extern "C" {
 
 int kvs_attn4_launch_size(void) { return static_cast<int>(sizeof(Attn4Launch)); }
 
-long long kvs_attn4_scratch_bytes(const Attn4Launch*) { return 0; }
+long long kvs_attn4_scratch_bytes(const Attn4Launch* L) {
+  const Grid g = grid_of(L);
+  return 16ll * g.ctas + 2ll * g.ctas * g.rows * (8 + 512);
+}
 
 int kvs_attention_kv4(const Attn4Launch* L, void* stream) {
-  if (L->seqs <= 0 || L->max_q <= 0 || L->tokens <= 0) return 0;
-  if (L->seqs > 65535) return -2;
-  const dim3 grid(static_cast<unsigned>(L->max_q) * L->q_heads, L->seqs);
+  if (L->seqs <= 0 || L->max_q <= 0 || L->tokens <= 0 || L->heads <= 0) return 0;
+  const Grid g = grid_of(L);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (L->fp16)
-    k_attn4_simple<true><<<grid, 128, 0, s>>>(*L);
-  else
-    k_attn4_simple<false><<<grid, 128, 0, s>>>(*L);
-  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+  const cudaError_t e =
+      L->fp16 ? launch_groups<true>(*L, g, s) : launch_groups<false>(*L, g, s);
+  return e == cudaSuccess ? 0 : -1;
 }
 
 }  // extern "C"
