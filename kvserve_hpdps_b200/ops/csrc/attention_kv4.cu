@@ -22,6 +22,8 @@
 // bits and read again, 4 + 4 bytes for each byte that HBM delivers.  At HBM's
 // rate (23 bytes a clock and SM) that is above what shared memory moves.
 // mma.sync takes the operands from the registers that unpack them.
+#include <type_traits>
+
 #include "kv4.cuh"
 
 namespace kvs {
@@ -31,6 +33,7 @@ namespace {
 constexpr int kWarps = 4;             // a CTA
 constexpr int kStep = 32;             // tokens a warp takes at a time
 constexpr int kUnit = kWarps * kStep; // tokens a CTA takes at a time: the unit of work
+constexpr int kOver = 1;              // what starting and ending an item costs, in units
 constexpr float kLowest = -1e30f;     // running maximum of a row that has seen nothing
 constexpr int kLowestExp = -100;      // smallest exponent that values are scaled by
 constexpr float kLazy = 8.f;          // log2 by which a score may pass its running maximum
@@ -131,10 +134,11 @@ KVS_DEV void lds_meta(uint32_t a, uint32_t (&m)[NG]) {
 
 // ------------------------------------------------------------- work split
 // The work is cut at the granularity of kUnit tokens and dealt out evenly:
-// item (sequence, kv head, row tile) has ceil(len / kUnit) units (at least one, so that rows
-// that see nothing are written), all items' units form one line, and CTA b
-// of B <= U takes [U b / B, U (b + 1) / B) of it.  Ragged batches load every CTA
-// alike and one long sequence is spread over all of them.  A CTA that holds
+// item (sequence, kv head, row tile) has ceil(len / kUnit) units (at least
+// one, so that rows that see nothing are written) and costs kOver more for
+// its queries and its result.  The items' costs form one line of length U,
+// and CTA b of B <= U takes [U b / B, U (b + 1) / B) of it.  Ragged batches
+// load every CTA alike and one long sequence is spread over all of them.  A CTA that holds
 // an item whole writes its output; else it leaves a partial result (at most
 // two: one for an item that began before its share, one for an item that
 // goes on behind it) and k_attn4_combine joins an item's parts in order, so
@@ -153,14 +157,14 @@ KVS_DEV Parts parts(void* scratch, int B, int rows) {
 }
 
 struct Work {
-  long long units;  // a sequence's units
+  long long units;  // a sequence's share of the line
   int tiles, per;   // row tiles a head, units an item
 };
 KVS_DEV Work work_of(const Attn4Launch& L, const Seq& s, int rows, int group) {
   Work w;
   w.tiles = (s.n * group + rows - 1) / rows;
   w.per = s.len > 0 ? (s.len + kUnit - 1) / kUnit : 1;
-  w.units = static_cast<long long>(w.tiles) * L.heads * w.per;
+  w.units = static_cast<long long>(w.tiles) * L.heads * (w.per + kOver);
   return w;
 }
 
@@ -262,10 +266,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       continue;
     }
     const long long rem = pos - begin;
-    const int item = static_cast<int>(rem / wk.per);
-    const int unit0 = static_cast<int>(rem - static_cast<long long>(item) * wk.per);
-    const long long left = end - pos;
-    const int units = static_cast<int>(left < wk.per - unit0 ? left : wk.per - unit0);
+    const int cost = wk.per + kOver;
+    const int item = static_cast<int>(rem / cost);
+    const int from0 = static_cast<int>(rem - static_cast<long long>(item) * cost);
+    const int share = static_cast<int>(min(end - pos, static_cast<long long>(cost - from0)));
+    // an item's overhead lies in front of its units
+    const int unit0 = max(0, from0 - kOver), units = max(0, from0 + share - kOver) - unit0;
+    pos += share;
+    if (units <= 0) continue;
     const int h = item / wk.tiles, ti = item - h * wk.tiles;
     // low and high tiles in turn: with causal limits, neighbours add up to alike work
     const int tile = (ti & 1) ? wk.tiles - 1 - (ti >> 1) : ti >> 1;
@@ -273,6 +281,57 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
     const int last_row = min(nrows, (tile + 1) * ROWS) - 1;
     const int min_seen = max(0, s.len - s.n + tile * ROWS / group + 1);
     const int limit = max(0, s.len - s.n + last_row / group + 1);
+
+    // ---- this warp's steps: tokens first + kUnit k + [0, 32)
+    const int first = unit0 * kUnit + warp * kStep;
+    const int stop = min(limit, (unit0 + units) * kUnit);
+    const int steps = first < stop ? (stop - first + kUnit - 1) / kUnit : 0;
+    const uint8_t* const head = static_cast<const uint8_t*>(L.cache) + h * L.head_stride;
+    const int32_t* const table = L.table + r * L.table_stride;
+    int ids = -1, offs = 0;      // of step k % 16 = lane / 2, half lane % 2
+    uint32_t have = 0;           // bit 2 (k % 2) + half: that half was copied
+    auto copy_step = [&](int k) {
+      if ((k & 15) == 0) {
+        const int tok = first + (k + (lane >> 1)) * kUnit + 16 * (lane & 1);
+        ids = -1;
+        if (tok < stop) {
+          const int page = tok / 16 / granules;
+          offs = tok - page * L.block_size;
+          ids = table[page];
+          if (ids < 0 || ids >= L.num_blocks) {
+            record_error(L.err, ERR_BOUNDS);
+            ids = -1;
+          }
+        }
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int from = 2 * (k & 15) + hf;
+        const int id = __shfl_sync(0xFFFFFFFFu, ids, from);
+        const int off = __shfl_sync(0xFFFFFFFFu, offs, from);
+        const uint32_t bit = 1u << (2 * (k & 1) + hf);
+        have &= ~bit;
+        if (id >= 0) {
+          have |= bit;
+          const uint8_t* rec = head + id * L.block_stride;
+          const uint32_t dst = ring + ((k & 1) * 2 + hf) * HALF;
+          const uint8_t* kc = rec + off * 64 + lane * 16;
+          const uint8_t* vc = kc + L.block_size * 64;
+          cp_async16(dst + ck_dst, kc);
+          cp_async16(dst + ck_dst + 512, kc + 512);
+          cp_async16(dst + cv_dst, vc);
+          cp_async16(dst + cv_dst + 512, vc + 512);
+          if (lane < 8 * NG) {
+            const int value = lane >= 4 * NG;
+            cp_async16(dst + 2048 + lane * 16,
+                       rec + L.block_size * (128 + value * 4 * NG) + off * 4 * NG +
+                           (lane - value * 4 * NG) * 16);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+    if (steps > 0) copy_step(0);
 
     // ---- query fragments: fp16, each row scaled by a power of two so that its largest
     // element is in [2^14, 2^15); exact unless 2^-31 of the largest
@@ -355,69 +414,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
     }
     int E = kLowestExp;
 
-    // ---- this warp's steps: tokens first + kUnit k + [0, 32)
-    const int first = unit0 * kUnit + warp * kStep;
-    const int stop = min(limit, (unit0 + units) * kUnit);
-    const int steps = first < stop ? (stop - first + kUnit - 1) / kUnit : 0;
-    const uint8_t* const head = static_cast<const uint8_t*>(L.cache) + h * L.head_stride;
-    const int32_t* const table = L.table + r * L.table_stride;
-    int ids = -1, offs = 0;      // of step k % 16 = lane / 2, half lane % 2
-    uint32_t have = 0;           // bit 2 (k % 2) + half: that half was copied
-    auto copy_step = [&](int k) {
-      if ((k & 15) == 0) {
-        const int tok = first + (k + (lane >> 1)) * kUnit + 16 * (lane & 1);
-        ids = -1;
-        if (tok < stop) {
-          const int page = tok / 16 / granules;
-          offs = tok - page * L.block_size;
-          ids = table[page];
-          if (ids < 0 || ids >= L.num_blocks) {
-            record_error(L.err, ERR_BOUNDS);
-            ids = -1;
-          }
-        }
-      }
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int from = 2 * (k & 15) + hf;
-        const int id = __shfl_sync(0xFFFFFFFFu, ids, from);
-        const int off = __shfl_sync(0xFFFFFFFFu, offs, from);
-        const uint32_t bit = 1u << (2 * (k & 1) + hf);
-        have &= ~bit;
-        if (id >= 0) {
-          have |= bit;
-          const uint8_t* rec = head + id * L.block_stride;
-          const uint32_t dst = ring + ((k & 1) * 2 + hf) * HALF;
-          const uint8_t* kc = rec + off * 64 + lane * 16;
-          const uint8_t* vc = kc + L.block_size * 64;
-          cp_async16(dst + ck_dst, kc);
-          cp_async16(dst + ck_dst + 512, kc + 512);
-          cp_async16(dst + cv_dst, vc);
-          cp_async16(dst + cv_dst + 512, vc + 512);
-          if (lane < 8 * NG) {
-            const int value = lane >= 4 * NG;
-            cp_async16(dst + 2048 + lane * 16,
-                       rec + L.block_size * (128 + value * 4 * NG) + off * 4 * NG +
-                           (lane - value * 4 * NG) * 16);
-          }
-        }
-      }
-      cp_async_commit();
-    };
-    if (steps > 0) copy_step(0);
-    for (int k = 0; k < steps; ++k) {
-      const uint32_t had = have >> (2 * (k & 1));
-      if (k + 1 < steps) {
-        copy_step(k + 1);
-        cp_async_wait<1>();
-      } else {
-        cp_async_wait<0>();
-      }
-      __syncwarp();
-      const int t0 = first + k * kUnit;
-      const bool masked = (had & 3u) != 3u || t0 + kStep > min_seen;
-      const uint32_t st = ring + (k & 1) * 2 * HALF;
-
+    auto step = [&](auto tag, int t0, uint32_t st, uint32_t had) {
+      constexpr bool MASKED = decltype(tag)::value;
       float sc[2][NT][4];
       uint32_t vm[2][2][NG];  // [half][row g, g + 8] (step, mid) of the values
       uint32_t big = 0;
@@ -431,7 +429,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
         lds_meta<NG>(at + m_at + 32 * NG, km1);
         lds_meta<NG>(at + m_at + 64 * NG, vm[hf][0]);
         lds_meta<NG>(at + m_at + 96 * NG, vm[hf][1]);
-        if (masked) {  // what no row of the tile sees counts as zeros, whatever its bytes are
+        if (MASKED) {  // what no row of the tile sees counts as zeros, whatever its bytes are
 #pragma unroll
           for (int i = 0; i < 2; ++i)
             if (!(had >> hf & 1u) || t0 + 16 * hf + sg + 8 * i >= limit) {
@@ -465,16 +463,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float zq = (i < 2 ? z0 : z1) * qs[gr][nt][i & 1];
-              const float add = fmaf(i < 2 ? s0 : s1, a[nt][i], zq);
-              sc[hf][nt][i] = gr == 0 ? add : sc[hf][nt][i] + add;
+              const float z = i < 2 ? z0 : z1, y = qs[gr][nt][i & 1];
+              sc[hf][nt][i] = fmaf(i < 2 ? s0 : s1, a[nt][i],
+                                   gr == 0 ? z * y : fmaf(z, y, sc[hf][nt][i]));
             }
           big = __vmaxu2(big, __vmaxu2(vm[hf][0][gr] & 0x7FFF7FFFu, vm[hf][1][gr] & 0x7FFF7FFFu));
         }
-      }
-      if (masked) {
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
+        if (MASKED) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -482,23 +477,23 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
               const int tok = t0 + 16 * hf + sg + (i < 2 ? 0 : 8);
               if (!(had >> hf & 1u) || tok >= seen[nt][i & 1]) sc[hf][nt][i] = -INFINITY;
             }
+        }
       }
       // ---- reference M of the exponentials: a row's running maximum, passed by up to
       // 2^kLazy before it is moved, plus the exponent E of the largest step or
       // mid seen (moved when passed by 2^4): w then stays inside fp16's range
       // whatever the values' scale, and sums keep one scale.
-      float t[2][NT][4];
       const float most = fmaxf(h2f<FP16>(big & 0xFFFFu), h2f<FP16>(big >> 16));
       bool move = most > __uint_as_float(static_cast<uint32_t>(127 + 4 + E) << 23);
+      float top[NT][2];
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            t[hf][nt][i] = fmaf(sc[hf][nt][i], f[nt][i & 1], -M[nt][i & 1]);
-            move |= t[hf][nt][i] > kLazy - E;
-          }
+        for (int j = 0; j < 2; ++j) {
+          top[nt][j] = fmaxf(fmaxf(sc[0][nt][j], sc[0][nt][j + 2]),
+                             fmaxf(sc[1][nt][j], sc[1][nt][j + 2])) * f[nt][j];
+          move |= top[nt][j] - M[nt][j] > kLazy - E;
+        }
       if (__any_sync(0xFFFFFFFFu, move)) {
         const uint32_t all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
         const int e = min(max(static_cast<int>(all >> 23) - 127, E), 100);
@@ -506,13 +501,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float top = fmaxf(fmaxf(sc[0][nt][j], sc[0][nt][j + 2]),
-                              fmaxf(sc[1][nt][j], sc[1][nt][j + 2])) * f[nt][j];
+            float x = top[nt][j];
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1)
-              top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, o));
             const float old = M[nt][j];
-            const float m = fmaxf(fmaxf(old - E, top) + e, kLowest);
+            const float m = fmaxf(fmaxf(old - E, x) + e, kLowest);
             M[nt][j] = m;
             const float k2 = ex2(old - m);
             l[nt][j] *= k2;
@@ -523,11 +516,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
             for (int d = 0; d < 8; ++d) {
               acc[d][nt][j] *= k2;
               acc[d][nt][j + 2] *= k2;
-            }
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-              t[hf][nt][j] = fmaf(sc[hf][nt][j], f[nt][j], -m);
-              t[hf][nt][j + 2] = fmaf(sc[hf][nt][j + 2], f[nt][j], -m);
             }
           }
         E = e;
@@ -540,7 +528,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            p[nt][i] = ex2(t[hf][nt][i]);
+            p[nt][i] = ex2(fmaf(sc[hf][nt][i], f[nt][i & 1], -M[nt][i & 1]));
             l[nt][i & 1] += p[nt][i];
           }
         const uint2 v0 = lds64(at + v_at), v1 = lds64(at + v_at + 256),
@@ -552,16 +540,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
           uint32_t b0[NT], b1[NT];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float w[4], y[4];
+            float w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               w[i] = p[nt][i] * (i < 2 ? s0 : s1);
-              y[i] = p[nt][i] * (i < 2 ? z0 : z1);
-              // a row that does not see the token takes nothing of it, NaN or not
-              if (masked && t[hf][nt][i] == -INFINITY) w[i] = y[i] = 0.f;
+              float& ms = msum[gr][nt][i & 1];
+              if (MASKED) {  // a row takes nothing of a token it does not see, NaN or not
+                const bool hid = sc[hf][nt][i] == -INFINITY;
+                if (hid) w[i] = 0.f;
+                ms += hid ? 0.f : p[nt][i] * (i < 2 ? z0 : z1);
+              } else {
+                ms = fmaf(p[nt][i], i < 2 ? z0 : z1, ms);
+              }
             }
-            msum[gr][nt][0] += y[0] + y[2];
-            msum[gr][nt][1] += y[1] + y[3];
             b0[nt] = transpose8(half2_bits(w[0], w[1]));
             b1[nt] = transpose8(half2_bits(w[2], w[3]));
             // row gr of this product is the sum of the rounded weights
@@ -584,6 +575,22 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
           }
         }
       }
+    };
+    for (int k = 0; k < steps; ++k) {
+      const uint32_t had = have >> (2 * (k & 1));
+      if (k + 1 < steps) {
+        copy_step(k + 1);
+        cp_async_wait<1>();
+      } else {
+        cp_async_wait<0>();
+      }
+      __syncwarp();
+      const int t0 = first + k * kUnit;
+      const uint32_t st = ring + (k & 1) * 2 * HALF;
+      if ((had & 3u) != 3u || t0 + kStep > min_seen)
+        step(std::true_type{}, t0, st, had);
+      else
+        step(std::false_type{}, t0, st, had);
       __syncwarp();  // the stage may be overwritten
     }
 
@@ -646,12 +653,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
     }
     if (!whole && unit0 == 0 && tid == 0) {
       // the CTA that holds the item's last unit x: the smallest b' whose share ends behind it
-      const long long x = pos + wk.per - 1;
+      const long long x = begin + static_cast<long long>(item + 1) * cost - 1;
       const long long last = ((x + 1) * used + U - 1) / U - 1;
       P.desc[b] = make_int4(r, h, tile, static_cast<int>(last - b) + 1);
     }
     __syncthreads();
-    pos += units;
   }
 }
 
