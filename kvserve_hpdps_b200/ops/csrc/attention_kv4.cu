@@ -137,8 +137,9 @@ KVS_DEV void lds_meta(uint32_t a, uint32_t (&m)[NG]) {
 // item (sequence, kv head, row tile) has ceil(len / kUnit) units (at least
 // one, so that rows that see nothing are written) and costs kOver more for
 // its queries and its result.  The items' costs form one line of length U,
-// and CTA b of B <= U takes [U b / B, U (b + 1) / B) of it.  Ragged batches
-// load every CTA alike and one long sequence is spread over all of them.  A CTA that holds
+// and CTA b of B <= U takes U / B of it, the first U % B CTAs one more.
+// Ragged batches load every CTA alike and one long sequence is spread over
+// all of them (U < 2^31: the host refuses more).  A CTA that holds
 // an item whole writes its output; else it leaves a partial result (at most
 // two: one for an item that began before its share, one for an item that
 // goes on behind it) and k_attn4_combine joins an item's parts in order, so
@@ -156,15 +157,25 @@ KVS_DEV Parts parts(void* scratch, int B, int rows) {
   return p;
 }
 
+// CTA b's share of a line of length U dealt to B: [begin(b), begin(b + 1)).
+struct Deal {
+  int each, more;  // U / B, U % B
+  KVS_DEV int begin(int b) const { return each * b + min(b, more); }
+  KVS_DEV int owner(int x) const {
+    const int wide = more * (each + 1);
+    return x < wide ? x / (each + 1) : more + (x - wide) / each;
+  }
+};
+
 struct Work {
-  long long units;  // a sequence's share of the line
-  int tiles, per;   // row tiles a head, units an item
+  int units;       // a sequence's share of the line
+  int tiles, per;  // row tiles a head, units an item
 };
 KVS_DEV Work work_of(const Attn4Launch& L, const Seq& s, int rows, int group) {
   Work w;
   w.tiles = (s.n * group + rows - 1) / rows;
   w.per = s.len > 0 ? (s.len + kUnit - 1) / kUnit : 1;
-  w.units = static_cast<long long>(w.tiles) * L.heads * (w.per + kOver);
+  w.units = w.tiles * L.heads * (w.per + kOver);
   return w;
 }
 
@@ -186,9 +197,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
   constexpr int ROWS = 8 * NT;
   constexpr int HALF = half_bytes<NG>();
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long s_scan[kWarps];
-  __shared__ long long s_begin;
-  __shared__ int s_seq;
+  __shared__ int s_scan[kWarps], s_begin, s_seq;
   __shared__ float2 s_ml[kWarps][ROWS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   const int group = L.q_heads / L.heads;
@@ -197,36 +206,35 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- this CTA's share [pos, end) and the sequence that it begins in
-  long long mine = 0;
+  int mine = 0;
   for (int r = tid; r < L.seqs; r += kWarps * 32)
     mine += work_of(L, sequence(L, r, b == 0), ROWS, group).units;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, o);
   if (lane == 0) s_scan[warp] = mine;
   __syncthreads();
-  long long U = 0;
+  int U = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) U += s_scan[w];
-  const long long used = U < B ? U : B;  // no CTA in the line has an empty share
+  const int used = min(U, B);  // no CTA in the line has an empty share
   if (tid == 0) P.desc[b] = make_int4(-1, 0, 0, 0);
   if (b >= used) return;
-  long long pos = U * b / used;
-  const long long end = U * (b + 1) / used;
-  long long base = 0;
+  const Deal deal{U / used, U % used};
+  int pos = deal.begin(b), base = 0;
+  const int end = deal.begin(b + 1);
   for (int r0 = 0; r0 < L.seqs; r0 += kWarps * 32) {
     const int r = r0 + tid;
-    const long long v =
-        r < L.seqs ? work_of(L, sequence(L, r, false), ROWS, group).units : 0;
-    long long inc = v;
+    const int v = r < L.seqs ? work_of(L, sequence(L, r, false), ROWS, group).units : 0;
+    int inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      const int x = __shfl_up_sync(0xFFFFFFFFu, inc, o);
       if (lane >= o) inc += x;
     }
     __syncthreads();
     if (lane == 31) s_scan[warp] = inc;
     __syncthreads();
-    long long before = base;
+    int before = base;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) before += s_scan[w];
@@ -240,7 +248,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
   }
   __syncthreads();
   int r = s_seq;
-  long long begin = s_begin;  // of sequence r on the line
+  int begin = s_begin;  // of sequence r on the line
 
   const uint32_t ring = smem_u32(smem) + warp * (4 * HALF);  // two stages of two halves
   float* const s_o = reinterpret_cast<float*>(smem + warp * (4 * HALF));  // later: [ROWS][128]
@@ -265,11 +273,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       ++r;
       continue;
     }
-    const long long rem = pos - begin;
     const int cost = wk.per + kOver;
-    const int item = static_cast<int>(rem / cost);
-    const int from0 = static_cast<int>(rem - static_cast<long long>(item) * cost);
-    const int share = static_cast<int>(min(end - pos, static_cast<long long>(cost - from0)));
+    const int item = (pos - begin) / cost;
+    const int from0 = pos - begin - item * cost;
+    const int share = min(end - pos, cost - from0);
     // an item's overhead lies in front of its units
     const int unit0 = max(0, from0 - kOver), units = max(0, from0 + share - kOver) - unit0;
     pos += share;
@@ -625,112 +632,137 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
     __syncthreads();
     const bool whole = unit0 == 0 && units == wk.per;
     const int slot = 2 * b + (unit0 == 0 ? 1 : 0);
-    for (int row = 0; row < ROWS; ++row) {
-      const int rr = tile * ROWS + row;
-      if (rr >= nrows) break;
-      float m = kLowest;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ml[w][row].x);
-      float ls = 0.f, o = 0.f;
+    for (int it = 0; it < ROWS / kWarps; ++it) {  // a warp a row, four channels a lane
+      const int row = it * kWarps + warp, rr = tile * ROWS + row;
+      if (rr >= nrows) break;
+      float m = kLowest, ls = 0.f;
+      float2 ml[kWarps];
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float k2 = ex2(s_ml[w][row].x - m);
-        ls += s_ml[w][row].y * k2;
-        o += reinterpret_cast<const float*>(smem + w * (4 * HALF))[row * 128 + tid] * k2;
+        ml[w] = s_ml[w][row];
+        m = fmaxf(m, ml[w].x);
+      }
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float k2 = ex2(ml[w].x - m);
+        const float4 x =
+            *reinterpret_cast<const float4*>(smem + w * (4 * HALF) + row * 512 + lane * 16);
+        ls = fmaf(ml[w].y, k2, ls);
+        o.x = fmaf(x.x, k2, o.x);
+        o.y = fmaf(x.y, k2, o.y);
+        o.z = fmaf(x.z, k2, o.z);
+        o.w = fmaf(x.w, k2, o.w);
       }
       if (whole) {
         const long long tq = s.row0 + rr / group;
         const int hq = h * group + rr % group;
-        static_cast<uint16_t*>(L.out)[tq * L.o_ts + hq * L.o_hs + tid] =
-            static_cast<uint16_t>(f2h<FP16>(ls == 0.f ? 0.f : o / ls));
-        if (L.lse != nullptr && tid == 0)
+        const float inv = ls == 0.f ? 0.f : __fdividef(1.f, ls);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + tq * L.o_ts + hq * L.o_hs +
+                                  lane * 4) =
+            make_uint2(f2h2<FP16>(o.x * inv, o.y * inv), f2h2<FP16>(o.z * inv, o.w * inv));
+        if (L.lse != nullptr && lane == 0)
           L.lse[tq * L.q_heads + hq] =
               ls == 0.f ? -INFINITY : (m + log2f(ls)) * 0.69314718055994531f;
       } else {
-        P.o[(static_cast<long long>(slot) * ROWS + row) * 128 + tid] = o;
-        if (tid == 0) P.ml[slot * ROWS + row] = make_float2(m, ls);
+        *reinterpret_cast<float4*>(
+            P.o + (static_cast<long long>(slot) * ROWS + row) * 128 + lane * 4) = o;
+        if (lane == 0) P.ml[slot * ROWS + row] = make_float2(m, ls);
       }
     }
-    if (!whole && unit0 == 0 && tid == 0) {
-      // the CTA that holds the item's last unit x: the smallest b' whose share ends behind it
-      const long long x = begin + static_cast<long long>(item + 1) * cost - 1;
-      const long long last = ((x + 1) * used + U - 1) / U - 1;
-      P.desc[b] = make_int4(r, h, tile, static_cast<int>(last - b) + 1);
-    }
+    if (!whole && unit0 == 0 && tid == 0)  // parts: up to the CTA that holds the item's end
+      P.desc[b] = make_int4(r, h, tile, deal.owner(begin + (item + 1) * cost - 1) - b + 1);
     __syncthreads();
   }
 }
 
 // Joins the parts of the item that begins in CTA blockIdx.x and goes on in
-// the next ones: 8 rows a CTA, four groups of parts at a time.
+// the next ones: a CTA a row, a warp every eighth part.
 template <bool FP16, int NT>
-__global__ void __launch_bounds__(1024) k_attn4_combine(const __grid_constant__ Attn4Launch L) {
+__global__ void __launch_bounds__(256) k_attn4_combine(const __grid_constant__ Attn4Launch L) {
   constexpr int ROWS = 8 * NT;
-  extern __shared__ float s_f[];  // [parts][8] factors
-  __shared__ float s_m[32], s_l[32], s_acc[4][8][128];
+  __shared__ float s_m[8], s_l[8];
+  __shared__ float4 s_acc[8][32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int B = gridDim.x, b = blockIdx.x;
+  const int B = gridDim.x, b = blockIdx.x, row = blockIdx.y;
   const Parts P = parts(L.scratch, B, ROWS);
   const int4 d = P.desc[b];
   if (d.x < 0) return;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = warp & 7, quarter = warp >> 3;
-  const int np = d.w, in_tile = blockIdx.y * 8 + row;
-  // slot of part i: the item's beginning is CTA b's second slot, the rest the first ones of the next
-  auto slot = [&](int i) { return i == 0 ? 2 * b + 1 : 2 * (b + i); };
-  float m = kLowest;
-  for (int i = quarter * 32 + lane; i < np; i += 128) m = fmaxf(m, P.ml[slot(i) * ROWS + in_tile].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-  if (lane == 0) s_m[warp] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_m[row], s_m[row + 8]), fmaxf(s_m[row + 16], s_m[row + 24]));
-  float ls = 0.f;
-  for (int i = quarter * 32 + lane; i < np; i += 128) {
-    const float2 ml = P.ml[slot(i) * ROWS + in_tile];
-    const float k2 = ex2(ml.x - m);
-    s_f[i * 8 + row] = k2;
-    ls += ml.y * k2;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xFFFFFFFFu, ls, o);
-  if (lane == 0) s_l[warp] = ls;
-  __syncthreads();
-  ls = (s_l[row] + s_l[row + 8]) + (s_l[row + 16] + s_l[row + 24]);
+  const int group = L.q_heads / L.heads;
+  const Seq s = sequence(L, d.x, false);
+  const int rr = d.z * ROWS + row, np = d.w;
+  if (rr >= s.n * group) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // part 0 is in CTA b's second slot, the others in the first ones of the next CTAs
+  auto slot = [&](int i) { return (i == 0 ? 2 * b + 1 : 2 * (b + i)) * ROWS + row; };
+  float m = kLowest, ls = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int i = quarter; i < np; i += 4) {
-    const float4 x = *reinterpret_cast<const float4*>(
-        P.o + (static_cast<long long>(slot(i)) * ROWS + in_tile) * 128 + lane * 4);
-    const float k2 = s_f[i * 8 + row];
+  for (int i0 = warp; i0 < np; i0 += 32) {  // four parts at a time, their loads together
+    float2 ml[4];
+    float4 x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + 8 * u;
+      ml[u] = make_float2(kLowest, 0.f);
+      x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < np) {
+        ml[u] = P.ml[slot(i)];
+        x[u] = *reinterpret_cast<const float4*>(P.o + slot(i) * 128ll + lane * 4);
+      }
+    }
+    const float top = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
+    const float k0 = ex2(m - top);
+    m = top;
+    ls *= k0;
+    a.x *= k0;
+    a.y *= k0;
+    a.z *= k0;
+    a.w *= k0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float k2 = ex2(ml[u].x - top);
+      ls = fmaf(ml[u].y, k2, ls);
+      a.x = fmaf(x[u].x, k2, a.x);
+      a.y = fmaf(x[u].y, k2, a.y);
+      a.z = fmaf(x[u].z, k2, a.z);
+      a.w = fmaf(x[u].w, k2, a.w);
+    }
+  }
+  s_acc[warp][lane] = a;
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = ls;
+  }
+  __syncthreads();
+  if (warp != 0) return;
+  m = kLowest;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, s_m[w]);
+  ls = 0.f;
+  a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const float k2 = ex2(s_m[w] - m);
+    const float4 x = s_acc[w][lane];
+    ls = fmaf(s_l[w], k2, ls);
     a.x = fmaf(x.x, k2, a.x);
     a.y = fmaf(x.y, k2, a.y);
     a.z = fmaf(x.z, k2, a.z);
     a.w = fmaf(x.w, k2, a.w);
   }
-  *reinterpret_cast<float4*>(&s_acc[quarter][row][lane * 4]) = a;
-  __syncthreads();
-  if (quarter != 0) return;
-  const int group = L.q_heads / L.heads;
-  const Seq s = sequence(L, d.x, false);
-  const int rr = d.z * ROWS + in_tile;
-  if (rr >= s.n * group) return;
   const long long tq = s.row0 + rr / group;
   const int hq = d.y * group + rr % group;
-  float o4[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float o = (s_acc[0][row][lane * 4 + k] + s_acc[1][row][lane * 4 + k]) +
-                    (s_acc[2][row][lane * 4 + k] + s_acc[3][row][lane * 4 + k]);
-    o4[k] = ls == 0.f ? 0.f : o / ls;
-  }
+  const float inv = ls == 0.f ? 0.f : __fdividef(1.f, ls);
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + tq * L.o_ts + hq * L.o_hs + lane * 4) =
-      make_uint2(f2h2<FP16>(o4[0], o4[1]), f2h2<FP16>(o4[2], o4[3]));
+      make_uint2(f2h2<FP16>(a.x * inv, a.y * inv), f2h2<FP16>(a.z * inv, a.w * inv));
   if (L.lse != nullptr && lane == 0)
     L.lse[tq * L.q_heads + hq] = ls == 0.f ? -INFINITY : (m + log2f(ls)) * 0.69314718055994531f;
 }
 
 struct Grid {
   int ctas, rows;
+  bool fits;   // the line's length is an int
   bool split;  // whether an item can have more than one unit
 };
 
@@ -742,8 +774,10 @@ Grid grid_of(const Attn4Launch* L) {
   const long long rows = static_cast<long long>(L->max_q) * group;
   g.rows = rows <= 8 ? 8 : 16;
   const long long per = (static_cast<long long>(L->table_cols) * L->block_size + kUnit - 1) / kUnit;
-  const long long units = static_cast<long long>(L->seqs) * L->heads *
-                          ((rows + g.rows - 1) / g.rows) * (per > 0 ? per : 1);
+  const long long items = static_cast<long long>(L->seqs) * L->heads *
+                          ((rows + g.rows - 1) / g.rows);
+  const long long units = items * (per > 0 ? per : 1);
+  g.fits = items < (1ll << 31) && items * (per + 1 + kOver) < (1ll << 31);
   const long long most = 148ll * (g.rows == 8 ? 4 : 3);  // resident at once
   g.ctas = static_cast<int>(units < most ? units : most);
   g.split = per > 1;
@@ -759,9 +793,8 @@ cudaError_t launch(const Attn4Launch& L, const Grid& g, cudaStream_t s) {
   k_attn4<FP16, NG, NT><<<g.ctas, kWarps * 32, smem, s>>>(L);
   if ((e = cudaGetLastError()) != cudaSuccess || !g.split) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(g.ctas, NT);
-  cfg.blockDim = dim3(1024);
-  cfg.dynamicSmemBytes = static_cast<size_t>(g.ctas) * 8 * sizeof(float);
+  cfg.gridDim = dim3(g.ctas, 8 * NT);
+  cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -799,6 +832,7 @@ long long kvs_attn4_scratch_bytes(const Attn4Launch* L) {
 int kvs_attention_kv4(const Attn4Launch* L, void* stream) {
   if (L->seqs <= 0 || L->max_q <= 0 || L->tokens <= 0 || L->heads <= 0) return 0;
   const Grid g = grid_of(L);
+  if (!g.fits) return -2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e =
       L->fp16 ? launch_groups<true>(*L, g, s) : launch_groups<false>(*L, g, s);
