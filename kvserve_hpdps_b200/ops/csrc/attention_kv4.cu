@@ -2,20 +2,20 @@
 //
 // With n query rows of a sequence whose cache holds `len` tokens, row i sees
 // keys j < len - n + i + 1.  Over a group g of channels,
-//   q . k_j = sum_g [ step_jg * sum_d q_d code_jd + (mid_jg - 8 step_jg) * Q_g ],
+//   q . k_j = sum_g [ step_jg * sum_d q_d (code_jd - 8) + mid_jg * Q_g ],
 // Q_g = sum of q over the group, and the output is
-//   o_d = [ sum_j w_jg code_jd - 8 sum_j w_jg + sum_j p_j mid_jg ] / sum_j p_j,
+//   o_d = [ sum_j w_jg (code_jd - 8) + sum_j p_j mid_jg ] / sum_j p_j,
 // w_jg = p_j step_jg.  A row that sees no key returns zeros and lse = -inf.
 //
-// Codes never become 16-bit values of their own: a code in bits 4..7 of an
-// fp16 is the subnormal code * 2^-20, which the matrix instructions take
-// exactly.  One AND, and a shift for three of four, makes two operands out
-// of a packed word, and products with the (power-of-two scaled) query are
-// exact.  The place matters: sums are aligned to the operands' exponent
-// fields, 2^-14 for every subnormal, so a code at 2^-24 loses 4 bits more of
-// the 24 (measured: 2^-16 of the largest product against 2^-20).  For the
-// output the one rounding is that of w to fp16, relative 2^-11; the -8 is
-// taken off with the same rounded w.
+// A code is turned into the fp16 code - 8 by one AND-OR that puts it into the
+// mantissa of 1024 and one exact fused multiply-add, for two codes at a time
+// (and a shift for every second pair): the integer pipe, which has half the
+// rate, shares the work with the floating-point one.  Products with the
+// power-of-two scaled query are then exact and sums are fp32, so scores are
+// as good as fp32's.  For the output the one rounding is that of w to fp16,
+// relative 2^-11.  (Codes taken as fp16 subnormals by the AND alone cost one
+// instruction less, but sums are aligned to the operands' exponent fields, so
+// they lose the bits that a subnormal has in front of its first one.)
 //
 // Why mma.sync and not tcgen05 for few query rows: tcgen05 reads its operands
 // from shared or tensor memory, so every code would be written there as 16
@@ -33,7 +33,7 @@ namespace {
 constexpr int kWarps = 4;             // a CTA
 constexpr int kStep = 32;             // tokens a warp takes at a time
 constexpr int kUnit = kWarps * kStep; // tokens a CTA takes at a time: the unit of work
-constexpr int kOver = 1;              // what starting and ending an item costs, in units
+constexpr int kOver = 2;              // what starting and ending an item costs, in units
 constexpr float kLowest = -1e30f;     // running maximum of a row that has seen nothing
 constexpr int kLowestExp = -100;      // smallest exponent that values are scaled by
 constexpr float kLazy = 8.f;          // log2 by which a score may pass its running maximum
@@ -80,15 +80,35 @@ KVS_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint
 // Transposes an 8x8 matrix of 16-bit elements held two to a lane.
 KVS_DEV uint32_t transpose8(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-// Two codes as fp16 operands, code * 2^-20, out of bits 4..7 of both halves.
-KVS_DEV uint32_t code2(uint32_t w) { return w & 0x00F000F0u; }
+// The codes in nibbles 0..3 of both halves of a word, each less 8, as fp16 pairs.
+KVS_DEV uint32_t and_or(uint32_t a, uint32_t mask, uint32_t with) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(with));
+  return d;
+}
+KVS_DEV void codes4(uint32_t w, uint32_t k1024, uint32_t (&r)[4]) {
+  const uint32_t v = w >> 8;
+  const __half2 low = __float2half2_rn(-1032.f), part = __float2half2_rn(0.0625f),
+                high = __float2half2_rn(-72.f);
+  auto as_half2 = [](uint32_t x) { return *reinterpret_cast<const __half2*>(&x); };
+  auto bits = [](__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); };
+  r[0] = bits(__hadd2(as_half2(and_or(w, 0x000F000Fu, k1024)), low));
+  r[1] = bits(__hfma2(as_half2(and_or(w, 0x00F000F0u, k1024)), part, high));
+  r[2] = bits(__hadd2(as_half2(and_or(v, 0x000F000Fu, k1024)), low));
+  r[3] = bits(__hfma2(as_half2(and_or(v, 0x00F000F0u, k1024)), part, high));
+}
 KVS_DEV uint32_t half2_bits(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+KVS_DEV uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 KVS_DEV void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -98,25 +118,11 @@ template <int N>
 KVS_DEV void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-KVS_DEV uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(a));
-  return v;
-}
-KVS_DEV uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-KVS_DEV uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
+KVS_DEV uint4 lds128(const uint8_t* a) { return *reinterpret_cast<const uint4*>(a); }
+KVS_DEV uint2 lds64(const uint8_t* a) { return *reinterpret_cast<const uint2*>(a); }
+KVS_DEV uint32_t lds32(const uint8_t* a) { return *reinterpret_cast<const uint32_t*>(a); }
 template <int NG>
-KVS_DEV void lds_meta(uint32_t a, uint32_t (&m)[NG]) {
+KVS_DEV void lds_meta(const uint8_t* a, uint32_t (&m)[NG]) {
   if constexpr (NG == 4) {
     const uint4 v = lds128(a);
     m[0] = v.x;
@@ -252,6 +258,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
 
   const uint32_t ring = smem_u32(smem) + warp * (4 * HALF);  // two stages of two halves
   float* const s_o = reinterpret_cast<float*>(smem + warp * (4 * HALF));  // later: [ROWS][128]
+  uint32_t k1024;  // fp16 1024 twice, kept in a register: and_or's third operand
+  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(k1024));
   const int granules = L.block_size / 16;
   const int sg = (g >> 1) + 4 * (g & 1);  // the token of fragment row g
   // fragment addresses inside a half
@@ -261,6 +269,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
   const uint32_t m_at = 2048 + sg * 4 * NG;
   // copy addresses inside a half: chunk `lane` of K, of V (chunk lane + 32 is
   // 512 bytes on in both places: eight rows further, the same swizzle)
+  const int v_src = L.block_size * 64;
+  const int m_src = lane < 4 * NG ? L.block_size * 128 + lane * 16
+                                  : L.block_size * (128 + 4 * NG) + (lane - 4 * NG) * 16;
   const int crow = lane >> 2, cc = lane & 3;
   const uint32_t ck_dst = (crow >> 1) * 128 + (((((crow & 1) << 2) | cc) ^ (crow & 4)) << 4);
   const uint32_t cv_dst = 1024 + (crow >> 1) * 128 + (crow & 1) * 64 + ((cc ^ (crow & 2)) << 4);
@@ -320,20 +331,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
         have &= ~bit;
         if (id >= 0) {
           have |= bit;
-          const uint8_t* rec = head + id * L.block_stride;
+          const uint8_t* rec = head + static_cast<uint64_t>(static_cast<uint32_t>(id)) *
+                                          static_cast<uint32_t>(L.block_stride);
+          const uint8_t* kc = rec + (off * 64 + lane * 16);
+          const uint8_t* vc = kc + v_src;
           const uint32_t dst = ring + ((k & 1) * 2 + hf) * HALF;
-          const uint8_t* kc = rec + off * 64 + lane * 16;
-          const uint8_t* vc = kc + L.block_size * 64;
           cp_async16(dst + ck_dst, kc);
           cp_async16(dst + ck_dst + 512, kc + 512);
           cp_async16(dst + cv_dst, vc);
           cp_async16(dst + cv_dst + 512, vc + 512);
-          if (lane < 8 * NG) {
-            const int value = lane >= 4 * NG;
-            cp_async16(dst + 2048 + lane * 16,
-                       rec + L.block_size * (128 + value * 4 * NG) + off * 4 * NG +
-                           (lane - value * 4 * NG) * 16);
-          }
+          if (lane < 8 * NG) cp_async16(dst + 2048 + lane * 16, rec + (off * (4 * NG) + m_src));
         }
       }
       cp_async_commit();
@@ -370,7 +377,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23) *
                        (L.scale < 0.f ? -1.f : 1.f);
       const float fr = fabsf(L.scale) * 1.4426950408889634f *
-                       __uint_as_float(static_cast<uint32_t>(127 + 6 + e) << 23);
+                       __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
       float sum[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -382,7 +389,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
         }
         sum[q] += __shfl_xor_sync(0xFFFFFFFFu, sum[q], 1);
         sum[q] += __shfl_xor_sync(0xFFFFFFFFu, sum[q], 2);
-        sum[q] *= 9.5367431640625e-7f;  // 2^-20, the codes' unit
         qf[nt][q][0][0] = half2_bits(x[q][0], x[q][4]);
         qf[nt][q][0][1] = half2_bits(x[q][2], x[q][6]);
         qf[nt][q][1][0] = half2_bits(x[q][1], x[q][5]);
@@ -402,15 +408,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       }
     }
 
-    float acc[8][NT][4], wsum[NT][4], msum[NG][NT][2], l[NT][2], M[NT][2];
+    float acc[8][NT][4], msum[NG][NT][2], l[NT][2], M[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[j][nt][i] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) wsum[nt][i] = 0.f;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         l[nt][j] = 0.f;
@@ -421,14 +425,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
     }
     int E = kLowestExp;
 
-    auto step = [&](auto tag, int t0, uint32_t st, uint32_t had) {
+    auto step = [&](auto tag, int t0, const uint8_t* st, uint32_t had) {
       constexpr bool MASKED = decltype(tag)::value;
       float sc[2][NT][4];
       uint32_t vm[2][2][NG];  // [half][row g, g + 8] (step, mid) of the values
       uint32_t big = 0;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const uint32_t at = st + hf * HALF;
+        const uint8_t* const at = st + hf * HALF;
         const uint4 ka = lds128(at + k_at), kb = lds128(at + k_at + 512);
         const uint32_t kw0[4] = {ka.x, ka.y, ka.z, ka.w}, kw1[4] = {kb.x, kb.y, kb.z, kb.w};
         uint32_t km0[NG], km1[NG];
@@ -453,19 +457,18 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
             for (int i = 0; i < 4; ++i) a[nt][i] = 0.f;
 #pragma unroll
           for (int q = gr * 4 / NG; q < (gr + 1) * 4 / NG; ++q) {
-            const uint32_t w0 = kw0[q], w1 = kw1[q];
+            uint32_t u[4], v[4];
+            codes4(kw0[q], k1024, u);
+            codes4(kw1[q], k1024, v);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816(a[nt], code2(w0 << 4), code2(w1 << 4), code2(w0 >> 4), code2(w1 >> 4),
-                       qf[nt][q][0][0], qf[nt][q][0][1]);
+              mma16816(a[nt], u[0], v[0], u[2], v[2], qf[nt][q][0][0], qf[nt][q][0][1]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816(a[nt], code2(w0), code2(w1), code2(w0 >> 8), code2(w1 >> 8),
-                       qf[nt][q][1][0], qf[nt][q][1][1]);
+              mma16816(a[nt], u[1], v[1], u[3], v[3], qf[nt][q][1][0], qf[nt][q][1][1]);
           }
           const float s0 = h2f<FP16>(km0[gr] & 0xFFFFu), s1 = h2f<FP16>(km1[gr] & 0xFFFFu);
-          const float z0 = fmaf(-8.f, s0, h2f<FP16>(km0[gr] >> 16));
-          const float z1 = fmaf(-8.f, s1, h2f<FP16>(km1[gr] >> 16));
+          const float z0 = h2f<FP16>(km0[gr] >> 16), z1 = h2f<FP16>(km1[gr] >> 16);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -474,7 +477,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
               sc[hf][nt][i] = fmaf(i < 2 ? s0 : s1, a[nt][i],
                                    gr == 0 ? z * y : fmaf(z, y, sc[hf][nt][i]));
             }
-          big = __vmaxu2(big, __vmaxu2(vm[hf][0][gr] & 0x7FFF7FFFu, vm[hf][1][gr] & 0x7FFF7FFFu));
+          big = max_u16x2(big, max_u16x2(vm[hf][0][gr] & 0x7FFF7FFFu, vm[hf][1][gr] & 0x7FFF7FFFu));
         }
         if (MASKED) {
 #pragma unroll
@@ -516,7 +519,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
             M[nt][j] = m;
             const float k2 = ex2(old - m);
             l[nt][j] *= k2;
-            wsum[nt][j] *= k2;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) msum[gr][nt][j] *= k2;
 #pragma unroll
@@ -529,7 +531,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       }
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const uint32_t at = st + hf * HALF;
+        const uint8_t* const at = st + hf * HALF;
         float p[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -562,23 +564,21 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
             }
             b0[nt] = transpose8(half2_bits(w[0], w[1]));
             b1[nt] = transpose8(half2_bits(w[2], w[3]));
-            // row gr of this product is the sum of the rounded weights
-            const uint32_t one = g == gr ? 0x3C003C00u : 0u;
-            mma16816(wsum[nt], one, 0u, one, 0u, b0[nt], b1[nt]);
           }
 #pragma unroll
           for (int q = gr * 4 / NG; q < (gr + 1) * 4 / NG; ++q) {
             const uint32_t pick = (q & 1) ? 0x7632u : 0x5410u;
             const uint32_t x01 = __byte_perm(q < 2 ? v0.x : v0.y, q < 2 ? v1.x : v1.y, pick);
             const uint32_t x23 = __byte_perm(q < 2 ? v2.x : v2.y, q < 2 ? v3.x : v3.y, pick);
+            uint32_t u[4], v[4];
+            codes4(x01, k1024, u);
+            codes4(x23, k1024, v);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816(acc[2 * q][nt], code2(x01 << 4), code2(x01 >> 4), code2(x23 << 4),
-                       code2(x23 >> 4), b0[nt], b1[nt]);
+              mma16816(acc[2 * q][nt], u[0], u[2], v[0], v[2], b0[nt], b1[nt]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816(acc[2 * q + 1][nt], code2(x01), code2(x01 >> 8), code2(x23),
-                       code2(x23 >> 8), b0[nt], b1[nt]);
+              mma16816(acc[2 * q + 1][nt], u[1], u[3], v[1], v[3], b0[nt], b1[nt]);
           }
         }
       }
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       }
       __syncwarp();
       const int t0 = first + k * kUnit;
-      const uint32_t st = ring + (k & 1) * 2 * HALF;
+      const uint8_t* const st = smem + warp * (4 * HALF) + (k & 1) * 2 * HALF;
       if ((had & 3u) != 3u || t0 + kStep > min_seen)
         step(std::true_type{}, t0, st, had);
       else
@@ -615,17 +615,17 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
           float ms = msum[gr][nt][j];
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) ms += __shfl_xor_sync(0xFFFFFFFFu, ms, o);
-          corr[gr] = ms - 8.f * __shfl_sync(0xFFFFFFFFu, wsum[nt][j], 4 * gr + c);
+          corr[gr] = ms;
         }
         if (g == 0) s_ml[warp][row] = make_float2(M[nt][j], ls);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const float z = corr[q * NG / 4];
           float4 o4;  // channels 32 q + 4 g + 0..3
-          o4.x = fmaf(acc[2 * q][nt][j], 1048576.f, z);
-          o4.y = fmaf(acc[2 * q + 1][nt][j], 1048576.f, z);
-          o4.z = fmaf(acc[2 * q][nt][j + 2], 1048576.f, z);
-          o4.w = fmaf(acc[2 * q + 1][nt][j + 2], 1048576.f, z);
+          o4.x = acc[2 * q][nt][j] + z;
+          o4.y = acc[2 * q + 1][nt][j] + z;
+          o4.z = acc[2 * q][nt][j + 2] + z;
+          o4.w = acc[2 * q + 1][nt][j + 2] + z;
           *reinterpret_cast<float4*>(s_o + row * 128 + 32 * q + 4 * g) = o4;
         }
       }
@@ -777,7 +777,8 @@ Grid grid_of(const Attn4Launch* L) {
   const long long items = static_cast<long long>(L->seqs) * L->heads *
                           ((rows + g.rows - 1) / g.rows);
   const long long units = items * (per > 0 ? per : 1);
-  g.fits = items < (1ll << 31) && items * (per + 1 + kOver) < (1ll << 31);
+  // block offsets are 32 x 32 -> 64 bit products
+  g.fits = L->block_stride >= 0 && L->block_stride < (1ll << 32) && items < (1ll << 31) && items * (per + 1 + kOver) < (1ll << 31);
   const long long most = 148ll * (g.rows == 8 ? 4 : 3);  // resident at once
   g.ctas = static_cast<int>(units < most ? units : most);
   g.split = per > 1;
