@@ -34,6 +34,7 @@ constexpr int kWarps = 4;             // a CTA
 constexpr int kStep = 32;             // tokens a warp takes at a time
 constexpr int kUnit = kWarps * kStep; // tokens a CTA takes at a time: the unit of work
 constexpr int kOver = 2;              // what starting and ending an item costs, in units
+constexpr int kLeast = 4;             // a CTA's share of the line is no shorter than this
 constexpr float kLowest = -1e30f;     // running maximum of a row that has seen nothing
 constexpr int kLowestExp = -100;      // smallest exponent that values are scaled by
 constexpr float kLazy = 8.f;          // log2 by which a score may pass its running maximum
@@ -143,7 +144,8 @@ KVS_DEV void lds_meta(const uint8_t* a, uint32_t (&m)[NG]) {
 // item (sequence, kv head, row tile) has ceil(len / kUnit) units (at least
 // one, so that rows that see nothing are written) and costs kOver more for
 // its queries and its result.  The items' costs form one line of length U,
-// and CTA b of B <= U takes U / B of it, the first U % B CTAs one more.
+// and CTA b of B takes U / B of it, the first U % B CTAs one more, B being
+// what is resident at once or, for little work, U / kLeast.
 // Ragged batches load every CTA alike and one long sequence is spread over
 // all of them (U < 2^31: the host refuses more).  A CTA that holds
 // an item whole writes its output; else it leaves a partial result (at most
@@ -212,26 +214,29 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- this CTA's share [pos, end) and the sequence that it begins in
-  int mine = 0;
-  for (int r = tid; r < L.seqs; r += kWarps * 32)
-    mine += work_of(L, sequence(L, r, b == 0), ROWS, group).units;
+  if (tid == 0) P.desc[b] = make_int4(-1, 0, 0, 0);
+  int U = 0, mine = 0;
+  for (int r = tid; r < L.seqs; r += kWarps * 32) {
+    mine = work_of(L, sequence(L, r, b == 0), ROWS, group).units;
+    U += mine;
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, o);
-  if (lane == 0) s_scan[warp] = mine;
+  for (int o = 16; o > 0; o >>= 1) U += __shfl_xor_sync(0xFFFFFFFFu, U, o);
+  if (lane == 0) s_scan[warp] = U;
   __syncthreads();
-  int U = 0;
+  U = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) U += s_scan[w];
-  const int used = min(U, B);  // no CTA in the line has an empty share
-  if (tid == 0) P.desc[b] = make_int4(-1, 0, 0, 0);
+  const int used = min(B, (U + kLeast - 1) / kLeast);
   if (b >= used) return;
   const Deal deal{U / used, U % used};
   int pos = deal.begin(b), base = 0;
   const int end = deal.begin(b + 1);
   for (int r0 = 0; r0 < L.seqs; r0 += kWarps * 32) {
     const int r = r0 + tid;
-    const int v = r < L.seqs ? work_of(L, sequence(L, r, false), ROWS, group).units : 0;
-    int inc = v;
+    if (L.seqs > kWarps * 32)  // else `mine` is it
+      mine = r < L.seqs ? work_of(L, sequence(L, r, false), ROWS, group).units : 0;
+    int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xFFFFFFFFu, inc, o);
@@ -246,9 +251,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       if (w < warp) before += s_scan[w];
       base += s_scan[w];
     }
-    if (before + inc - v <= pos && pos < before + inc) {
+    if (before + inc - mine <= pos && pos < before + inc) {
       s_seq = r;
-      s_begin = before + inc - v;
+      s_begin = before + inc - mine;
     }
     if (pos < base) break;  // the same for every thread
   }
@@ -345,6 +350,18 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       }
       cp_async_commit();
     };
+    uint4 raw[NT][4] = {};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = tile * ROWS + nt * 8 + g;
+      if (row < nrows) {
+        const uint16_t* qp = static_cast<const uint16_t*>(L.q) +
+                             (s.row0 + row / group) * L.q_ts +
+                             (h * group + row % group) * L.q_hs + 8 * c;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) raw[nt][q] = *reinterpret_cast<const uint4*>(qp + 32 * q);
+      }
+    }
     if (steps > 0) copy_step(0);
 
     // ---- query fragments: fp16, each row scaled by a power of two so that its largest
@@ -354,19 +371,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
     int seen[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = tile * ROWS + nt * 8 + g;
-      uint4 raw[4] = {};
-      if (row < nrows) {
-        const uint16_t* qp = static_cast<const uint16_t*>(L.q) +
-                             (s.row0 + row / group) * L.q_ts +
-                             (h * group + row % group) * L.q_hs + 8 * c;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) raw[q] = *reinterpret_cast<const uint4*>(qp + 32 * q);
-      }
       float x[4][8], top = 0.f;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        unpack8<FP16>(raw[q], x[q]);
+        unpack8<FP16>(raw[nt][q], x[q]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[q][i]));
       }
@@ -678,32 +686,30 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
 }
 
 // Joins the parts of the item that begins in CTA blockIdx.x and goes on in
-// the next ones: a CTA a row, a warp every eighth part.
+// the next ones: eight rows a CTA, four warps a row, each every fourth part.
 template <bool FP16, int NT>
-__global__ void __launch_bounds__(256) k_attn4_combine(const __grid_constant__ Attn4Launch L) {
+__global__ void __launch_bounds__(1024) k_attn4_combine(const __grid_constant__ Attn4Launch L) {
   constexpr int ROWS = 8 * NT;
-  __shared__ float s_m[8], s_l[8];
-  __shared__ float4 s_acc[8][32];
+  __shared__ float s_m[4][8], s_l[4][8];
+  __shared__ float4 s_acc[4][8][32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int B = gridDim.x, b = blockIdx.x, row = blockIdx.y;
+  const int B = gridDim.x, b = blockIdx.x;
   const Parts P = parts(L.scratch, B, ROWS);
   const int4 d = P.desc[b];
   if (d.x < 0) return;
-  const int group = L.q_heads / L.heads;
-  const Seq s = sequence(L, d.x, false);
-  const int rr = d.z * ROWS + row, np = d.w;
-  if (rr >= s.n * group) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = L.q_heads / L.heads, np = d.w;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r8 = warp & 7, quarter = warp >> 3;
+  const int row = blockIdx.y * 8 + r8;
   // part 0 is in CTA b's second slot, the others in the first ones of the next CTAs
   auto slot = [&](int i) { return (i == 0 ? 2 * b + 1 : 2 * (b + i)) * ROWS + row; };
   float m = kLowest, ls = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = warp; i0 < np; i0 += 32) {  // four parts at a time, their loads together
+  for (int i0 = quarter; i0 < np; i0 += 16) {  // four parts at a time, their loads together
     float2 ml[4];
     float4 x[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int i = i0 + 8 * u;
+      const int i = i0 + 4 * u;
       ml[u] = make_float2(kLowest, 0.f);
       x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i < np) {
@@ -729,23 +735,24 @@ __global__ void __launch_bounds__(256) k_attn4_combine(const __grid_constant__ A
       a.w = fmaf(x[u].w, k2, a.w);
     }
   }
-  s_acc[warp][lane] = a;
+  s_acc[quarter][r8][lane] = a;
   if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = ls;
+    s_m[quarter][r8] = m;
+    s_l[quarter][r8] = ls;
   }
   __syncthreads();
-  if (warp != 0) return;
-  m = kLowest;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) m = fmaxf(m, s_m[w]);
+  if (quarter != 0) return;
+  const Seq s = sequence(L, d.x, false);
+  const int rr = d.z * ROWS + row;
+  if (rr >= s.n * group) return;  // rows behind the tile's last were not written either
+  m = fmaxf(fmaxf(s_m[0][r8], s_m[1][r8]), fmaxf(s_m[2][r8], s_m[3][r8]));
   ls = 0.f;
   a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const float k2 = ex2(s_m[w] - m);
-    const float4 x = s_acc[w][lane];
-    ls = fmaf(s_l[w], k2, ls);
+  for (int w = 0; w < 4; ++w) {
+    const float k2 = ex2(s_m[w][r8] - m);
+    const float4 x = s_acc[w][r8][lane];
+    ls = fmaf(s_l[w][r8], k2, ls);
     a.x = fmaf(x.x, k2, a.x);
     a.y = fmaf(x.y, k2, a.y);
     a.z = fmaf(x.z, k2, a.z);
@@ -794,8 +801,8 @@ cudaError_t launch(const Attn4Launch& L, const Grid& g, cudaStream_t s) {
   k_attn4<FP16, NG, NT><<<g.ctas, kWarps * 32, smem, s>>>(L);
   if ((e = cudaGetLastError()) != cudaSuccess || !g.split) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(g.ctas, 8 * NT);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(g.ctas, NT);
+  cfg.blockDim = dim3(1024);
   cfg.stream = s;
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
