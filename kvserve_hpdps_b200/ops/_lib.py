@@ -77,40 +77,6 @@ class RawLaunch(ctypes.Structure):
                 ("pad_", c_int)]
 
 
-class AppendLaunch(ctypes.Structure):
-    _fields_ = [("key", c_void_p), ("value", c_void_p), ("query", c_void_p),
-                ("query_out", c_void_p), ("slots", c_void_p), ("pos", c_void_p),
-                ("table", c_void_p), ("cache", c_void_p), ("err", c_void_p),
-                ("key_ts", c_longlong), ("key_hs", c_longlong), ("val_ts", c_longlong),
-                ("val_hs", c_longlong), ("q_ts", c_longlong), ("q_hs", c_longlong),
-                ("qo_ts", c_longlong), ("qo_hs", c_longlong), ("block_stride", c_longlong),
-                ("kv_stride", c_longlong), ("slot_stride", c_longlong),
-                ("head_stride", c_longlong), ("num_slots", c_longlong), ("max_pos", c_longlong),
-                ("table_stride", c_longlong), ("tokens", c_int), ("heads", c_int),
-                ("q_heads", c_int), ("block_size", c_int), ("rotary", c_int),
-                ("interleaved", c_int), ("fp16", c_int), ("slots64", c_int), ("pos64", c_int),
-                ("table32", c_int), ("groups", c_int), ("pad_", c_int)]
-
-
-class Read4Launch(ctypes.Structure):
-    _fields_ = [("cache", c_void_p), ("slots", c_void_p), ("out", c_void_p), ("err", c_void_p),
-                ("block_stride", c_longlong), ("head_stride", c_longlong),
-                ("num_slots", c_longlong), ("tokens", c_int), ("heads", c_int),
-                ("block_size", c_int), ("groups", c_int), ("fp16", c_int), ("slots64", c_int)]
-
-
-class Attn4Launch(ctypes.Structure):
-    _fields_ = [("q", c_void_p), ("out", c_void_p), ("lse", c_void_p), ("cache", c_void_p),
-                ("table", c_void_p), ("lens", c_void_p), ("start", c_void_p),
-                ("scratch", c_void_p), ("err", c_void_p), ("q_ts", c_longlong),
-                ("q_hs", c_longlong), ("o_ts", c_longlong), ("o_hs", c_longlong),
-                ("block_stride", c_longlong), ("head_stride", c_longlong),
-                ("table_stride", c_longlong), ("seqs", c_int), ("tokens", c_int),
-                ("table_cols", c_int), ("num_blocks", c_int), ("q_heads", c_int),
-                ("heads", c_int), ("block_size", c_int), ("groups", c_int), ("fp16", c_int),
-                ("max_q", c_int), ("scale", c_float), ("pad_", c_int)]
-
-
 _lock = threading.Lock()
 _lib = None
 
@@ -160,13 +126,6 @@ def _declare(lib: ctypes.CDLL) -> None:
         "kvs_probe_push": ([P, P, c_longlong, P, c_int, P], c_int),
         "kvs_kv_error": ([P, P, c_longlong, P, P, P], c_int),
         "kvs_logit_agreement": ([P, P, c_int, c_int, P, P], c_int),
-        "kvs_append_launch_size": ([], c_int),
-        "kvs_read4_launch_size": ([], c_int),
-        "kvs_attn4_launch_size": ([], c_int),
-        "kvs_append_kv": ([POINTER(AppendLaunch), P], c_int),
-        "kvs_read_kv4": ([POINTER(Read4Launch), P], c_int),
-        "kvs_attn4_scratch_bytes": ([POINTER(Attn4Launch)], c_longlong),
-        "kvs_attention_kv4": ([POINTER(Attn4Launch), P], c_int),
         "kvs_device_count": ([], c_int),
         "kvs_malloc": ([c_int, c_uint64, POINTER(c_void_p)], c_int),
         "kvs_free": ([c_int, P], c_int),
@@ -204,10 +163,7 @@ def lib() -> ctypes.CDLL:
                               ("kvs_paged_kv_size", PagedKV),
                               ("kvs_raw_launch_size", RawLaunch),
                               ("kvs_rans_msg_size", RansMsg),
-                              ("kvs_raw_item_size", RawItem),
-                              ("kvs_append_launch_size", AppendLaunch),
-                              ("kvs_read4_launch_size", Read4Launch),
-                              ("kvs_attn4_launch_size", Attn4Launch)):
+                              ("kvs_raw_item_size", RawItem)):
                 got = getattr(handle, name)()
                 if got != ctypes.sizeof(cls):
                     raise RuntimeError(f"{cls.__name__} size mismatch: C {got} vs Python "
@@ -231,5 +187,5 @@ def check(rc: int, what: str) -> None:
 
 
 __all__ = ["lib", "available", "check", "PagedKV", "ReqTable", "LayerParams", "LayerLaunch",
-           "RansMsg", "AppendLaunch", "Read4Launch", "Attn4Launch",
+           "RansMsg",
            "MAX_HEADS", "c_double", "c_ulonglong"]

@@ -8,6 +8,10 @@ encoding) are fetched at run time with ``cudaGetDriverEntryPoint``, so the
 library also loads on machines without a GPU driver (its CPU codec then
 works and its device entry points return errors).
 
+``csrc/torch/*.cpp`` (host code that takes torch tensors) is compiled against
+this interpreter's torch into a second module, ``_paged_ops.so``, linked to
+the library next to it.
+
 Usage: ``python -m kvserve_hpdps_b200.ops.build [-v] [--force]``.
 Objects go to ``ops/_build/``; rebuilding is incremental on file mtimes.
 """
@@ -27,6 +31,8 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB_NAME = "libkvs_b200.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
+BIND_NAME = "_paged_ops"
+BIND_PATH = os.path.join(HERE, BIND_NAME + ".so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -67,6 +73,42 @@ def _compile(src: str, obj: str, cuda: str, verbose: bool) -> tuple[str, str]:
     return src, (res.stdout + res.stderr)
 
 
+def _build_bindings(jobs: int, force: bool) -> str:
+    """Compile csrc/torch/*.cpp against torch and link it to the library."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    srcs = sorted(glob.glob(os.path.join(CSRC, "torch", "*.cpp")))
+    deps = _headers()
+    objs, todo = [], []
+    flags = [f"-DTORCH_EXTENSION_NAME={BIND_NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    incs = cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"]]
+    for src in srcs:
+        obj = os.path.join(BUILD, f"torch_{torch.__version__}_{os.path.basename(src)}.o")
+        objs.append(obj)
+        if force or _stale(obj, src, deps):
+            todo.append(["g++", "-O2", "-fPIC", "-std=c++17", "-fvisibility=hidden", *flags,
+                         *[x for i in incs for x in ("-isystem", i)], "-c", src, "-o", obj])
+
+    def run(cmd):
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        list(ex.map(run, todo))
+    if todo or not os.path.exists(BIND_PATH) or any(
+            os.path.getmtime(o) > os.path.getmtime(BIND_PATH) for o in objs):
+        libdir = cpp_extension.library_paths("cuda")[0]
+        tmp = BIND_PATH + ".tmp"
+        run(["g++", "-shared", "-o", tmp, *objs, f"-L{HERE}", f"-l:{LIB_NAME}",
+             "-Wl,-rpath,$ORIGIN", f"-L{libdir}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+             "-ltorch_cuda", "-ltorch", "-ltorch_python"])
+        os.replace(tmp, BIND_PATH)
+    return BIND_PATH
+
+
 def build(verbose: bool = False, force: bool = False, jobs: int | None = None) -> str:
     """Compile and link; returns the library path."""
     cuda = _cuda_home()
@@ -96,6 +138,7 @@ def build(verbose: bool = False, force: bool = False, jobs: int | None = None) -
         if res.returncode != 0:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB_PATH)
+    _build_bindings(jobs or min(8, os.cpu_count() or 4), force)
     return LIB_PATH
 
 

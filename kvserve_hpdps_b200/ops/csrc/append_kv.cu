@@ -284,9 +284,6 @@ using namespace kvs;
 
 extern "C" {
 
-int kvs_append_launch_size(void) { return static_cast<int>(sizeof(AppendLaunch)); }
-int kvs_read4_launch_size(void) { return static_cast<int>(sizeof(Read4Launch)); }
-
 int kvs_append_kv(const AppendLaunch* L, void* stream) {
   const long long items = static_cast<long long>(L->tokens) * (L->q_heads + 2 * L->heads);
   if (items <= 0) return 0;

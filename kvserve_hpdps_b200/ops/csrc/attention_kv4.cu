@@ -200,7 +200,7 @@ constexpr int half_bytes() {  // 16 tokens in shared memory: K, V codes, K, V me
 // Row m of a 16-token tile is token (m / 2) + 4 (m % 2) (+ 8): with the
 // swizzle below both kinds of fragment loads are free of bank conflicts.
 template <bool FP16, int NG, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     k_attn4(const __grid_constant__ Attn4Launch L) {
   constexpr int ROWS = 8 * NT;
   constexpr int HALF = half_bytes<NG>();
@@ -786,7 +786,7 @@ Grid grid_of(const Attn4Launch* L) {
   const long long units = items * (per > 0 ? per : 1);
   // block offsets are 32 x 32 -> 64 bit products
   g.fits = L->block_stride >= 0 && L->block_stride < (1ll << 32) && items < (1ll << 31) && items * (per + 1 + kOver) < (1ll << 31);
-  const long long most = 148ll * (g.rows == 8 ? 4 : 3);  // resident at once
+  const long long most = 148ll * (g.rows == 8 ? 3 : 2);  // resident at once
   g.ctas = static_cast<int>(units < most ? units : most);
   g.split = per > 1;
   return g;
@@ -794,12 +794,11 @@ Grid grid_of(const Attn4Launch* L) {
 
 template <bool FP16, int NG, int NT>
 cudaError_t launch(const Attn4Launch& L, const Grid& g, cudaStream_t s) {
-  const int smem = kWarps * 4 * half_bytes<NG>();
-  cudaError_t e = cudaFuncSetAttribute(k_attn4<FP16, NG, NT>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
+  const int smem = kWarps * 4 * half_bytes<NG>();  // at most 40 KB: no opt-in needed
+  static_assert(kWarps * 4 * half_bytes<NG>() <= 46 * 1024);
   k_attn4<FP16, NG, NT><<<g.ctas, kWarps * 32, smem, s>>>(L);
-  if ((e = cudaGetLastError()) != cudaSuccess || !g.split) return e;
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || !g.split) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(g.ctas, NT);
   cfg.blockDim = dim3(1024);
@@ -829,8 +828,6 @@ cudaError_t launch_groups(const Attn4Launch& L, const Grid& g, cudaStream_t s) {
 using namespace kvs;
 
 extern "C" {
-
-int kvs_attn4_launch_size(void) { return static_cast<int>(sizeof(Attn4Launch)); }
 
 long long kvs_attn4_scratch_bytes(const Attn4Launch* L) {
   const Grid g = grid_of(L);

@@ -106,6 +106,8 @@ def test_read_refuses(change, error):
     (dict(seq_lens=torch.zeros(2, dtype=torch.int64)), TypeError),
     (dict(seq_lens=torch.zeros(3, dtype=torch.int32)), TypeError),
     (dict(max_query_len=2), ValueError),
+    (dict(scale=0.0), ValueError),
+    (dict(scale=math.inf), ValueError),
     (dict(query_start=torch.zeros(2, dtype=torch.int32)), TypeError),
     (dict(query_start=torch.zeros(3, dtype=torch.int32), max_query_len=0), ValueError),
     (dict(out=_kv(t=3, h=4)), ValueError),
