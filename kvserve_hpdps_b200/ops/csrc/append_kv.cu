@@ -9,7 +9,7 @@
 // multiply-add), so codes equal those of the same formula in plain fp32.
 // A 16-bit cache takes the result rounded once; a 4-bit cache (kv4.cuh) takes
 // it quantised per group of g channels, without a 16-bit rounding in between:
-//   step = T((max - min) / 15), mid = T(min + 8 step),
+//   step = T((max - min) (1 / 15)), mid = T(min + 8 step),
 //   code = clamp(floor((x - mid) * (1 / step) + 8.5), 0, 15),
 // T being the 16-bit type.  Codes are taken against the rounded (step, mid):
 // the pair that readers use.
@@ -79,7 +79,7 @@ KVS_DEV void group_extremes(uint32_t mask, int lanes, float& lo, float& hi) {
 // (step, mid) of a group, packed, and the numbers its codes are taken with.
 template <bool FP16>
 KVS_DEV uint32_t group_meta(float lo, float hi, float& mid, float& inv) {
-  uint32_t sb = f2h<FP16>(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
+  uint32_t sb = f2h<FP16>(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f));
   float step = h2f<FP16>(sb);
   if (step < 1.17549435e-38f) {  // 1 / step would overflow: the group is its mid
     sb = 0;

@@ -171,6 +171,34 @@ def test_append_4bit(dt, g_size, tokens, h, bs, rd):
         assert torch.equal(a, z)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("g_size", [32, 64, 128])
+def test_append_4bit_is_the_fp32_formula(dt, g_size):
+    """The stored bytes are those of the formula in fp32, one rounding an operation."""
+    g = _gen(g_size)
+    T, h, bs, rd = 600, 3, 16, 128
+    k, v = (torch.randn((T, h, 128), generator=g) for _ in range(2))
+    k[..., ::17] *= 12
+    k, v = k.to(dt), v.to(dt)
+    pos = torch.randint(0, 300, (T,), generator=g)
+    table = _table(300, rd).cpu()
+    cache = P.kv4_cache(T // bs + 1, h, bs, g_size)
+    P.append_kv(cache, k.cuda(), v.cuda(), torch.arange(T).cuda(), pos.cuda(), table.cuda())
+    c, s = table[pos][:, None, :64], table[pos][:, None, 64:]
+    a, b = k.float()[..., :64], k.float()[..., 64:]
+    x = torch.stack([torch.cat([a * c - b * s, b * c + a * s], -1), v.float()])
+    x = x.unflatten(-1, (128 // g_size, g_size))
+    lo, hi = x.amin(-1), x.amax(-1)
+    step = ((hi - lo) * torch.tensor(1 / 15)).to(dt)
+    mid = (lo + 8 * step.float()).to(dt)
+    code = ((x - mid.float()[..., None]) * (1 / step.float())[..., None] + 8.5).floor()
+    code = code.clamp(0, 15).flatten(-2).long()
+    got = O.unpack(cache.cpu(), dt)
+    for have, want in zip(got, (code, step, mid)):
+        have = have.transpose(2, 3).flatten(1, 2)[:, :T]  # [2, tokens, heads, ...]
+        assert torch.equal(have, want)
+
+
 def test_append_4bit_infinities_and_nans_stay_in_their_group():
     k = torch.zeros((4, 1, 128), dtype=torch.bfloat16)
     k[:] = torch.arange(128) / 8
