@@ -87,7 +87,7 @@ KVS_DEV uint32_t group_meta(float lo, float hi, float& mid, float& inv) {
   }
   const uint32_t mb = f2h<FP16>(__fadd_rn(lo, __fmul_rn(8.f, step)));
   mid = h2f<FP16>(mb);
-  inv = step == 0.f ? 0.f : __fdiv_rn(1.f, step);  // 0: every code is 8, the mid
+  inv = step == 0.f ? 0.f : __frcp_rn(step);  // 0: every code is 8, the mid
   return sb | (mb << 16);
 }
 
@@ -154,7 +154,7 @@ KVS_DEV void store_row4(const AppendLaunch& L, uint8_t* rec, int value, int off,
 // Bound by memory: measured at 16384 tokens of 32 + 8 heads into a bf16 cache, and
 // for a decode step by the launch.
 template <bool FP16, int MODE, bool FOUR, int EACH>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 3)
     k_append_kv(const __grid_constant__ AppendLaunch L, const __grid_constant__ Spread S) {
   const int l = threadIdx.x & 7, gi = threadIdx.x >> 3;
   const uint32_t mask = 0xFFu << (threadIdx.x & 24);
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kThreads)
 // Eight lanes read one row: key rows of a token, then value rows; slot < 0 reads zeros.  Lane
 // 4 hi + c holds the codes of q = 2 hi and 2 hi + 1, i.e. the chunks 8 hi + c and 8 hi + 4 + c.
 template <bool FP16, int EACH>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 3)
     k_read_kv4(const __grid_constant__ Read4Launch L, const __grid_constant__ Spread S) {
   const int l = threadIdx.x & 7, gi = threadIdx.x >> 3, c = l & 3, hi = l >> 2;
   const int t = static_cast<int>(blockIdx.x) * (kGroups / S.across) + gi / S.across;
