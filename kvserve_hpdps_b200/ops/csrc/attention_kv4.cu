@@ -24,7 +24,7 @@
 // mma.sync takes the operands from the registers that unpack them.
 #include <type_traits>
 
-#include "kv4.cuh"
+#include "attention_kv4.cuh"
 
 namespace kvs {
 
@@ -35,42 +35,6 @@ constexpr int kStep = 32;             // tokens a warp takes at a time
 constexpr int kUnit = kWarps * kStep; // tokens a CTA takes at a time: the unit of work
 constexpr int kOver = 2;              // what starting and ending an item costs, in units
 constexpr int kLeast = 4;             // a CTA's share of the line is no shorter than this
-constexpr float kLowest = -1e30f;     // running maximum of a row that has seen nothing
-constexpr int kLowestExp = -100;      // smallest exponent that values are scaled by
-constexpr float kLazy = 8.f;          // log2 by which a score may pass its running maximum
-
-struct Seq {
-  int row0, n, len;  // first query row, query rows, cached tokens
-};
-
-// The sequence's extents, held to what the launch's arrays cover.
-KVS_DEV Seq sequence(const Attn4Launch& L, int r, bool report) {
-  Seq s;
-  int end;
-  if (L.start != nullptr) {
-    s.row0 = L.start[r];
-    end = L.start[r + 1];
-  } else {
-    s.row0 = r;
-    end = r + 1;
-  }
-  s.n = end - s.row0;
-  s.len = L.lens[r];
-  const long long cap = static_cast<long long>(L.table_cols) * L.block_size;
-  const bool bad = s.row0 < 0 || end < s.row0 || end > L.tokens || s.n > L.max_q || s.len < 0 ||
-                   s.len > cap;
-  if (bad) {
-    if (report) record_error(L.err, ERR_BOUNDS);
-    s.n = 0;
-  }
-  return s;
-}
-
-KVS_DEV float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 KVS_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                       uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -82,33 +46,6 @@ KVS_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint
 KVS_DEV uint32_t transpose8(uint32_t a) {
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
-  return d;
-}
-// The codes in nibbles 0..3 of both halves of a word, each less 8, as fp16 pairs.
-KVS_DEV uint32_t and_or(uint32_t a, uint32_t mask, uint32_t with) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(with));
-  return d;
-}
-KVS_DEV void codes4(uint32_t w, uint32_t k1024, uint32_t (&r)[4]) {
-  const uint32_t v = w >> 8;
-  const __half2 low = __float2half2_rn(-1032.f), part = __float2half2_rn(0.0625f),
-                high = __float2half2_rn(-72.f);
-  auto as_half2 = [](uint32_t x) { return *reinterpret_cast<const __half2*>(&x); };
-  auto bits = [](__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); };
-  r[0] = bits(__hadd2(as_half2(and_or(w, 0x000F000Fu, k1024)), low));
-  r[1] = bits(__hfma2(as_half2(and_or(w, 0x00F000F0u, k1024)), part, high));
-  r[2] = bits(__hadd2(as_half2(and_or(v, 0x000F000Fu, k1024)), low));
-  r[3] = bits(__hfma2(as_half2(and_or(v, 0x00F000F0u, k1024)), part, high));
-}
-KVS_DEV uint32_t half2_bits(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-KVS_DEV uint32_t max_u16x2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 KVS_DEV void cp_async16(uint32_t dst, const void* src) {
@@ -152,19 +89,6 @@ KVS_DEV void lds_meta(const uint8_t* a, uint32_t (&m)[NG]) {
 // two: one for an item that began before its share, one for an item that
 // goes on behind it) and k_attn4_combine joins an item's parts in order, so
 // results do not depend on timing.
-struct Parts {
-  int4* desc;   // [B] item that begins in CTA b and goes on: (r, h, tile, parts) or r < 0
-  float2* ml;   // [2 B][rows] running maximum and sum
-  float* o;     // [2 B][rows][128]
-};
-KVS_DEV Parts parts(void* scratch, int B, int rows) {
-  Parts p;
-  p.desc = static_cast<int4*>(scratch);
-  p.ml = reinterpret_cast<float2*>(p.desc + B);
-  p.o = reinterpret_cast<float*>(p.ml + 2ll * B * rows);
-  return p;
-}
-
 // CTA b's share of a line of length U dealt to B: [begin(b), begin(b + 1)).
 struct Deal {
   int each, more;  // U / B, U % B
@@ -685,88 +609,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
   }
 }
 
-// Joins the parts of the item that begins in CTA blockIdx.x and goes on in
-// the next ones: eight rows a CTA, four warps a row, each every fourth part.
-template <bool FP16, int NT>
-__global__ void __launch_bounds__(1024) k_attn4_combine(const __grid_constant__ Attn4Launch L) {
-  constexpr int ROWS = 8 * NT;
-  __shared__ float s_m[4][8], s_l[4][8];
-  __shared__ float4 s_acc[4][8][32];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int B = gridDim.x, b = blockIdx.x;
-  const Parts P = parts(L.scratch, B, ROWS);
-  const int4 d = P.desc[b];
-  if (d.x < 0) return;
-  const int group = L.q_heads / L.heads, np = d.w;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r8 = warp & 7, quarter = warp >> 3;
-  const int row = blockIdx.y * 8 + r8;
-  // part 0 is in CTA b's second slot, the others in the first ones of the next CTAs
-  auto slot = [&](int i) { return (i == 0 ? 2 * b + 1 : 2 * (b + i)) * ROWS + row; };
-  float m = kLowest, ls = 0.f;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = quarter; i0 < np; i0 += 16) {  // four parts at a time, their loads together
-    float2 ml[4];
-    float4 x[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = i0 + 4 * u;
-      ml[u] = make_float2(kLowest, 0.f);
-      x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (i < np) {
-        ml[u] = P.ml[slot(i)];
-        x[u] = *reinterpret_cast<const float4*>(P.o + slot(i) * 128ll + lane * 4);
-      }
-    }
-    const float top = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
-    const float k0 = ex2(m - top);
-    m = top;
-    ls *= k0;
-    a.x *= k0;
-    a.y *= k0;
-    a.z *= k0;
-    a.w *= k0;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float k2 = ex2(ml[u].x - top);
-      ls = fmaf(ml[u].y, k2, ls);
-      a.x = fmaf(x[u].x, k2, a.x);
-      a.y = fmaf(x[u].y, k2, a.y);
-      a.z = fmaf(x[u].z, k2, a.z);
-      a.w = fmaf(x[u].w, k2, a.w);
-    }
-  }
-  s_acc[quarter][r8][lane] = a;
-  if (lane == 0) {
-    s_m[quarter][r8] = m;
-    s_l[quarter][r8] = ls;
-  }
-  __syncthreads();
-  if (quarter != 0) return;
-  const Seq s = sequence(L, d.x, false);
-  const int rr = d.z * ROWS + row;
-  if (rr >= s.n * group) return;  // rows behind the tile's last were not written either
-  m = fmaxf(fmaxf(s_m[0][r8], s_m[1][r8]), fmaxf(s_m[2][r8], s_m[3][r8]));
-  ls = 0.f;
-  a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float k2 = ex2(s_m[w][r8] - m);
-    const float4 x = s_acc[w][r8][lane];
-    ls = fmaf(s_l[w][r8], k2, ls);
-    a.x = fmaf(x.x, k2, a.x);
-    a.y = fmaf(x.y, k2, a.y);
-    a.z = fmaf(x.z, k2, a.z);
-    a.w = fmaf(x.w, k2, a.w);
-  }
-  const long long tq = s.row0 + rr / group;
-  const int hq = d.y * group + rr % group;
-  const float inv = ls == 0.f ? 0.f : __fdividef(1.f, ls);
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + tq * L.o_ts + hq * L.o_hs + lane * 4) =
-      make_uint2(f2h2<FP16>(a.x * inv, a.y * inv), f2h2<FP16>(a.z * inv, a.w * inv));
-  if (L.lse != nullptr && lane == 0)
-    L.lse[tq * L.q_heads + hq] = ls == 0.f ? -INFINITY : (m + log2f(ls)) * 0.69314718055994531f;
-}
-
 struct Grid {
   int ctas, rows;
   bool fits;   // the line's length is an int
@@ -792,6 +634,12 @@ Grid grid_of(const Attn4Launch* L) {
   return g;
 }
 
+// More rows a kv head than this go to attention_kv4_tile.cu.
+constexpr int kManyRows = 64;
+bool many_rows(const Attn4Launch* L) {
+  return static_cast<long long>(L->max_q) * (L->q_heads / L->heads) > kManyRows;
+}
+
 template <bool FP16, int NG, int NT>
 cudaError_t launch(const Attn4Launch& L, const Grid& g, cudaStream_t s) {
   const int smem = kWarps * 4 * half_bytes<NG>();  // at most 40 KB: no opt-in needed
@@ -799,16 +647,7 @@ cudaError_t launch(const Attn4Launch& L, const Grid& g, cudaStream_t s) {
   k_attn4<FP16, NG, NT><<<g.ctas, kWarps * 32, smem, s>>>(L);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || !g.split) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(g.ctas, NT);
-  cfg.blockDim = dim3(1024);
-  cfg.stream = s;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_attn4_combine<FP16, NT>, L);
+  return launch_combine<FP16, NT>(L, g.ctas, s);
 }
 
 template <bool FP16, int NG>
@@ -830,15 +669,17 @@ using namespace kvs;
 extern "C" {
 
 long long kvs_attn4_scratch_bytes(const Attn4Launch* L) {
+  if (many_rows(L)) return attn4_tile_scratch(*L);
   const Grid g = grid_of(L);
   return 16ll * g.ctas + 2ll * g.ctas * g.rows * (8 + 512);
 }
 
 int kvs_attention_kv4(const Attn4Launch* L, void* stream) {
   if (L->seqs <= 0 || L->max_q <= 0 || L->tokens <= 0 || L->heads <= 0) return 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (many_rows(L)) return attn4_tile_launch(*L, s) == cudaSuccess ? 0 : -1;
   const Grid g = grid_of(L);
   if (!g.fits) return -2;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e =
       L->fp16 ? launch_groups<true>(*L, g, s) : launch_groups<false>(*L, g, s);
   return e == cudaSuccess ? 0 : -1;

@@ -1,0 +1,693 @@
+// Attention over a paged 4-bit cache for many query rows (prefill chunks).
+//
+// The mathematics is attention_kv4.cu's; here 2 x 128 query rows (several
+// tokens times the query heads of one kv head) share each key, so the keys
+// are worth turning into 16-bit tiles once, for tcgen05:
+//   S = Q K^T, O += P V, 128 x 128 x 128 fp16 products into tensor memory.
+// K and V become fp16 with one power of two for each 32 tokens, chosen from the largest
+// step and mid among them, so any scale keeps fp16's relative 2^-11; the power
+// goes into the softmax's factor (K) and into the exponent's reference (V).
+//
+// Roles of a CTA (one an SM, 13 warps):
+//   warps 0-3, 4-7   softmax of query tile 0, 1: a thread a row.  A first pass
+//                    over the row's scores in tensor memory finds their
+//                    maximum, a second writes exp as fp16 over them, the A
+//                    operand of O += P V.
+//   warps 8-11       packed rows to fp16 tiles in shared memory, a thread a token
+//   warp 12          issues the matrix instructions
+// Two query tiles take turns: while one's scores go through the exponentials,
+// the other's products run.  O stays in tensor memory; it is rescaled by the
+// softmax warps when a row's maximum has grown by more than 2^kLazy, which
+// after the first tiles is rare.  What bounds it: the exponentials (16 a
+// clock and SM: 2048 clocks for 2 x 128 x 128 scores) next to the products
+// (2048 clocks at the nominal rate).
+//
+// The work is dealt out as in attention_kv4.cu, here by the number of visible
+// keys a tile has, so that causal tiles of a long chunk load all SMs alike.
+#include "attention_kv4.cuh"
+
+namespace kvs {
+
+namespace {
+
+constexpr int kRows = 256;       // an item's query rows, two tiles
+constexpr int kTile = 128;       // tokens a step
+constexpr int kThreads = 13 * 32;
+constexpr int kOverTile = 2;     // an item's own cost, in steps
+constexpr int kLeastTile = 2;    // steps a CTA takes at least
+constexpr int kHalfTile = 16384; // 128 rows x 64 channels of fp16
+
+struct Ctrl {
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_full[2], o_full[2], e_full[4];
+  uint32_t tmem;
+  // What the converting warps say of a step (ring of four), by 32 tokens:
+  float k_up[4][4];        // K in shared memory times this is K
+  int v_exp[4][4];         // V in shared memory times 2^this is V
+  uint32_t gone[4][4];     // tokens whose block does not exist
+  uint32_t bad[4][4][4];   // [..][group] tokens with a step or mid of V that is not finite
+  uint32_t flags[4][4];    // whether any of the two is set
+  long long scan[kThreads / 32];
+  long long begin;
+  int seq;
+};
+
+constexpr int kSmem = 1024 + 6 * 2 * kHalfTile + static_cast<int>(sizeof(Ctrl));
+
+// Instruction descriptor: fp16 x fp16 -> fp32, M = N = 128; B K-major or MN-major.
+constexpr uint32_t kIdescQK = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+constexpr uint32_t kIdescPV = kIdescQK | (1u << 16);
+
+// Tile [128 rows][128 channels] in shared memory: two halves of 64 channels, rows of 128
+// bytes, 16-byte chunks swizzled by the row.  As K (rows: N, channels: K) it is K-major;
+// as V (rows: K, channels: N) it is MN-major: 64 channels a block, blocks 16 KB apart
+// (leading offset), groups of 8 tokens 1 KB apart (stride offset).
+KVS_DEV uint64_t mn_desc(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(kHalfTile >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+KVS_DEV uint32_t chunk_at(int row, int chunk) {
+  return (chunk >> 3) * kHalfTile + (row >> 3) * 1024 + (row & 7) * 128 +
+         (((chunk & 7) ^ (row & 7)) << 4);
+}
+KVS_DEV void mma_pv(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a_tmem), "l"(b), "r"(kIdescPV), "r"(accumulate)
+      : "memory");
+}
+KVS_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
+      : "memory");
+}
+KVS_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ------------------------------------------------------------- work split
+// A tile's cost is linear in its number: with n rows' worth of queries and `len` tokens,
+// tile t's last row sees about len - n + (256 t + 255) / group + 1 of them.  In units of
+// 1 / group tokens: cost(t) = first + 256 t, which sums up in closed form.
+struct TileWork {
+  int tiles;
+  long long first, head;  // cost of tile 0; of a head's tiles together
+  KVS_DEV long long before(long long t) const { return t * first + kRows * (t * (t - 1) / 2); }
+};
+KVS_DEV TileWork tile_work(const Seq& s, int group) {
+  TileWork w;
+  w.tiles = static_cast<int>((static_cast<long long>(s.n) * group + kRows - 1) / kRows);
+  w.first = static_cast<long long>(group) * (kOverTile * kTile + max(s.len - s.n, 0) + 1) +
+            kRows - 1;
+  w.head = w.before(w.tiles);
+  return w;
+}
+
+struct Piece {
+  Seq s;
+  int r, h, tile, nrows;     // nrows: the sequence's query rows times heads of the group
+  int start, stop, steps;    // tokens [start, stop) in `steps` tiles
+  bool two, whole, begins;   // second query tile in use; not shared; the item's first part
+  int parts;                 // begins and not whole: CTAs that share it
+};
+
+// Walks the pieces of a CTA's share; every thread does the same.
+struct Walk {
+  long long U, pos, end, begin;
+  int r, used, b;
+  KVS_DEV long long share(int i) const { return U * i / used; }
+  KVS_DEV bool next(const Attn4Launch& L, int group, Piece& p) {
+    const long long unit = static_cast<long long>(kTile) * group;
+    while (pos < end) {
+      p.s = sequence(L, r, false);
+      const TileWork w = tile_work(p.s, group);
+      if (pos >= begin + w.head * L.heads) {
+        begin += w.head * L.heads;
+        ++r;
+        continue;
+      }
+      long long off = pos - begin;
+      const int h = static_cast<int>(off / w.head);
+      off -= h * w.head;
+      int lo = 0, hi = w.tiles - 1;  // the last tile that begins at or before off
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (w.before(mid) <= off) lo = mid;
+        else hi = mid - 1;
+      }
+      const long long item = begin + h * w.head + w.before(lo);
+      const long long cost = w.first + static_cast<long long>(kRows) * lo;
+      const long long body = item + kOverTile * unit;  // the steps lie behind the item's own cost
+      const long long to = min(end, item + cost);
+      p.nrows = p.s.n * group;
+      const int last_row = min(p.nrows, (lo + 1) * kRows) - 1;
+      const int limit = max(0, p.s.len - p.s.n + last_row / group + 1);
+      const int all = max(1, (limit + kTile - 1) / kTile);
+      auto step_of = [&](long long x) {
+        if (x >= item + cost) return all;
+        if (x <= body) return 0;
+        const long long k = (x - body) / unit;
+        return static_cast<int>(k < all ? k : all);
+      };
+      const int u0 = step_of(pos), u1 = step_of(to);
+      pos = to;
+      if (u0 >= u1) continue;
+      p.r = r;
+      p.h = h;
+      p.tile = lo;
+      p.start = u0 * kTile;
+      p.stop = min(limit, u1 * kTile);
+      p.steps = p.stop > p.start ? (p.stop - p.start + kTile - 1) / kTile : 0;
+      p.two = p.nrows - lo * kRows > 128;
+      p.begins = u0 == 0;
+      p.whole = u0 == 0 && u1 == all;
+      if (p.begins && !p.whole) {  // the last part is the CTA's whose share reaches the last step
+        const long long x = min(item + cost, body + all * unit) - 1;
+        p.parts = static_cast<int>(((x + 1) * used + U - 1) / U - 1) - b + 1;
+      }
+      return true;
+    }
+    return false;
+  }
+};
+
+#define KVS_WAIT(bar, parity) __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, L.err, ERR_MBAR_TIMEOUT))
+
+// ---------------------------------------------------- packed rows to tiles
+template <bool FP16, int NG>
+KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* k_tile,
+                          uint8_t* v_tile, Ctrl* C) {
+  const int lane = threadIdx.x & 31, seg = (threadIdx.x >> 5) & 3, row = seg * 32 + lane;
+  constexpr uint32_t kInf = FP16 ? 0x7C00u : 0x7F80u;
+  constexpr uint32_t k1024 = 0x64006400u;
+  uint32_t step_no = 0;
+  Piece p;
+  while (walk.next(L, group, p)) {
+    const uint8_t* const head = static_cast<const uint8_t*>(L.cache) + p.h * L.head_stride;
+    const int32_t* const table = L.table + p.r * L.table_stride;
+    for (int j = 0; j < p.steps; ++j, ++step_no) {
+      const int tok = p.start + j * kTile + row;
+      uint4 code[2][4] = {};
+      uint32_t meta[2][NG] = {};
+      bool gone = false;
+      if (tok < p.stop) {
+        const int page = tok / L.block_size, off = tok - page * L.block_size;
+        const int id = table[page];
+        gone = id < 0 || id >= L.num_blocks;
+        if (gone) {
+          record_error(L.err, ERR_BOUNDS);
+        } else {
+          const uint8_t* rec = head + id * L.block_stride;
+          const Kv4Record R{NG, L.block_size};
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            const uint4* src = reinterpret_cast<const uint4*>(rec + R.codes(v, off));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) code[v][i] = src[i];
+            const uint32_t* ms = reinterpret_cast<const uint32_t*>(rec + R.meta(v, off));
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) meta[v][gr] = ms[gr];
+          }
+        }
+      }
+      // exponent of the largest finite step or mid of the warp's 32 tokens
+      float up[2];
+      uint32_t bad[NG];
+      const int ring = step_no & 3;
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) bad[gr] = 0;
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          const uint32_t a = meta[v][gr] & 0x7FFFu, z = (meta[v][gr] >> 16) & 0x7FFFu;
+          const bool fine = a < kInf && z < kInf;
+          if (fine) top = max(top, max(a, z));
+          if (v == 1) {
+            bad[gr] = __ballot_sync(0xFFFFFFFFu, !fine);
+            if (!fine) meta[v][gr] = 0;  // rows that see it are marked instead
+          }
+        }
+        const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h2f<FP16>(top)));
+        const int e = max(static_cast<int>(most >> 23) - 127, kLowestExp) - 8;
+        up[v] = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        if (lane == 0) {
+          if (v == 0) C->k_up[ring][seg] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+          else C->v_exp[ring][seg] = e;
+        }
+      }
+      const uint32_t lost = __ballot_sync(0xFFFFFFFFu, gone);
+      if (lane == 0) {
+        uint32_t any = lost;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          C->bad[ring][seg][gr] = bad[gr];
+          any |= bad[gr];
+        }
+        C->gone[ring][seg] = lost;
+        C->flags[ring][seg] = any;
+        mbar_arrive(&C->e_full[ring]);
+      }
+      const int stage = step_no & 1;
+      const uint32_t again = ((step_no >> 1) & 1) ^ 1;
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        uint64_t* const empty = v ? &C->v_empty[stage] : &C->k_empty[stage];
+        if (!KVS_WAIT(empty, again)) return;
+        uint8_t* const dst = (v ? v_tile : k_tile) + stage * 2 * kHalfTile;
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[4 * i] = code[v][i].x;
+          w[4 * i + 1] = code[v][i].y;
+          w[4 * i + 2] = code[v][i].z;
+          w[4 * i + 3] = code[v][i].w;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t m = meta[v][q * NG / 4];
+          const __half2 step = __float2half2_rn(h2f<FP16>(m & 0xFFFFu) * up[v]);
+          const __half2 mid = __float2half2_rn(h2f<FP16>(m >> 16) * up[v]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            // the eight codes of channels 32 q + 8 c + 0..7, pairs (i, i + 4)
+            const uint32_t x = v == 0 ? w[4 * c + q]
+                                      : __byte_perm(w[4 * c + (q >> 1)], w[4 * c + 2 + (q >> 1)],
+                                                    (q & 1) ? 0x7632 : 0x5410);
+            uint32_t u[4];
+            codes4(x, k1024, u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&u[i]), step, mid);
+              u[i] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+            *reinterpret_cast<uint4*>(dst + chunk_at(row, 4 * q + c)) =
+                make_uint4(u[0], u[1], u[2], u[3]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v ? &C->v_full[stage] : &C->k_full[stage]);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------ matrix instructions
+KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, uint32_t q_tile, uint32_t k_tile,
+                      uint32_t v_tile, uint32_t tmem, Ctrl* C) {
+  uint32_t step_no = 0, piece_no[2] = {0, 0}, p_no[2] = {0, 0};
+  Piece p;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait(bar, parity, L.err, ERR_MBAR_TIMEOUT);
+  };
+  auto qk = [&](int x, uint32_t no) {
+    const uint32_t a = q_tile + x * 2 * kHalfTile, b = k_tile + (no & 1) * 2 * kHalfTile;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      const uint32_t off = (ks >> 2) * kHalfTile + (ks & 3) * 32;
+      umma_bf16_f32(tmem + 128 * x, sw128_kmajor_desc(a + off), sw128_kmajor_desc(b + off),
+                    kIdescQK, ks > 0 ? 1u : 0u);
+    }
+    umma_commit(&C->s_full[x]);
+  };
+  auto pv = [&](int x, uint32_t no, bool first) {
+    const uint32_t b = v_tile + (no & 1) * 2 * kHalfTile;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks)  // 16 tokens: two groups of eight rows, 8 columns of P
+      mma_pv(tmem + 256 + 128 * x, tmem + 128 * x + 8 * ks, mn_desc(b + ks * 2048),
+             first && ks == 0 ? 0u : 1u);
+  };
+  while (walk.next(L, group, p)) {
+    if (p.steps == 0) continue;
+    const int n = p.two ? 2 : 1;
+    for (int x = 0; x < n; ++x)
+      if (!wait(&C->q_full[x], piece_no[x]++ & 1)) return;
+    if (!wait(&C->k_full[step_no & 1], (step_no >> 1) & 1)) return;
+    tc_fence_after();
+    for (int x = 0; x < n; ++x) qk(x, step_no);
+    umma_commit(&C->k_empty[step_no & 1]);
+    for (int j = 0; j < p.steps; ++j, ++step_no) {
+      const uint32_t parity = (step_no >> 1) & 1, next = step_no + 1;
+      for (int x = 0; x < n; ++x) {
+        if (!wait(&C->p_full[x], p_no[x]++ & 1)) return;
+        if (x == 0 && !wait(&C->v_full[step_no & 1], parity)) return;
+        tc_fence_after();
+        pv(x, step_no, j == 0);
+        if (j + 1 < p.steps) {
+          if (x == 0 && !wait(&C->k_full[next & 1], (next >> 1) & 1)) return;
+          tc_fence_after();
+          qk(x, next);
+        } else {
+          umma_commit(&C->o_full[x]);
+        }
+      }
+      umma_commit(&C->v_empty[step_no & 1]);
+      if (j + 1 < p.steps) umma_commit(&C->k_empty[next & 1]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ softmax
+template <bool FP16, int NG>
+KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q_tile,
+                          uint32_t tmem, const Parts& P, Ctrl* C) {
+  const int x = threadIdx.x >> 7, row = threadIdx.x & 127;
+  const uint32_t lanes = static_cast<uint32_t>((threadIdx.x >> 5) & 3) << 21;  // 32 TMEM lanes a warp
+  const uint32_t S = tmem + 128 * x + lanes, O = tmem + 256 + 128 * x + lanes;
+  uint8_t* const qt = q_tile + x * 2 * kHalfTile;
+  uint32_t step_no = 0, s_no = 0, o_no = 0;
+  Piece p;
+  while (walk.next(L, group, p)) {
+    if (x == 1 && !p.two) {
+      step_no += p.steps;
+      continue;
+    }
+    const int rr = p.tile * kRows + x * 128 + row;
+    const bool mine = rr < p.nrows;
+    const long long tq = p.s.row0 + rr / group;
+    const int hq = p.h * group + rr % group;
+    const int seen = mine ? p.s.len - p.s.n + rr / group + 1 : 0;
+    float m = kLowest, l = 0.f, f = 0.f;
+    int E = kLowestExp;
+    uint32_t poison = 0;
+    if (p.steps > 0) {
+      // ---- the row as fp16, scaled by a power of two: largest element in [2^14, 2^15)
+      uint4 raw[16] = {};
+      if (mine) {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(L.q) +
+                                                          tq * L.q_ts + hq * L.q_hs);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) raw[i] = src[i];
+      }
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float y[8];
+        unpack8<FP16>(raw[i], y);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(y[k]));
+      }
+      int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+      e = top == 0.f ? 0 : max(kLowestExp, min(e, 100));
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23) *
+                       (L.scale < 0.f ? -1.f : 1.f);
+      f = fabsf(L.scale) * 1.4426950408889634f *
+          __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float y[8];
+        unpack8<FP16>(raw[i], y);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] *= up;
+        *reinterpret_cast<uint4*>(qt + chunk_at(row, i)) =
+            make_uint4(half2_bits(y[0], y[4]), half2_bits(y[1], y[5]), half2_bits(y[2], y[6]),
+                       half2_bits(y[3], y[7]));
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&C->q_full[x]);
+      // tokens that every row of this warp sees
+      const int all_see = __reduce_min_sync(0xFFFFFFFFu, mine ? max(seen, 0) : 0x7FFFFFFF);
+      for (int j = 0; j < p.steps; ++j, ++step_no, ++s_no) {
+        const int ring = step_no & 3, t0 = p.start + j * kTile;
+        if (!KVS_WAIT(&C->e_full[ring], (step_no >> 2) & 1)) return;
+        if (!KVS_WAIT(&C->s_full[x], s_no & 1)) return;
+        tc_fence_after();
+        const uint32_t flag = C->flags[ring][0] | C->flags[ring][1] | C->flags[ring][2] |
+                              C->flags[ring][3];
+        const bool masked = t0 + kTile > min(all_see, p.stop) || flag != 0;
+        // columns of segment g that this row sees
+        auto visible = [&](int sg) {
+          const int n = min(seen, p.stop) - t0 - 32 * sg;
+          const uint32_t v = n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
+          return v & ~C->gone[ring][sg];
+        };
+        // ---- maximum
+        float mx = -INFINITY;
+        int e_new = E;
+#pragma unroll
+        for (int sg = 0; sg < 4; ++sg) {
+          float v[32];
+          tmem_ld32(S + 32 * sg, v);
+          float part = -INFINITY;
+          if (masked) {
+            const uint32_t vis = visible(sg);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (vis >> i & 1u) part = fmaxf(part, v[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) part = fmaxf(part, v[i]);
+          }
+          mx = fmaxf(mx, part * (f * C->k_up[ring][sg]));
+          e_new = max(e_new, C->v_exp[ring][sg]);
+        }
+        if (__any_sync(0xFFFFFFFFu, mx > m + kLazy) || e_new != E) {
+          const float m_new = fmaxf(m, mx), k2 = ex2(m - m_new);
+          l *= k2;
+          if (j > 0) {
+            const float ko = k2 * ex2(static_cast<float>(E - e_new));
+#pragma unroll
+            for (int cg = 0; cg < 4; ++cg) {
+              float v[32];
+              tmem_ld32(O + 32 * cg, v);
+              uint32_t a[16], b[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                a[i] = __float_as_uint(v[i] * ko);
+                b[i] = __float_as_uint(v[i + 16] * ko);
+              }
+              tmem_st16(O + 32 * cg, a);
+              tmem_st16(O + 32 * cg + 16, b);
+            }
+          }
+          m = m_new;
+          E = e_new;
+        }
+        // ---- exponentials, to where the scores were
+#pragma unroll
+        for (int sg = 0; sg < 4; ++sg) {
+          float v[32];
+          tmem_ld32(S + 32 * sg, v);
+          const float fs = f * C->k_up[ring][sg];
+          const int ev = C->v_exp[ring][sg];
+          const float ref = m + static_cast<float>(E - ev);
+          float sum0 = 0.f, sum1 = 0.f;
+          uint32_t h[16];
+          const uint32_t vis = masked ? visible(sg) : 0xFFFFFFFFu;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float p0 = ex2(fmaf(v[2 * i], fs, -ref)), p1 = ex2(fmaf(v[2 * i + 1], fs, -ref));
+            if (masked) {
+              p0 = vis >> (2 * i) & 1u ? p0 : 0.f;
+              p1 = vis >> (2 * i + 1) & 1u ? p1 : 0.f;
+            }
+            sum0 += p0;
+            sum1 += p1;
+            h[i] = half2_bits(p0, p1);
+          }
+          l = fmaf(sum0 + sum1, ex2(static_cast<float>(E - ev)), l);
+          tmem_st16(S + 16 * sg, h);
+          if (flag) {
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr)
+              if (C->bad[ring][sg][gr] & vis) poison |= 1u << gr;
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&C->p_full[x]);
+      }
+      if (!KVS_WAIT(&C->o_full[x], o_no++ & 1)) return;
+      tc_fence_after();
+    }
+    // ---- the result, or this part of it
+    const float scale_o = p.steps > 0 ? ex2(static_cast<float>(E)) : 0.f;
+    const float inv = l == 0.f ? 0.f : __fdividef(scale_o, l);
+    const int slot = 2 * static_cast<int>(blockIdx.x) + (p.begins ? 1 : 0);
+    uint16_t* const out = static_cast<uint16_t*>(L.out) + tq * L.o_ts + hq * L.o_hs;
+    float* const part = P.o + (static_cast<long long>(slot) * kRows + x * 128 + row) * 128;
+#pragma unroll
+    for (int cg = 0; cg < 4; ++cg) {  // 32 channels: one group or part of one
+      float v[32];
+      if (p.steps > 0) {
+        tmem_ld32(O + 32 * cg, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0.f;
+      }
+      if (poison >> (cg * NG / 4) & 1u) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(0x7FC00000u);
+      }
+      if (!mine) continue;
+      const float k = p.whole ? inv : scale_o;
+#pragma unroll
+      for (int ch = 0; ch < 4; ++ch) {  // columns hold channels 0, 4, 1, 5, 2, 6, 3, 7 of eight
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[(i >> 1) + 4 * (i & 1)] = v[8 * ch + i] * k;
+        if (p.whole) {
+          *reinterpret_cast<uint4*>(out + 32 * cg + 8 * ch) = pack8<FP16>(y);
+        } else {
+          float4* d = reinterpret_cast<float4*>(part + 32 * cg + 8 * ch);
+          d[0] = make_float4(y[0], y[1], y[2], y[3]);
+          d[1] = make_float4(y[4], y[5], y[6], y[7]);
+        }
+      }
+    }
+    if (mine) {
+      if (!p.whole)
+        P.ml[slot * kRows + x * 128 + row] = make_float2(m, l);
+      else if (L.lse != nullptr)
+        L.lse[tq * L.q_heads + hq] =
+            l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    }
+    if (!p.whole && p.begins && threadIdx.x == 0)
+      P.desc[blockIdx.x] = make_int4(p.r, p.h, p.tile, p.parts);
+    tc_fence_before();
+    __syncwarp();
+  }
+}
+
+template <bool FP16, int NG>
+__global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constant__ Attn4Launch L) {
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t *const q_tile = smem, *const k_tile = smem + 4 * kHalfTile,
+                 *const v_tile = smem + 8 * kHalfTile;
+  Ctrl* const C = reinterpret_cast<Ctrl*>(smem + 12 * kHalfTile);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int group = L.q_heads / L.heads, B = gridDim.x, b = blockIdx.x;
+  const Parts P = parts(L.scratch, B, kRows);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) {
+    P.desc[b] = make_int4(-1, 0, 0, 0);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&C->q_full[i], 128);
+      mbar_init(&C->k_full[i], 4);
+      mbar_init(&C->k_empty[i], 1);
+      mbar_init(&C->v_full[i], 4);
+      mbar_init(&C->v_empty[i], 1);
+      mbar_init(&C->s_full[i], 1);
+      mbar_init(&C->p_full[i], 128);
+      mbar_init(&C->o_full[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(&C->e_full[i], 4);
+    fence_mbar_init();
+  }
+  if (warp == 12) tmem_alloc(&C->tmem, 512);
+  tc_fence_before();
+
+  // ---- this CTA's share of the line
+  long long total = 0, mine = 0;
+  for (int r = tid; r < L.seqs; r += kThreads) {
+    mine = tile_work(sequence(L, r, b == 0), group).head * L.heads;
+    total += mine;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+  if (lane == 0) C->scan[warp] = total;
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = C->tmem;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) total += C->scan[w];
+  const long long least = static_cast<long long>(kLeastTile) * kTile * group;
+  Walk walk;
+  walk.U = total;
+  walk.b = b;
+  walk.used = static_cast<int>(min(static_cast<long long>(B), (total + least - 1) / least));
+  if (b < walk.used) {
+    walk.pos = walk.share(b);
+    walk.end = walk.share(b + 1);
+    long long base = 0;
+    for (int r0 = 0; r0 < L.seqs; r0 += kThreads) {
+      const int r = r0 + tid;
+      if (L.seqs > kThreads)  // else `mine` is it
+        mine = r < L.seqs ? tile_work(sequence(L, r, false), group).head * L.heads : 0;
+      long long inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+        if (lane >= o) inc += y;
+      }
+      __syncthreads();
+      if (lane == 31) C->scan[warp] = inc;
+      __syncthreads();
+      long long before = base;
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) before += C->scan[w];
+        base += C->scan[w];
+      }
+      if (before + inc - mine <= walk.pos && walk.pos < before + inc) {
+        C->seq = r;
+        C->begin = before + inc - mine;
+      }
+      if (walk.pos < base) break;  // the same for every thread
+    }
+    __syncthreads();
+    walk.r = C->seq;
+    walk.begin = C->begin;
+    if (warp < 8) {
+      softmax_role<FP16, NG>(L, walk, group, q_tile, tmem, P, C);
+    } else if (warp < 12) {
+      convert_role<FP16, NG>(L, walk, group, k_tile, v_tile, C);
+    } else if (lane == 0) {
+      mma_role(L, walk, group, smem_u32(q_tile), smem_u32(k_tile), smem_u32(v_tile), tmem, C);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+int tile_ctas(const Attn4Launch& L) {
+  const int group = L.q_heads / L.heads;
+  const long long tiles = (static_cast<long long>(L.max_q) * group + kRows - 1) / kRows;
+  const long long steps =
+      (static_cast<long long>(L.table_cols) * L.block_size + kTile - 1) / kTile;
+  const long long most = static_cast<long long>(L.seqs) * L.heads * tiles * (steps + kOverTile + 1);
+  return static_cast<int>(most < 148 ? (most > 0 ? most : 1) : 148);
+}
+
+template <bool FP16, int NG>
+cudaError_t launch(const Attn4Launch& L, cudaStream_t s) {
+  cudaError_t e = cudaFuncSetAttribute(k_attn4_tile<FP16, NG>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  const int ctas = tile_ctas(L);
+  k_attn4_tile<FP16, NG><<<ctas, kThreads, kSmem, s>>>(L);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  return launch_combine<FP16, kRows / 8>(L, ctas, s);
+}
+
+}  // namespace
+
+cudaError_t attn4_tile_launch(const Attn4Launch& L, cudaStream_t s) {
+  if (L.fp16)
+    return L.groups == 1 ? launch<true, 1>(L, s) : L.groups == 2 ? launch<true, 2>(L, s)
+                                                                 : launch<true, 4>(L, s);
+  return L.groups == 1 ? launch<false, 1>(L, s) : L.groups == 2 ? launch<false, 2>(L, s)
+                                                                : launch<false, 4>(L, s);
+}
+
+long long attn4_tile_scratch(const Attn4Launch& L) {
+  return 16ll * tile_ctas(L) + 2ll * tile_ctas(L) * kRows * (8 + 512);
+}
+
+}  // namespace kvs

@@ -78,7 +78,7 @@ def values(cache, dt):
     return m + (c - 8) * s, m, s
 
 
-def attend(q, cache, table, lens, start, scale=None):
+def attend(q, cache, table, lens, start, scale=None, tiles=False):
     """fp64 (out, lse, tolerance) of attention over a 4-bit cache; NaN rows where
     no sequence has a row.  Tolerance, element by element, of an implementation that
     takes scores and sums in fp32 and probabilities times steps in fp16, before
@@ -89,6 +89,11 @@ def attend(q, cache, table, lens, start, scale=None):
       weights: fp16's half step, 2^-11, of p |code - 8| step; below fp16's
         normal range half of 2^-24 of the largest step, times 8;
       exponentials, sums and the division: 2^-18 of p |v| together.
+    ``tiles``: the kernel for many rows rounds more. Keys and values become fp16, so a
+      key's product with the query is off by at most half a step, 2^-11, of each
+      |q_d k_d|, which adds to the scores' error; a value by 2^-11 |v|, and p itself
+      (there is no step in it) by 2^-11 p: together 2^-10 of p |v| and the
+      product of both errors, in the place of 2^-11 of p |code - 8| step.
     """
     dt = q.dtype
     q, cache = q.double().cpu(), cache.cpu()
@@ -121,13 +126,19 @@ def attend(q, cache, table, lens, start, scale=None):
                 continue
             w = torch.einsum("hgd,hld->hgl", qi, k[:, :seen]) * scale
             werr = torch.einsum("hgd,hld->hgl", qi.abs(), kmag[:, :seen]) * abs(scale) * 2 ** -18
+            if tiles:
+                werr = werr + 2 ** -11 * abs(scale) * torch.einsum("hgd,hld->hgl", qi.abs(),
+                                                                   k[:, :seen].abs())
             z = torch.logsumexp(w, -1, keepdim=True)
             p = torch.exp(w - z)
             out[a + i] = torch.einsum("hgl,hld->hgd", p, v[:, :seen]).reshape(hq, D)
             lse[a + i] = z.reshape(hq)
             e = torch.einsum("hgl,hld->hgd", p * (2 * werr.amax(-1, keepdim=True) + 2 ** -18),
                              vmag[:, :seen])
-            e = e + 2 ** -11 * torch.einsum("hgl,hld->hgd", p, dev[:, :seen])
+            if tiles:
+                e = e + (2 ** -10 + 2 ** -21) * torch.einsum("hgl,hld->hgd", p, v[:, :seen].abs())
+            else:
+                e = e + 2 ** -11 * torch.einsum("hgl,hld->hgd", p, dev[:, :seen])
             e = e + 8 * 2 ** -25 * top * seen * torch.exp(w.amax(-1, keepdim=True) - z)
             tol[a + i] = e.reshape(hq, D)
             ltol[a + i] = werr.amax(-1).reshape(hq) + 2 ** -20 * (1 + lse[a + i].abs())

@@ -291,6 +291,11 @@ def _problem(seqs, hq, h, bs, g_size, dt, seed, spare_rows=0, cols_more=2, sprea
     return q, cache, table, lens, start
 
 
+def _tiles(seqs, hq, h):
+    """Whether a call takes the kernel for many rows: over 64 rows a kv head."""
+    return max(n for n, _ in seqs) * (hq // h) > 64
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("g_size", [32, 64, 128])
 @pytest.mark.parametrize("hq,h,bs", [(7, 1, 16), (8, 8, 32), (28, 4, 16), (16, 1, 16), (48, 2, 48)])
@@ -311,6 +316,9 @@ def test_attention_one_token(dt, g_size, hq, h, bs):
     (7, 1, [(130, 130), (33, 160)]),
     (8, 2, [(64, 300), (17, 17)]),
     (3, 3, [(100, 37)]),
+    (8, 1, [(16, 500), (0, 30), (33, 0), (40, 129), (1, 128)]),   # one tile and two, no keys
+    (16, 2, [(300, 300), (5, 1000), (64, 64)]),
+    (4, 4, [(65, 1111), (1, 1), (257, 256)]),
 ])
 def test_attention_several_rows(dt, g_size, hq, h, seqs):
     q, cache, table, lens, start = _problem(seqs, hq, h, 16, g_size, dt, hq * 7, spare_rows=3)
@@ -320,9 +328,69 @@ def test_attention_several_rows(dt, g_size, hq, h, seqs):
     torch.cuda.synchronize()
     assert got is out
     K.check_device_error(out.device)
-    ref = O.attend(q, cache, table, lens, start)
+    ref = O.attend(q, cache, table, lens, start, tiles=_tiles(seqs, hq, h))
     _check(out, lse, ref, dt)
     assert (out[int(start[-1]):] == 9.0).all()  # rows of no sequence
+
+
+def test_attention_many_rows_magnitudes_and_growth():
+    """Values far from 1, steps and scores that rise along the sequence, a negative scale."""
+    for dt, mag in ((torch.bfloat16, 1e-18), (torch.bfloat16, 1e6), (torch.float16, 1.0)):
+        q, cache, table, lens, start = _problem([(90, 700), (20, 20)], 4, 2, 16, 64, dt, 31)
+        codes, step, mid = O.unpack(cache, dt)
+        grow = torch.zeros(cache.shape[0])
+        used = table[0][:44].long()
+        grow[used] = torch.linspace(-6, 3, 44)
+        grow = torch.exp2(grow)[:, None, None, None].double()
+        up = torch.tensor([1 / mag, mag]).double()[:, None, None, None, None]
+        up = up * torch.stack([grow.sqrt(), grow])
+        step, mid = (step.double() * up).to(dt), (mid.double() * up).to(dt)
+        cache = O.pack(codes, step, mid)
+        q = (q.double() * mag).to(dt)
+        out, lse = P.attention_kv4(q.cuda(), cache.cuda(), table.cuda(), lens.cuda(),
+                                   start.cuda(), 90, scale=-0.11, return_lse=True)
+        torch.cuda.synchronize()
+        K.check_device_error(out.device)
+        want, wlse, tol, ltol = O.attend(q, cache, table, lens, start, scale=-0.11, tiles=True)
+        bound = tol + O.half_step(dt) * (want.abs() + tol)
+        assert ((out.double().cpu() - want).abs() <= bound).all()
+        assert ((lse.double().cpu() - wlse).abs() <= ltol).all()
+
+
+def test_attention_many_rows_bad_blocks_and_numbers():
+    """A block id outside the cache hides its tokens; NaN and infinities behind the length or
+    behind a row's own position do not reach it, and those that it sees stay in their group."""
+    dt, h, hq = torch.bfloat16, 2, 8
+    q, cache, table, lens, start = _problem([(40, 100), (30, 77)], hq, h, 16, 64, dt, 12)
+    ref = O.attend(q, cache, table, lens, start, tiles=True)
+    codes, step, mid = O.unpack(cache, dt)
+    for r, n in enumerate(lens.tolist()):
+        last = int(table[r, (n - 1) // 16])
+        step[:, last, :, n % 16:] = math.nan
+        mid[:, last, :, n % 16:] = -math.inf
+    hurt = O.pack(codes, step, mid)
+    args = [x.cuda() for x in (table, lens, start)]
+    out = P.attention_kv4(q.cuda(), hurt.cuda(), *args, 40)
+    _check(out, None, ref, dt)
+    # token 90 of sequence 0 holds a NaN value in the second group of head 1: rows 30 and on see it
+    mid[1, int(table[0, 5]), 1, 10, 1] = math.nan
+    out = P.attention_kv4(q.cuda(), O.pack(codes, step, mid).cuda(), *args, 40).cpu()
+    bad = torch.zeros(out.shape, dtype=torch.bool)
+    bad[30:40, 4:, 64:] = True
+    assert torch.equal(out.isnan(), bad)
+    want, _, tol, _ = ref
+    d = (out.double() - want).abs() / (tol + O.half_step(dt) * (want.abs() + tol) + 1e-30)
+    assert (d[~bad & ~want.isnan()] <= 1).all()
+    # the last two blocks of sequence 0 are full of hidden tokens
+    gone = table.clone()
+    gone[0, 5], gone[0, 6] = cache.shape[0] + 7, -2
+    out, lse = P.attention_kv4(q.cuda(), cache.cuda(), gone.cuda(), *args[1:], 40,
+                               return_lse=True)
+    assert _error() == 3
+    for i in (0, 19, 39):  # row i sees tokens up to 60 + i, of them those below 80
+        n = min(61 + i, 80)
+        one = O.attend(q[i:i + 1], cache, table[:1], torch.tensor([n]).int(), None, tiles=True)
+        _check(out[i:i + 1], lse[i:i + 1], one, dt)
 
 
 @pytest.mark.parametrize("n", [5000, 20011])
@@ -530,7 +598,7 @@ def test_decode_steps_eager_and_captured(dt, g_size):
         lens = torch.tensor(prompt).int().cuda()
         turned = P.append_kv(cache, pk, pv, slots.cuda(), pos.cuda(), cos_sin, pq)
         first = P.attention_kv4(turned, cache, table, lens, start, max(prompt))
-        ref = O.attend(turned.cpu(), cache, table, lens, start)
+        ref = O.attend(turned.cpu(), cache, table, lens, start, tiles=True)
         _check(first, None, ref, dt)
         state = {"lens": lens}
         if captured:
