@@ -308,8 +308,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       e = top == 0.f ? 0 : max(kLowestExp, min(e, 100));
       const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23) *
                        (L.scale < 0.f ? -1.f : 1.f);
-      const float fr = fabsf(L.scale) * 1.4426950408889634f *
-                       __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+      // not zero: a hidden score is -inf times it
+      const float fr = fmaxf(fabsf(L.scale) * 1.4426950408889634f *
+                                 __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23),
+                             1.17549435e-38f);
       float sum[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -449,8 +451,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
             const float old = M[nt][j];
             const float m = fmaxf(fmaxf(old - E, x) + e, kLowest);
             M[nt][j] = m;
-            const float k2 = ex2(old - m);
-            l[nt][j] *= k2;
+            // in two factors: E alone may move by more than the range of one (tokens whose
+            // values are zero, then large ones), and their part of the sum has to stay
+            const float k1 = ex2(0.5f * (old - m)), k2 = k1 * k1;
+            l[nt][j] = l[nt][j] * k1 * k1;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) msum[gr][nt][j] *= k2;
 #pragma unroll
@@ -549,15 +553,17 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
           for (int o = 4; o < 32; o <<= 1) ms += __shfl_xor_sync(0xFFFFFFFFu, ms, o);
           corr[gr] = ms;
         }
-        if (g == 0) s_ml[warp][row] = make_float2(M[nt][j], ls);
+        // out of the units of this warp's E, which the others need not share
+        const float unit = __uint_as_float(static_cast<uint32_t>(127 + E) << 23);
+        if (g == 0) s_ml[warp][row] = make_float2(fmaxf(M[nt][j] - E, kLowest), ls * unit);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const float z = corr[q * NG / 4];
           float4 o4;  // channels 32 q + 4 g + 0..3
-          o4.x = acc[2 * q][nt][j] + z;
-          o4.y = acc[2 * q + 1][nt][j] + z;
-          o4.z = acc[2 * q][nt][j + 2] + z;
-          o4.w = acc[2 * q + 1][nt][j + 2] + z;
+          o4.x = (acc[2 * q][nt][j] + z) * unit;
+          o4.y = (acc[2 * q + 1][nt][j] + z) * unit;
+          o4.z = (acc[2 * q][nt][j + 2] + z) * unit;
+          o4.w = (acc[2 * q + 1][nt][j + 2] + z) * unit;
           *reinterpret_cast<float4*>(s_o + row * 128 + 32 * q + 4 * g) = o4;
         }
       }

@@ -4,17 +4,17 @@
 // tokens times the query heads of one kv head) share each key, so the keys
 // are worth turning into 16-bit tiles once, for tcgen05:
 //   S = Q K^T, O += P V, 128 x 128 x 128 fp16 products into tensor memory.
-// K and V become fp16 with one power of two for each 32 tokens, chosen from the largest
-// step and mid among them, so any scale keeps fp16's relative 2^-11; the power
-// goes into the softmax's factor (K) and into the exponent's reference (V).
+// K and V become fp16 with one power of two for each 32 tokens, chosen from
+// the largest step and mid among them, so any scale keeps fp16's relative
+// 2^-11; the power goes into the softmax's factor (K) and, where it is not the largest so
+// far, into the weights (V), O being kept in units of the largest.
 //
-// Roles of a CTA (one an SM, 13 warps):
-//   warps 0-3, 4-7   softmax of query tile 0, 1: a thread a row.  A first pass
-//                    over the row's scores in tensor memory finds their
-//                    maximum, a second writes exp as fp16 over them, the A
-//                    operand of O += P V.
+// Roles of a CTA (one an SM, 16 warps whose registers are dealt out anew):
+//   warps 0-3, 4-7   softmax of query tile 0, 1: a thread a row, which it reads
+//                    from tensor memory and writes back as fp16 exponentials
+//                    over the scores, the A operand of O += P V
 //   warps 8-11       packed rows to fp16 tiles in shared memory, a thread a token
-//   warp 12          issues the matrix instructions
+//   warp 12          issues the matrix instructions (13-15 have no work)
 // Two query tiles take turns: while one's scores go through the exponentials,
 // the other's products run.  O stays in tensor memory; it is rescaled by the
 // softmax warps when a row's maximum has grown by more than 2^kLazy, which
@@ -32,7 +32,7 @@ namespace {
 
 constexpr int kRows = 256;       // an item's query rows, two tiles
 constexpr int kTile = 128;       // tokens a step
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 16 * 32;
 constexpr int kOverTile = 2;     // an item's own cost, in steps
 constexpr int kLeastTile = 2;    // steps a CTA takes at least
 constexpr int kHalfTile = 16384; // 128 rows x 64 channels of fp16
@@ -82,6 +82,32 @@ KVS_DEV void mma_pv(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t accumulate
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
       "r"(a_tmem), "l"(b), "r"(kIdescPV), "r"(accumulate)
       : "memory");
+}
+// A load of 32 columns that is waited for later: tmem_arrived() orders the uses behind it.
+KVS_DEV void tmem_ld32_start(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(taddr));
+}
+KVS_DEV void tmem_arrived(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+  asm volatile(""
+               : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                 "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
 KVS_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -239,7 +265,9 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* k
           }
         }
         const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h2f<FP16>(top)));
-        const int e = max(static_cast<int>(most >> 23) - 127, kLowestExp) - 8;
+        // in steps of 16, so that V's powers seldom differ; K of zeros gets any
+        int e = max(static_cast<int>(most >> 23) - 127, kLowestExp);
+        e = (v == 0 && most == 0 ? 0 : (e + 3) & ~3) - 8;
         up[v] = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
         if (lane == 0) {
           if (v == 0) C->k_up[ring][seg] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
@@ -432,73 +460,104 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
           const uint32_t v = n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
           return v & ~C->gone[ring][sg];
         };
-        // ---- maximum
-        float mx = -INFINITY;
         int e_new = E;
 #pragma unroll
-        for (int sg = 0; sg < 4; ++sg) {
-          float v[32];
-          tmem_ld32(S + 32 * sg, v);
-          float part = -INFINITY;
-          if (masked) {
-            const uint32_t vis = visible(sg);
+        for (int sg = 0; sg < 4; ++sg) e_new = max(e_new, C->v_exp[ring][sg]);
+        // Against the reference that there is, the scores only pass through once; a row that
+        // has grown by more than 2^kLazy, or larger values, make the warp find the maximum,
+        // rescale and take the scores again (the first step always does).
+        uint32_t h[4][16];
+        float sum = 0.f;
+        for (bool fresh = j == 0 || e_new != E;; fresh = true) {
+          if (fresh) {
+            float mx = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (vis >> i & 1u) part = fmaxf(part, v[i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) part = fmaxf(part, v[i]);
-          }
-          mx = fmaxf(mx, part * (f * C->k_up[ring][sg]));
-          e_new = max(e_new, C->v_exp[ring][sg]);
-        }
-        if (__any_sync(0xFFFFFFFFu, mx > m + kLazy) || e_new != E) {
-          const float m_new = fmaxf(m, mx), k2 = ex2(m - m_new);
-          l *= k2;
-          if (j > 0) {
-            const float ko = k2 * ex2(static_cast<float>(E - e_new));
-#pragma unroll
-            for (int cg = 0; cg < 4; ++cg) {
+            for (int sg = 0; sg < 4; ++sg) {
               float v[32];
-              tmem_ld32(O + 32 * cg, v);
-              uint32_t a[16], b[16];
+              tmem_ld32(S + 32 * sg, v);
+              float part = -INFINITY;
+              if (masked) {
+                const uint32_t vis = visible(sg);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (vis >> i & 1u) part = fmaxf(part, v[i]);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) part = fmaxf(part, v[i]);
+              }
+              mx = fmaxf(mx, part * (f * C->k_up[ring][sg]));
+            }
+            const float m_new = fmaxf(m, mx), k2 = ex2(m - m_new);
+            l *= k2;
+            if (j > 0) {
+              const float ko = k2 * ex2(static_cast<float>(E - e_new));
+#pragma unroll
+              for (int cg = 0; cg < 4; ++cg) {
+                float v[32];
+                tmem_ld32(O + 32 * cg, v);
+                uint32_t a[16], b[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  a[i] = __float_as_uint(v[i] * ko);
+                  b[i] = __float_as_uint(v[i + 16] * ko);
+                }
+                tmem_st16(O + 32 * cg, a);
+                tmem_st16(O + 32 * cg + 16, b);
+              }
+            }
+            m = m_new;
+            E = e_new;
+          }
+          f32x2_t s2 = f2_pack(0.f, 0.f);
+          float high = -INFINITY;
+          uint32_t v[2][32];
+          tmem_ld32_start(S, v[0]);
+#pragma unroll
+          for (int sg = 0; sg < 4; ++sg) {
+            uint32_t(&w)[32] = v[sg & 1];
+            tmem_arrived(w);
+            if (sg < 3) tmem_ld32_start(S + 32 * (sg + 1), v[(sg + 1) & 1]);
+            if (masked) {
+              const uint32_t vis = visible(sg);
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!(vis >> i & 1u)) w[i] = 0xFF800000u;
+            }
+            // not zero: a hidden score is -inf times it
+            const float fs = fmaxf(f * C->k_up[ring][sg], 1.17549435e-38f);
+            const f32x2_t fs2 = f2_pack(fs, fs), ref2 = f2_pack(-m, -m);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float t0_, t1_;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])),
+                               fs2, ref2), t0_, t1_);
+              high = fmaxf(fmaxf(t0_, t1_), high);
+              const float p0 = ex2(t0_), p1 = ex2(t1_);
+              s2 = f2_add(s2, f2_pack(p0, p1));
+              h[sg][i] = half2_bits(p0, p1);
+            }
+            const int down = E - C->v_exp[ring][sg];
+            if (down != 0) {  // these tokens' V is in smaller units than O
+              const __half2 g = __float2half2_rn(ex2(static_cast<float>(-down)));
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
-                a[i] = __float_as_uint(v[i] * ko);
-                b[i] = __float_as_uint(v[i + 16] * ko);
+                const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h[sg][i]), g);
+                h[sg][i] = *reinterpret_cast<const uint32_t*>(&y);
               }
-              tmem_st16(O + 32 * cg, a);
-              tmem_st16(O + 32 * cg + 16, b);
             }
           }
-          m = m_new;
-          E = e_new;
+          float s0, s1;
+          f2_unpack(s2, s0, s1);
+          sum = s0 + s1;
+          if (fresh || !__any_sync(0xFFFFFFFFu, high > kLazy)) break;
         }
-        // ---- exponentials, to where the scores were
+        l += sum;
 #pragma unroll
-        for (int sg = 0; sg < 4; ++sg) {
-          float v[32];
-          tmem_ld32(S + 32 * sg, v);
-          const float fs = f * C->k_up[ring][sg];
-          const int ev = C->v_exp[ring][sg];
-          const float ref = m + static_cast<float>(E - ev);
-          float sum0 = 0.f, sum1 = 0.f;
-          uint32_t h[16];
-          const uint32_t vis = masked ? visible(sg) : 0xFFFFFFFFu;
+        for (int sg = 0; sg < 4; ++sg) tmem_st16(S + 16 * sg, h[sg]);
+        if (flag) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float p0 = ex2(fmaf(v[2 * i], fs, -ref)), p1 = ex2(fmaf(v[2 * i + 1], fs, -ref));
-            if (masked) {
-              p0 = vis >> (2 * i) & 1u ? p0 : 0.f;
-              p1 = vis >> (2 * i + 1) & 1u ? p1 : 0.f;
-            }
-            sum0 += p0;
-            sum1 += p1;
-            h[i] = half2_bits(p0, p1);
-          }
-          l = fmaf(sum0 + sum1, ex2(static_cast<float>(E - ev)), l);
-          tmem_st16(S + 16 * sg, h);
-          if (flag) {
+          for (int sg = 0; sg < 4; ++sg) {
+            const uint32_t vis = visible(sg);
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr)
               if (C->bad[ring][sg][gr] & vis) poison |= 1u << gr;
@@ -641,12 +700,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
     __syncthreads();
     walk.r = C->seq;
     walk.begin = C->begin;
+    // 256 x 168 + 128 x 104 + 128 x 72 = the 512 x 128 registers of the launch
     if (warp < 8) {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
       softmax_role<FP16, NG>(L, walk, group, q_tile, tmem, P, C);
     } else if (warp < 12) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
       convert_role<FP16, NG>(L, walk, group, k_tile, v_tile, C);
-    } else if (lane == 0) {
-      mma_role(L, walk, group, smem_u32(q_tile), smem_u32(k_tile), smem_u32(v_tile), tmem, C);
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+      if (warp == 12 && lane == 0)
+        mma_role(L, walk, group, smem_u32(q_tile), smem_u32(k_tile), smem_u32(v_tile), tmem, C);
     }
   }
   __syncwarp();

@@ -357,6 +357,25 @@ def test_attention_many_rows_magnitudes_and_growth():
         assert ((lse.double().cpu() - wlse).abs() <= ltol).all()
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_values_of_zero_and_tiny_scales(rows):
+    """Tokens whose values are all zero still count in the sum, next to large ones; scales
+    and keys so small that every score is the same."""
+    dt = torch.bfloat16
+    q, cache, table, lens, start = _problem([(rows, 150), (rows, rows)], 8, 2, 16, 64, dt, 44)
+    codes, step, mid = O.unpack(cache, dt)
+    big = step[1].double() * 2.0 ** 40
+    big[table[0][2:9].long()] = 0  # tokens 32 to 143 of sequence 0
+    step[1], mid[1] = big.to(dt), 0
+    cache = O.pack(codes, step, mid)
+    for scale in (0.1, 1e-37):
+        out, lse = P.attention_kv4(q.cuda(), cache.cuda(), table.cuda(), lens.cuda(),
+                                   start.cuda(), rows, scale=scale, return_lse=True)
+        torch.cuda.synchronize()
+        K.check_device_error(out.device)
+        _check(out, lse, O.attend(q, cache, table, lens, start, scale=scale, tiles=rows > 16), dt)
+
+
 def test_attention_many_rows_bad_blocks_and_numbers():
     """A block id outside the cache hides its tokens; NaN and infinities behind the length or
     behind a row's own position do not reach it, and those that it sees stay in their group."""
