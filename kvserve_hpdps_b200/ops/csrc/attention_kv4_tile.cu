@@ -3,7 +3,7 @@
 // The mathematics is attention_kv4.cu's; here 2 x 128 query rows (several
 // tokens times the query heads of one kv head) share each key, so the keys
 // are worth turning into 16-bit tiles once, for tcgen05:
-//   S = Q K^T, O += P V, 128 x 128 x 128 fp16 products into tensor memory.
+//   S = Q K^T, O += P V, fp16 products of 128 rows and 64 tokens into tensor memory.
 // K and V become fp16 with one power of two for each 32 tokens, chosen from
 // the largest step and mid among them, so any scale keeps fp16's relative
 // 2^-11; the power goes into the softmax's factor (K) and, where it is not the largest so
@@ -15,8 +15,8 @@
 //                    over the scores, the A operand of O += P V
 //   warps 8-11       packed rows to fp16 tiles in shared memory, a thread a token
 //   warp 12          issues the matrix instructions (13-15 have no work)
-// Two query tiles take turns: while one's scores go through the exponentials,
-// the other's products run.  O stays in tensor memory; it is rescaled by the
+// Scores are double buffered in tensor memory, 64 tokens at a time for each of two query
+// tiles, so the softmax warps need not wait for the products.  O stays in tensor memory; it is rescaled by the
 // softmax warps when a row's maximum has grown by more than 2^kLazy, which
 // after the first tiles is rare.  What bounds it: the exponentials (16 a
 // clock and SM: 2048 clocks for 2 x 128 x 128 scores) next to the products
@@ -39,7 +39,7 @@ constexpr int kHalfTile = 16384; // 128 rows x 64 channels of fp16
 
 struct Ctrl {
   uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_full[2], o_full[2], e_full[4];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2], e_full[4];  // [query tile][score buffer]
   uint32_t tmem;
   // What the converting warps say of a step (ring of four), by 32 tokens:
   float k_up[4][4];        // K in shared memory times this is K
@@ -54,33 +54,58 @@ struct Ctrl {
 
 constexpr int kSmem = 1024 + 6 * 2 * kHalfTile + static_cast<int>(sizeof(Ctrl));
 
-// Instruction descriptor: fp16 x fp16 -> fp32, M = N = 128; B K-major or MN-major.
-constexpr uint32_t kIdescQK = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-constexpr uint32_t kIdescPV = kIdescQK | (1u << 16);
+// Instruction descriptors: fp16 x fp16 -> fp32, M = 128; N = 64 tokens with B K-major, N = 128
+// channels with B MN-major.
+constexpr uint32_t kIdescQK = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
+constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+
+// Tensor memory: scores of query tile x in buffer b at 128 x + 64 b, O of tile x behind them.
+constexpr uint32_t kOutAt = 256;
 
 // Tile [128 rows][128 channels] in shared memory: two halves of 64 channels, rows of 128
 // bytes, 16-byte chunks swizzled by the row.  As K (rows: N, channels: K) it is K-major;
 // as V (rows: K, channels: N) it is MN-major: 64 channels a block, blocks 16 KB apart
-// (leading offset), groups of 8 tokens 1 KB apart (stride offset).
-KVS_DEV uint64_t mn_desc(uint32_t saddr) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>(kHalfTile >> 4) << 16;
-  d |= static_cast<uint64_t>(1024u >> 4) << 32;
-  d |= static_cast<uint64_t>(1u) << 46;
-  d |= static_cast<uint64_t>(2u) << 61;
-  return d;
+// (leading offset), groups of 8 tokens 1 KB apart (stride offset).  Descriptors: the lower
+// word is start address / 16 and leading offset / 16, the upper one stride offset / 16,
+// version and 128-byte swizzle; moving along the tile adds to the lower word.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+KVS_DEV uint32_t k_desc(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+KVS_DEV uint32_t mn_desc(uint32_t saddr) {
+  return (saddr >> 4) | (static_cast<uint32_t>(kHalfTile >> 4) << 16);
+}
+// The value of lane 0 in a uniform register, where the matrix instructions want their operands:
+// from there each takes one uniform addition, from a vector register four moves (measured: the
+// issuing warp was what the kernel waited for).
+KVS_DEV uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }
+KVS_DEV bool elected() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
 }
 KVS_DEV uint32_t chunk_at(int row, int chunk) {
   return (chunk >> 3) * kHalfTile + (row >> 3) * 1024 + (row & 7) * 128 +
          (((chunk & 7) ^ (row & 7)) << 4);
 }
-KVS_DEV void mma_pv(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t accumulate) {
+KVS_DEV void mma_qk(uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a_tmem), "l"(b), "r"(kIdescPV), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%1, %4};\n\tmov.b64 y, {%2, %4};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(kIdescQK), "n"(kDescHigh), "r"(accumulate)
+      : "memory");
+}
+KVS_DEV void mma_pv(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\t"
+      "mov.b64 y, {%2, %4};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a_tmem), "r"(b), "r"(kIdescPV), "n"(kDescHigh), "r"(accumulate)
       : "memory");
 }
 // A load of 32 columns that is waited for later: tmem_arrived() orders the uses behind it.
@@ -141,7 +166,8 @@ KVS_DEV TileWork tile_work(const Seq& s, int group) {
 struct Piece {
   Seq s;
   int r, h, tile, nrows;     // nrows: the sequence's query rows times heads of the group
-  int start, stop, steps;    // tokens [start, stop) in `steps` tiles
+  int start, stop;           // tokens [start, stop), in
+  int steps, halves;         // tiles and halves of 64
   bool two, whole, begins;   // second query tile in use; not shared; the item's first part
   int parts;                 // begins and not whole: CTAs that share it
 };
@@ -192,7 +218,8 @@ struct Walk {
       p.tile = lo;
       p.start = u0 * kTile;
       p.stop = min(limit, u1 * kTile);
-      p.steps = p.stop > p.start ? (p.stop - p.start + kTile - 1) / kTile : 0;
+      p.halves = p.stop > p.start ? (p.stop - p.start + 63) / 64 : 0;
+      p.steps = (p.halves + 1) / 2;
       p.two = p.nrows - lo * kRows > 128;
       p.begins = u0 == 0;
       p.whole = u0 == 0 && u1 == all;
@@ -332,57 +359,89 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* k
 }
 
 // ------------------------------------------------------ matrix instructions
+// Scores of half i + 2 are asked for right behind the output of half i, so the softmax warps
+// find the next half ready when they are through with one.  QK(i + 2) writes where PV(i) reads
+// its weights, and products of different shapes need not run in the order of issue: it waits.
 KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, uint32_t q_tile, uint32_t k_tile,
                       uint32_t v_tile, uint32_t tmem, Ctrl* C) {
-  uint32_t step_no = 0, piece_no[2] = {0, 0}, p_no[2] = {0, 0};
+  uint32_t step_no = 0, piece_no[2] = {0, 0}, half_no[2] = {0, 0};
   Piece p;
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    return mbar_wait(bar, parity, L.err, ERR_MBAR_TIMEOUT);
-  };
-  auto qk = [&](int x, uint32_t no) {
-    const uint32_t a = q_tile + x * 2 * kHalfTile, b = k_tile + (no & 1) * 2 * kHalfTile;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return KVS_WAIT(bar, parity); };
+  auto qk = [&](int x, int i) {
+    const uint32_t buf = (half_no[x] + i) & 1;
+    const uint32_t a = uniform(k_desc(q_tile + x * 2 * kHalfTile));
+    const uint32_t b = uniform(
+        k_desc(k_tile + ((step_no + (i >> 1)) & 1) * 2 * kHalfTile + (i & 1) * 8192));
+    const uint32_t d = uniform(tmem + 128 * x + 64 * buf);
+    if (elected()) {
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-      const uint32_t off = (ks >> 2) * kHalfTile + (ks & 3) * 32;
-      umma_bf16_f32(tmem + 128 * x, sw128_kmajor_desc(a + off), sw128_kmajor_desc(b + off),
-                    kIdescQK, ks > 0 ? 1u : 0u);
+      for (int ks = 0; ks < 8; ++ks) {
+        const uint32_t off = ((ks >> 2) * kHalfTile + (ks & 3) * 32) >> 4;
+        mma_qk(d, a + off, b + off, ks > 0 ? 1u : 0u);
+      }
+      umma_commit(&C->s_full[x][buf]);
     }
-    umma_commit(&C->s_full[x]);
+    __syncwarp();
   };
-  auto pv = [&](int x, uint32_t no, bool first) {
-    const uint32_t b = v_tile + (no & 1) * 2 * kHalfTile;
+  auto pv = [&](int x, int i) {
+    const uint32_t buf = (half_no[x] + i) & 1;
+    const uint32_t b = uniform(
+        mn_desc(v_tile + ((step_no + (i >> 1)) & 1) * 2 * kHalfTile + (i & 1) * 8192));
+    const uint32_t pw = uniform(tmem + 128 * x + 64 * buf);
+    const uint32_t d = uniform(tmem + kOutAt + 128 * x);
+    const uint32_t add = uniform(i > 0);
+    if (elected()) {
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks)  // 16 tokens: two groups of eight rows, 8 columns of P
-      mma_pv(tmem + 256 + 128 * x, tmem + 128 * x + 8 * ks, mn_desc(b + ks * 2048),
-             first && ks == 0 ? 0u : 1u);
+      for (int ks = 0; ks < 4; ++ks)  // 16 tokens: two groups of eight rows, 8 columns of P
+        mma_pv(d, pw + 8 * ks, b + ks * (2048 >> 4), ks > 0 ? 1u : add);
+      umma_commit(&C->pv_done[x]);
+    }
+    __syncwarp();
+  };
+  auto commit = [&](uint64_t* bar) {
+    if (elected()) umma_commit(bar);
+    __syncwarp();
   };
   while (walk.next(L, group, p)) {
     if (p.steps == 0) continue;
-    const int n = p.two ? 2 : 1;
+    const int n = p.two ? 2 : 1, H = p.halves;
+    auto k_ready = [&](int i) {  // before the first half of a step
+      const uint32_t no = step_no + (i >> 1);
+      return (i & 1) || wait(&C->k_full[no & 1], (no >> 1) & 1);
+    };
+    auto k_used = [&](int i) {  // behind the last half of a step
+      if ((i & 1) || i == H - 1) commit(&C->k_empty[(step_no + (i >> 1)) & 1]);
+    };
     for (int x = 0; x < n; ++x)
       if (!wait(&C->q_full[x], piece_no[x]++ & 1)) return;
-    if (!wait(&C->k_full[step_no & 1], (step_no >> 1) & 1)) return;
-    tc_fence_after();
-    for (int x = 0; x < n; ++x) qk(x, step_no);
-    umma_commit(&C->k_empty[step_no & 1]);
-    for (int j = 0; j < p.steps; ++j, ++step_no) {
-      const uint32_t parity = (step_no >> 1) & 1, next = step_no + 1;
+    for (int i = 0; i < 2 && i < H; ++i) {
+      if (!k_ready(i)) return;
+      tc_fence_after();
+      for (int x = 0; x < n; ++x) qk(x, i);
+      k_used(i);
+    }
+    for (int i = 0; i < H; ++i) {
+      const uint32_t no = step_no + (i >> 1);
       for (int x = 0; x < n; ++x) {
-        if (!wait(&C->p_full[x], p_no[x]++ & 1)) return;
-        if (x == 0 && !wait(&C->v_full[step_no & 1], parity)) return;
+        const uint32_t hn = half_no[x] + i;
+        if (!wait(&C->p_full[x][hn & 1], (hn >> 1) & 1)) return;
+        if (x == 0 && !(i & 1) && !wait(&C->v_full[no & 1], (no >> 1) & 1)) return;
         tc_fence_after();
-        pv(x, step_no, j == 0);
-        if (j + 1 < p.steps) {
-          if (x == 0 && !wait(&C->k_full[next & 1], (next >> 1) & 1)) return;
+        pv(x, i);
+      }
+      if (i + 2 < H) {
+        if (!k_ready(i + 2)) return;
+        for (int x = 0; x < n; ++x) {
+          if (!wait(&C->pv_done[x], (half_no[x] + i) & 1)) return;
           tc_fence_after();
-          qk(x, next);
-        } else {
-          umma_commit(&C->o_full[x]);
+          qk(x, i + 2);
         }
       }
-      umma_commit(&C->v_empty[step_no & 1]);
-      if (j + 1 < p.steps) umma_commit(&C->k_empty[next & 1]);
+      if ((i & 1) || i == H - 1) commit(&C->v_empty[no & 1]);
+      if (i + 2 < H) k_used(i + 2);
     }
+    step_no += p.steps;
+    for (int x = 0; x < n; ++x) half_no[x] += H;
   }
 }
 
@@ -392,9 +451,9 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
                           uint32_t tmem, const Parts& P, Ctrl* C) {
   const int x = threadIdx.x >> 7, row = threadIdx.x & 127;
   const uint32_t lanes = static_cast<uint32_t>((threadIdx.x >> 5) & 3) << 21;  // 32 TMEM lanes a warp
-  const uint32_t S = tmem + 128 * x + lanes, O = tmem + 256 + 128 * x + lanes;
+  const uint32_t O = tmem + kOutAt + 128 * x + lanes;
   uint8_t* const qt = q_tile + x * 2 * kHalfTile;
-  uint32_t step_no = 0, s_no = 0, o_no = 0;
+  uint32_t step_no = 0, half_no = 0;
   Piece p;
   while (walk.next(L, group, p)) {
     if (x == 1 && !p.two) {
@@ -446,60 +505,80 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
       mbar_arrive(&C->q_full[x]);
       // tokens that every row of this warp sees
       const int all_see = __reduce_min_sync(0xFFFFFFFFu, mine ? max(seen, 0) : 0x7FFFFFFF);
-      for (int j = 0; j < p.steps; ++j, ++step_no, ++s_no) {
-        const int ring = step_no & 3, t0 = p.start + j * kTile;
-        if (!KVS_WAIT(&C->e_full[ring], (step_no >> 2) & 1)) return;
-        if (!KVS_WAIT(&C->s_full[x], s_no & 1)) return;
+      for (int i = 0; i < p.halves; ++i, ++half_no) {
+        const uint32_t no = step_no + (i >> 1);
+        const int ring = no & 3, seg0 = 2 * (i & 1), t0 = p.start + 64 * i;
+        const uint32_t S = tmem + 128 * x + 64 * (half_no & 1) + lanes;
+        if (!KVS_WAIT(&C->e_full[ring], (no >> 2) & 1)) return;
+        if (!KVS_WAIT(&C->s_full[x][half_no & 1], (half_no >> 1) & 1)) return;
         tc_fence_after();
-        const uint32_t flag = C->flags[ring][0] | C->flags[ring][1] | C->flags[ring][2] |
-                              C->flags[ring][3];
-        const bool masked = t0 + kTile > min(all_see, p.stop) || flag != 0;
-        // columns of segment g that this row sees
+        const uint32_t flag = C->flags[ring][seg0] | C->flags[ring][seg0 + 1];
+        // columns of a segment of 32 that this row sees
         auto visible = [&](int sg) {
           const int n = min(seen, p.stop) - t0 - 32 * sg;
           const uint32_t v = n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
-          return v & ~C->gone[ring][sg];
+          return v & ~C->gone[ring][seg0 + sg];
         };
-        int e_new = E;
+        if (t0 + 64 > min(all_see, p.stop) || flag != 0) {  // hidden scores become -inf
+#pragma unroll 1
+          for (int sg = 0; sg < 2; ++sg) {
+            const uint32_t vis = visible(sg);
+            uint32_t v[32];
+            tmem_ld32_start(S + 32 * sg, v);
+            tmem_arrived(v);
+            uint32_t a[16], b[16];
 #pragma unroll
-        for (int sg = 0; sg < 4; ++sg) e_new = max(e_new, C->v_exp[ring][sg]);
+            for (int k = 0; k < 16; ++k) {
+              a[k] = vis >> k & 1u ? v[k] : 0xFF800000u;
+              b[k] = vis >> (k + 16) & 1u ? v[k + 16] : 0xFF800000u;
+            }
+            tmem_st16(S + 32 * sg, a);
+            tmem_st16(S + 32 * sg + 16, b);
+            if (flag) {
+#pragma unroll
+              for (int gr = 0; gr < NG; ++gr)
+                if (C->bad[ring][seg0 + sg][gr] & vis) poison |= 1u << gr;
+            }
+          }
+          tmem_st_wait();
+        }
+        const int e_new = max(E, max(C->v_exp[ring][seg0], C->v_exp[ring][seg0 + 1]));
+        // not zero: a hidden score is -inf times it
+        float fs[2];
+#pragma unroll
+        for (int sg = 0; sg < 2; ++sg)
+          fs[sg] = fmaxf(f * C->k_up[ring][seg0 + sg], 1.17549435e-38f);
         // Against the reference that there is, the scores only pass through once; a row that
         // has grown by more than 2^kLazy, or larger values, make the warp find the maximum,
-        // rescale and take the scores again (the first step always does).
-        uint32_t h[4][16];
-        float sum = 0.f;
-        for (bool fresh = j == 0 || e_new != E;; fresh = true) {
+        // rescale and take the scores again (the first half always does).
+        uint32_t h[2][16];
+        float sum;
+        for (bool fresh = i == 0 || e_new != E;; fresh = true) {
           if (fresh) {
             float mx = -INFINITY;
-#pragma unroll
-            for (int sg = 0; sg < 4; ++sg) {
-              float v[32];
+#pragma unroll 1
+            for (int sg = 0; sg < 2; ++sg) {
+              float v[32], part = -INFINITY;
               tmem_ld32(S + 32 * sg, v);
-              float part = -INFINITY;
-              if (masked) {
-                const uint32_t vis = visible(sg);
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (vis >> i & 1u) part = fmaxf(part, v[i]);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) part = fmaxf(part, v[i]);
-              }
-              mx = fmaxf(mx, part * (f * C->k_up[ring][sg]));
+              for (int k = 0; k < 32; ++k) part = fmaxf(part, v[k]);
+              mx = fmaxf(mx, part * (sg ? fs[1] : fs[0]));
             }
             const float m_new = fmaxf(m, mx), k2 = ex2(m - m_new);
             l *= k2;
-            if (j > 0) {
+            if (i > 0) {
+              if (!KVS_WAIT(&C->pv_done[x], (half_no - 1) & 1)) return;
+              tc_fence_after();
               const float ko = k2 * ex2(static_cast<float>(E - e_new));
-#pragma unroll
+#pragma unroll 1
               for (int cg = 0; cg < 4; ++cg) {
                 float v[32];
                 tmem_ld32(O + 32 * cg, v);
                 uint32_t a[16], b[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  a[i] = __float_as_uint(v[i] * ko);
-                  b[i] = __float_as_uint(v[i + 16] * ko);
+                for (int k = 0; k < 16; ++k) {
+                  a[k] = __float_as_uint(v[k] * ko);
+                  b[k] = __float_as_uint(v[k + 16] * ko);
                 }
                 tmem_st16(O + 32 * cg, a);
                 tmem_st16(O + 32 * cg + 16, b);
@@ -509,41 +588,25 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
             E = e_new;
           }
           f32x2_t s2 = f2_pack(0.f, 0.f);
+          const f32x2_t ref2 = f2_pack(-m, -m);
           float high = -INFINITY;
           uint32_t v[2][32];
           tmem_ld32_start(S, v[0]);
+          tmem_ld32_start(S + 32, v[1]);
+          tmem_arrived(v[0]);
+          tmem_arrived(v[1]);
 #pragma unroll
-          for (int sg = 0; sg < 4; ++sg) {
-            uint32_t(&w)[32] = v[sg & 1];
-            tmem_arrived(w);
-            if (sg < 3) tmem_ld32_start(S + 32 * (sg + 1), v[(sg + 1) & 1]);
-            if (masked) {
-              const uint32_t vis = visible(sg);
+          for (int sg = 0; sg < 2; ++sg) {
+            const f32x2_t fs2 = f2_pack(fs[sg], fs[sg]);
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(vis >> i & 1u)) w[i] = 0xFF800000u;
-            }
-            // not zero: a hidden score is -inf times it
-            const float fs = fmaxf(f * C->k_up[ring][sg], 1.17549435e-38f);
-            const f32x2_t fs2 = f2_pack(fs, fs), ref2 = f2_pack(-m, -m);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float t0_, t1_;
-              f2_unpack(f2_fma(f2_pack(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])),
-                               fs2, ref2), t0_, t1_);
-              high = fmaxf(fmaxf(t0_, t1_), high);
-              const float p0 = ex2(t0_), p1 = ex2(t1_);
+            for (int k = 0; k < 16; ++k) {
+              float u0, u1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(v[sg][2 * k]),
+                                       __uint_as_float(v[sg][2 * k + 1])), fs2, ref2), u0, u1);
+              high = fmaxf(fmaxf(u0, u1), high);
+              const float p0 = ex2(u0), p1 = ex2(u1);
               s2 = f2_add(s2, f2_pack(p0, p1));
-              h[sg][i] = half2_bits(p0, p1);
-            }
-            const int down = E - C->v_exp[ring][sg];
-            if (down != 0) {  // these tokens' V is in smaller units than O
-              const __half2 g = __float2half2_rn(ex2(static_cast<float>(-down)));
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h[sg][i]), g);
-                h[sg][i] = *reinterpret_cast<const uint32_t*>(&y);
-              }
+              h[sg][k] = half2_bits(p0, p1);
             }
           }
           float s0, s1;
@@ -553,21 +616,27 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         }
         l += sum;
 #pragma unroll
-        for (int sg = 0; sg < 4; ++sg) tmem_st16(S + 16 * sg, h[sg]);
-        if (flag) {
+        for (int sg = 0; sg < 2; ++sg) {
+          const int down = E - C->v_exp[ring][seg0 + sg];
+          if (down != 0) {  // these tokens' V is in smaller units than O
+            const __half2 g = __float2half2_rn(ex2(static_cast<float>(-down)));
 #pragma unroll
-          for (int sg = 0; sg < 4; ++sg) {
-            const uint32_t vis = visible(sg);
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr)
-              if (C->bad[ring][sg][gr] & vis) poison |= 1u << gr;
+            for (int k = 0; k < 16; ++k) {
+              const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h[sg][k]), g);
+              h[sg][k] = *reinterpret_cast<const uint32_t*>(&y);
+            }
           }
+          tmem_st16(S + 16 * sg, h[sg]);
         }
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&C->p_full[x]);
+        mbar_arrive(&C->p_full[x][half_no & 1]);
       }
-      if (!KVS_WAIT(&C->o_full[x], o_no++ & 1)) return;
+      step_no += p.steps;
+      // one phase after the other: a wait for the last alone could take the one before the
+      // last but one, of the same parity, for it
+      if (p.halves > 1 && !KVS_WAIT(&C->pv_done[x], half_no & 1)) return;
+      if (!KVS_WAIT(&C->pv_done[x], (half_no - 1) & 1)) return;
       tc_fence_after();
     }
     // ---- the result, or this part of it
@@ -639,9 +708,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
       mbar_init(&C->k_empty[i], 1);
       mbar_init(&C->v_full[i], 4);
       mbar_init(&C->v_empty[i], 1);
-      mbar_init(&C->s_full[i], 1);
-      mbar_init(&C->p_full[i], 128);
-      mbar_init(&C->o_full[i], 1);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&C->s_full[i][k], 1);
+        mbar_init(&C->p_full[i][k], 128);
+      }
+      mbar_init(&C->pv_done[i], 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&C->e_full[i], 4);
     fence_mbar_init();
@@ -709,7 +780,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
       convert_role<FP16, NG>(L, walk, group, k_tile, v_tile, C);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-      if (warp == 12 && lane == 0)
+      if (warp == 12)
         mma_role(L, walk, group, smem_u32(q_tile), smem_u32(k_tile), smem_u32(v_tile), tmem, C);
     }
   }
