@@ -11,12 +11,12 @@
 //
 // Roles of a CTA (one an SM, 16 warps whose registers are dealt out anew):
 //   warps 0-3, 4-7   softmax of query tile 0, 1: a thread a row, which it reads
-//                    from tensor memory and writes back as fp16 exponentials
-//                    over the scores, the A operand of O += P V
+//                    from tensor memory and writes back as fp16 exponentials,
+//                    the A operand of O += P V
 //   warps 8-11       packed rows to fp16 tiles in shared memory, a thread a token
 //   warp 12          issues the matrix instructions (13-15 have no work)
-// Scores are double buffered in tensor memory, 64 tokens at a time for each of two query
-// tiles, so the softmax warps need not wait for the products.  O stays in tensor memory; it is rescaled by the
+// The softmax warps take 64 tokens' scores at a time into registers, so that the next ones are
+// computed while they work.  O stays in tensor memory; it is rescaled by the
 // softmax warps when a row's maximum has grown by more than 2^kLazy, which
 // after the first tiles is rare.  What bounds it: the exponentials (16 a
 // clock and SM: 2048 clocks for 2 x 128 x 128 scores) next to the products
@@ -39,7 +39,7 @@ constexpr int kHalfTile = 16384; // 128 rows x 64 channels of fp16
 
 struct Ctrl {
   uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2][2], p_full[2][2], pv_done[2], e_full[4];  // [query tile][score buffer]
+  uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2][2], e_full[4];  // [tile][buffer]
   uint32_t tmem;
   // What the converting warps say of a step (ring of four), by 32 tokens:
   float k_up[4][4];        // K in shared memory times this is K
@@ -59,8 +59,9 @@ constexpr int kSmem = 1024 + 6 * 2 * kHalfTile + static_cast<int>(sizeof(Ctrl));
 constexpr uint32_t kIdescQK = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
 constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 
-// Tensor memory: scores of query tile x in buffer b at 128 x + 64 b, O of tile x behind them.
-constexpr uint32_t kOutAt = 256;
+// Tensor memory: scores of query tile x at 64 x, its weights in buffer b at 128 + 64 x + 32 b
+// (fp16 pairs), its output at 256 + 128 x.
+constexpr uint32_t kWeightsAt = 128, kOutAt = 256;
 
 // Tile [128 rows][128 channels] in shared memory: two halves of 64 channels, rows of 128
 // bytes, 16-byte chunks swizzled by the row.  As K (rows: N, channels: K) it is K-major;
@@ -233,7 +234,10 @@ struct Walk {
   }
 };
 
-#define KVS_WAIT(bar, parity) __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, L.err, ERR_MBAR_TIMEOUT))
+KVS_DEV bool wait_phase(uint64_t* bar, uint32_t parity, uint32_t* err) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, err, ERR_MBAR_TIMEOUT));
+}
+#define KVS_WAIT(bar, parity) wait_phase(bar, parity, L.err)
 
 // ---------------------------------------------------- packed rows to tiles
 template <bool FP16, int NG>
@@ -247,31 +251,52 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* k
   while (walk.next(L, group, p)) {
     const uint8_t* const head = static_cast<const uint8_t*>(L.cache) + p.h * L.head_stride;
     const int32_t* const table = L.table + p.r * L.table_stride;
-    for (int j = 0; j < p.steps; ++j, ++step_no) {
+    const Kv4Record R{NG, L.block_size};
+    // A step's row of this thread: nothing behind `stop`, nor in a block that is not there.
+    const uint8_t* rec = nullptr;
+    int off = 0;
+    bool gone = false;
+    auto locate = [&](int j) {
       const int tok = p.start + j * kTile + row;
-      uint4 code[2][4] = {};
-      uint32_t meta[2][NG] = {};
-      bool gone = false;
+      rec = nullptr;
+      gone = false;
       if (tok < p.stop) {
-        const int page = tok / L.block_size, off = tok - page * L.block_size;
+        const int page = tok / L.block_size;
+        off = tok - page * L.block_size;
         const int id = table[page];
         gone = id < 0 || id >= L.num_blocks;
-        if (gone) {
-          record_error(L.err, ERR_BOUNDS);
-        } else {
-          const uint8_t* rec = head + id * L.block_stride;
-          const Kv4Record R{NG, L.block_size};
-#pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            const uint4* src = reinterpret_cast<const uint4*>(rec + R.codes(v, off));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) code[v][i] = src[i];
-            const uint32_t* ms = reinterpret_cast<const uint32_t*>(rec + R.meta(v, off));
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr) meta[v][gr] = ms[gr];
-          }
-        }
+        if (gone) record_error(L.err, ERR_BOUNDS);
+        else rec = head + id * L.block_stride;
       }
+    };
+    uint4 code[2][4];
+    uint32_t meta[2][NG], coming[2][NG];
+    auto load_codes = [&](int v) {
+      const uint4* src = reinterpret_cast<const uint4*>(rec + R.codes(v, off));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) code[v][i] = rec ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+    };
+    auto load_meta = [&]() {
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(rec + R.meta(v, off));
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) coming[v][gr] = rec ? src[gr] : 0u;
+      }
+    };
+    if (p.steps > 0) {
+      locate(0);
+      load_meta();
+      load_codes(0);
+      load_codes(1);
+    }
+    for (int j = 0; j < p.steps; ++j, ++step_no) {
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) meta[v][gr] = coming[v][gr];
+      const uint32_t lost = __ballot_sync(0xFFFFFFFFu, gone);
+      if (j + 1 < p.steps) locate(j + 1);  // its loads go out as registers become free
       // exponent of the largest finite step or mid of the warp's 32 tokens
       float up[2];
       uint32_t bad[NG];
@@ -301,7 +326,6 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* k
           else C->v_exp[ring][seg] = e;
         }
       }
-      const uint32_t lost = __ballot_sync(0xFFFFFFFFu, gone);
       if (lane == 0) {
         uint32_t any = lost;
 #pragma unroll
@@ -350,6 +374,10 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* k
                 make_uint4(u[0], u[1], u[2], u[3]);
           }
         }
+        if (j + 1 < p.steps) {
+          if (v == 0) load_meta();
+          load_codes(v);
+        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(v ? &C->v_full[stage] : &C->k_full[stage]);
@@ -359,42 +387,41 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* k
 }
 
 // ------------------------------------------------------ matrix instructions
-// Scores of half i + 2 are asked for right behind the output of half i, so the softmax warps
-// find the next half ready when they are through with one.  QK(i + 2) writes where PV(i) reads
-// its weights, and products of different shapes need not run in the order of issue: it waits.
+// Scores of half i + 1 are asked for as soon as the softmax warps have those of half i in their
+// registers, so they find them ready when they are through; the weights have two buffers of
+// their own.
 KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, uint32_t q_tile, uint32_t k_tile,
                       uint32_t v_tile, uint32_t tmem, Ctrl* C) {
   uint32_t step_no = 0, piece_no[2] = {0, 0}, half_no[2] = {0, 0};
   Piece p;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return KVS_WAIT(bar, parity); };
+  const uint32_t qd = uniform(k_desc(q_tile)), kd = uniform(k_desc(k_tile)),
+                 vd = uniform(mn_desc(v_tile)), tm = uniform(tmem);
   auto qk = [&](int x, int i) {
-    const uint32_t buf = (half_no[x] + i) & 1;
-    const uint32_t a = uniform(k_desc(q_tile + x * 2 * kHalfTile));
-    const uint32_t b = uniform(
-        k_desc(k_tile + ((step_no + (i >> 1)) & 1) * 2 * kHalfTile + (i & 1) * 8192));
-    const uint32_t d = uniform(tmem + 128 * x + 64 * buf);
+    const uint32_t a = qd + x * (2 * kHalfTile >> 4);
+    const uint32_t b = kd + ((step_no + (i >> 1)) & 1) * (2 * kHalfTile >> 4) + (i & 1) * (8192 >> 4);
+    const uint32_t d = tm + 64 * x;
     if (elected()) {
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
         const uint32_t off = ((ks >> 2) * kHalfTile + (ks & 3) * 32) >> 4;
         mma_qk(d, a + off, b + off, ks > 0 ? 1u : 0u);
       }
-      umma_commit(&C->s_full[x][buf]);
+      umma_commit(&C->s_full[x]);
     }
     __syncwarp();
   };
   auto pv = [&](int x, int i) {
     const uint32_t buf = (half_no[x] + i) & 1;
-    const uint32_t b = uniform(
-        mn_desc(v_tile + ((step_no + (i >> 1)) & 1) * 2 * kHalfTile + (i & 1) * 8192));
-    const uint32_t pw = uniform(tmem + 128 * x + 64 * buf);
-    const uint32_t d = uniform(tmem + kOutAt + 128 * x);
-    const uint32_t add = uniform(i > 0);
+    const uint32_t b = vd + ((step_no + (i >> 1)) & 1) * (2 * kHalfTile >> 4) + (i & 1) * (8192 >> 4);
+    const uint32_t w = tm + kWeightsAt + 64 * x + 32 * buf;
+    const uint32_t d = tm + kOutAt + 128 * x;
+    const uint32_t add = i > 0;
     if (elected()) {
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)  // 16 tokens: two groups of eight rows, 8 columns of P
-        mma_pv(d, pw + 8 * ks, b + ks * (2048 >> 4), ks > 0 ? 1u : add);
-      umma_commit(&C->pv_done[x]);
+        mma_pv(d, w + 8 * ks, b + ks * (2048 >> 4), ks > 0 ? 1u : add);
+      umma_commit(&C->pv_done[x][buf]);
     }
     __syncwarp();
   };
@@ -404,7 +431,7 @@ KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, uint32_t q_til
   };
   while (walk.next(L, group, p)) {
     if (p.steps == 0) continue;
-    const int n = p.two ? 2 : 1, H = p.halves;
+    const int n = static_cast<int>(uniform(p.two ? 2u : 1u)), H = static_cast<int>(uniform(p.halves));
     auto k_ready = [&](int i) {  // before the first half of a step
       const uint32_t no = step_no + (i >> 1);
       return (i & 1) || wait(&C->k_full[no & 1], (no >> 1) & 1);
@@ -412,36 +439,46 @@ KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, uint32_t q_til
     auto k_used = [&](int i) {  // behind the last half of a step
       if ((i & 1) || i == H - 1) commit(&C->k_empty[(step_no + (i >> 1)) & 1]);
     };
-    for (int x = 0; x < n; ++x)
-      if (!wait(&C->q_full[x], piece_no[x]++ & 1)) return;
-    for (int i = 0; i < 2 && i < H; ++i) {
-      if (!k_ready(i)) return;
-      tc_fence_after();
-      for (int x = 0; x < n; ++x) qk(x, i);
-      k_used(i);
-    }
+    #pragma unroll
+    for (int x = 0; x < 2; ++x)  // unrolled: what is indexed by x stays in registers
+      if (x < n && !wait(&C->q_full[x], piece_no[x]++ & 1)) return;
+    if (!k_ready(0)) return;
+    tc_fence_after();
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      if (x < n) qk(x, 0);
+    k_used(0);
     for (int i = 0; i < H; ++i) {
       const uint32_t no = step_no + (i >> 1);
-      for (int x = 0; x < n; ++x) {
+      if (i + 1 < H) {
+        if (!k_ready(i + 1)) return;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (x >= n) break;
+          if (!wait(&C->s_free[x], (half_no[x] + i) & 1)) return;
+          tc_fence_after();
+          qk(x, i + 1);
+        }
+        k_used(i + 1);
+      }
+      if (!(i & 1) && !wait(&C->v_full[no & 1], (no >> 1) & 1)) return;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (x >= n) break;
         const uint32_t hn = half_no[x] + i;
         if (!wait(&C->p_full[x][hn & 1], (hn >> 1) & 1)) return;
-        if (x == 0 && !(i & 1) && !wait(&C->v_full[no & 1], (no >> 1) & 1)) return;
         tc_fence_after();
         pv(x, i);
       }
-      if (i + 2 < H) {
-        if (!k_ready(i + 2)) return;
-        for (int x = 0; x < n; ++x) {
-          if (!wait(&C->pv_done[x], (half_no[x] + i) & 1)) return;
-          tc_fence_after();
-          qk(x, i + 2);
-        }
-      }
       if ((i & 1) || i == H - 1) commit(&C->v_empty[no & 1]);
-      if (i + 2 < H) k_used(i + 2);
     }
+    // the last half's scores were taken, too: one phase of s_free a half
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      if (x < n && !wait(&C->s_free[x], (half_no[x] + H - 1) & 1)) return;
     step_no += p.steps;
-    for (int x = 0; x < n; ++x) half_no[x] += H;
+    half_no[0] += H;
+    if (n == 2) half_no[1] += H;
   }
 }
 
@@ -451,7 +488,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
                           uint32_t tmem, const Parts& P, Ctrl* C) {
   const int x = threadIdx.x >> 7, row = threadIdx.x & 127;
   const uint32_t lanes = static_cast<uint32_t>((threadIdx.x >> 5) & 3) << 21;  // 32 TMEM lanes a warp
-  const uint32_t O = tmem + kOutAt + 128 * x + lanes;
+  const uint32_t S = tmem + 64 * x + lanes, O = tmem + kOutAt + 128 * x + lanes;
   uint8_t* const qt = q_tile + x * 2 * kHalfTile;
   uint32_t step_no = 0, half_no = 0;
   Piece p;
@@ -502,17 +539,32 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
                        half2_bits(y[3], y[7]));
       }
       fence_proxy_async_smem();
-      mbar_arrive(&C->q_full[x]);
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&C->q_full[x]);
       // tokens that every row of this warp sees
       const int all_see = __reduce_min_sync(0xFFFFFFFFu, mine ? max(seen, 0) : 0x7FFFFFFF);
       for (int i = 0; i < p.halves; ++i, ++half_no) {
         const uint32_t no = step_no + (i >> 1);
         const int ring = no & 3, seg0 = 2 * (i & 1), t0 = p.start + 64 * i;
-        const uint32_t S = tmem + 128 * x + 64 * (half_no & 1) + lanes;
-        if (!KVS_WAIT(&C->e_full[ring], (no >> 2) & 1)) return;
-        if (!KVS_WAIT(&C->s_full[x][half_no & 1], (half_no >> 1) & 1)) return;
-        tc_fence_after();
+        const uint32_t buf = half_no & 1, W = tmem + kWeightsAt + 64 * x + 32 * buf + lanes;
+        // what the converting warps say of the tokens comes long before the scores
+        if (!(i & 1) && !KVS_WAIT(&C->e_full[ring], (no >> 2) & 1)) return;
         const uint32_t flag = C->flags[ring][seg0] | C->flags[ring][seg0 + 1];
+        const int v_exp[2] = {C->v_exp[ring][seg0], C->v_exp[ring][seg0 + 1]};
+        const int e_new = max(E, max(v_exp[0], v_exp[1]));
+        // not zero: a hidden score is -inf times it
+        const float fs[2] = {fmaxf(f * C->k_up[ring][seg0], 1.17549435e-38f),
+                             fmaxf(f * C->k_up[ring][seg0 + 1], 1.17549435e-38f)};
+        if (!KVS_WAIT(&C->s_full[x], half_no & 1)) return;
+        tc_fence_after();
+        uint32_t v[2][32];
+        tmem_ld32_start(S, v[0]);
+        tmem_ld32_start(S + 32, v[1]);
+        tmem_arrived(v[0]);
+        tmem_arrived(v[1]);
+        tc_fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&C->s_free[x]);
         // columns of a segment of 32 that this row sees
         auto visible = [&](int sg) {
           const int n = min(seen, p.stop) - t0 - 32 * sg;
@@ -520,34 +572,18 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
           return v & ~C->gone[ring][seg0 + sg];
         };
         if (t0 + 64 > min(all_see, p.stop) || flag != 0) {  // hidden scores become -inf
-#pragma unroll 1
+#pragma unroll
           for (int sg = 0; sg < 2; ++sg) {
             const uint32_t vis = visible(sg);
-            uint32_t v[32];
-            tmem_ld32_start(S + 32 * sg, v);
-            tmem_arrived(v);
-            uint32_t a[16], b[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              a[k] = vis >> k & 1u ? v[k] : 0xFF800000u;
-              b[k] = vis >> (k + 16) & 1u ? v[k + 16] : 0xFF800000u;
-            }
-            tmem_st16(S + 32 * sg, a);
-            tmem_st16(S + 32 * sg + 16, b);
+            for (int k = 0; k < 32; ++k) v[sg][k] = vis >> k & 1u ? v[sg][k] : 0xFF800000u;
             if (flag) {
 #pragma unroll
               for (int gr = 0; gr < NG; ++gr)
                 if (C->bad[ring][seg0 + sg][gr] & vis) poison |= 1u << gr;
             }
           }
-          tmem_st_wait();
         }
-        const int e_new = max(E, max(C->v_exp[ring][seg0], C->v_exp[ring][seg0 + 1]));
-        // not zero: a hidden score is -inf times it
-        float fs[2];
-#pragma unroll
-        for (int sg = 0; sg < 2; ++sg)
-          fs[sg] = fmaxf(f * C->k_up[ring][seg0 + sg], 1.17549435e-38f);
         // Against the reference that there is, the scores only pass through once; a row that
         // has grown by more than 2^kLazy, or larger values, make the warp find the maximum,
         // rescale and take the scores again (the first half always does).
@@ -555,19 +591,17 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         float sum;
         for (bool fresh = i == 0 || e_new != E;; fresh = true) {
           if (fresh) {
-            float mx = -INFINITY;
-#pragma unroll 1
-            for (int sg = 0; sg < 2; ++sg) {
-              float v[32], part = -INFINITY;
-              tmem_ld32(S + 32 * sg, v);
+            float part[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-              for (int k = 0; k < 32; ++k) part = fmaxf(part, v[k]);
-              mx = fmaxf(mx, part * (sg ? fs[1] : fs[0]));
+            for (int k = 0; k < 32; ++k) {
+              part[0] = fmaxf(part[0], __uint_as_float(v[0][k]));
+              part[1] = fmaxf(part[1], __uint_as_float(v[1][k]));
             }
+            const float mx = fmaxf(part[0] * fs[0], part[1] * fs[1]);
             const float m_new = fmaxf(m, mx), k2 = ex2(m - m_new);
             l *= k2;
             if (i > 0) {
-              if (!KVS_WAIT(&C->pv_done[x], (half_no - 1) & 1)) return;
+              if (!KVS_WAIT(&C->pv_done[x][buf ^ 1], ((half_no - 1) >> 1) & 1)) return;
               tc_fence_after();
               const float ko = k2 * ex2(static_cast<float>(E - e_new));
 #pragma unroll 1
@@ -590,11 +624,6 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
           f32x2_t s2 = f2_pack(0.f, 0.f);
           const f32x2_t ref2 = f2_pack(-m, -m);
           float high = -INFINITY;
-          uint32_t v[2][32];
-          tmem_ld32_start(S, v[0]);
-          tmem_ld32_start(S + 32, v[1]);
-          tmem_arrived(v[0]);
-          tmem_arrived(v[1]);
 #pragma unroll
           for (int sg = 0; sg < 2; ++sg) {
             const f32x2_t fs2 = f2_pack(fs[sg], fs[sg]);
@@ -615,9 +644,11 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
           if (fresh || !__any_sync(0xFFFFFFFFu, high > kLazy)) break;
         }
         l += sum;
+        // The buffer is free: the scores' barrier is committed behind the products with the
+        // weights of half i - 2, and a commit covers all that its thread has issued before.
 #pragma unroll
         for (int sg = 0; sg < 2; ++sg) {
-          const int down = E - C->v_exp[ring][seg0 + sg];
+          const int down = E - v_exp[sg];
           if (down != 0) {  // these tokens' V is in smaller units than O
             const __half2 g = __float2half2_rn(ex2(static_cast<float>(-down)));
 #pragma unroll
@@ -626,17 +657,18 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
               h[sg][k] = *reinterpret_cast<const uint32_t*>(&y);
             }
           }
-          tmem_st16(S + 16 * sg, h[sg]);
+          tmem_st16(W + 16 * sg, h[sg]);
         }
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&C->p_full[x][half_no & 1]);
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&C->p_full[x][half_no & 1]);
       }
       step_no += p.steps;
-      // one phase after the other: a wait for the last alone could take the one before the
-      // last but one, of the same parity, for it
-      if (p.halves > 1 && !KVS_WAIT(&C->pv_done[x], half_no & 1)) return;
-      if (!KVS_WAIT(&C->pv_done[x], (half_no - 1) & 1)) return;
+      for (int back = p.halves > 1 ? 2 : 1; back > 0; --back) {  // both buffers' last products
+        const uint32_t no = half_no - back;
+        if (!KVS_WAIT(&C->pv_done[x][no & 1], (no >> 1) & 1)) return;
+      }
       tc_fence_after();
     }
     // ---- the result, or this part of it
@@ -703,16 +735,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
   if (tid == 0) {
     P.desc[b] = make_int4(-1, 0, 0, 0);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&C->q_full[i], 128);
+      mbar_init(&C->q_full[i], 4);
       mbar_init(&C->k_full[i], 4);
       mbar_init(&C->k_empty[i], 1);
       mbar_init(&C->v_full[i], 4);
       mbar_init(&C->v_empty[i], 1);
+      mbar_init(&C->s_full[i], 1);
+      mbar_init(&C->s_free[i], 4);
       for (int k = 0; k < 2; ++k) {
-        mbar_init(&C->s_full[i][k], 1);
-        mbar_init(&C->p_full[i][k], 128);
+        mbar_init(&C->p_full[i][k], 4);
+        mbar_init(&C->pv_done[i][k], 1);
       }
-      mbar_init(&C->pv_done[i], 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&C->e_full[i], 4);
     fence_mbar_init();
