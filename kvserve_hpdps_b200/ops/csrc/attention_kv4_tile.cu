@@ -7,7 +7,10 @@
 // K and V become fp16 with one power of two for each 32 tokens, chosen from
 // the largest step and mid among them, so any scale keeps fp16's relative
 // 2^-11; the power goes into the softmax's factor (K) and, where it is not the largest so
-// far, into the weights (V), O being kept in units of the largest.
+// far, into the weights (V), O being kept in units of the largest.  K's tile holds
+// step (code - 8) alone, which is exact in fp16 for bf16 steps (8 bits times 3); mid times the
+// sum of the group's query elements is 16 more columns of the product: that sum in three
+// fp16 parts against mid three times, so the scores of a bf16 cache are fp32's.
 //
 // Roles of a CTA (one an SM, 16 warps whose registers are dealt out anew):
 //   warps 0-3, 4-7   softmax of query tile 0, 1: a thread a row, which it reads
@@ -52,7 +55,10 @@ struct Ctrl {
   int seq;
 };
 
-constexpr int kSmem = 1024 + 6 * 2 * kHalfTile + static_cast<int>(sizeof(Ctrl));
+// Behind the tiles: [128 rows][16] fp16, two for the queries, two for the keys' stages.
+constexpr int kMidTile = 4096;
+constexpr int kMidAt = 12 * kHalfTile, kCtrlAt = kMidAt + 4 * kMidTile;
+constexpr int kSmem = 1024 + kCtrlAt + static_cast<int>(sizeof(Ctrl));
 
 // Instruction descriptors: fp16 x fp16 -> fp32, M = 128; N = 64 tokens with B K-major, N = 128
 // channels with B MN-major.
@@ -87,17 +93,38 @@ KVS_DEV bool elected() {
       : "=r"(p));
   return p != 0;
 }
+// The 16 extra columns: no swizzle, cores of 8 rows by 16 bytes, the two of a row 128 bytes
+// apart (leading offset), groups of 8 rows 256 bytes (stride offset).
+constexpr uint32_t kMidHigh = (256u >> 4) | (1u << 14);
+KVS_DEV uint32_t mid_desc(uint32_t saddr) { return (saddr >> 4) | ((128u >> 4) << 16); }
+KVS_DEV uint32_t mid_at(int row) { return (row >> 3) * 256 + (row & 7) * 16; }
+// Column 3 g + 0..2 of the extra ones belongs to group g: `part(g, i)` packed into a row's two
+// 16-byte chunks.
+template <int NG, class F>
+KVS_DEV void store_mids(uint8_t* tile, int row, F part) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int a = 2 * i, b = 2 * i + 1;
+    const uint32_t lo = a < 3 * NG ? part(a / 3, a % 3) : 0u, hi = b < 3 * NG ? part(b / 3, b % 3) : 0u;
+    w[i] = lo | (hi << 16);
+  }
+  *reinterpret_cast<uint4*>(tile + mid_at(row)) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint4*>(tile + mid_at(row) + 128) = make_uint4(w[4], w[5], w[6], w[7]);
+}
+constexpr float kMidUp = 128.f;  // mids times this, query sums by it: both inside fp16's range
 KVS_DEV uint32_t chunk_at(int row, int chunk) {
   return (chunk >> 3) * kHalfTile + (row >> 3) * 1024 + (row & 7) * 128 +
          (((chunk & 7) ^ (row & 7)) << 4);
 }
+template <uint32_t HIGH>
 KVS_DEV void mma_qk(uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
       "mov.b64 x, {%1, %4};\n\tmov.b64 y, {%2, %4};\n\t"
       "setp.ne.b32 p, %5, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "r"(b), "r"(kIdescQK), "n"(kDescHigh), "r"(accumulate)
+      "r"(a), "r"(b), "r"(kIdescQK), "n"(HIGH), "r"(accumulate)
       : "memory");
 }
 KVS_DEV void mma_pv(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t accumulate) {
@@ -241,8 +268,8 @@ KVS_DEV bool wait_phase(uint64_t* bar, uint32_t parity, uint32_t* err) {
 
 // ---------------------------------------------------- packed rows to tiles
 template <bool FP16, int NG>
-KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* k_tile,
-                          uint8_t* v_tile, Ctrl* C) {
+KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q_tile,
+                          uint8_t* k_tile, uint8_t* v_tile, Ctrl* C) {
   const int lane = threadIdx.x & 31, seg = (threadIdx.x >> 5) & 3, row = seg * 32 + lane;
   constexpr uint32_t kInf = FP16 ? 0x7C00u : 0x7F80u;
   constexpr uint32_t k1024 = 0x64006400u;
@@ -319,7 +346,7 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* k
         const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h2f<FP16>(top)));
         // in steps of 16, so that V's powers seldom differ; K of zeros gets any
         int e = max(static_cast<int>(most >> 23) - 127, kLowestExp);
-        e = (v == 0 && most == 0 ? 0 : (e + 3) & ~3) - 8;
+        e = (v == 0 && most == 0 ? 0 : (e + 3) & ~3) - 7;
         up[v] = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
         if (lane == 0) {
           if (v == 0) C->k_up[ring][seg] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
@@ -367,13 +394,18 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* k
             codes4(x, k1024, u);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&u[i]), step, mid);
+              const __half2 code2 = *reinterpret_cast<const __half2*>(&u[i]);
+              const __half2 y = v == 0 ? __hmul2(code2, step) : __hfma2(code2, step, mid);
               u[i] = *reinterpret_cast<const uint32_t*>(&y);
             }
             *reinterpret_cast<uint4*>(dst + chunk_at(row, 4 * q + c)) =
                 make_uint4(u[0], u[1], u[2], u[3]);
           }
         }
+        if (v == 0)
+          store_mids<NG>(q_tile + kMidAt + (2 + stage) * kMidTile, row, [&](int gr, int) {
+            return f2h<true>(h2f<FP16>(meta[0][gr] >> 16) * (up[0] * kMidUp));
+          });
         if (j + 1 < p.steps) {
           if (v == 0) load_meta();
           load_codes(v);
@@ -396,17 +428,22 @@ KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, uint32_t q_til
   Piece p;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return KVS_WAIT(bar, parity); };
   const uint32_t qd = uniform(k_desc(q_tile)), kd = uniform(k_desc(k_tile)),
-                 vd = uniform(mn_desc(v_tile)), tm = uniform(tmem);
+                 vd = uniform(mn_desc(v_tile)), tm = uniform(tmem),
+                 qm = uniform(mid_desc(q_tile + kMidAt)),
+                 km = uniform(mid_desc(q_tile + kMidAt + 2 * kMidTile));
   auto qk = [&](int x, int i) {
     const uint32_t a = qd + x * (2 * kHalfTile >> 4);
     const uint32_t b = kd + ((step_no + (i >> 1)) & 1) * (2 * kHalfTile >> 4) + (i & 1) * (8192 >> 4);
+    const uint32_t am = qm + x * (kMidTile >> 4);
+    const uint32_t bm = km + ((step_no + (i >> 1)) & 1) * (kMidTile >> 4) + (i & 1) * (2048 >> 4);
     const uint32_t d = tm + 64 * x;
     if (elected()) {
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
         const uint32_t off = ((ks >> 2) * kHalfTile + (ks & 3) * 32) >> 4;
-        mma_qk(d, a + off, b + off, ks > 0 ? 1u : 0u);
+        mma_qk<kDescHigh>(d, a + off, b + off, ks > 0 ? 1u : 0u);
       }
+      mma_qk<kMidHigh>(d, am, bm, 1u);
       umma_commit(&C->s_full[x]);
     }
     __syncwarp();
@@ -528,16 +565,31 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
                        (L.scale < 0.f ? -1.f : 1.f);
       f = fabsf(L.scale) * 1.4426950408889634f *
           __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+      float sums[NG];
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) sums[gr] = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float y[8];
         unpack8<FP16>(raw[i], y);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] *= up;
+        for (int k = 0; k < 8; ++k) {
+          y[k] *= up;
+          sums[i * NG / 16] += y[k];
+        }
         *reinterpret_cast<uint4*>(qt + chunk_at(row, i)) =
             make_uint4(half2_bits(y[0], y[4]), half2_bits(y[1], y[5]), half2_bits(y[2], y[6]),
                        half2_bits(y[3], y[7]));
       }
+      store_mids<NG>(q_tile + kMidAt + x * kMidTile, row, [&](int gr, int i) {
+        float rest = sums[gr] * (1.f / kMidUp);
+        uint32_t part = f2h<true>(rest);
+        for (; i > 0; --i) {  // what the parts before leave over
+          rest -= h2f<true>(part);
+          part = f2h<true>(rest);
+        }
+        return part;
+      });
       fence_proxy_async_smem();
       __syncwarp();
       if ((threadIdx.x & 31) == 0) mbar_arrive(&C->q_full[x]);
@@ -727,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
       (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t *const q_tile = smem, *const k_tile = smem + 4 * kHalfTile,
                  *const v_tile = smem + 8 * kHalfTile;
-  Ctrl* const C = reinterpret_cast<Ctrl*>(smem + 12 * kHalfTile);
+  Ctrl* const C = reinterpret_cast<Ctrl*>(smem + kCtrlAt);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = L.q_heads / L.heads, B = gridDim.x, b = blockIdx.x;
   const Parts P = parts(L.scratch, B, kRows);
@@ -810,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
       softmax_role<FP16, NG>(L, walk, group, q_tile, tmem, P, C);
     } else if (warp < 12) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-      convert_role<FP16, NG>(L, walk, group, k_tile, v_tile, C);
+      convert_role<FP16, NG>(L, walk, group, q_tile, k_tile, v_tile, C);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
       if (warp == 12)
