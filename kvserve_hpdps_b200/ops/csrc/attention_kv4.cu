@@ -640,10 +640,19 @@ Grid grid_of(const Attn4Launch* L) {
   return g;
 }
 
-// More rows a kv head than this go to attention_kv4_tile.cu.
-constexpr int kManyRows = 64;
+// Whether a call goes to attention_kv4_tile.cu: many rows a kv head, and enough of them.
+// Measured, us here / there, bf16, groups of 64: 16 sequences of 2000 tokens, 8 heads: 96
+// rows 93 / 107, 128 rows 117 / 108; 8 of 8000, 4 heads: 84 rows 84 / 78, 448 rows 333 / 148.
+// With little to do the first tiles decide: one of 1024 tokens, 4 heads: 448 rows (1.8 Mi rows
+// times tokens times heads) 21 / 33, 896 rows (3.5 Mi) 31 / 37, 1792 rows (7 Mi) 43 / 39; one of
+// 512 tokens, 8 heads: 2048 rows (8 Mi) 61 / 37.
+constexpr int kManyRows = 96;
+constexpr long long kMuchWork = 5ll << 20;
 bool many_rows(const Attn4Launch* L) {
-  return static_cast<long long>(L->max_q) * (L->q_heads / L->heads) > kManyRows;
+  const long long rows = static_cast<long long>(L->max_q) * (L->q_heads / L->heads);
+  const double work = static_cast<double>(rows) * L->seqs * L->heads * L->table_cols *
+                      L->block_size;
+  return rows > kManyRows && work > static_cast<double>(kMuchWork);
 }
 
 template <bool FP16, int NG, int NT>
@@ -653,7 +662,7 @@ cudaError_t launch(const Attn4Launch& L, const Grid& g, cudaStream_t s) {
   k_attn4<FP16, NG, NT><<<g.ctas, kWarps * 32, smem, s>>>(L);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || !g.split) return e;
-  return launch_combine<FP16, NT>(L, g.ctas, s);
+  return launch_combine<FP16, NT, 4>(L, g.ctas, s);
 }
 
 template <bool FP16, int NG>

@@ -87,12 +87,14 @@ KVS_DEV Parts parts(void* scratch, int B, int rows) {
 }
 
 // Joins the parts of the item that begins in CTA blockIdx.x and goes on in
-// the next ones: eight rows a CTA, four warps a row, each every fourth part.
-template <bool FP16, int NT>
-__global__ void __launch_bounds__(1024) k_attn4_combine(const __grid_constant__ Attn4Launch L) {
+// the next ones: eight rows a CTA, WARPS warps a row, each every WARPS-th part.  Few rows an
+// item come with many parts (one long sequence on all SMs): four warps.  Tiles of 256 rows
+// come with few, but a CTA for eight rows of each: small ones, most of which have nothing to do.
+template <bool FP16, int NT, int WARPS>
+__global__ void __launch_bounds__(256 * WARPS) k_attn4_combine(const __grid_constant__ Attn4Launch L) {
   constexpr int ROWS = 8 * NT;
-  __shared__ float s_m[4][8], s_l[4][8];
-  __shared__ float4 s_acc[4][8][32];
+  __shared__ float s_m[WARPS][8], s_l[WARPS][8];
+  __shared__ float4 s_acc[WARPS][8][32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int B = gridDim.x, b = blockIdx.x;
   const Parts P = parts(L.scratch, B, ROWS);
@@ -105,12 +107,12 @@ __global__ void __launch_bounds__(1024) k_attn4_combine(const __grid_constant__ 
   auto slot = [&](int i) { return (i == 0 ? 2 * b + 1 : 2 * (b + i)) * ROWS + row; };
   float m = kLowest, ls = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = quarter; i0 < np; i0 += 16) {  // four parts at a time, their loads together
+  for (int i0 = quarter; i0 < np; i0 += 4 * WARPS) {  // four parts at a time, their loads together
     float2 ml[4];
     float4 x[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int i = i0 + 4 * u;
+      const int i = i0 + WARPS * u;
       ml[u] = make_float2(kLowest, 0.f);
       x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i < np) {
@@ -146,11 +148,13 @@ __global__ void __launch_bounds__(1024) k_attn4_combine(const __grid_constant__ 
   const Seq s = sequence(L, d.x, false);
   const int rr = d.z * ROWS + row;
   if (rr >= s.n * group) return;  // rows behind the tile's last were not written either
-  m = fmaxf(fmaxf(s_m[0][r8], s_m[1][r8]), fmaxf(s_m[2][r8], s_m[3][r8]));
+  m = kLowest;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) m = fmaxf(m, s_m[w][r8]);
   ls = 0.f;
   a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     const float k2 = ex2(s_m[w][r8] - m);
     const float4 x = s_acc[w][r8][lane];
     ls = fmaf(s_l[w][r8], k2, ls);
@@ -169,18 +173,18 @@ __global__ void __launch_bounds__(1024) k_attn4_combine(const __grid_constant__ 
 }
 
 // Launches the join behind the attention kernel, allowed to start while that ends.
-template <bool FP16, int NT>
+template <bool FP16, int NT, int WARPS>
 cudaError_t launch_combine(const Attn4Launch& L, int ctas, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas, NT);
-  cfg.blockDim = dim3(1024);
+  cfg.blockDim = dim3(256 * WARPS);
   cfg.stream = s;
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_attn4_combine<FP16, NT>, L);
+  return cudaLaunchKernelEx(&cfg, k_attn4_combine<FP16, NT, WARPS>, L);
 }
 
 }  // namespace

@@ -893,7 +893,7 @@ cudaError_t launch(const Attn4Launch& L, cudaStream_t s) {
   const int ctas = tile_ctas(L);
   k_attn4_tile<FP16, NG><<<ctas, kThreads, kSmem, s>>>(L);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  return launch_combine<FP16, kRows / 8>(L, ctas, s);
+  return launch_combine<FP16, kRows / 8, 1>(L, ctas, s);
 }
 
 }  // namespace

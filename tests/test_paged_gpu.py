@@ -291,9 +291,16 @@ def _problem(seqs, hq, h, bs, g_size, dt, seed, spare_rows=0, cols_more=2, sprea
     return q, cache, table, lens, start
 
 
-def _tiles(seqs, hq, h):
-    """Whether a call takes the kernel for many rows: over 64 rows a kv head."""
-    return max(n for n, _ in seqs) * (hq // h) > 64
+def _tiles(table, rows, hq, h, bs):
+    """Whether a call takes the kernel for many rows, going by what the host knows: rows a kv
+    head, and rows times tokens that the table has room for."""
+    rows *= hq // h
+    return rows > 96 and rows * h * table.numel() * bs > 5 << 20
+
+
+def _wide(rows, seqs, hq, h, bs=16):
+    """Table columns that take a call of few tokens there all the same."""
+    return (6 << 20) // (rows * (hq // h) * h * seqs * bs) + 1
 
 
 @pytest.mark.parametrize("dt", DTYPES)
@@ -320,15 +327,23 @@ def test_attention_one_token(dt, g_size, hq, h, bs):
     (16, 2, [(300, 300), (5, 1000), (64, 64)]),
     (4, 4, [(65, 1111), (1, 1), (257, 256)]),
 ])
-def test_attention_several_rows(dt, g_size, hq, h, seqs):
-    q, cache, table, lens, start = _problem(seqs, hq, h, 16, g_size, dt, hq * 7, spare_rows=3)
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_several_rows(dt, g_size, hq, h, seqs, wide):
+    most = max(n for n, _ in seqs)
+    if wide and most * (hq // h) <= 96:
+        pytest.skip("too few rows for the other kernel")
+    q, cache, table, lens, start = _problem(
+        seqs, hq, h, 16, g_size, dt, hq * 7, spare_rows=3,
+        cols_more=_wide(most, len(seqs), hq, h) if wide else 2)
+    tiles = _tiles(table, most, hq, h, 16)
+    assert tiles or not wide
     out = torch.full_like(q, 9.0).cuda()
     got, lse = P.attention_kv4(q.cuda(), cache.cuda(), table.cuda(), lens.cuda(), start.cuda(),
                                max(n for n, _ in seqs), out=out, return_lse=True)
     torch.cuda.synchronize()
     assert got is out
     K.check_device_error(out.device)
-    ref = O.attend(q, cache, table, lens, start, tiles=_tiles(seqs, hq, h))
+    ref = O.attend(q, cache, table, lens, start, tiles=tiles)
     _check(out, lse, ref, dt)
     assert (out[int(start[-1]):] == 9.0).all()  # rows of no sequence
 
@@ -336,7 +351,9 @@ def test_attention_several_rows(dt, g_size, hq, h, seqs):
 def test_attention_many_rows_magnitudes_and_growth():
     """Values far from 1, steps and scores that rise along the sequence, a negative scale."""
     for dt, mag in ((torch.bfloat16, 1e-18), (torch.bfloat16, 1e6), (torch.float16, 1.0)):
-        q, cache, table, lens, start = _problem([(90, 700), (20, 20)], 4, 2, 16, 64, dt, 31)
+        q, cache, table, lens, start = _problem([(90, 700), (20, 20)], 4, 2, 16, 64, dt, 31,
+                                                cols_more=_wide(90, 2, 4, 2))
+        assert _tiles(table, 90, 4, 2, 16)
         codes, step, mid = O.unpack(cache, dt)
         grow = torch.zeros(cache.shape[0])
         used = table[0][:44].long()
@@ -362,7 +379,9 @@ def test_attention_values_of_zero_and_tiny_scales(rows):
     """Tokens whose values are all zero still count in the sum, next to large ones; scales
     and keys so small that every score is the same."""
     dt = torch.bfloat16
-    q, cache, table, lens, start = _problem([(rows, 150), (rows, rows)], 8, 2, 16, 64, dt, 44)
+    q, cache, table, lens, start = _problem([(rows, 150), (rows, rows)], 8, 2, 16, 64, dt, 44,
+                                            cols_more=_wide(40, 2, 8, 2))
+    assert _tiles(table, rows, 8, 2, 16) == (rows == 40)
     codes, step, mid = O.unpack(cache, dt)
     big = step[1].double() * 2.0 ** 40
     big[table[0][2:9].long()] = 0  # tokens 32 to 143 of sequence 0
@@ -380,7 +399,9 @@ def test_attention_many_rows_bad_blocks_and_numbers():
     """A block id outside the cache hides its tokens; NaN and infinities behind the length or
     behind a row's own position do not reach it, and those that it sees stay in their group."""
     dt, h, hq = torch.bfloat16, 2, 8
-    q, cache, table, lens, start = _problem([(40, 100), (30, 77)], hq, h, 16, 64, dt, 12)
+    q, cache, table, lens, start = _problem([(40, 100), (30, 77)], hq, h, 16, 64, dt, 12,
+                                            cols_more=_wide(40, 2, hq, h))
+    assert _tiles(table, 40, hq, h, 16)
     ref = O.attend(q, cache, table, lens, start, tiles=True)
     codes, step, mid = O.unpack(cache, dt)
     for r, n in enumerate(lens.tolist()):
@@ -617,7 +638,7 @@ def test_decode_steps_eager_and_captured(dt, g_size):
         lens = torch.tensor(prompt).int().cuda()
         turned = P.append_kv(cache, pk, pv, slots.cuda(), pos.cuda(), cos_sin, pq)
         first = P.attention_kv4(turned, cache, table, lens, start, max(prompt))
-        ref = O.attend(turned.cpu(), cache, table, lens, start, tiles=True)
+        ref = O.attend(turned.cpu(), cache, table, lens, start)
         _check(first, None, ref, dt)
         state = {"lens": lens}
         if captured:
@@ -684,11 +705,19 @@ def test_results_do_not_change_from_call_to_call():
     q, cache, table, lens, start = _problem([(9, 1500), (2, 800), (1, 5)], 12, 3, 16, 32,
                                             torch.float16, 2)
     a = [x.cuda() for x in (q, cache, table, lens, start)]
-    first = P.attention_kv4(*a, 9)
+    _same_again(a, 9)
+    q, cache, table, lens, start = _problem([(200, 900), (77, 300)], 8, 2, 16, 64,
+                                            torch.bfloat16, 6, cols_more=_wide(200, 2, 8, 2))
+    assert _tiles(table, 200, 8, 2, 16)
+    _same_again([x.cuda() for x in (q, cache, table, lens, start)], 200)
+
+
+def _same_again(a, most):
+    first = P.attention_kv4(*a, most)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     for i in range(5):
         with torch.cuda.stream(side if i % 2 else torch.cuda.current_stream()):
-            again = P.attention_kv4(*a, 9)
+            again = P.attention_kv4(*a, most)
         torch.cuda.synchronize()
         assert torch.equal(first, again)
