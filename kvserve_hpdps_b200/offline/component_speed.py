@@ -23,6 +23,14 @@ reference quantizer formula per (head, channel) for keys and per token for
 values (quantize / dequantize).  CUDA figures are event times; CPU figures
 are wall time.
 
+``--serving`` times the operators of a serving step on one layer's paged cache
+(``ops/paged.py``): ``append`` (rotated keys and values into a bf16 cache, the
+queries rotated too), ``append4`` (into a 4-bit cache), ``read4`` (its rows back
+as bf16), ``attn4_decode`` (one query token of each of ``--requests`` sequences
+over its ``--tokens`` cached ones) and ``attn4_chunk`` (the last ``--chunk``
+tokens of one sequence).  Their rates are GB/s of the bf16 KV that the stage
+writes, reads or attends over.
+
 Every fused-stage figure is CUDA-event time on the launching stream after warm-up,
 averaged over ``--iters`` launches; the input of a full request (28 layers,
 8K tokens, 4 heads: 470 MB) is larger than L2, so no flush is needed at
@@ -33,6 +41,7 @@ Usage::
   python -m kvserve_hpdps_b200.offline.component_speed --layers 28 --tokens 8192
   python -m kvserve_hpdps_b200.offline.component_speed --only quant --layers 2 --iters 3
   python -m kvserve_hpdps_b200.offline.component_speed --methods kivi,cachegen --tokens 4096
+  python -m kvserve_hpdps_b200.offline.component_speed --serving --requests 32 --group-size 64
 """
 
 from __future__ import annotations
@@ -46,6 +55,7 @@ import torch
 STAGES = ("quant", "dequant", "rans_enc", "rans_dec", "lc_enc", "lc_dec", "block_copy")
 PEER_STAGES = ("quant_peer", "rans_enc_peer")
 METHODS = ("custom", "kivi", "cachegen", "hadamard", "minmax")
+SERVING = ("append", "append4", "read4", "attn4_decode", "attn4_chunk")
 
 
 def _timeit(fn, iters: int, warmup: int = 3) -> float:
@@ -265,6 +275,62 @@ def run(layers: int = 28, tokens: int = 8192, heads: int = 4, iters: int = 10,
     return rows
 
 
+def run_serving(tokens: int = 8192, heads: int = 4, q_heads: int = 28, requests: int = 32,
+                chunk: int = 1024, group_size: int = 64, block_size: int = 16, iters: int = 10,
+                warmup: int = 3, seed: int = 1, theta: float = 1e6) -> list[dict]:
+    """Stage timings of :mod:`kvserve_hpdps_b200.ops.paged` on one layer of bf16 KV with
+    outlier key channels, requests of ``tokens`` each at shuffled blocks."""
+    from kvserve_hpdps_b200.ops import paged as P
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    per = (tokens + block_size - 1) // block_size
+    nb = requests * per
+    table = torch.randperm(nb, generator=g, device="cuda").view(requests, per).int()
+    place = torch.arange(tokens, device="cuda")
+    freq = 1.0 / theta ** (torch.arange(0, 128, 2, device="cuda", dtype=torch.float64) / 128)
+    angle = place.double()[:, None] * freq
+    cos_sin = torch.cat([angle.cos(), angle.sin()], 1).float()
+    cache = torch.zeros((2, nb, block_size, heads, 128), dtype=torch.bfloat16, device="cuda")
+    cache4 = P.kv4_cache(nb, heads, block_size, group_size)
+
+    def rows(n, h):
+        return torch.randn((n, h, 128), generator=g, device="cuda").bfloat16()
+
+    k, v, q = rows(tokens, heads), rows(tokens, heads), rows(tokens, q_heads)
+    k[..., :4] *= 12.0
+    for r in range(requests):  # every request holds the same tokens at its own blocks
+        slots = table[r].long()[place // block_size] * block_size + place % block_size
+        P.append_kv(cache4, k, v, slots, place, cos_sin)
+    lens = torch.full((requests,), tokens, dtype=torch.int32, device="cuda")
+    qd = rows(requests, q_heads)
+    chunk = min(chunk, tokens)
+    start = torch.tensor([0, chunk], dtype=torch.int32, device="cuda")
+    stages = {
+        "append": (lambda: P.append_kv(cache, k, v, slots, place, cos_sin, q), 1),
+        "append4": (lambda: P.append_kv(cache4, k, v, slots, place, cos_sin, q), 1),
+        "read4": (lambda: P.read_kv4(cache4, slots, torch.bfloat16), 1),
+        "attn4_decode": (lambda: P.attention_kv4(qd, cache4, table, lens), requests),
+        "attn4_chunk": (lambda: P.attention_kv4(q[-chunk:], cache4, table[:1], lens[:1], start,
+                                                chunk), 1),
+    }
+    out = []
+    for stage in SERVING:
+        fn, n = stages[stage]
+        ms = _timeit(fn, iters, warmup)
+        out.append({"stage": stage, "ms": round(ms, 5),
+                    "gbps": round(n * tokens * heads * 512 / ms / 1e6, 1), "tokens": tokens,
+                    "heads": heads, "q_heads": q_heads, "requests": n, "group_size": group_size})
+        if stage == "attn4_chunk":
+            out[-1]["chunk"] = chunk
+    from kvserve_hpdps_b200.ops import kernels as K
+    back = P.read_kv4(cache4, slots, torch.bfloat16)
+    err = K.kv_error(torch.stack([cache.flatten(1, 2)[p][slots] for p in range(2)]), back)
+    out.append({"stage": "summary", "bytes_per_token_head": P.kv4_row_bytes(group_size),
+                "compression_ratio": round(512 / P.kv4_row_bytes(group_size), 3),
+                "rel_mse": err["rel_mse"], "cosine": err["cosine"],
+                "device_error": K.read_device_error(cache.device)})
+    return out
+
+
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(description="component speed of the compression kernels")
     ap.add_argument("--layers", type=int, default=28)
@@ -283,6 +349,12 @@ def main(argv=None) -> int:
     ap.add_argument("--device", default=None, help="--methods device (default: cuda if present)")
     ap.add_argument("--peer", type=int, default=None,
                     help="second GPU for the direct-path stages (--only quant_peer,rans_enc_peer)")
+    ap.add_argument("--serving", action="store_true",
+                    help=f"time a serving step's operators instead: {','.join(SERVING)}")
+    ap.add_argument("--requests", type=int, default=32, help="--serving: sequences of a decode step")
+    ap.add_argument("--chunk", type=int, default=1024, help="--serving: query tokens of a chunk")
+    ap.add_argument("--q-heads", type=int, default=28, help="--serving: query heads")
+    ap.add_argument("--group-size", type=int, default=64, help="--serving: channels a group")
     args = ap.parse_args(argv)
     if args.methods:
         for r in run_methods(tuple(args.methods.split(",")), args.layers, args.tokens, args.heads,
@@ -291,6 +363,11 @@ def main(argv=None) -> int:
         return 0
     if not torch.cuda.is_available():
         print(json.dumps({"unavailable": "no CUDA device"}))
+        return 0
+    if args.serving:
+        for r in run_serving(args.tokens, args.heads, args.q_heads, args.requests, args.chunk,
+                             args.group_size, iters=args.iters, warmup=args.warmup):
+            print(json.dumps(r))
         return 0
     for r in run(args.layers, args.tokens, args.heads, args.iters,
                  tuple(args.only.split(",")), args.engine, warmup=args.warmup,

@@ -701,6 +701,14 @@ def test_two_graphs_at_once():
         assert torch.equal(o, w)
 
 
+def test_component_speed_times_the_serving_operators():
+    from kvserve_hpdps_b200.offline import component_speed as CS
+    rows = CS.run_serving(tokens=300, heads=2, q_heads=8, requests=3, chunk=40, iters=2, warmup=1)
+    assert [r["stage"] for r in rows] == [*CS.SERVING, "summary"]
+    assert all(r["ms"] > 0 for r in rows[:-1])
+    assert rows[-1]["device_error"] == 0 and rows[-1]["cosine"] > 0.98
+
+
 def test_results_do_not_change_from_call_to_call():
     q, cache, table, lens, start = _problem([(9, 1500), (2, 800), (1, 5)], 12, 3, 16, 32,
                                             torch.float16, 2)
