@@ -439,7 +439,20 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
           move |= top[nt][j] - M[nt][j] > kLazy - E;
         }
       if (__any_sync(0xFFFFFFFFu, move)) {
-        const uint32_t all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
+        // the largest that is finite: an infinite step or mid makes its own channels NaN and
+        // must not put the other channels' weights out of range
+        constexpr uint32_t kInf = FP16 ? 0x7C00u : 0x7F80u;
+        uint32_t fine = 0;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+          for (int r2 = 0; r2 < 2; ++r2)
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+              const uint32_t a = vm[hf][r2][gr] & 0x7FFFu, z = vm[hf][r2][gr] >> 16 & 0x7FFFu;
+              fine = max(fine, max(a < kInf ? a : 0u, z < kInf ? z : 0u));
+            }
+        const uint32_t all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h2f<FP16>(fine)));
         const int e = min(max(static_cast<int>(all >> 23) - 127, E), 100);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)

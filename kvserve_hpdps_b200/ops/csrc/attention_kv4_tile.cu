@@ -673,9 +673,15 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
             m = m_new;
             E = e_new;
           }
-          f32x2_t s2 = f2_pack(0.f, 0.f);
+          // four sums and maxima: one of each would be a chain as long as the row
+          f32x2_t s2[4];
+          float top[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            s2[k] = f2_pack(0.f, 0.f);
+            top[k] = -INFINITY;
+          }
           const f32x2_t ref2 = f2_pack(-m, -m);
-          float high = -INFINITY;
 #pragma unroll
           for (int sg = 0; sg < 2; ++sg) {
             const f32x2_t fs2 = f2_pack(fs[sg], fs[sg]);
@@ -684,15 +690,16 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
               float u0, u1;
               f2_unpack(f2_fma(f2_pack(__uint_as_float(v[sg][2 * k]),
                                        __uint_as_float(v[sg][2 * k + 1])), fs2, ref2), u0, u1);
-              high = fmaxf(fmaxf(u0, u1), high);
+              top[k & 3] = fmaxf(fmaxf(u0, u1), top[k & 3]);
               const float p0 = ex2(u0), p1 = ex2(u1);
-              s2 = f2_add(s2, f2_pack(p0, p1));
+              s2[k & 3] = f2_add(s2[k & 3], f2_pack(p0, p1));
               h[sg][k] = half2_bits(p0, p1);
             }
           }
           float s0, s1;
-          f2_unpack(s2, s0, s1);
+          f2_unpack(f2_add(f2_add(s2[0], s2[1]), f2_add(s2[2], s2[3])), s0, s1);
           sum = s0 + s1;
+          const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
           if (fresh || !__any_sync(0xFFFFFFFFu, high > kLazy)) break;
         }
         l += sum;

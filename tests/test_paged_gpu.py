@@ -93,6 +93,29 @@ def test_append_16bit(dt, form, tokens, hq, h, rd, inter):
     assert torch.equal(planes, old)
 
 
+def test_append_any_block_size_and_many_slots():
+    """16-bit caches have no rule for the block size; enough tokens for four rows a group."""
+    g = _gen(8)
+    for bs, h, hq in ((7, 3, 5), (1, 2, 2), (24, 8, 32)):
+        T = 3000
+        nb = T // bs + 3
+        cache = _layer(nb, bs, h, torch.float16, "nhd", g)
+        k, v = (torch.randn((T, h, 128), generator=g).half().cuda() for _ in range(2))
+        q = torch.randn((T, hq, 128), generator=g).half().cuda()
+        slots = torch.randperm(nb * bs, generator=g)[:T]
+        pos = torch.randint(0, 99, (T,), generator=g)
+        for rd, inter in ((128, False), (48, False), (128, True)):
+            table = _table(99, rd)
+            out = P.append_kv(cache, k, v, slots.cuda(), pos.cuda(), table, q, interleaved=inter)
+            for got, x in ((out, q), (cache[0].flatten(0, 1)[slots.cuda()], k)):
+                ref, mag = O.rotate(x, table, pos, inter)
+                bound = O.half_step(torch.float16) * ref.abs() * (1 + 2 ** -20) + \
+                    2 ** -23 * mag + 2 ** -24
+                assert ((got.double().cpu() - ref).abs() <= bound).all()
+            assert torch.equal(cache[1].flatten(0, 1)[slots.cuda()], v)
+    K.check_device_error(cache.device)
+
+
 def test_append_plain_padded_and_in_place():
     g = _gen(3)
     cache = _layer(9, 16, 2, torch.bfloat16, "nhd", g)
@@ -372,6 +395,24 @@ def test_attention_many_rows_magnitudes_and_growth():
         bound = tol + O.half_step(dt) * (want.abs() + tol)
         assert ((out.double().cpu() - want).abs() <= bound).all()
         assert ((lse.double().cpu() - wlse).abs() <= ltol).all()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_infinite_values_stay_in_their_channels(rows):
+    dt = torch.bfloat16
+    q, cache, table, lens, start = _problem([(rows, 300), (rows, 200)], 8, 2, 16, 64, dt, 45,
+                                            cols_more=_wide(40, 2, 8, 2))
+    ref = O.attend(q, cache, table, lens, start, tiles=rows > 16)
+    codes, step, mid = O.unpack(cache, dt)
+    step[1, int(table[0, 3]), 1, 5, 0] = math.inf  # token 53 of sequence 0: every row sees it
+    mid[1, int(table[1, 8]), 0, 2, 1] = -math.inf  # token 130 of sequence 1
+    out = P.attention_kv4(q.cuda(), O.pack(codes, step, mid).cuda(), table.cuda(), lens.cuda(),
+                          start.cuda(), rows).cpu().double()
+    bad = torch.zeros(out.shape, dtype=torch.bool)
+    bad[:rows, 4:, :64] = bad[rows:, :4, 64:] = True
+    assert not out[bad].isfinite().any()
+    want, _, tol, _ = ref
+    assert ((out - want).abs() <= tol + O.half_step(dt) * (want.abs() + tol) + 1e-30)[~bad].all()
 
 
 @pytest.mark.parametrize("rows", [1, 40])
