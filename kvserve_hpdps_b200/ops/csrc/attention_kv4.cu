@@ -106,7 +106,7 @@ struct Work {
 KVS_DEV Work work_of(const Attn4Launch& L, const Seq& s, int rows, int group) {
   Work w;
   w.tiles = (s.n * group + rows - 1) / rows;
-  w.per = s.len > 0 ? (s.len + kUnit - 1) / kUnit : 1;
+  w.per = s.len > 0 && !L.whole ? (s.len + kUnit - 1) / kUnit : 1;
   w.units = w.tiles * L.heads * (w.per + kOver);
   return w;
 }
@@ -151,7 +151,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
   U = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) U += s_scan[w];
-  const int used = min(B, (U + kLeast - 1) / kLeast);
+  const int least = L.whole ? 1 + kOver : kLeast;  // whole: an item a CTA
+  const int used = min(B, (U + least - 1) / least);
   if (b >= used) return;
   const Deal deal{U / used, U % used};
   int pos = deal.begin(b), base = 0;
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
 
     // ---- this warp's steps: tokens first + kUnit k + [0, 32)
     const int first = unit0 * kUnit + warp * kStep;
-    const int stop = min(limit, (unit0 + units) * kUnit);
+    const int stop = L.whole ? limit : min(limit, (unit0 + units) * kUnit);
     const int steps = first < stop ? (stop - first + kUnit - 1) / kUnit : 0;
     const uint8_t* const head = static_cast<const uint8_t*>(L.cache) + h * L.head_stride;
     const int32_t* const table = L.table + r * L.table_stride;
@@ -631,8 +632,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
 struct Grid {
   int ctas, rows;
   bool fits;   // the line's length is an int
-  bool split;  // whether an item can have more than one unit
+  bool split;  // whether items may be split
 };
+
+// Tables of at most so many units are not split: the launch that joins the parts takes longer
+// than a second step (150 tokens, one sequence: 10.5 us against 8.4 on the device).
+constexpr int kWholeUnits = 2;
 
 // Rows a tile: 8 hold a decode step's query heads of one kv head (up to 8);
 // more rows take 16, which unpack each code once for twice the rows.
@@ -644,12 +649,13 @@ Grid grid_of(const Attn4Launch* L) {
   const long long per = (static_cast<long long>(L->table_cols) * L->block_size + kUnit - 1) / kUnit;
   const long long items = static_cast<long long>(L->seqs) * L->heads *
                           ((rows + g.rows - 1) / g.rows);
-  const long long units = items * (per > 0 ? per : 1);
+  const long long units = items * (per > kWholeUnits ? per : 1);
   // block offsets are 32 x 32 -> 64 bit products
-  g.fits = L->block_stride >= 0 && L->block_stride < (1ll << 32) && items < (1ll << 31) && items * (per + 1 + kOver) < (1ll << 31);
+  g.fits = L->block_stride >= 0 && L->block_stride < (1ll << 32) && items < (1ll << 31) &&
+           items * (per + 1 + kOver) < (1ll << 31);
   const long long most = 148ll * (g.rows == 8 ? 3 : 2);  // resident at once
   g.ctas = static_cast<int>(units < most ? units : most);
-  g.split = per > 1;
+  g.split = per > kWholeUnits;
   return g;
 }
 
@@ -708,8 +714,9 @@ int kvs_attention_kv4(const Attn4Launch* L, void* stream) {
   if (many_rows(L)) return attn4_tile_launch(*L, s) == cudaSuccess ? 0 : -1;
   const Grid g = grid_of(L);
   if (!g.fits) return -2;
-  const cudaError_t e =
-      L->fp16 ? launch_groups<true>(*L, g, s) : launch_groups<false>(*L, g, s);
+  Attn4Launch A = *L;
+  A.whole = !g.split;
+  const cudaError_t e = L->fp16 ? launch_groups<true>(A, g, s) : launch_groups<false>(A, g, s);
   return e == cudaSuccess ? 0 : -1;
 }
 

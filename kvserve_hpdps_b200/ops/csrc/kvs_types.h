@@ -146,7 +146,7 @@ struct Attn4Launch {
   long long q_ts, q_hs, o_ts, o_hs, block_stride, head_stride, table_stride;
   int seqs, tokens, table_cols, num_blocks, q_heads, heads, block_size, groups, fp16, max_q;
   float scale;
-  int pad_;
+  int whole;  // set by the launcher: tables so short that items are not split
 };
 
 }  // namespace kvs
