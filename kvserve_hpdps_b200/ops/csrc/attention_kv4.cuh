@@ -91,7 +91,8 @@ KVS_DEV Parts parts(void* scratch, int B, int rows) {
 // item come with many parts (one long sequence on all SMs): four warps.  Tiles of 256 rows
 // come with few, but a CTA for eight rows of each: small ones, most of which have nothing to do.
 template <bool FP16, int NT, int WARPS>
-__global__ void __launch_bounds__(256 * WARPS) k_attn4_combine(const __grid_constant__ Attn4Launch L) {
+__global__ void __launch_bounds__(256 * WARPS)
+    k_attn4_combine(const __grid_constant__ Attn4Launch L) {
   constexpr int ROWS = 8 * NT;
   __shared__ float s_m[WARPS][8], s_l[WARPS][8];
   __shared__ float4 s_acc[WARPS][8][32];

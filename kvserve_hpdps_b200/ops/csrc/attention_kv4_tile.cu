@@ -21,9 +21,12 @@
 // The softmax warps take 64 tokens' scores at a time into registers, so that the next ones are
 // computed while they work.  O stays in tensor memory; it is rescaled by the
 // softmax warps when a row's maximum has grown by more than 2^kLazy, which
-// after the first tiles is rare.  What bounds it: the exponentials (16 a
-// clock and SM: 2048 clocks for 2 x 128 x 128 scores) next to the products
-// (2048 clocks at the nominal rate).
+// after the first tiles is rare.
+//
+// What bounds it: the softmax warps' chain of barriers, tensor memory and exponentials, about
+// 2900 clocks for 64 tokens of both tiles, of which the exponentials' rate (16 a clock and SM)
+// is 1024 and the products take 1320.  2 x 2048 tokens over up to 8193, 28/4 heads (361 GFLOP):
+// 522 us, 690 TFLOP/s; on mma.sync, a warp 16 rows, it was 2000 us.
 //
 // The work is dealt out as in attention_kv4.cu, here by the number of visible
 // keys a tile has, so that causal tiles of a long chunk load all SMs alike.
@@ -81,8 +84,8 @@ KVS_DEV uint32_t mn_desc(uint32_t saddr) {
   return (saddr >> 4) | (static_cast<uint32_t>(kHalfTile >> 4) << 16);
 }
 // The value of lane 0 in a uniform register, where the matrix instructions want their operands:
-// from there each takes one uniform addition, from a vector register four moves (measured: the
-// issuing warp was what the kernel waited for).
+// from there each takes one uniform addition, from a vector register four moves (736 us at 2 x
+// 2048 tokens against 536: the issuing warp was what the kernel waited for).
 KVS_DEV uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }
 KVS_DEV bool elected() {
   uint32_t p;
@@ -106,7 +109,8 @@ KVS_DEV void store_mids(uint8_t* tile, int row, F part) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int a = 2 * i, b = 2 * i + 1;
-    const uint32_t lo = a < 3 * NG ? part(a / 3, a % 3) : 0u, hi = b < 3 * NG ? part(b / 3, b % 3) : 0u;
+    const uint32_t lo = a < 3 * NG ? part(a / 3, a % 3) : 0u;
+    const uint32_t hi = b < 3 * NG ? part(b / 3, b % 3) : 0u;
     w[i] = lo | (hi << 16);
   }
   *reinterpret_cast<uint4*>(tile + mid_at(row)) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -433,7 +437,8 @@ KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, uint32_t q_til
                  km = uniform(mid_desc(q_tile + kMidAt + 2 * kMidTile));
   auto qk = [&](int x, int i) {
     const uint32_t a = qd + x * (2 * kHalfTile >> 4);
-    const uint32_t b = kd + ((step_no + (i >> 1)) & 1) * (2 * kHalfTile >> 4) + (i & 1) * (8192 >> 4);
+    const uint32_t b =
+        kd + ((step_no + (i >> 1)) & 1) * (2 * kHalfTile >> 4) + (i & 1) * (8192 >> 4);
     const uint32_t am = qm + x * (kMidTile >> 4);
     const uint32_t bm = km + ((step_no + (i >> 1)) & 1) * (kMidTile >> 4) + (i & 1) * (2048 >> 4);
     const uint32_t d = tm + 64 * x;
@@ -450,7 +455,8 @@ KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, uint32_t q_til
   };
   auto pv = [&](int x, int i) {
     const uint32_t buf = (half_no[x] + i) & 1;
-    const uint32_t b = vd + ((step_no + (i >> 1)) & 1) * (2 * kHalfTile >> 4) + (i & 1) * (8192 >> 4);
+    const uint32_t b =
+        vd + ((step_no + (i >> 1)) & 1) * (2 * kHalfTile >> 4) + (i & 1) * (8192 >> 4);
     const uint32_t w = tm + kWeightsAt + 64 * x + 32 * buf;
     const uint32_t d = tm + kOutAt + 128 * x;
     const uint32_t add = i > 0;
@@ -468,7 +474,8 @@ KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, uint32_t q_til
   };
   while (walk.next(L, group, p)) {
     if (p.steps == 0) continue;
-    const int n = static_cast<int>(uniform(p.two ? 2u : 1u)), H = static_cast<int>(uniform(p.halves));
+    const int n = static_cast<int>(uniform(p.two ? 2u : 1u));
+    const int H = static_cast<int>(uniform(p.halves));
     auto k_ready = [&](int i) {  // before the first half of a step
       const uint32_t no = step_no + (i >> 1);
       return (i & 1) || wait(&C->k_full[no & 1], (no >> 1) & 1);
@@ -524,7 +531,7 @@ template <bool FP16, int NG>
 KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q_tile,
                           uint32_t tmem, const Parts& P, Ctrl* C) {
   const int x = threadIdx.x >> 7, row = threadIdx.x & 127;
-  const uint32_t lanes = static_cast<uint32_t>((threadIdx.x >> 5) & 3) << 21;  // 32 TMEM lanes a warp
+  const uint32_t lanes = static_cast<uint32_t>((threadIdx.x >> 5) & 3) << 21;  // a warp's 32
   const uint32_t S = tmem + 64 * x + lanes, O = tmem + kOutAt + 128 * x + lanes;
   uint8_t* const qt = q_tile + x * 2 * kHalfTile;
   uint32_t step_no = 0, half_no = 0;

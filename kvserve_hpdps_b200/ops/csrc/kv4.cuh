@@ -10,9 +10,10 @@
 // floats of the cache's 16-bit type; a channel reads
 //   value = mid + (code - 8) * step,  code in [0, 15].
 //
-// Code order.  The attention kernel feeds matrix instructions from these
-// bytes with one AND (and one shift) per two codes, so channels are placed where its
-// fragments want them.  With channel d = 32 q + r:
+// Code order.  The attention kernels make matrix operands from these bytes
+// pair by pair with one AND-OR and one fused multiply-add (and a shift for
+// every second pair), so channels are placed where their fragments want
+// them.  With channel d = 32 q + r:
 //   K: r = 8 c + i: nibble i of the 32-bit word at byte 16 c + 4 q;
 //   V: r = 4 j + i: nibble i of the 16-bit word at byte 8 j + 2 q.
 #pragma once

@@ -79,7 +79,8 @@ def test_append_16bit(dt, form, tokens, hq, h, rd, inter):
     half = O.half_step(dt)
 
     def near(a, ref, mag):
-        bound = half * ref.abs() * (1 + 2 ** -20) + 2 ** -23 * mag + torch.finfo(dt).eps * torch.finfo(dt).tiny
+        smallest = torch.finfo(dt).eps * torch.finfo(dt).tiny
+        bound = half * ref.abs() * (1 + 2 ** -20) + 2 ** -23 * mag + smallest
         assert ((a.double().cpu() - ref).abs() <= bound).all()
 
     near(got, *O.rotate(q, table, pos, inter))
