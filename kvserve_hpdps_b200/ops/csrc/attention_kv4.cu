@@ -40,7 +40,10 @@ constexpr int kWarps = 4;             // a CTA
 constexpr int kStep = 32;             // tokens a warp takes at a time
 constexpr int kUnit = kWarps * kStep; // tokens a CTA takes at a time: the unit of work
 constexpr int kOver = 2;              // what starting and ending an item costs, in units
-constexpr int kLeast = 4;             // a CTA's share of the line is no shorter than this
+// A CTA's share of the line is no shorter than kLeast, or kFew while that takes no more than
+// kSpread CTAs: short chains against few parts to join (kFew and kLeast alone: one sequence of
+// 2000 tokens, 8 heads, 11.5 and 12.5 us; of 32768, 4 heads, 22.8 and 20.7).
+constexpr int kLeast = 4, kFew = 2, kSpread = 148;
 KVS_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                       uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -88,7 +91,7 @@ KVS_DEV void lds_meta(const uint8_t* a, uint32_t (&m)[NG]) {
 // one, so that rows that see nothing are written) and costs kOver more for
 // its queries and its result.  The items' costs form one line of length U,
 // and CTA b of B takes U / B of it, the first U % B CTAs one more, B being
-// what is resident at once or, for little work, U / kLeast.
+// what is resident at once or, for little work, less.
 // Ragged batches load every CTA alike and one long sequence is spread over
 // all of them (U < 2^31: the host refuses more).  A CTA that holds
 // an item whole writes its output; else it leaves a partial result (at most
@@ -157,8 +160,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
   U = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) U += s_scan[w];
-  const int least = L.whole ? 1 + kOver : kLeast;  // whole: an item a CTA
-  const int used = min(B, (U + least - 1) / least);
+  const int used =
+      min(B, L.whole ? U / (1 + kOver)  // an item a CTA
+                     : max((U + kLeast - 1) / kLeast, min(kSpread, (U + kFew - 1) / kFew)));
   if (b >= used) return;
   const Deal deal{U / used, U % used};
   int pos = deal.begin(b), base = 0;

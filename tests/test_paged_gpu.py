@@ -372,6 +372,23 @@ def test_attention_several_rows(dt, g_size, hq, h, seqs, wide):
     assert (out[int(start[-1]):] == 9.0).all()  # rows of no sequence
 
 
+@pytest.mark.parametrize("first", [1, 30])
+def test_attention_more_sequences_than_threads(first):
+    """Both kernels find a share's beginning in several rounds over the lengths."""
+    g = torch.Generator().manual_seed(first)
+    dt, hq, h = torch.bfloat16, 4, 1
+    seqs = [(int(n > 0), n) for n in torch.randint(0, 60, (700,), generator=g).tolist()]
+    seqs[3] = (0, 25)
+    seqs[650] = (first, 77)
+    q, cache, table, lens, start = _problem(seqs, hq, h, 16, 64, dt, first, cols_more=2)
+    assert _tiles(table, first, hq, h, 16) == (first == 30)
+    out, lse = P.attention_kv4(q.cuda(), cache.cuda(), table.cuda(), lens.cuda(), start.cuda(),
+                               first, return_lse=True)
+    torch.cuda.synchronize()
+    K.check_device_error(out.device)
+    _check(out, lse, O.attend(q, cache, table, lens, start, tiles=first == 30), dt)
+
+
 def test_attention_many_rows_magnitudes_and_growth():
     """Values far from 1, steps and scores that rise along the sequence, a negative scale."""
     for dt, mag in ((torch.bfloat16, 1e-18), (torch.bfloat16, 1e6), (torch.float16, 1.0)):
