@@ -670,12 +670,16 @@ Grid grid_of(const Attn4Launch* L) {
 }
 
 // Whether a call goes to attention_kv4_tile.cu: many rows a kv head, and enough of them.
-// Measured, us here / there, bf16, groups of 64: 16 sequences of 2000 tokens, 8 heads: 96
-// rows 93 / 107, 128 rows 117 / 108; 8 of 8000, 4 heads: 84 rows 84 / 78, 448 rows 333 / 148.
-// With little to do the first tiles decide: one of 1024 tokens, 4 heads: 448 rows (1.8 Mi rows
-// times tokens times heads) 21 / 33, 896 rows (3.5 Mi) 31 / 37, 1792 rows (7 Mi) 43 / 39; one of
-// 512 tokens, 8 heads: 2048 rows (8 Mi) 61 / 37.
-constexpr int kManyRows = 96;
+// Measured, us here / there, bf16, groups of 64: 32 sequences of 2000 tokens, 8 heads: 48
+// rows 98 / 103, 52 rows 121 / 104; 16 of 2000: 48 rows 58 / 59, 64 rows 71 / 61, 96 rows
+// 97 / 64; 8 of 8000, 4 heads: 42 rows 51 / 53, 56 rows 63 / 54; 64 of 1000, 4 heads: 42 rows
+// 70 / 72, 56 rows 85 / 74.
+// With little to do the tiles' fixed cost decides (Mi rows times tokens times heads): one of
+// 1024 tokens, 4 heads: 448 rows (1.8 Mi) 22 / 35, 896 rows (3.5 Mi) 31 / 39, 1792 rows (7 Mi)
+// 41 / 41; one of 4000, 8 heads: 128 rows (3.9 Mi) 27 / 33, 192 rows (5.9 Mi) 41 / 41; 4 of
+// 2000: 64 rows (3.9 Mi) 29 / 29, 96 rows (5.9 Mi) 37 / 33; 8 of 2000: 52 rows (6.3 Mi) 44 / 39.
+// Many short ones lose a little there: 64 of 200, 8 heads: 64 rows (6.2 Mi) 58 / 63.
+constexpr int kManyRows = 48;
 constexpr long long kMuchWork = 5ll << 20;
 bool many_rows(const Attn4Launch* L) {
   const long long rows = static_cast<long long>(L->max_q) * (L->q_heads / L->heads);

@@ -87,9 +87,10 @@ KVS_DEV Parts parts(void* scratch, int B, int rows) {
 }
 
 // Joins the parts of the item that begins in CTA blockIdx.x and goes on in
-// the next ones: eight rows a CTA, WARPS warps a row, each every WARPS-th part.  Few rows an
+// the next ones: eight rows at a time, WARPS warps a row, each every WARPS-th part.  Few rows an
 // item come with many parts (one long sequence on all SMs): four warps.  Tiles of 256 rows
-// come with few, but a CTA for eight rows of each: small ones, most of which have nothing to do.
+// come with few parts: one warp, and eight small CTAs an item, most of which have nothing to
+// do (32 of them, a CTA for eight rows, cost 5 to 10 us more a call).
 template <bool FP16, int NT, int WARPS>
 __global__ void __launch_bounds__(256 * WARPS)
     k_attn4_combine(const __grid_constant__ Attn4Launch L) {
@@ -103,81 +104,91 @@ __global__ void __launch_bounds__(256 * WARPS)
   if (d.x < 0) return;
   const int group = L.q_heads / L.heads, np = d.w;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r8 = warp & 7, quarter = warp >> 3;
-  const int row = blockIdx.y * 8 + r8;
-  // part 0 is in CTA b's second slot, the others in the first ones of the next CTAs
-  auto slot = [&](int i) { return (i == 0 ? 2 * b + 1 : 2 * (b + i)) * ROWS + row; };
-  float m = kLowest, ls = 0.f;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = quarter; i0 < np; i0 += 4 * WARPS) {  // four parts at a time, their loads together
-    float2 ml[4];
-    float4 x[4];
+  const Seq s = sequence(L, d.x, false);
+  const int rows = min(ROWS, s.n * group - d.z * ROWS);  // of this tile
+  for (int r0 = blockIdx.y * 8; r0 < rows; r0 += gridDim.y * 8) {
+    const int row = r0 + r8;
+    // part 0 is in CTA b's second slot, the others in the first ones of the next CTAs
+    auto slot = [&](int i) { return (i == 0 ? 2 * b + 1 : 2 * (b + i)) * ROWS + row; };
+    float m = kLowest, ls = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = quarter; i0 < np; i0 += 4 * WARPS) {  // four parts at a time, loads together
+      float2 ml[4];
+      float4 x[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = i0 + WARPS * u;
-      ml[u] = make_float2(kLowest, 0.f);
-      x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (i < np) {
-        ml[u] = P.ml[slot(i)];
-        x[u] = *reinterpret_cast<const float4*>(P.o + slot(i) * 128ll + lane * 4);
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + WARPS * u;
+        ml[u] = make_float2(kLowest, 0.f);
+        x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < np && row < rows) {
+          ml[u] = P.ml[slot(i)];
+          x[u] = *reinterpret_cast<const float4*>(P.o + slot(i) * 128ll + lane * 4);
+        }
+      }
+      const float top = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
+      const float k0 = ex2(m - top);
+      m = top;
+      ls *= k0;
+      a.x *= k0;
+      a.y *= k0;
+      a.z *= k0;
+      a.w *= k0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float k2 = ex2(ml[u].x - top);
+        ls = fmaf(ml[u].y, k2, ls);
+        a.x = fmaf(x[u].x, k2, a.x);
+        a.y = fmaf(x[u].y, k2, a.y);
+        a.z = fmaf(x[u].z, k2, a.z);
+        a.w = fmaf(x[u].w, k2, a.w);
       }
     }
-    const float top = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
-    const float k0 = ex2(m - top);
-    m = top;
-    ls *= k0;
-    a.x *= k0;
-    a.y *= k0;
-    a.z *= k0;
-    a.w *= k0;
+    if constexpr (WARPS > 1) {
+      s_acc[quarter][r8][lane] = a;
+      if (lane == 0) {
+        s_m[quarter][r8] = m;
+        s_l[quarter][r8] = ls;
+      }
+      __syncthreads();
+      if (quarter == 0) {
+        m = kLowest;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float k2 = ex2(ml[u].x - top);
-      ls = fmaf(ml[u].y, k2, ls);
-      a.x = fmaf(x[u].x, k2, a.x);
-      a.y = fmaf(x[u].y, k2, a.y);
-      a.z = fmaf(x[u].z, k2, a.z);
-      a.w = fmaf(x[u].w, k2, a.w);
+        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, s_m[w][r8]);
+        ls = 0.f;
+        a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const float k2 = ex2(s_m[w][r8] - m);
+          const float4 x = s_acc[w][r8][lane];
+          ls = fmaf(s_l[w][r8], k2, ls);
+          a.x = fmaf(x.x, k2, a.x);
+          a.y = fmaf(x.y, k2, a.y);
+          a.z = fmaf(x.z, k2, a.z);
+          a.w = fmaf(x.w, k2, a.w);
+        }
+      }
     }
+    if (quarter == 0 && row < rows) {
+      const int rr = d.z * ROWS + row;
+      const long long tq = s.row0 + rr / group;
+      const int hq = d.y * group + rr % group;
+      const float inv = ls == 0.f ? 0.f : __fdividef(1.f, ls);
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + tq * L.o_ts + hq * L.o_hs +
+                                lane * 4) =
+          make_uint2(f2h2<FP16>(a.x * inv, a.y * inv), f2h2<FP16>(a.z * inv, a.w * inv));
+      if (L.lse != nullptr && lane == 0)
+        L.lse[tq * L.q_heads + hq] =
+            ls == 0.f ? -INFINITY : (m + log2f(ls)) * 0.69314718055994531f;
+    }
+    if constexpr (WARPS > 1) __syncthreads();  // the next rows' sums take their place
   }
-  s_acc[quarter][r8][lane] = a;
-  if (lane == 0) {
-    s_m[quarter][r8] = m;
-    s_l[quarter][r8] = ls;
-  }
-  __syncthreads();
-  if (quarter != 0) return;
-  const Seq s = sequence(L, d.x, false);
-  const int rr = d.z * ROWS + row;
-  if (rr >= s.n * group) return;  // rows behind the tile's last were not written either
-  m = kLowest;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) m = fmaxf(m, s_m[w][r8]);
-  ls = 0.f;
-  a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    const float k2 = ex2(s_m[w][r8] - m);
-    const float4 x = s_acc[w][r8][lane];
-    ls = fmaf(s_l[w][r8], k2, ls);
-    a.x = fmaf(x.x, k2, a.x);
-    a.y = fmaf(x.y, k2, a.y);
-    a.z = fmaf(x.z, k2, a.z);
-    a.w = fmaf(x.w, k2, a.w);
-  }
-  const long long tq = s.row0 + rr / group;
-  const int hq = d.y * group + rr % group;
-  const float inv = ls == 0.f ? 0.f : __fdividef(1.f, ls);
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + tq * L.o_ts + hq * L.o_hs + lane * 4) =
-      make_uint2(f2h2<FP16>(a.x * inv, a.y * inv), f2h2<FP16>(a.z * inv, a.w * inv));
-  if (L.lse != nullptr && lane == 0)
-    L.lse[tq * L.q_heads + hq] = ls == 0.f ? -INFINITY : (m + log2f(ls)) * 0.69314718055994531f;
 }
 
 // Launches the join behind the attention kernel, allowed to start while that ends.
 template <bool FP16, int NT, int WARPS>
 cudaError_t launch_combine(const Attn4Launch& L, int ctas, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, NT);
+  cfg.gridDim = dim3(ctas, NT < 8 ? NT : 8);
   cfg.blockDim = dim3(256 * WARPS);
   cfg.stream = s;
   cudaLaunchAttribute attr = {};

@@ -319,7 +319,7 @@ def _tiles(table, rows, hq, h, bs):
     """Whether a call takes the kernel for many rows, going by what the host knows: rows a kv
     head, and rows times tokens that the table has room for."""
     rows *= hq // h
-    return rows > 96 and rows * h * table.numel() * bs > 5 << 20
+    return rows > 48 and rows * h * table.numel() * bs > 5 << 20
 
 
 def _wide(rows, seqs, hq, h, bs=16):
@@ -354,7 +354,7 @@ def test_attention_one_token(dt, g_size, hq, h, bs):
 @pytest.mark.parametrize("wide", [False, True])
 def test_attention_several_rows(dt, g_size, hq, h, seqs, wide):
     most = max(n for n, _ in seqs)
-    if wide and most * (hq // h) <= 96:
+    if wide and most * (hq // h) <= 48:
         pytest.skip("too few rows for the other kernel")
     q, cache, table, lens, start = _problem(
         seqs, hq, h, 16, g_size, dt, hq * 7, spare_rows=3,
