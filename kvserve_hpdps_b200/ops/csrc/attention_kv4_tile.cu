@@ -17,16 +17,16 @@
 //                    from tensor memory and writes back as fp16 exponentials,
 //                    the A operand of O += P V
 //   warps 8-11       packed rows to fp16 tiles in shared memory, a thread a token
-//   warp 12          issues the matrix instructions (13-15 have no work)
+//   warps 12-15      issue the matrix instructions: S of tile 0, 1, O of tile 0, 1
 // The softmax warps take 64 tokens' scores at a time into registers, so that the next ones are
 // computed while they work.  O stays in tensor memory; it is rescaled by the
-// softmax warps when a row's maximum has grown by more than 2^kLazy, which
+// softmax warps when 64 weights of a row sum up to more than kMostSum, which
 // after the first tiles is rare.
 //
 // What bounds it: the softmax warps' chain of barriers, tensor memory and exponentials, about
-// 2900 clocks for 64 tokens of both tiles, of which the exponentials' rate (16 a clock and SM)
+// 2400 clocks for 64 tokens of both tiles, of which the exponentials' rate (16 a clock and SM)
 // is 1024 and the products take 1320.  2 x 2048 tokens over up to 8193, 28/4 heads (361 GFLOP):
-// 522 us, 690 TFLOP/s; on mma.sync, a warp 16 rows, it was 2000 us.
+// 466 us, 775 TFLOP/s; on mma.sync, a warp 16 rows, it was 2000 us.
 //
 // The work is dealt out as in attention_kv4.cu, here by the number of visible
 // keys a tile has, so that causal tiles of a long chunk load all SMs alike.
@@ -41,6 +41,7 @@ constexpr int kTile = 128;       // tokens a step
 constexpr int kThreads = 16 * 32;
 constexpr int kOverTile = 2;     // an item's own cost, in steps
 constexpr int kLeastTile = 2;    // steps a CTA takes at least
+constexpr float kMostSum = 256.f;  // of 64 weights, without a new maximum (fp16 ends at 65504)
 constexpr int kHalfTile = 16384; // 128 rows x 64 channels of fp16
 
 struct Ctrl {
@@ -269,6 +270,18 @@ KVS_DEV bool wait_phase(uint64_t* bar, uint32_t parity, uint32_t* err) {
   return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, err, ERR_MBAR_TIMEOUT));
 }
 #define KVS_WAIT(bar, parity) wait_phase(bar, parity, L.err)
+// Whether the phase is over; nothing waits for the answer before it is used.
+KVS_DEV uint32_t peek_phase(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done;
+}
 
 // ---------------------------------------------------- packed rows to tiles
 template <bool FP16, int NG>
@@ -423,106 +436,72 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
 }
 
 // ------------------------------------------------------ matrix instructions
+// Four warps issue them, one a query tile x and product, each on a scheduler of its own: all
+// from one warp, its scheduler's two softmax warps were a third slower than the others.
+//
 // Scores of half i + 1 are asked for as soon as the softmax warps have those of half i in their
 // registers, so they find them ready when they are through; the weights have two buffers of
-// their own.
-KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, uint32_t q_tile, uint32_t k_tile,
-                      uint32_t v_tile, uint32_t tmem, Ctrl* C) {
-  uint32_t step_no = 0, piece_no[2] = {0, 0}, half_no[2] = {0, 0};
+// their own.  A stage is free when both tiles' products with it are done; without a second tile
+// its warps only say so.
+template <bool QK>
+KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, int x, uint32_t q_tile,
+                      uint32_t kv_tile, uint32_t tmem, Ctrl* C) {
+  uint32_t step_no = 0, piece_no = 0, half_no = 0;
   Piece p;
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return KVS_WAIT(bar, parity); };
-  const uint32_t qd = uniform(k_desc(q_tile)), kd = uniform(k_desc(k_tile)),
-                 vd = uniform(mn_desc(v_tile)), tm = uniform(tmem),
-                 qm = uniform(mid_desc(q_tile + kMidAt)),
-                 km = uniform(mid_desc(q_tile + kMidAt + 2 * kMidTile));
-  auto qk = [&](int x, int i) {
-    const uint32_t a = qd + x * (2 * kHalfTile >> 4);
-    const uint32_t b =
-        kd + ((step_no + (i >> 1)) & 1) * (2 * kHalfTile >> 4) + (i & 1) * (8192 >> 4);
-    const uint32_t am = qm + x * (kMidTile >> 4);
-    const uint32_t bm = km + ((step_no + (i >> 1)) & 1) * (kMidTile >> 4) + (i & 1) * (2048 >> 4);
-    const uint32_t d = tm + 64 * x;
-    if (elected()) {
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        const uint32_t off = ((ks >> 2) * kHalfTile + (ks & 3) * 32) >> 4;
-        mma_qk<kDescHigh>(d, a + off, b + off, ks > 0 ? 1u : 0u);
-      }
-      mma_qk<kMidHigh>(d, am, bm, 1u);
-      umma_commit(&C->s_full[x]);
-    }
-    __syncwarp();
-  };
-  auto pv = [&](int x, int i) {
-    const uint32_t buf = (half_no[x] + i) & 1;
-    const uint32_t b =
-        vd + ((step_no + (i >> 1)) & 1) * (2 * kHalfTile >> 4) + (i & 1) * (8192 >> 4);
-    const uint32_t w = tm + kWeightsAt + 64 * x + 32 * buf;
-    const uint32_t d = tm + kOutAt + 128 * x;
-    const uint32_t add = i > 0;
-    if (elected()) {
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)  // 16 tokens: two groups of eight rows, 8 columns of P
-        mma_pv(d, w + 8 * ks, b + ks * (2048 >> 4), ks > 0 ? 1u : add);
-      umma_commit(&C->pv_done[x][buf]);
-    }
-    __syncwarp();
-  };
-  auto commit = [&](uint64_t* bar) {
-    if (elected()) umma_commit(bar);
-    __syncwarp();
-  };
+  const uint32_t qd = uniform(k_desc(q_tile) + x * (2 * kHalfTile >> 4)),
+                 qm = uniform(mid_desc(q_tile + kMidAt) + x * (kMidTile >> 4)),
+                 km = uniform(mid_desc(q_tile + kMidAt + 2 * kMidTile)),
+                 kvd = uniform(QK ? k_desc(kv_tile) : mn_desc(kv_tile)),
+                 scores = uniform(tmem + 64 * x), weights = uniform(tmem + kWeightsAt + 64 * x),
+                 result = uniform(tmem + kOutAt + 128 * x);
   while (walk.next(L, group, p)) {
     if (p.steps == 0) continue;
-    const int n = static_cast<int>(uniform(p.two ? 2u : 1u));
     const int H = static_cast<int>(uniform(p.halves));
-    auto k_ready = [&](int i) {  // before the first half of a step
-      const uint32_t no = step_no + (i >> 1);
-      return (i & 1) || wait(&C->k_full[no & 1], (no >> 1) & 1);
-    };
-    auto k_used = [&](int i) {  // behind the last half of a step
-      if ((i & 1) || i == H - 1) commit(&C->k_empty[(step_no + (i >> 1)) & 1]);
-    };
-    #pragma unroll
-    for (int x = 0; x < 2; ++x)  // unrolled: what is indexed by x stays in registers
-      if (x < n && !wait(&C->q_full[x], piece_no[x]++ & 1)) return;
-    if (!k_ready(0)) return;
-    tc_fence_after();
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-      if (x < n) qk(x, 0);
-    k_used(0);
+    const bool idle = x == 1 && !p.two;
+    if (QK && !idle && !KVS_WAIT(&C->q_full[x], piece_no++ & 1)) return;
     for (int i = 0; i < H; ++i) {
-      const uint32_t no = step_no + (i >> 1);
-      if (i + 1 < H) {
-        if (!k_ready(i + 1)) return;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (x >= n) break;
-          if (!wait(&C->s_free[x], (half_no[x] + i) & 1)) return;
-          tc_fence_after();
-          qk(x, i + 1);
-        }
-        k_used(i + 1);
+      const uint32_t no = step_no + (i >> 1), stage = no & 1;
+      const bool last = (i & 1) || i == H - 1;
+      if (!(i & 1) && !KVS_WAIT(QK ? &C->k_full[stage] : &C->v_full[stage], (no >> 1) & 1)) return;
+      uint64_t* const empty = QK ? &C->k_empty[stage] : &C->v_empty[stage];
+      if (idle) {
+        if (last && (threadIdx.x & 31) == 0) mbar_arrive(empty);
+        continue;
       }
-      if (!(i & 1) && !wait(&C->v_full[no & 1], (no >> 1) & 1)) return;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if (x >= n) break;
-        const uint32_t hn = half_no[x] + i;
-        if (!wait(&C->p_full[x][hn & 1], (hn >> 1) & 1)) return;
+      const uint32_t b = kvd + stage * (2 * kHalfTile >> 4) + (i & 1) * (8192 >> 4);
+      if constexpr (QK) {
+        if (i > 0 && !KVS_WAIT(&C->s_free[x], (half_no - 1) & 1)) return;
         tc_fence_after();
-        pv(x, i);
+        const uint32_t bm = km + stage * (kMidTile >> 4) + (i & 1) * (2048 >> 4);
+        if (elected()) {
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const uint32_t off = ((ks >> 2) * kHalfTile + (ks & 3) * 32) >> 4;
+            mma_qk<kDescHigh>(scores, qd + off, b + off, ks > 0 ? 1u : 0u);
+          }
+          mma_qk<kMidHigh>(scores, qm, bm, 1u);
+          umma_commit(&C->s_full[x]);
+          if (last) umma_commit(empty);
+        }
+      } else {
+        const uint32_t buf = half_no & 1;
+        if (!KVS_WAIT(&C->p_full[x][buf], (half_no >> 1) & 1)) return;
+        tc_fence_after();
+        if (elected()) {
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)  // 16 tokens: two groups of eight rows, 8 columns of P
+            mma_pv(result, weights + 32 * buf + 8 * ks, b + ks * (2048 >> 4),
+                   ks > 0 || i > 0 ? 1u : 0u);
+          umma_commit(&C->pv_done[x][buf]);
+          if (last) umma_commit(empty);
+        }
       }
-      if ((i & 1) || i == H - 1) commit(&C->v_empty[no & 1]);
+      __syncwarp();
+      ++half_no;
     }
     // the last half's scores were taken, too: one phase of s_free a half
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-      if (x < n && !wait(&C->s_free[x], (half_no[x] + H - 1) & 1)) return;
+    if (QK && !idle && !KVS_WAIT(&C->s_free[x], (half_no - 1) & 1)) return;
     step_no += p.steps;
-    half_no[0] += H;
-    if (n == 2) half_no[1] += H;
   }
 }
 
@@ -602,23 +581,43 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
       if ((threadIdx.x & 31) == 0) mbar_arrive(&C->q_full[x]);
       // tokens that every row of this warp sees
       const int all_see = __reduce_min_sync(0xFFFFFFFFu, mine ? max(seen, 0) : 0x7FFFFFFF);
+      // what the converting warps say of half i's tokens, read a half ahead
+      struct {
+        uint32_t flag;
+        int v_exp[2];
+        float k_up[2];
+      } said;
+      auto listen = [&](int i) {
+        const uint32_t ring = (step_no + (i >> 1)) & 3, seg0 = 2 * (i & 1);
+        said.flag = C->flags[ring][seg0] | C->flags[ring][seg0 + 1];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          said.v_exp[k] = C->v_exp[ring][seg0 + k];
+          said.k_up[k] = C->k_up[ring][seg0 + k];
+        }
+      };
+      if (!KVS_WAIT(&C->e_full[step_no & 3], (step_no >> 2) & 1)) return;
+      listen(0);
       for (int i = 0; i < p.halves; ++i, ++half_no) {
-        const uint32_t no = step_no + (i >> 1);
-        const int ring = no & 3, seg0 = 2 * (i & 1), t0 = p.start + 64 * i;
+        const int ring = (step_no + (i >> 1)) & 3, seg0 = 2 * (i & 1), t0 = p.start + 64 * i;
         const uint32_t buf = half_no & 1, W = tmem + kWeightsAt + 64 * x + 32 * buf + lanes;
-        // what the converting warps say of the tokens comes long before the scores
-        if (!(i & 1) && !KVS_WAIT(&C->e_full[ring], (no >> 2) & 1)) return;
-        const uint32_t flag = C->flags[ring][seg0] | C->flags[ring][seg0 + 1];
-        const int v_exp[2] = {C->v_exp[ring][seg0], C->v_exp[ring][seg0 + 1]};
+        const uint32_t flag = said.flag;
+        const int v_exp[2] = {said.v_exp[0], said.v_exp[1]};
         const int e_new = max(E, max(v_exp[0], v_exp[1]));
         // not zero: a hidden score is -inf times it
-        const float fs[2] = {fmaxf(f * C->k_up[ring][seg0], 1.17549435e-38f),
-                             fmaxf(f * C->k_up[ring][seg0 + 1], 1.17549435e-38f)};
+        const float fs[2] = {fmaxf(f * said.k_up[0], 1.17549435e-38f),
+                             fmaxf(f * said.k_up[1], 1.17549435e-38f)};
         if (!KVS_WAIT(&C->s_full[x], half_no & 1)) return;
         tc_fence_after();
         uint32_t v[2][32];
         tmem_ld32_start(S, v[0]);
         tmem_ld32_start(S + 32, v[1]);
+        // Asked long before the answers are needed: a wait costs 140 clocks even when it is over.
+        const bool next = i + 1 < p.halves;
+        const uint32_t no = step_no + ((i + 1) >> 1);  // of the next half
+        const uint32_t ahead =
+            peek_phase(&C->pv_done[x][buf], ((half_no >> 1) & 1) ^ 1) &
+            ((i & 1) && next ? peek_phase(&C->e_full[no & 3], (no >> 2) & 1) : 1u);
         tmem_arrived(v[0]);
         tmem_arrived(v[1]);
         tc_fence_before();
@@ -643,11 +642,12 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
             }
           }
         }
-        // Against the reference that there is, the scores only pass through once; a row that
-        // has grown by more than 2^kLazy, or larger values, make the warp find the maximum,
+        // Against the reference that there is, the scores only pass through once; a row
+        // whose weights' sum has passed kMostSum, or larger values, make the warp find the maximum,
         // rescale and take the scores again (the first half always does).
         uint32_t h[2][16];
         float sum;
+        bool ready = false;
         for (bool fresh = i == 0 || e_new != E;; fresh = true) {
           if (fresh) {
             float part[2] = {-INFINITY, -INFINITY};
@@ -680,14 +680,10 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
             m = m_new;
             E = e_new;
           }
-          // four sums and maxima: one of each would be a chain as long as the row
+          // four sums: one would be a chain as long as the row
           f32x2_t s2[4];
-          float top[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            s2[k] = f2_pack(0.f, 0.f);
-            top[k] = -INFINITY;
-          }
+          for (int k = 0; k < 4; ++k) s2[k] = f2_pack(0.f, 0.f);
           const f32x2_t ref2 = f2_pack(-m, -m);
 #pragma unroll
           for (int sg = 0; sg < 2; ++sg) {
@@ -697,7 +693,6 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
               float u0, u1;
               f2_unpack(f2_fma(f2_pack(__uint_as_float(v[sg][2 * k]),
                                        __uint_as_float(v[sg][2 * k + 1])), fs2, ref2), u0, u1);
-              top[k & 3] = fmaxf(fmaxf(u0, u1), top[k & 3]);
               const float p0 = ex2(u0), p1 = ex2(u1);
               s2[k & 3] = f2_add(s2[k & 3], f2_pack(p0, p1));
               h[sg][k] = half2_bits(p0, p1);
@@ -706,12 +701,18 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
           float s0, s1;
           f2_unpack(f2_add(f2_add(s2[0], s2[1]), f2_add(s2[2], s2[3])), s0, s1);
           sum = s0 + s1;
-          const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-          if (fresh || !__any_sync(0xFFFFFFFFu, high > kLazy)) break;
+          if (fresh) break;
+          ready = __all_sync(0xFFFFFFFFu, ahead != 0 && !(sum > kMostSum));
+          if (ready || !__any_sync(0xFFFFFFFFu, sum > kMostSum)) break;
         }
         l += sum;
-        // The buffer is free: the scores' barrier is committed behind the products with the
-        // weights of half i - 2, and a commit covers all that its thread has issued before.
+        if (!ready) {
+          // the products with the weights two halves ago; what is said of the next half
+          if (!KVS_WAIT(&C->pv_done[x][buf], ((half_no >> 1) & 1) ^ 1)) return;
+          if ((i & 1) && next && !KVS_WAIT(&C->e_full[no & 3], (no >> 2) & 1)) return;
+        }
+        tc_fence_after();
+        if (next) listen(i + 1);
 #pragma unroll
         for (int sg = 0; sg < 2; ++sg) {
           const int down = E - v_exp[sg];
@@ -803,9 +804,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
     for (int i = 0; i < 2; ++i) {
       mbar_init(&C->q_full[i], 4);
       mbar_init(&C->k_full[i], 4);
-      mbar_init(&C->k_empty[i], 1);
+      mbar_init(&C->k_empty[i], 2);
       mbar_init(&C->v_full[i], 4);
-      mbar_init(&C->v_empty[i], 1);
+      mbar_init(&C->v_empty[i], 2);
       mbar_init(&C->s_full[i], 1);
       mbar_init(&C->s_free[i], 4);
       for (int k = 0; k < 2; ++k) {
@@ -879,8 +880,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
       convert_role<FP16, NG>(L, walk, group, q_tile, k_tile, v_tile, C);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-      if (warp == 12)
-        mma_role(L, walk, group, smem_u32(q_tile), smem_u32(k_tile), smem_u32(v_tile), tmem, C);
+      if (warp < 14)
+        mma_role<true>(L, walk, group, warp & 1, smem_u32(q_tile), smem_u32(k_tile), tmem, C);
+      else
+        mma_role<false>(L, walk, group, warp & 1, smem_u32(q_tile), smem_u32(v_tile), tmem, C);
     }
   }
   __syncwarp();
