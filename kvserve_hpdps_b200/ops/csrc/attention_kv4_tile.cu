@@ -26,7 +26,7 @@
 // What bounds it: the softmax warps' chain of barriers, tensor memory and exponentials, about
 // 2400 clocks for 64 tokens of both tiles, of which the exponentials' rate (16 a clock and SM)
 // is 1024 and the products take 1320.  2 x 2048 tokens over up to 8193, 28/4 heads (361 GFLOP):
-// 466 us, 775 TFLOP/s; on mma.sync, a warp 16 rows, it was 2000 us.
+// 464 us, 778 TFLOP/s; on mma.sync, a warp 16 rows, it was 2000 us.
 //
 // The work is dealt out as in attention_kv4.cu, here by the number of visible
 // keys a tile has, so that causal tiles of a long chunk load all SMs alike.
@@ -598,6 +598,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
       };
       if (!KVS_WAIT(&C->e_full[step_no & 3], (step_no >> 2) & 1)) return;
       listen(0);
+      uint32_t s_ready = 0;
       for (int i = 0; i < p.halves; ++i, ++half_no) {
         const int ring = (step_no + (i >> 1)) & 3, seg0 = 2 * (i & 1), t0 = p.start + 64 * i;
         const uint32_t buf = half_no & 1, W = tmem + kWeightsAt + 64 * x + 32 * buf + lanes;
@@ -607,12 +608,13 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         // not zero: a hidden score is -inf times it
         const float fs[2] = {fmaxf(f * said.k_up[0], 1.17549435e-38f),
                              fmaxf(f * said.k_up[1], 1.17549435e-38f)};
-        if (!KVS_WAIT(&C->s_full[x], half_no & 1)) return;
+        if (!__all_sync(0xFFFFFFFFu, s_ready) && !KVS_WAIT(&C->s_full[x], half_no & 1)) return;
         tc_fence_after();
         uint32_t v[2][32];
         tmem_ld32_start(S, v[0]);
         tmem_ld32_start(S + 32, v[1]);
-        // Asked long before the answers are needed: a wait costs 140 clocks even when it is over.
+        // Asked long before the answers are needed: a wait costs 140 clocks even when it is over
+        // (asking saves 30 us of 500 at 2 x 2048 tokens).
         const bool next = i + 1 < p.halves;
         const uint32_t no = step_no + ((i + 1) >> 1);  // of the next half
         const uint32_t ahead =
@@ -713,6 +715,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         }
         tc_fence_after();
         if (next) listen(i + 1);
+        s_ready = next ? peek_phase(&C->s_full[x], (half_no + 1) & 1) : 0u;
 #pragma unroll
         for (int sg = 0; sg < 2; ++sg) {
           const int down = E - v_exp[sg];
