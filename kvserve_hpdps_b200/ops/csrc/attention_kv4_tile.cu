@@ -596,9 +596,14 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
           said.k_up[k] = C->k_up[ring][seg0 + k];
         }
       };
+      // The first scores' barrier before the converting warps' one: tile 1 walks past pieces
+      // without a second tile and waits for nothing there, so it can be many steps ahead, and a
+      // parity cannot tell the phase wanted from the one two before it.  Once the scores are there,
+      // e_full is past this step and cannot be a phase further.
+      if (!KVS_WAIT(&C->s_full[x], half_no & 1)) return;
       if (!KVS_WAIT(&C->e_full[step_no & 3], (step_no >> 2) & 1)) return;
       listen(0);
-      uint32_t s_ready = 0;
+      uint32_t s_ready = 1;
       for (int i = 0; i < p.halves; ++i, ++half_no) {
         const int ring = (step_no + (i >> 1)) & 3, seg0 = 2 * (i & 1), t0 = p.start + 64 * i;
         const uint32_t buf = half_no & 1, W = tmem + kWeightsAt + 64 * x + 32 * buf + lanes;
