@@ -433,6 +433,13 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
       }
     }
   }
+  // The last products' commits arrive on their own: not after the CTA has gone.
+  for (uint32_t back = 2; back > 0; --back) {
+    if (step_no < back) continue;
+    const uint32_t no = step_no - back;
+    if (!KVS_WAIT(&C->k_empty[no & 1], (no >> 1) & 1)) return;
+    if (!KVS_WAIT(&C->v_empty[no & 1], (no >> 1) & 1)) return;
+  }
 }
 
 // ------------------------------------------------------ matrix instructions
