@@ -5,12 +5,22 @@
 // are worth turning into 16-bit tiles once, for tcgen05:
 //   S = Q K^T, O += P V, fp16 products of 128 rows and 64 tokens into tensor memory.
 // K and V become fp16 with one power of two for each 32 tokens, chosen from
-// the largest step and mid among them, so any scale keeps fp16's relative
-// 2^-11; the power goes into the softmax's factor (K) and, where it is not the largest so
-// far, into the weights (V), O being kept in units of the largest.  K's tile holds
-// step (code - 8) alone, which is exact in fp16 for bf16 steps (8 bits times 3); mid times the
-// sum of the group's query elements is 16 more columns of the product: that sum in three
-// fp16 parts against mid three times, so the scores of a bf16 cache are fp32's.
+// the largest step and mid among them; the power goes into the softmax's factor (K) and, where it
+// is not the largest so far, into the weights (V), O being kept in units of the largest.  K's tile
+// holds step (code - 8) alone; mid times the sum of the group's query elements is 16 more columns
+// of the product: that sum in three fp16 parts against mid three times.
+//
+// Roundings to fewer bits than fp32's:
+//   K, bf16 caches: none, step (code - 8) has 8 + 3 bits and fp16 holds 11.
+//   K and V, fp16 caches: none to speak of.  A step has 11 bits, so a second tile holds what the
+//     first one's rounding leaves over, and each product is taken with both.  Without it scores
+//     were off by 2^-11 of |q| |k| (errors of outputs and lse four times those of fp32 arithmetic;
+//     2 x 700 rows over 3000 tokens, 28/4 heads, 100 us); with it 135 us.
+//   V, bf16 caches: to fp16, 2^-11 of |v| at most, an eighth of the output's own rounding.
+//   Weights: to fp16, 2^-11, as the matrix instructions' A operand has to be of V's type; their
+//     sum is taken before that.  An fp16 output's error grows by a third (2.1e-4 to 2.8e-4 of the
+//     norm), a bf16 output's does not change; three parts of fp32 weights would need twice the
+//     products and tensor memory, of which none is left.
 //
 // Roles of a CTA (one an SM, 16 warps whose registers are dealt out anew):
 //   warps 0-3, 4-7   softmax of query tile 0, 1: a thread a row, which it reads
@@ -284,6 +294,19 @@ KVS_DEV uint32_t peek_phase(uint64_t* bar, uint32_t parity) {
 }
 
 // ---------------------------------------------------- packed rows to tiles
+// Where a step's tiles lie.  bf16 caches: two slots of 128 tokens, a step in each in turn.  fp16
+// caches: tokens 0..63 of every step are slot 0, 64..127 slot 1; the first 32 KB hold the tile
+// rounded to fp16, the next 32 KB, kRestAt on, what that leaves over.
+template <bool FP16>
+KVS_DEV uint32_t slot_of(uint32_t step, uint32_t half) {
+  return FP16 ? half : step & 1;
+}
+template <bool FP16>
+KVS_DEV uint32_t phase_of(uint32_t step) {  // of its slot's barriers
+  return (FP16 ? step : step >> 1) & 1;
+}
+constexpr int kRestAt = 2 * kHalfTile;
+
 template <bool FP16, int NG>
 KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q_tile,
                           uint8_t* k_tile, uint8_t* v_tile, Ctrl* C) {
@@ -381,13 +404,13 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         C->flags[ring][seg] = any;
         mbar_arrive(&C->e_full[ring]);
       }
-      const int stage = step_no & 1;
-      const uint32_t again = ((step_no >> 1) & 1) ^ 1;
+      const uint32_t slot = slot_of<FP16>(step_no, seg >> 1);
+      const uint32_t again = phase_of<FP16>(step_no) ^ 1;
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
-        uint64_t* const empty = v ? &C->v_empty[stage] : &C->k_empty[stage];
+        uint64_t* const empty = v ? &C->v_empty[slot] : &C->k_empty[slot];
         if (!KVS_WAIT(empty, again)) return;
-        uint8_t* const dst = (v ? v_tile : k_tile) + stage * 2 * kHalfTile;
+        uint8_t* const dst = (v ? v_tile : k_tile) + (FP16 ? 0 : slot * 2 * kHalfTile);
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -407,20 +430,36 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
             const uint32_t x = v == 0 ? w[4 * c + q]
                                       : __byte_perm(w[4 * c + (q >> 1)], w[4 * c + 2 + (q >> 1)],
                                                     (q & 1) ? 0x7632 : 0x5410);
-            uint32_t u[4];
+            uint32_t u[4], low[4];
             codes4(x, k1024, u);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const __half2 code2 = *reinterpret_cast<const __half2*>(&u[i]);
-              const __half2 y = v == 0 ? __hmul2(code2, step) : __hfma2(code2, step, mid);
+              __half2 y, rest;
+              if constexpr (FP16) {
+                y = __hmul2(code2, step);
+                rest = __hfma2(code2, step, __hneg2(y));  // exact
+                if (v == 1) {  // what y + mid leaves over, by the two-sum of its terms
+                  const __half2 z = __hadd2_rn(y, mid), w = __hsub2_rn(z, y);
+                  rest = __hadd2_rn(rest, __hadd2_rn(__hsub2_rn(y, __hsub2_rn(z, w)),
+                                                     __hsub2_rn(mid, w)));
+                  y = z;
+                }
+              } else {
+                y = v == 0 ? __hmul2(code2, step) : __hfma2(code2, step, mid);
+                rest = y;
+              }
               u[i] = *reinterpret_cast<const uint32_t*>(&y);
+              low[i] = *reinterpret_cast<const uint32_t*>(&rest);
             }
-            *reinterpret_cast<uint4*>(dst + chunk_at(row, 4 * q + c)) =
-                make_uint4(u[0], u[1], u[2], u[3]);
+            uint8_t* const at = dst + chunk_at(row, 4 * q + c);
+            *reinterpret_cast<uint4*>(at) = make_uint4(u[0], u[1], u[2], u[3]);
+            if constexpr (FP16)
+              *reinterpret_cast<uint4*>(at + kRestAt) = make_uint4(low[0], low[1], low[2], low[3]);
           }
         }
         if (v == 0)
-          store_mids<NG>(q_tile + kMidAt + (2 + stage) * kMidTile, row, [&](int gr, int) {
+          store_mids<NG>(q_tile + kMidAt + (FP16 ? 2 : 2 + slot) * kMidTile, row, [&](int gr, int) {
             return f2h<true>(h2f<FP16>(meta[0][gr] >> 16) * (up[0] * kMidUp));
           });
         if (j + 1 < p.steps) {
@@ -429,16 +468,16 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(v ? &C->v_full[stage] : &C->k_full[stage]);
+        if (lane == 0) mbar_arrive(v ? &C->v_full[slot] : &C->k_full[slot]);
       }
     }
   }
   // The last products' commits arrive on their own: not after the CTA has gone.
-  for (uint32_t back = 2; back > 0; --back) {
+  for (uint32_t back = FP16 ? 1 : 2; back > 0; --back) {
     if (step_no < back) continue;
-    const uint32_t no = step_no - back;
-    if (!KVS_WAIT(&C->k_empty[no & 1], (no >> 1) & 1)) return;
-    if (!KVS_WAIT(&C->v_empty[no & 1], (no >> 1) & 1)) return;
+    const uint32_t no = step_no - back, slot = slot_of<FP16>(no, seg >> 1);
+    if (!KVS_WAIT(&C->k_empty[slot], phase_of<FP16>(no))) return;
+    if (!KVS_WAIT(&C->v_empty[slot], phase_of<FP16>(no))) return;
   }
 }
 
@@ -450,7 +489,7 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
 // registers, so they find them ready when they are through; the weights have two buffers of
 // their own.  A stage is free when both tiles' products with it are done; without a second tile
 // its warps only say so.
-template <bool QK>
+template <bool FP16, bool QK>
 KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, int x, uint32_t q_tile,
                       uint32_t kv_tile, uint32_t tmem, Ctrl* C) {
   uint32_t step_no = 0, piece_no = 0, half_no = 0;
@@ -466,25 +505,27 @@ KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, int x, uint32_
     const int H = static_cast<int>(uniform(p.halves));
     const bool idle = x == 1 && !p.two;
     if (QK && !idle && !KVS_WAIT(&C->q_full[x], piece_no++ & 1)) return;
+    uint64_t *const fulls = QK ? C->k_full : C->v_full, *const empties = QK ? C->k_empty : C->v_empty;
     for (int i = 0; i < H; ++i) {
-      const uint32_t no = step_no + (i >> 1), stage = no & 1;
-      const bool last = (i & 1) || i == H - 1;
-      if (!(i & 1) && !KVS_WAIT(QK ? &C->k_full[stage] : &C->v_full[stage], (no >> 1) & 1)) return;
-      uint64_t* const empty = QK ? &C->k_empty[stage] : &C->v_empty[stage];
+      const uint32_t no = step_no + (i >> 1), slot = slot_of<FP16>(no, i & 1);
+      const bool last = FP16 || (i & 1) || i == H - 1;  // half of the slot
+      if ((FP16 || !(i & 1)) && !KVS_WAIT(&fulls[slot], phase_of<FP16>(no))) return;
+      uint64_t* const empty = &empties[slot];
       if (idle) {
         if (last && (threadIdx.x & 31) == 0) mbar_arrive(empty);
         continue;
       }
-      const uint32_t b = kvd + stage * (2 * kHalfTile >> 4) + (i & 1) * (8192 >> 4);
+      const uint32_t b = kvd + (FP16 ? 0 : slot * (2 * kHalfTile >> 4)) + (i & 1) * (8192 >> 4);
       if constexpr (QK) {
         if (i > 0 && !KVS_WAIT(&C->s_free[x], (half_no - 1) & 1)) return;
         tc_fence_after();
-        const uint32_t bm = km + stage * (kMidTile >> 4) + (i & 1) * (2048 >> 4);
+        const uint32_t bm = km + (FP16 ? 0 : slot * (kMidTile >> 4)) + (i & 1) * (2048 >> 4);
         if (elected()) {
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
             const uint32_t off = ((ks >> 2) * kHalfTile + (ks & 3) * 32) >> 4;
             mma_qk<kDescHigh>(scores, qd + off, b + off, ks > 0 ? 1u : 0u);
+            if constexpr (FP16) mma_qk<kDescHigh>(scores, qd + off, b + (kRestAt >> 4) + off, 1u);
           }
           mma_qk<kMidHigh>(scores, qm, bm, 1u);
           umma_commit(&C->s_full[x]);
@@ -496,15 +537,21 @@ KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, int x, uint32_
         tc_fence_after();
         if (elected()) {
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)  // 16 tokens: two groups of eight rows, 8 columns of P
-            mma_pv(result, weights + 32 * buf + 8 * ks, b + ks * (2048 >> 4),
-                   ks > 0 || i > 0 ? 1u : 0u);
+          for (int ks = 0; ks < 4; ++ks) {  // 16 tokens: two groups of eight rows, 8 columns of P
+            const uint32_t p = weights + 32 * buf + 8 * ks, at = b + ks * (2048 >> 4);
+            mma_pv(result, p, at, ks > 0 || i > 0 ? 1u : 0u);
+            if constexpr (FP16) mma_pv(result, p, at + (kRestAt >> 4), 1u);
+          }
           umma_commit(&C->pv_done[x][buf]);
           if (last) umma_commit(empty);
         }
       }
       __syncwarp();
       ++half_no;
+    }
+    if (FP16 && (H & 1)) {  // the step's second half, which nothing needs
+      if (!KVS_WAIT(&fulls[1], phase_of<FP16>(step_no + (H >> 1)))) return;
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&empties[1]);
     }
     // the last half's scores were taken, too: one phase of s_free a half
     if (QK && !idle && !KVS_WAIT(&C->s_free[x], (half_no - 1) & 1)) return;
@@ -818,9 +865,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
     P.desc[b] = make_int4(-1, 0, 0, 0);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&C->q_full[i], 4);
-      mbar_init(&C->k_full[i], 4);
+      mbar_init(&C->k_full[i], FP16 ? 2 : 4);
       mbar_init(&C->k_empty[i], 2);
-      mbar_init(&C->v_full[i], 4);
+      mbar_init(&C->v_full[i], FP16 ? 2 : 4);
       mbar_init(&C->v_empty[i], 2);
       mbar_init(&C->s_full[i], 1);
       mbar_init(&C->s_free[i], 4);
@@ -896,9 +943,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
       if (warp < 14)
-        mma_role<true>(L, walk, group, warp & 1, smem_u32(q_tile), smem_u32(k_tile), tmem, C);
+        mma_role<FP16, true>(L, walk, group, warp & 1, smem_u32(q_tile), smem_u32(k_tile), tmem, C);
       else
-        mma_role<false>(L, walk, group, warp & 1, smem_u32(q_tile), smem_u32(v_tile), tmem, C);
+        mma_role<FP16, false>(L, walk, group, warp & 1, smem_u32(q_tile), smem_u32(v_tile), tmem, C);
     }
   }
   __syncwarp();
