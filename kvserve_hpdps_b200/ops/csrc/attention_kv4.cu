@@ -368,7 +368,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
         for (int gr = 0; gr < NG; ++gr) msum[gr][nt][j] = 0.f;
       }
     }
-    int E = kLowestExp;
+    float E[NT][2], most_in = __uint_as_float(static_cast<uint32_t>(127 + 4 + kLowestExp) << 23);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) E[nt][0] = E[nt][1] = kLowestExp;
 
     auto step = [&](auto tag, int t0, const uint8_t* st, uint32_t had) {
       constexpr bool MASKED = decltype(tag)::value;
@@ -436,10 +438,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       }
       // ---- reference M of the exponentials: a row's running maximum, passed by up to
       // 2^kLazy before it is moved, plus the exponent E of the largest step or
-      // mid seen (moved when passed by 2^4): w then stays inside fp16's range
-      // whatever the values' scale, and sums keep one scale.
+      // mid that the row has seen (moved when passed by 2^4, `most_in`): w then stays inside
+      // fp16's range whatever the values' scale, and sums keep one scale.
       const float most = fmaxf(h2f<FP16>(big & 0xFFFFu), h2f<FP16>(big >> 16));
-      bool move = most > __uint_as_float(static_cast<uint32_t>(127 + 4 + E) << 23);
+      bool move = most > most_in;
       float top[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -447,34 +449,48 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
         for (int j = 0; j < 2; ++j) {
           top[nt][j] = fmaxf(fmaxf(sc[0][nt][j], sc[0][nt][j + 2]),
                              fmaxf(sc[1][nt][j], sc[1][nt][j + 2])) * f[nt][j];
-          move |= top[nt][j] - M[nt][j] > kLazy - E;
+          move |= top[nt][j] - M[nt][j] > kLazy - E[nt][j];
         }
       if (__any_sync(0xFFFFFFFFu, move)) {
         // the largest that is finite: an infinite step or mid makes its own channels NaN and
-        // must not put the other channels' weights out of range
+        // must not put the other channels' weights out of range; nor must a token that the row
+        // does not see
         constexpr uint32_t kInf = FP16 ? 0x7C00u : 0x7F80u;
-        uint32_t fine = 0;
+        uint32_t fine[2][2];
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-          for (int r2 = 0; r2 < 2; ++r2)
+          for (int r2 = 0; r2 < 2; ++r2) {
+            fine[hf][r2] = 0;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
               const uint32_t a = vm[hf][r2][gr] & 0x7FFFu, z = vm[hf][r2][gr] >> 16 & 0x7FFFu;
-              fine = max(fine, max(a < kInf ? a : 0u, z < kInf ? z : 0u));
+              fine[hf][r2] = max(fine[hf][r2], max(a < kInf ? a : 0u, z < kInf ? z : 0u));
             }
-        const uint32_t all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h2f<FP16>(fine)));
-        const int e = min(max(static_cast<int>(all >> 23) - 127, E), 100);
+          }
+        float low = 100.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             float x = top[nt][j];
+            uint32_t all = 0;
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, o));
-            const float old = M[nt][j];
-            const float m = fmaxf(fmaxf(old - E, x) + e, kLowest);
+            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+              for (int r2 = 0; r2 < 2; ++r2)
+                if (!MASKED || sc[hf][nt][2 * r2 + j] != -INFINITY) all = max(all, fine[hf][r2]);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+              x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, o));
+              all = max(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
+            }
+            const int bits = static_cast<int>(__float_as_uint(h2f<FP16>(all)) >> 23) - 127;
+            const float old = M[nt][j], e = fminf(fmaxf(static_cast<float>(bits), E[nt][j]), 100.f);
+            const float m = fmaxf(fmaxf(old - E[nt][j], x) + e, kLowest);
             M[nt][j] = m;
+            E[nt][j] = e;
+            low = fminf(low, e);
             // in two factors: E alone may move by more than the range of one (tokens whose
             // values are zero, then large ones), and their part of the sum has to stay
             const float k1 = ex2(0.5f * (old - m)), k2 = k1 * k1;
@@ -487,7 +503,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
               acc[d][nt][j + 2] *= k2;
             }
           }
-        E = e;
+        most_in = __uint_as_float(static_cast<uint32_t>(127 + 4 + static_cast<int>(low)) << 23);
       }
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
@@ -578,8 +594,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
           corr[gr] = ms;
         }
         // out of the units of this warp's E, which the others need not share
-        const float unit = __uint_as_float(static_cast<uint32_t>(127 + E) << 23);
-        if (g == 0) s_ml[warp][row] = make_float2(fmaxf(M[nt][j] - E, kLowest), ls * unit);
+        const float unit =
+            __uint_as_float(static_cast<uint32_t>(127 + static_cast<int>(E[nt][j])) << 23);
+        if (g == 0) s_ml[warp][row] = make_float2(fmaxf(M[nt][j] - E[nt][j], kLowest), ls * unit);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const float z = corr[q * NG / 4];

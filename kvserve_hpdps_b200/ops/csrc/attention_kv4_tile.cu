@@ -6,7 +6,9 @@
 //   S = Q K^T, O += P V, fp16 products of 128 rows and 64 tokens into tensor memory.
 // K and V become fp16 with one power of two for each 32 tokens, chosen from
 // the largest step and mid among them; the power goes into the softmax's factor (K) and, where it
-// is not the largest so far, into the weights (V), O being kept in units of the largest.  K's tile
+// is not the largest that the row has seen, into the weights (V), a row's O being kept in units of
+// that one.  Where 32 tokens' scales are more than 2^kApart apart, each takes its own power: else
+// a large token would take the small ones' bits from the rows that do not see it.  K's tile
 // holds step (code - 8) alone; mid times the sum of the group's query elements is 16 more columns
 // of the product: that sum in three fp16 parts against mid three times.
 //
@@ -53,6 +55,10 @@ constexpr int kOverTile = 2;     // an item's own cost, in steps
 constexpr int kLeastTile = 2;    // steps a CTA takes at least
 constexpr float kMostSum = 256.f;  // of 64 weights, without a new maximum (fp16 ends at 65504)
 constexpr int kHalfTile = 16384; // 128 rows x 64 channels of fp16
+// Tokens (of 32) whose scales are further apart than 2^kApart take a scale each: a row may see only
+// the small ones, or need their bits.
+constexpr uint32_t kApart = 8;
+constexpr uint32_t kHides = 1, kWideK = 2, kWideV = 4;
 
 struct Ctrl {
   uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
@@ -63,7 +69,9 @@ struct Ctrl {
   int v_exp[4][4];         // V in shared memory times 2^this is V
   uint32_t gone[4][4];     // tokens whose block does not exist
   uint32_t bad[4][4][4];   // [..][group] tokens with a step or mid of V that is not finite
-  uint32_t flags[4][4];    // whether any of the two is set
+  uint32_t flags[4][4];    // kHides: any of the two is set; kWideK, kWideV: a scale each token,
+  float k_tok[4][kTile];   //   in the place of k_up
+  int v_tok[4][kTile];     //   and v_exp
   long long scan[kThreads / 32];
   long long begin;
   int seq;
@@ -364,9 +372,9 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         for (int gr = 0; gr < NG; ++gr) meta[v][gr] = coming[v][gr];
       const uint32_t lost = __ballot_sync(0xFFFFFFFFu, gone);
       if (j + 1 < p.steps) locate(j + 1);  // its loads go out as registers become free
-      // exponent of the largest finite step or mid of the warp's 32 tokens
+      // exponent of the largest finite step or mid of the warp's 32 tokens, or of each one's
       float up[2];
-      uint32_t bad[NG];
+      uint32_t bad[NG], wide = 0;
       const int ring = step_no & 3;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) bad[gr] = 0;
@@ -383,16 +391,29 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
             if (!fine) meta[v][gr] = 0;  // rows that see it are marked instead
           }
         }
-        const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h2f<FP16>(top)));
+        const uint32_t own = __float_as_uint(h2f<FP16>(top));
+        uint32_t most = __reduce_max_sync(0xFFFFFFFFu, own);
+        const uint32_t least = __reduce_min_sync(0xFFFFFFFFu, own ? own : most);
+        const bool apart = (most >> 23) - (least >> 23) > kApart;
+        if (apart) {
+          wide |= v ? kWideV : kWideK;
+          most = own;
+        }
         // in steps of 16, so that V's powers seldom differ; K of zeros gets any
         int e = max(static_cast<int>(most >> 23) - 127, kLowestExp);
         e = (v == 0 && most == 0 ? 0 : (e + 3) & ~3) - 7;
         up[v] = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        if (lane == 0) {
-          if (v == 0) C->k_up[ring][seg] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        const float down = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        if (apart) {
+          if (v == 0) C->k_tok[ring][row] = down;
+          else C->v_tok[ring][row] = e;
+        }
+        if (lane == 0) {  // not looked at where they are apart
+          if (v == 0) C->k_up[ring][seg] = down;
           else C->v_exp[ring][seg] = e;
         }
       }
+      if (wide) __syncwarp();
       if (lane == 0) {
         uint32_t any = lost;
 #pragma unroll
@@ -401,7 +422,7 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
           any |= bad[gr];
         }
         C->gone[ring][seg] = lost;
-        C->flags[ring][seg] = any;
+        C->flags[ring][seg] = (any ? kHides : 0u) | wide;
         mbar_arrive(&C->e_full[ring]);
       }
       const uint32_t slot = slot_of<FP16>(step_no, seg >> 1);
@@ -580,7 +601,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
     const int hq = p.h * group + rr % group;
     const int seen = mine ? p.s.len - p.s.n + rr / group + 1 : 0;
     float m = kLowest, l = 0.f, f = 0.f;
-    int E = kLowestExp;
+    int E = kLowestExp, E_low = kLowestExp;  // of this row, the warp's lowest
     uint32_t poison = 0;
     if (p.steps > 0) {
       // ---- the row as fp16, scaled by a power of two: largest element in [2^14, 2^15)
@@ -662,11 +683,10 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         const int ring = (step_no + (i >> 1)) & 3, seg0 = 2 * (i & 1), t0 = p.start + 64 * i;
         const uint32_t buf = half_no & 1, W = tmem + kWeightsAt + 64 * x + 32 * buf + lanes;
         const uint32_t flag = said.flag;
-        const int v_exp[2] = {said.v_exp[0], said.v_exp[1]};
-        const int e_new = max(E, max(v_exp[0], v_exp[1]));
+        int v_exp[2] = {said.v_exp[0], said.v_exp[1]};
         // not zero: a hidden score is -inf times it
-        const float fs[2] = {fmaxf(f * said.k_up[0], 1.17549435e-38f),
-                             fmaxf(f * said.k_up[1], 1.17549435e-38f)};
+        float fs[2] = {fmaxf(f * said.k_up[0], 1.17549435e-38f),
+                       fmaxf(f * said.k_up[1], 1.17549435e-38f)};
         if (!__all_sync(0xFFFFFFFFu, s_ready) && !KVS_WAIT(&C->s_full[x], half_no & 1)) return;
         tc_fence_after();
         uint32_t v[2][32];
@@ -690,10 +710,18 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
           const uint32_t v = n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
           return v & ~C->gone[ring][seg0 + sg];
         };
+        bool raise;
         if (t0 + 64 > min(all_see, p.stop) || flag != 0) {  // hidden scores become -inf
 #pragma unroll
           for (int sg = 0; sg < 2; ++sg) {
-            const uint32_t vis = visible(sg);
+            const uint32_t vis = visible(sg), what = flag ? C->flags[ring][seg0 + sg] : 0u;
+            if (what & kWideK) {
+              const float* const up = C->k_tok[ring] + 32 * (seg0 + sg);
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                v[sg][k] = __float_as_uint(__uint_as_float(v[sg][k]) * (f * up[k]));
+              fs[sg] = 1.f;
+            }
 #pragma unroll
             for (int k = 0; k < 32; ++k) v[sg][k] = vis >> k & 1u ? v[sg][k] : 0xFF800000u;
             if (flag) {
@@ -701,16 +729,27 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
               for (int gr = 0; gr < NG; ++gr)
                 if (C->bad[ring][seg0 + sg][gr] & vis) poison |= 1u << gr;
             }
+            // values that the row does not see have no say in its units
+            if (what & kWideV) {
+              v_exp[sg] = kLowestExp;
+#pragma unroll 4
+              for (int k = 0; k < 32; ++k)
+                if (vis >> k & 1u) v_exp[sg] = max(v_exp[sg], C->v_tok[ring][32 * (seg0 + sg) + k]);
+            } else if (vis == 0) {
+              v_exp[sg] = kLowestExp;
+            }
           }
         }
+        raise = __any_sync(0xFFFFFFFFu, max(v_exp[0], v_exp[1]) > E);
         // Against the reference that there is, the scores only pass through once; a row
         // whose weights' sum has passed kMostSum, or larger values, make the warp find the maximum,
         // rescale and take the scores again (the first half always does).
         uint32_t h[2][16];
         float sum;
         bool ready = false;
-        for (bool fresh = i == 0 || e_new != E;; fresh = true) {
+        for (bool fresh = i == 0 || raise;; fresh = true) {
           if (fresh) {
+            const int e_new = max(E, max(v_exp[0], v_exp[1]));
             float part[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
@@ -778,7 +817,16 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
 #pragma unroll
         for (int sg = 0; sg < 2; ++sg) {
           const int down = E - v_exp[sg];
-          if (down != 0) {  // these tokens' V is in smaller units than O
+          if (flag & kWideV && C->flags[ring][seg0 + sg] & kWideV) {
+            const int* const exps = C->v_tok[ring] + 32 * (seg0 + sg);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {  // those that the row does not see weigh nothing
+              const __half2 g = __floats2half2_rn(ex2(static_cast<float>(min(exps[2 * k] - E, 0))),
+                                                  ex2(static_cast<float>(min(exps[2 * k + 1] - E, 0))));
+              const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h[sg][k]), g);
+              h[sg][k] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+          } else if (down != 0) {  // these tokens' V is in smaller units than O
             const __half2 g = __float2half2_rn(ex2(static_cast<float>(-down)));
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
