@@ -436,8 +436,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
             }
         }
       }
-      // ---- reference M of the exponentials: a row's running maximum, passed by up to
-      // 2^kLazy before it is moved, plus the exponent E of the largest step or
+      // ---- reference M + E of the exponentials: a row's running maximum, passed by up to
+      // 2^kLazy before it is moved, and the exponent of the largest step or
       // mid that the row has seen (moved when passed by 2^4, `most_in`): w then stays inside
       // fp16's range whatever the values' scale, and sums keep one scale.
       const float most = fmaxf(h2f<FP16>(big & 0xFFFFu), h2f<FP16>(big >> 16));
@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
         for (int j = 0; j < 2; ++j) {
           top[nt][j] = fmaxf(fmaxf(sc[0][nt][j], sc[0][nt][j + 2]),
                              fmaxf(sc[1][nt][j], sc[1][nt][j + 2])) * f[nt][j];
-          move |= top[nt][j] - M[nt][j] > kLazy - E[nt][j];
+          move |= top[nt][j] - M[nt][j] > kLazy;
         }
       if (__any_sync(0xFFFFFFFFu, move)) {
         // the largest that is finite: an infinite step or mid makes its own channels NaN and
@@ -483,17 +483,18 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
               x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, o));
-              all = max(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
+              if (MASKED) all = max(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
             }
+            if (!MASKED) all = __reduce_max_sync(0xFFFFFFFFu, all);
             const int bits = static_cast<int>(__float_as_uint(h2f<FP16>(all)) >> 23) - 127;
             const float old = M[nt][j], e = fminf(fmaxf(static_cast<float>(bits), E[nt][j]), 100.f);
-            const float m = fmaxf(fmaxf(old - E[nt][j], x) + e, kLowest);
+            const float m = fmaxf(old, x), less = (old - m) + (E[nt][j] - e);
             M[nt][j] = m;
             E[nt][j] = e;
             low = fminf(low, e);
             // in two factors: E alone may move by more than the range of one (tokens whose
             // values are zero, then large ones), and their part of the sum has to stay
-            const float k1 = ex2(0.5f * (old - m)), k2 = k1 * k1;
+            const float k1 = ex2(0.5f * less), k2 = k1 * k1;
             l[nt][j] = l[nt][j] * k1 * k1;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) msum[gr][nt][j] *= k2;
@@ -513,7 +514,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            p[nt][i] = ex2(fmaf(sc[hf][nt][i], f[nt][i & 1], -M[nt][i & 1]));
+            // rounded as the maximum was, and that taken off first: a fused multiply-add would
+            // leave the maximum's rounding over, which grows with the score
+            p[nt][i] = ex2(__fmul_rn(sc[hf][nt][i], f[nt][i & 1]) - M[nt][i & 1] - E[nt][i & 1]);
             l[nt][i & 1] += p[nt][i];
           }
         const uint2 v0 = lds64(at + v_at), v1 = lds64(at + v_at + 256),
@@ -596,7 +599,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
         // out of the units of this warp's E, which the others need not share
         const float unit =
             __uint_as_float(static_cast<uint32_t>(127 + static_cast<int>(E[nt][j])) << 23);
-        if (g == 0) s_ml[warp][row] = make_float2(fmaxf(M[nt][j] - E[nt][j], kLowest), ls * unit);
+        if (g == 0) s_ml[warp][row] = make_float2(M[nt][j], ls * unit);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const float z = corr[q * NG / 4];

@@ -8,7 +8,9 @@ namespace kvs {
 
 namespace {
 
-constexpr float kLowest = -1e30f;     // running maximum of a row that has seen nothing
+// Running maximum of a row that has seen nothing: finite, so that differences of two are numbers,
+// and below any score that fp32 holds in comfort.
+constexpr float kLowest = -3e38f;
 constexpr int kLowestExp = -100;      // smallest exponent that values are scaled by
 constexpr float kLazy = 8.f;          // log2 by which a score may pass its running maximum
 

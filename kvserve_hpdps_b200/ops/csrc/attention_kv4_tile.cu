@@ -59,6 +59,10 @@ constexpr int kHalfTile = 16384; // 128 rows x 64 channels of fp16
 // the small ones, or need their bits.
 constexpr uint32_t kApart = 8;
 constexpr uint32_t kHides = 1, kWideK = 2, kWideV = 4;
+// A score is a factor times 128 products of less than 2^15 and 2^11.  Where the factor lets it pass
+// 2^20, the product is rounded before the maximum is taken off: the fused multiply-add leaves
+// the maximum's own rounding over, which is 2^-24 of the score and no longer small.
+constexpr float kHuge = 0x1p-13f;
 
 struct Ctrl {
   uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
@@ -654,6 +658,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
       fence_proxy_async_smem();
       __syncwarp();
       if ((threadIdx.x & 31) == 0) mbar_arrive(&C->q_full[x]);
+      const float f_most = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(f)));
       // tokens that every row of this warp sees
       const int all_see = __reduce_min_sync(0xFFFFFFFFu, mine ? max(seen, 0) : 0x7FFFFFFF);
       // what the converting warps say of half i's tokens, read a half ahead
@@ -685,8 +690,9 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         const uint32_t flag = said.flag;
         int v_exp[2] = {said.v_exp[0], said.v_exp[1]};
         // not zero: a hidden score is -inf times it
-        float fs[2] = {fmaxf(f * said.k_up[0], 1.17549435e-38f),
-                       fmaxf(f * said.k_up[1], 1.17549435e-38f)};
+        const float said_up[2] = {said.k_up[0], said.k_up[1]};
+        float fs[2] = {fmaxf(f * said_up[0], 1.17549435e-38f),
+                       fmaxf(f * said_up[1], 1.17549435e-38f)};
         if (!__all_sync(0xFFFFFFFFu, s_ready) && !KVS_WAIT(&C->s_full[x], half_no & 1)) return;
         tc_fence_after();
         uint32_t v[2][32];
@@ -711,7 +717,8 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
           return v & ~C->gone[ring][seg0 + sg];
         };
         bool raise;
-        if (t0 + 64 > min(all_see, p.stop) || flag != 0) {  // hidden scores become -inf
+        const bool huge = f_most * fmaxf(said_up[0], said_up[1]) > kHuge;
+        if (t0 + 64 > min(all_see, p.stop) || flag != 0 || huge) {  // hidden scores become -inf
 #pragma unroll
           for (int sg = 0; sg < 2; ++sg) {
             const uint32_t vis = visible(sg), what = flag ? C->flags[ring][seg0 + sg] : 0u;
@@ -720,6 +727,11 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
 #pragma unroll
               for (int k = 0; k < 32; ++k)
                 v[sg][k] = __float_as_uint(__uint_as_float(v[sg][k]) * (f * up[k]));
+              fs[sg] = 1.f;
+            } else if (huge) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                v[sg][k] = __float_as_uint(__fmul_rn(__uint_as_float(v[sg][k]), fs[sg]));
               fs[sg] = 1.f;
             }
 #pragma unroll
