@@ -53,7 +53,10 @@ constexpr int kTile = 128;       // tokens a step
 constexpr int kThreads = 16 * 32;
 constexpr int kOverTile = 2;     // an item's own cost, in steps
 constexpr int kLeastTile = 2;    // steps a CTA takes at least
-constexpr float kMostSum = 256.f;  // of 64 weights, without a new maximum (fp16 ends at 65504)
+// The largest weight is 2^kAbove at its maximum's time, so that those down to 2^-21 of it are normal
+// fp16 numbers (a first token often takes nearly all of the weight and has a small value).
+constexpr float kAbove = 7.f;
+constexpr float kMostSum = 32768.f;  // of 64 weights, without a new maximum (fp16 ends at 65504)
 constexpr int kHalfTile = 16384; // 128 rows x 64 channels of fp16
 // Tokens (of 32) whose scales are further apart than 2^kApart take a scale each: a row may see only
 // the small ones, or need their bits.
@@ -768,7 +771,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
               part[0] = fmaxf(part[0], __uint_as_float(v[0][k]));
               part[1] = fmaxf(part[1], __uint_as_float(v[1][k]));
             }
-            const float mx = fmaxf(part[0] * fs[0], part[1] * fs[1]);
+            const float mx = fmaxf(part[0] * fs[0], part[1] * fs[1]) - kAbove;
             const float m_new = fmaxf(m, mx), k2 = ex2(m - m_new);
             l *= k2;
             if (i > 0) {

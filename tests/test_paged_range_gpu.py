@@ -88,3 +88,38 @@ def test_scores_of_any_size(dt, mag, rows):
             tol = tol + O.half_step(dt) * (want.abs() + tol)
             assert ((out[i, head].double().cpu() - want).abs() <= tol).all()
     assert clear > rows * hq // 2
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_many_rows_small_weights_beside_a_large_one(dt):
+    """A first token of no value takes nearly all the weight; the others, 2^-16 to 2^-20 of it,
+    make up the output and keep their bits: it is off by half a step of fp16 of their p |v|
+    (twice in bf16 caches, whose values are rounded too), not of the first one's."""
+    hq, h, bs, rows, length = 8, 2, 16, 60, 300
+    g = _gen(9)
+    cols = -(-length // bs)
+    table = torch.full((1, cols + _wide(rows, 1, hq, h)), -7, dtype=torch.int32)
+    table[0, :cols] = torch.arange(cols).int()
+    assert _tiles(table, rows, hq, h, bs)
+    codes, step, mid = O.unpack(_cache4(cols, h, bs, 64, dt, g, spread=0.0), dt)
+    step[0], mid[0] = step[0] * 0.125, 0
+    step[:, 0, :, 0], mid[1, 0, :, 0], mid[0, 0, :, 0] = 0, 0, 1.0  # token 0: all ones, and zeros
+    cache = O.pack(codes, step, mid)
+    q = (torch.randn((rows, hq, 128), generator=g) * 0.1 + 1.0).to(dt)
+    start, lens = torch.tensor([0, rows]).int(), torch.tensor([length]).int()
+    out = P.attention_kv4(q.cuda(), cache.cuda(), table.cuda(), lens.cuda(), start.cuda(), rows)
+    torch.cuda.synchronize()
+    K.check_device_error(out.device)
+    x = O.values(cache, dt)[0][:, table[0, :cols].long()].permute(0, 2, 1, 3, 4).flatten(2, 3)
+    seen = length - rows + 1 + torch.arange(rows)
+    for head in range(hq):
+        k, v = x[0, head // 4, :length], x[1, head // 4, :length]
+        want, _, pv, werr = one_head(q[:, head], k, v, seen, 1 / math.sqrt(128))
+        w = q[:, head].double() @ k.T / math.sqrt(128)
+        below = (w[:, :1] - w[:, 1:]) / math.log(2)
+        assert (below > 13).all() and (below < 21).all()
+        tol = (2 ** -11 * (2 if dt == BF else 1) + 2 ** -17 + 2 * werr[:, None]) * pv
+        tol = tol + O.half_step(dt) * (want.abs() + tol) + 2 ** -25
+        assert ((out[:, head].double().cpu() - want).abs() <= tol).all()
+        off = (out[:, head].double().cpu() - want).norm() / want.norm()
+        assert off <= 2 * O.half_step(dt)
