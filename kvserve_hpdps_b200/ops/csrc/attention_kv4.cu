@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_scan[kWarps], s_begin, s_seq;
   __shared__ float2 s_ml[kWarps][ROWS];
+  __shared__ int2 s_named[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   const int group = L.q_heads / L.heads;
   const int B = gridDim.x, b = blockIdx.x;
@@ -149,14 +150,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
   // ---- this CTA's share [pos, end) and the sequence that it begins in
   if (tid == 0) P.desc[b] = make_int4(-1, 0, 0, 0);
   int U = 0, mine = 0;
+  Named named;
   for (int r = tid; r < L.seqs; r += kWarps * 32) {
-    mine = work_of(L, sequence(L, r, b == 0), ROWS, group).units;
+    const Seq s = sequence(L, r, b == 0);
+    named.take(L, s, r);
+    mine = work_of(L, s, ROWS, group).units;
     U += mine;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) U += __shfl_xor_sync(0xFFFFFFFFu, U, o);
   if (lane == 0) s_scan[warp] = U;
+  named.leave(L, s_named);
   __syncthreads();
+  named.clear<kWarps>(L, s_named);
   U = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) U += s_scan[w];

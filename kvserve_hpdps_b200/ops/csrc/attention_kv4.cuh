@@ -16,6 +16,7 @@ constexpr float kLazy = 8.f;          // log2 by which a score may pass its runn
 
 struct Seq {
   int row0, n, len;  // first query row, query rows, cached tokens
+  bool bad;          // left out
 };
 
 // The sequence's extents, held to what the launch's arrays cover.
@@ -32,14 +33,80 @@ KVS_DEV Seq sequence(const Attn4Launch& L, int r, bool report) {
   s.n = end - s.row0;
   s.len = L.lens[r];
   const long long cap = static_cast<long long>(L.table_cols) * L.block_size;
-  const bool bad = s.row0 < 0 || end < s.row0 || end > L.tokens || s.n > L.max_q || s.len < 0 ||
-                   s.len > cap;
-  if (bad) {
+  s.bad = s.row0 < 0 || end < s.row0 || end > L.tokens || s.n > L.max_q || s.len < 0 ||
+          s.len > cap;
+  if (s.bad) {
     if (report) record_error(L.err, ERR_BOUNDS);
     s.n = 0;
   }
   return s;
 }
+
+// Rows [from, to) have no result: 16 bytes `at`, at + by, ... of them.
+KVS_DEV void clear_rows(const Attn4Launch& L, long long from, long long to, long long at,
+                        long long by) {
+  for (long long i = at; i < (to - from) * L.q_heads * 16; i += by) {
+    const long long row = i >> 4, t = from + row / L.q_heads;
+    const int h = static_cast<int>(row % L.q_heads);
+    if (L.clear)
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(L.out) + t * L.o_ts + h * L.o_hs +
+                                (i & 15) * 8) = make_uint4(0u, 0u, 0u, 0u);
+    if (L.lse != nullptr && (i & 15) == 0) L.lse[t * L.q_heads + h] = -INFINITY;
+  }
+}
+// The rows of a sequence that is left out, by one thread a CTA (few calls have any); not those
+// that another sequence names too and has results for.
+KVS_DEV void clear_sequence(const Attn4Launch& L, int r) {
+  const int from = max(0, L.start ? L.start[r] : r), to = min(L.tokens, L.start ? L.start[r + 1] : r + 1);
+  for (int t = from + static_cast<int>(blockIdx.x); t < to; t += gridDim.x) {
+    bool named = false;
+    for (int i = 0; L.start && i < L.seqs && !named; ++i) {
+      const Seq s = sequence(L, i, false);
+      named = !s.bad && t >= s.row0 && t - s.row0 < s.n;
+    }
+    if (!named) clear_rows(L, t, t + 1, 0, 1);
+  }
+}
+// Keeps the book of the rows that sequences have, for those in front of the first and behind the
+// last, which are dealt out to all threads.
+struct Named {
+  int lo, hi;
+  KVS_DEV Named() : lo(0x7FFFFFFF), hi(0) {}
+  KVS_DEV void take(const Attn4Launch& L, const Seq& s, int r) {
+    if (!L.clear && L.lse == nullptr) return;
+    if (s.bad) {
+      clear_sequence(L, r);
+    } else {
+      lo = min(lo, s.row0);
+      hi = max(hi, s.row0 + s.n);
+    }
+  }
+  // Between the two a __syncthreads.
+  KVS_DEV void leave(const Attn4Launch& L, int2* smem) {
+    if ((!L.clear && L.lse == nullptr) || L.start == nullptr) return;
+    const int a = __reduce_min_sync(0xFFFFFFFFu, lo), z = __reduce_max_sync(0xFFFFFFFFu, hi);
+    if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = make_int2(a, z);
+  }
+  template <int WARPS>
+  KVS_DEV void clear(const Attn4Launch& L, const int2* smem) {
+    if (!L.clear && L.lse == nullptr) return;
+    int a = 0, z = L.seqs;
+    if (L.start != nullptr) {
+      a = L.tokens;
+      z = 0;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        a = min(a, smem[w].x);
+        z = max(z, smem[w].y);
+      }
+    }
+    if (a == 0 && z == L.tokens) return;
+    const long long at = static_cast<long long>(blockIdx.x) * (32 * WARPS) + threadIdx.x,
+                    by = static_cast<long long>(gridDim.x) * (32 * WARPS);
+    clear_rows(L, 0, a, at, by);
+    clear_rows(L, z, L.tokens, at, by);
+  }
+};
 
 KVS_DEV float ex2(float x) {
   float y;

@@ -80,6 +80,7 @@ struct Ctrl {
   float k_tok[4][kTile];   //   in the place of k_up
   int v_tok[4][kTile];     //   and v_exp
   long long scan[kThreads / 32];
+  int2 named[kThreads / 32];
   long long begin;
   int seq;
 };
@@ -947,14 +948,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
 
   // ---- this CTA's share of the line
   long long total = 0, mine = 0;
+  Named named;
   for (int r = tid; r < L.seqs; r += kThreads) {
-    mine = tile_work(sequence(L, r, b == 0), group).head * L.heads;
+    const Seq s = sequence(L, r, b == 0);
+    named.take(L, s, r);
+    mine = tile_work(s, group).head * L.heads;
     total += mine;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
   if (lane == 0) C->scan[warp] = total;
+  named.leave(L, C->named);
   __syncthreads();
+  named.clear<kThreads / 32>(L, C->named);
   tc_fence_after();
   const uint32_t tmem = C->tmem;
   total = 0;

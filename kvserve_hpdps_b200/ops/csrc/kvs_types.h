@@ -147,6 +147,7 @@ struct Attn4Launch {
   int seqs, tokens, table_cols, num_blocks, q_heads, heads, block_size, groups, fp16, max_q;
   float scale;
   int whole;  // set by the launcher: tables so short that items are not split
+  int clear;  // rows of no sequence become zeros, too (their lse is -inf either way)
 };
 
 }  // namespace kvs

@@ -253,7 +253,11 @@ std::pair<Tensor, optional<Tensor>> attention_kv4(
   const Tensor out = out_in.has_value() ? *out_in : at::empty(query.sizes(), query.options());
   optional<Tensor> lse;
   if (return_lse) lse = at::empty({T, Hq}, query.options().dtype(at::kFloat));
-  if (R == 0 || T == 0 || Hq == 0) return {out, lse};
+  if (R == 0 || T == 0 || Hq == 0) {
+    if (!out_in.has_value()) out.zero_();
+    if (lse.has_value()) lse->fill_(-INFINITY);
+    return {out, lse};
+  }
   const Tensor q = rows(query), lens = seq_lens.contiguous();
   const Tensor table = block_table.stride(1) == 1 ? block_table : block_table.contiguous();
   const Tensor start = query_start.has_value() ? query_start->contiguous() : Tensor();
@@ -272,6 +276,7 @@ std::pair<Tensor, optional<Tensor>> attention_kv4(
   L.fp16 = query.scalar_type() == at::kHalf;
   L.max_q = static_cast<int>(std::min(max_query_len, T));
   L.scale = static_cast<float>(sc);
+  L.clear = !out_in.has_value();
   L.err = g_err[dev.index()];
   const long long bytes = kvs_attn4_scratch_bytes(&L);
   Tensor scratch;  // from the caching allocator: a captured graph has its own
