@@ -93,6 +93,13 @@ void on_device(const char* what, const at::Device& dev, std::initializer_list<co
   TORCH_CHECK_VALUE(dev.index() < kMaxDevices, what, ": device index too large");
   if (g_err[dev.index()] == nullptr) throw NoErrorWord("no error word");
 }
+// There is no backward pass: a gradient would be lost without a word.
+void no_gradient(const char* what, std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : ts)
+    TORCH_CHECK_VALUE(t == nullptr || !t->requires_grad(), what,
+                      " has no backward pass: call it under torch.no_grad() or on detached tensors");
+}
 const Tensor* opt(const optional<Tensor>& t) { return t.has_value() ? &*t : nullptr; }
 
 void launched(int rc, const char* what) {
@@ -176,6 +183,8 @@ optional<Tensor> append_kv(const Tensor& cache, const Tensor& key_in, const Tens
     TORCH_CHECK_VALUE(query->size(0) == T, "query has ", query->size(0), " rows, key ", T);
     if (query_out.has_value()) check_out("query_out", *query_out, *query);
   }
+  no_gradient("append_kv",
+              {&cache, &key_in, &value_in, opt(cos_sin), opt(query), opt(query_out)});
   on_device("append_kv", dev,
             {&cache, &value_in, &slot_mapping, opt(positions), opt(cos_sin), opt(query),
              opt(query_out)});
@@ -206,6 +215,7 @@ Tensor read_kv4(const Tensor& cache, const Tensor& slot_mapping, at::ScalarType 
     TORCH_CHECK_VALUE(out_in->sizes() == at::IntArrayRef(shape) && out_in->scalar_type() == dt &&
                           out_in->is_contiguous() && aligned16(*out_in),
                       "out must be a contiguous ", dt, " tensor of ", at::IntArrayRef(shape));
+  no_gradient("read_kv4", {opt(out_in)});
   on_device("read_kv4", dev, {&slot_mapping, opt(out_in)});
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor out = out_in.has_value() ? *out_in : at::empty(shape, cache.options().dtype(dt));
@@ -247,6 +257,7 @@ std::pair<Tensor, optional<Tensor>> attention_kv4(
   const double sc = scale.has_value() ? *scale : 0.08838834764831845;  // 1 / sqrt(128)
   TORCH_CHECK_VALUE(std::isfinite(sc) && sc != 0.0, "scale must be finite and not zero, got ", sc);
   if (out_in.has_value()) check_out("out", *out_in, query);
+  no_gradient("attention_kv4", {&query, opt(out_in)});
   on_device("attention_kv4", dev,
             {&cache, &block_table, &seq_lens, opt(query_start), opt(out_in)});
   const c10::cuda::CUDAGuard guard(dev);

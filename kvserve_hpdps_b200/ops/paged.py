@@ -20,6 +20,8 @@ has the dtype of the keys, values and queries the cache is used with: one
 dtype for the life of a cache.
 
 All functions run on the current CUDA stream and never synchronise the host.
+They have no backward pass and refuse tensors that require a gradient outside
+``torch.no_grad()``.
 Indices that only the device sees (slots, positions, block ids, lengths) are
 checked there: one out of range records ERR_BOUNDS in the device error word
 (:func:`kernels.check_device_error`), and its row, or the part of it that the
