@@ -402,7 +402,7 @@ using namespace kvs;
 extern "C" {
 
 int kvs_append_kv(const AppendLaunch* L, void* stream) {
-  if (L->tokens <= 0 || L->heads <= 0) return 0;
+  if (L->tokens <= 0 || L->q_heads + L->heads <= 0) return 0;
   const Spread S = spread_of(L->tokens, L->q_heads + 2 * L->heads);
   if (S.y > 65535u) return -2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -212,13 +212,16 @@ optional<Tensor> append_kv(const Tensor& cache, const Tensor& key_in, const Tens
   const c10::cuda::CUDAGuard guard(dev);
   if (query.has_value()) {
     src = rows(*query);
-    if (!query_out.has_value()) query_out = at::empty(query->sizes(), query->options());
+    if (!query_out.has_value()) {
+      query_out = at::empty(query->sizes(), query->options());
+      if (n < T) query_out->narrow(0, n, T - n).zero_();
+    }
     L.query = src.data_ptr(), L.query_out = query_out->data_ptr();
     L.q_heads = int_of("query heads", src.size(1));
     L.q_ts = src.stride(0), L.q_hs = src.stride(1);
     L.qo_ts = query_out->stride(0), L.qo_hs = query_out->stride(1);
   }
-  if (n == 0 || H == 0) return query_out;
+  if (n == 0 || H + L.q_heads == 0) return query_out;
   L.err = g_err[dev.index()];
   launched(kvs_append_kv(&L, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "append_kv");
   return query_out;

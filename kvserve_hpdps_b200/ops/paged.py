@@ -110,7 +110,8 @@ def append_kv(cache: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     channels of keys and queries are rotated: channel i with i + rotary_dim/2,
     or 2i with 2i + 1 when ``interleaved``.  Computed in fp32 and rounded once.
     ``query`` ``[T, Hq, 128]``: returned rotated, in ``query_out`` when given
-    (it may be ``query``); rows behind ``n`` are not written.  A position
+    (it may be ``query``); rows behind ``n`` are not written there, and zeros
+    without it.  A position
     outside the table records an error: its token is not appended and its
     query row is returned as it is.  Without ``positions`` nothing is rotated
     and ``query`` must be None.

@@ -125,3 +125,36 @@ def test_starts_out_of_order(rows):
                        tiles=wide)
         _check(out[at], lse[at], ref, dt)
     assert (out[2 * rows:] == 0).all() and (lse[2 * rows:] == -math.inf).all()
+
+
+@pytest.mark.parametrize("n", [0, 1, 13, 20])
+def test_query_rows_behind_the_slots(n):
+    q = torch.randn((20, 3, 128), generator=torch.Generator().manual_seed(n)).to(BF).cuda()
+    kv = torch.zeros((20, 2, 128), dtype=BF, device="cuda")
+    cache = torch.zeros((2, 4, 16, 2, 128), dtype=BF, device="cuda")
+    slots = torch.arange(n, device="cuda")
+    table = torch.rand((64, 128), device="cuda")
+    _dirty(q)
+    out = P.append_kv(cache, kv, kv, slots, slots, table, q)
+    want, _ = O.rotate(q[:n], table, slots, False)
+    assert ((out[:n].double().cpu() - want).abs() <= 2 ** -8 * want.abs() + 2 ** -20).all()
+    assert (out[n:] == 0).all()
+    kept = torch.full_like(q, 9.0)
+    P.append_kv(cache, kv, kv, slots, slots, table, q, query_out=kept)
+    assert torch.equal(kept[:n], out[:n]) and (kept[n:] == 9.0).all()
+
+
+@pytest.mark.parametrize("four", [False, True])
+def test_queries_are_rotated_when_there_are_no_kv_heads(four):
+    """A rank that holds no kv head of its own still gets its queries."""
+    q = torch.randn((5, 3, 128), generator=torch.Generator().manual_seed(3)).to(BF).cuda()
+    kv = torch.zeros((5, 0, 128), dtype=BF, device="cuda")
+    cache = P.kv4_cache(4, 0) if four else torch.zeros((2, 4, 16, 0, 128), dtype=BF, device="cuda")
+    pos = torch.arange(5, device="cuda")
+    table = torch.rand((64, 128), device="cuda")
+    _dirty(q)
+    out = P.append_kv(cache, kv, kv, pos, pos, table, q)
+    K.check_device_error(out.device)
+    want, _ = O.rotate(q, table, pos, False)
+    assert ((out.double().cpu() - want).abs() <= 2 ** -8 * want.abs() + 2 ** -20).all()
+    assert P.append_kv(cache, kv, kv, pos) is None
