@@ -32,7 +32,8 @@ KVS_DEV Seq sequence(const Attn4Launch& L, int r, bool report) {
   }
   s.n = end - s.row0;
   s.len = L.lens[r];
-  const long long cap = static_cast<long long>(L.table_cols) * L.block_size;
+  // what the table has room for, and tokens whose number plus a few steps is an int
+  const long long cap = min(static_cast<long long>(L.table_cols) * L.block_size, 0x7FFF0000ll);
   s.bad = s.row0 < 0 || end < s.row0 || end > L.tokens || s.n > L.max_q || s.len < 0 ||
           s.len > cap;
   if (s.bad) {

@@ -139,8 +139,8 @@ def attention_kv4(query: torch.Tensor, cache: torch.Tensor, block_table: torch.T
     """Causal attention of ``query`` ``[T, Hq, 128]`` over a 4-bit cache.
 
     ``block_table`` int32 ``[R, columns]``: block ids of each sequence;
-    ``seq_lens`` int32 ``[R]``: tokens of it in the cache, those of the query
-    rows among them (append first).  ``query_start`` int32 ``[R + 1]``: sequence r's
+    ``seq_lens`` int32 ``[R]``: tokens of it in the cache (up to 2^31 - 2^16), those
+    of the query rows among them (append first).  ``query_start`` int32 ``[R + 1]``: sequence r's
     query rows are ``query_start[r]..query_start[r + 1]``, at most
     ``max_query_len`` of them; row i of n sees the first
     ``seq_lens[r] - n + i + 1`` tokens.  Without it sequence r has the one row

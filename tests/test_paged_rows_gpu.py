@@ -158,3 +158,20 @@ def test_queries_are_rotated_when_there_are_no_kv_heads(four):
     want, _ = O.rotate(q, table, pos, False)
     assert ((out.double().cpu() - want).abs() <= 2 ** -8 * want.abs() + 2 ** -20).all()
     assert P.append_kv(cache, kv, kv, pos) is None
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_lengths_that_ints_cannot_walk(rows):
+    """A table wide enough for 2^31 tokens; a length near that is refused as one that does not fit."""
+    q = torch.ones((rows, 4, 128), dtype=BF, device="cuda")
+    cache = P.kv4_cache(2, 2)
+    table = torch.zeros((1, 2 ** 27), dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, rows]).int().cuda()
+    for n in (2 ** 31 - 1, 2 ** 31 - 2 ** 16 + 1):
+        out, lse = _call((q, cache, table, torch.tensor([n]).int().cuda(), start), rows)
+        assert K.read_device_error(out.device) == 3
+        assert (out == 0).all() and (lse == -math.inf).all()
+    out, lse = _call((q, cache, table, torch.tensor([rows + 9]).int().cuda(), start), rows)
+    K.check_device_error(out.device)
+    seen = torch.arange(10, 10 + rows).double()[:, None].log().expand(rows, 4)
+    assert (out == 0).all() and ((lse.double().cpu() - seen).abs() < 2 ** -18).all()
