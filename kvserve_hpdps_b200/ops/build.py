@@ -9,8 +9,9 @@ library also loads on machines without a GPU driver (its CPU codec then
 works and its device entry points return errors).
 
 ``csrc/torch/*.cpp`` (host code that takes torch tensors) is compiled against
-this interpreter's torch into a second module, ``_paged_ops.so``, linked to
-the library next to it.
+this interpreter's torch into a second module, ``_paged_ops`` with the
+interpreter's suffix, linked to the library next to it.  Without a torch for
+CUDA it is left out, with a warning: the library does not need one.
 
 Usage: ``python -m kvserve_hpdps_b200.ops.build [-v] [--force]``.
 Objects go to ``ops/_build/``; rebuilding is incremental on file mtimes.
@@ -25,6 +26,8 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
+import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -32,7 +35,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB_NAME = "libkvs_b200.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 BIND_NAME = "_paged_ops"
-BIND_PATH = os.path.join(HERE, BIND_NAME + ".so")
+BIND_PATH = os.path.join(HERE, BIND_NAME + sysconfig.get_config_var("EXT_SUFFIX"))
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -73,20 +76,31 @@ def _compile(src: str, obj: str, cuda: str, verbose: bool) -> tuple[str, str]:
     return src, (res.stdout + res.stderr)
 
 
+def _no_bindings() -> str | None:
+    """Why the torch module cannot be built here; None if it can."""
+    try:
+        import torch
+    except ImportError as e:
+        return f"torch cannot be imported ({e})"
+    if torch.version.cuda is None:
+        return f"torch {torch.__version__} is not built for CUDA"
+    return None
+
+
 def _build_bindings(jobs: int, force: bool) -> str:
     """Compile csrc/torch/*.cpp against torch and link it to the library."""
-    import sysconfig
-
     import torch
     from torch.utils import cpp_extension
     srcs = sorted(glob.glob(os.path.join(CSRC, "torch", "*.cpp")))
     deps = _headers()
     objs, todo = [], []
     flags = [f"-DTORCH_EXTENSION_NAME={BIND_NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             f'-DKVS_TORCH_VERSION="{torch.__version__}"',
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     incs = cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"]]
+    made_for = f"{torch.__version__}_{sysconfig.get_config_var('SOABI')}"
     for src in srcs:
-        obj = os.path.join(BUILD, f"torch_{torch.__version__}_{os.path.basename(src)}.o")
+        obj = os.path.join(BUILD, f"torch_{made_for}_{os.path.basename(src)}.o")
         objs.append(obj)
         if force or _stale(obj, src, deps):
             todo.append(["g++", "-O2", "-fPIC", "-std=c++17", "-fvisibility=hidden", *flags,
@@ -98,7 +112,14 @@ def _build_bindings(jobs: int, force: bool) -> str:
             raise RuntimeError(f"failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
         list(ex.map(run, todo))
-    if todo or not os.path.exists(BIND_PATH) or any(
+    # What the module was linked for: an older object of another torch is no newer than it.
+    stamp = os.path.join(BUILD, BIND_NAME + ".made_for")
+    if os.path.exists(stamp):
+        with open(stamp) as f:
+            last = f.read()
+    else:
+        last = None
+    if todo or last != made_for or not os.path.exists(BIND_PATH) or any(
             os.path.getmtime(o) > os.path.getmtime(BIND_PATH) for o in objs):
         libdir = cpp_extension.library_paths("cuda")[0]
         tmp = BIND_PATH + ".tmp"
@@ -106,11 +127,12 @@ def _build_bindings(jobs: int, force: bool) -> str:
              "-Wl,-rpath,$ORIGIN", f"-L{libdir}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
              "-ltorch_cuda", "-ltorch", "-ltorch_python"])
         os.replace(tmp, BIND_PATH)
+        with open(stamp, "w") as f:
+            f.write(made_for)
     return BIND_PATH
 
 
-def build(verbose: bool = False, force: bool = False, jobs: int | None = None) -> str:
-    """Compile and link; returns the library path."""
+def _build_library(verbose: bool, force: bool, jobs: int | None) -> None:
     cuda = _cuda_home()
     os.makedirs(BUILD, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cpp")))
@@ -138,7 +160,16 @@ def build(verbose: bool = False, force: bool = False, jobs: int | None = None) -
         if res.returncode != 0:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB_PATH)
-    _build_bindings(jobs or min(8, os.cpu_count() or 4), force)
+
+
+def build(verbose: bool = False, force: bool = False, jobs: int | None = None) -> str:
+    """Compile and link; returns the library path."""
+    _build_library(verbose, force, jobs)
+    why = _no_bindings()
+    if why is None:
+        _build_bindings(jobs or min(8, os.cpu_count() or 4), force)
+    else:
+        warnings.warn(f"built without the paged-cache operators: {why}", stacklevel=2)
     return LIB_PATH
 
 

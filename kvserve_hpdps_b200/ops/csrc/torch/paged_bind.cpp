@@ -328,6 +328,7 @@ std::pair<Tensor, optional<Tensor>> attention_kv4(
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   py::register_exception<NoErrorWord>(m, "NoErrorWord");
+  m.attr("torch_version") = KVS_TORCH_VERSION;
   m.def("set_error_word", [](int64_t device, int64_t ptr) {
     TORCH_CHECK_VALUE(device >= 0 && device < kMaxDevices, "device index out of range");
     g_err[device] = reinterpret_cast<uint32_t*>(ptr);

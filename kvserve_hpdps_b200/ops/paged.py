@@ -52,6 +52,10 @@ def _native():
         except ImportError as e:
             raise RuntimeError(f"native module _paged_ops cannot be loaded ({e}); build it with "
                                "`python -m kvserve_hpdps_b200.ops.build`") from e
+        if _paged_ops.torch_version != torch.__version__:
+            raise RuntimeError(f"native module _paged_ops is built for torch "
+                               f"{_paged_ops.torch_version}, this is {torch.__version__}; build it "
+                               "again with `python -m kvserve_hpdps_b200.ops.build`")
         _ops = _paged_ops
     return _ops
 
