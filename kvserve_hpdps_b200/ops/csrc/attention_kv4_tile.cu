@@ -6,8 +6,8 @@
 //   S = Q K^T, O += P V, fp16 products of 128 rows and 64 tokens into tensor memory.
 // K and V become fp16 with one power of two for each 32 tokens, chosen from
 // the largest step and mid among them; the power goes into the softmax's factor (K) and, where it
-// is not the largest that the row has seen, into the weights (V), a row's O being kept in units of
-// that one.  Where 32 tokens' scales are more than 2^kApart apart, each takes its own power: else
+// is not the largest that the row has seen, into the exponentials (V), a row's O being kept in units
+// of that one.  Where 32 tokens' scales are more than 2^8 apart, each takes its own power: else
 // a large token would take the small ones' bits from the rows that do not see it.  K's tile
 // holds step (code - 8) alone; mid times the sum of the group's query elements is 16 more columns
 // of the product: that sum in three fp16 parts against mid three times.
@@ -58,14 +58,16 @@ constexpr int kLeastTile = 2;    // steps a CTA takes at least
 constexpr float kAbove = 7.f;
 constexpr float kMostSum = 32768.f;  // of 64 weights, without a new maximum (fp16 ends at 65504)
 constexpr int kHalfTile = 16384; // 128 rows x 64 channels of fp16
-// Tokens (of 32) whose scales are further apart than 2^kApart take a scale each: a row may see only
+// Tokens (of 32) with scales less than kApart of the largest take a scale each: a row may see only
 // the small ones, or need their bits.
-constexpr uint32_t kApart = 8;
+constexpr float kApart = 0x1p-8f;
 constexpr uint32_t kHides = 1, kWideK = 2, kWideV = 4;
+constexpr int kFar = 60;
 // A score is a factor times 128 products of less than 2^15 and 2^11.  Where the factor lets it pass
-// 2^20, the product is rounded before the maximum is taken off: the fused multiply-add leaves
-// the maximum's own rounding over, which is 2^-24 of the score and no longer small.
-constexpr float kHuge = 0x1p-13f;
+// 2^27, the product is rounded before the maximum is taken off: the fused multiply-add leaves the
+// maximum's own rounding over, up to 2^-25 of it, and weights are 2 to that from where they should be
+// (the same for all of a row's, so that 2^4 does no harm).
+constexpr float kHuge = 0x1p-6f;
 
 struct Ctrl {
   uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
@@ -77,8 +79,8 @@ struct Ctrl {
   uint32_t gone[4][4];     // tokens whose block does not exist
   uint32_t bad[4][4][4];   // [..][group] tokens with a step or mid of V that is not finite
   uint32_t flags[4][4];    // kHides: any of the two is set; kWideK, kWideV: a scale each token,
-  float k_tok[4][kTile];   //   in the place of k_up
-  int v_tok[4][kTile];     //   and v_exp
+  float k_tok[4][kTile];   //   in the place of k_up,
+  float v_tok[4][kTile];   //   and 2^v_exp
   long long scan[kThreads / 32];
   int2 named[kThreads / 32];
   long long begin;
@@ -381,7 +383,8 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
       const uint32_t lost = __ballot_sync(0xFFFFFFFFu, gone);
       if (j + 1 < p.steps) locate(j + 1);  // its loads go out as registers become free
       // exponent of the largest finite step or mid of the warp's 32 tokens, or of each one's
-      float up[2];
+      float up[2], down[2];
+      int exps[2];
       uint32_t bad[NG], wide = 0;
       const int ring = step_no & 3;
 #pragma unroll
@@ -399,29 +402,24 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
             if (!fine) meta[v][gr] = 0;  // rows that see it are marked instead
           }
         }
-        const uint32_t own = __float_as_uint(h2f<FP16>(top));
-        uint32_t most = __reduce_max_sync(0xFFFFFFFFu, own);
-        const uint32_t least = __reduce_min_sync(0xFFFFFFFFu, own ? own : most);
-        const bool apart = (most >> 23) - (least >> 23) > kApart;
-        if (apart) {
+        const float own = h2f<FP16>(top);
+        float most = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(own)));
+        if (__any_sync(0xFFFFFFFFu, own < most * kApart && own != 0.f)) {
           wide |= v ? kWideV : kWideK;
           most = own;
         }
         // in steps of 16, so that V's powers seldom differ; K of zeros gets any
-        int e = max(static_cast<int>(most >> 23) - 127, kLowestExp);
-        e = (v == 0 && most == 0 ? 0 : (e + 3) & ~3) - 7;
+        int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, kLowestExp);
+        e = (v == 0 && most == 0.f ? 0 : (e + 3) & ~3) - 7;
         up[v] = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        const float down = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-        if (apart) {
-          if (v == 0) C->k_tok[ring][row] = down;
-          else C->v_tok[ring][row] = e;
-        }
-        if (lane == 0) {  // not looked at where they are apart
-          if (v == 0) C->k_up[ring][seg] = down;
-          else C->v_exp[ring][seg] = e;
-        }
+        down[v] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        exps[v] = e;
       }
-      if (wide) __syncwarp();
+      if (wide) {
+        C->k_tok[ring][row] = down[0];
+        C->v_tok[ring][row] = down[1];
+        __syncwarp();
+      }
       if (lane == 0) {
         uint32_t any = lost;
 #pragma unroll
@@ -429,6 +427,8 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
           C->bad[ring][seg][gr] = bad[gr];
           any |= bad[gr];
         }
+        C->k_up[ring][seg] = down[0];  // where they are apart, nobody takes these two
+        C->v_exp[ring][seg] = exps[1];
         C->gone[ring][seg] = lost;
         C->flags[ring][seg] = (any ? kHides : 0u) | wide;
         mbar_arrive(&C->e_full[ring]);
@@ -609,7 +609,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
     const int hq = p.h * group + rr % group;
     const int seen = mine ? p.s.len - p.s.n + rr / group + 1 : 0;
     float m = kLowest, l = 0.f, f = 0.f;
-    int E = kLowestExp, E_low = kLowestExp;  // of this row, the warp's lowest
+    int E = kLowestExp;  // of this row's units
     uint32_t poison = 0;
     if (p.steps > 0) {
       // ---- the row as fp16, scaled by a power of two: largest element in [2^14, 2^15)
@@ -662,9 +662,12 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
       fence_proxy_async_smem();
       __syncwarp();
       if ((threadIdx.x & 31) == 0) mbar_arrive(&C->q_full[x]);
-      const float f_most = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(f)));
+      // of the keys' scale, for scores that the exponentials take as they are
+      const float up_most =
+          kHuge / __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(f)));
       // tokens that every row of this warp sees
       const int all_see = __reduce_min_sync(0xFFFFFFFFu, mine ? max(seen, 0) : 0x7FFFFFFF);
+      const int plain_to = min(all_see, p.stop);
       // what the converting warps say of half i's tokens, read a half ahead
       struct {
         uint32_t flag;
@@ -721,8 +724,8 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
           return v & ~C->gone[ring][seg0 + sg];
         };
         bool raise;
-        const bool huge = f_most * fmaxf(said_up[0], said_up[1]) > kHuge;
-        if (t0 + 64 > min(all_see, p.stop) || flag != 0 || huge) {  // hidden scores become -inf
+        const bool huge = fmaxf(said_up[0], said_up[1]) > up_most;
+        if (t0 + 64 > plain_to || flag != 0 || huge) {  // hidden scores become -inf
 #pragma unroll
           for (int sg = 0; sg < 2; ++sg) {
             const uint32_t vis = visible(sg), what = flag ? C->flags[ring][seg0 + sg] : 0u;
@@ -747,10 +750,11 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
             }
             // values that the row does not see have no say in its units
             if (what & kWideV) {
-              v_exp[sg] = kLowestExp;
+              float most = 0.f;
 #pragma unroll 4
               for (int k = 0; k < 32; ++k)
-                if (vis >> k & 1u) v_exp[sg] = max(v_exp[sg], C->v_tok[ring][32 * (seg0 + sg) + k]);
+                if (vis >> k & 1u) most = fmaxf(most, C->v_tok[ring][32 * (seg0 + sg) + k]);
+              v_exp[sg] = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, kLowestExp);
             } else if (vis == 0) {
               v_exp[sg] = kLowestExp;
             }
@@ -796,27 +800,43 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
             m = m_new;
             E = e_new;
           }
+          // Tokens whose V is in units smaller by 2^d than O's weigh less by that, which their sum
+          // gets back; more than kFar is nothing beside O.
+          const int d[2] = {huge ? 0 : min(E - v_exp[0], kFar),  // lost beside a huge m
+                            huge ? 0 : min(E - v_exp[1], kFar)};
           // four sums: one would be a chain as long as the row
           f32x2_t s2[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) s2[k] = f2_pack(0.f, 0.f);
-          const f32x2_t ref2 = f2_pack(-m, -m);
+          float refs[2] = {-m, -m};
+          if ((d[0] | d[1]) != 0) {
+            refs[0] -= static_cast<float>(d[0]);
+            refs[1] -= static_cast<float>(d[1]);
+          }
 #pragma unroll
           for (int sg = 0; sg < 2; ++sg) {
-            const f32x2_t fs2 = f2_pack(fs[sg], fs[sg]);
+            const f32x2_t fs2 = f2_pack(fs[sg], fs[sg]), ref2 = f2_pack(refs[sg], refs[sg]);
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               float u0, u1;
               f2_unpack(f2_fma(f2_pack(__uint_as_float(v[sg][2 * k]),
                                        __uint_as_float(v[sg][2 * k + 1])), fs2, ref2), u0, u1);
               const float p0 = ex2(u0), p1 = ex2(u1);
-              s2[k & 3] = f2_add(s2[k & 3], f2_pack(p0, p1));
+              f32x2_t& part = s2[2 * sg + (k & 1)];
+              part = f2_add(part, f2_pack(p0, p1));
               h[sg][k] = half2_bits(p0, p1);
             }
           }
-          float s0, s1;
-          f2_unpack(f2_add(f2_add(s2[0], s2[1]), f2_add(s2[2], s2[3])), s0, s1);
-          sum = s0 + s1;
+          float s0, s1, s2a, s2b;
+          f2_unpack(f2_add(s2[0], s2[1]), s0, s1);
+          f2_unpack(f2_add(s2[2], s2[3]), s2a, s2b);
+          s0 += s1;
+          s2a += s2b;
+          if ((d[0] | d[1]) != 0) {
+            s0 *= __uint_as_float(static_cast<uint32_t>(127 + d[0]) << 23);
+            s2a *= __uint_as_float(static_cast<uint32_t>(127 + d[1]) << 23);
+          }
+          sum = s0 + s2a;
           if (fresh) break;
           ready = __all_sync(0xFFFFFFFFu, ahead != 0 && !(sum > kMostSum));
           if (ready || !__any_sync(0xFFFFFFFFu, sum > kMostSum)) break;
@@ -830,28 +850,25 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         tc_fence_after();
         if (next) listen(i + 1);
         s_ready = next ? peek_phase(&C->s_full[x], (half_no + 1) & 1) : 0u;
+        if (flag & kWideV || huge) {
 #pragma unroll
-        for (int sg = 0; sg < 2; ++sg) {
-          const int down = E - v_exp[sg];
-          if (flag & kWideV && C->flags[ring][seg0 + sg] & kWideV) {
-            const int* const exps = C->v_tok[ring] + 32 * (seg0 + sg);
+          for (int sg = 0; sg < 2; ++sg) {
+            const bool each = flag & kWideV && C->flags[ring][seg0 + sg] & kWideV;
+            const int from = huge ? E : v_exp[sg];  // what the exponentials did not do
+            const float unit = __uint_as_float(static_cast<uint32_t>(127 - from) << 23),
+                        one = ex2(static_cast<float>(v_exp[sg] - from));
+            const float* const tok = C->v_tok[ring] + 32 * (seg0 + sg);
 #pragma unroll
             for (int k = 0; k < 16; ++k) {  // those that the row does not see weigh nothing
-              const __half2 g = __floats2half2_rn(ex2(static_cast<float>(min(exps[2 * k] - E, 0))),
-                                                  ex2(static_cast<float>(min(exps[2 * k + 1] - E, 0))));
-              const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h[sg][k]), g);
-              h[sg][k] = *reinterpret_cast<const uint32_t*>(&y);
-            }
-          } else if (down != 0) {  // these tokens' V is in smaller units than O
-            const __half2 g = __float2half2_rn(ex2(static_cast<float>(-down)));
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
+              const __half2 g = __floats2half2_rn(each ? fminf(tok[2 * k] * unit, 1.f) : one,
+                                                  each ? fminf(tok[2 * k + 1] * unit, 1.f) : one);
               const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h[sg][k]), g);
               h[sg][k] = *reinterpret_cast<const uint32_t*>(&y);
             }
           }
-          tmem_st16(W + 16 * sg, h[sg]);
         }
+        tmem_st16(W, h[0]);
+        tmem_st16(W + 16, h[1]);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();

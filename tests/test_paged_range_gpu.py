@@ -123,3 +123,38 @@ def test_many_rows_small_weights_beside_a_large_one(dt):
         assert ((out[:, head].double().cpu() - want).abs() <= tol).all()
         off = (out[:, head].double().cpu() - want).norm() / want.norm()
         assert off <= 2 * O.half_step(dt)
+
+
+@pytest.mark.parametrize("mag", [1.0, 1e8, 1e16])
+@pytest.mark.parametrize("rows", [1, 60])
+def test_equal_scores_of_any_size_over_values_of_many_scales(rows, mag):
+    """Equal keys, scores of 10, 1e17 and 1e33; values of 2^0, 2^-6, 2^-30 and 0 by 32 tokens, or
+    by token: every token weighs the same, so that a row is the mean of what it sees."""
+    hq, h, bs, dt, length = 8, 2, 16, BF, 400
+    g = _gen(rows + 50)
+    cols = -(-length // bs)
+    tiles = rows == 60
+    table = torch.full((1, cols + (_wide(rows, 1, hq, h) if tiles else 0)), -7, dtype=torch.int32)
+    table[0, :cols] = torch.arange(cols).int()
+    start, lens = torch.tensor([0, rows]).int(), torch.tensor([length]).int()
+    q = (mag * (0.5 + torch.rand((rows, hq, 128), generator=g))).to(dt)
+    codes, step, mid = O.unpack(_cache4(cols, h, bs, 64, dt, g, spread=0.0), dt)
+    step[0], mid[0] = 0, mag
+    token = torch.arange(cols * bs).view(cols, 1, bs, 1)
+    for each in (token // 32, token * 7 // 5):
+        by = torch.tensor([1.0, 2.0 ** -6, 2.0 ** -30, 0.0], dtype=torch.float64)[each % 4]
+        s, m = step.clone(), mid.clone()
+        s[1], m[1] = (step[1].double() * by).to(dt), (mid[1].double() * by).to(dt)
+        cache = O.pack(codes, s, m)
+        out = P.attention_kv4(q.cuda(), cache.cuda(), table.cuda(), lens.cuda(), start.cuda(), rows)
+        torch.cuda.synchronize()
+        K.check_device_error(out.device)
+        x = O.values(cache, dt)[0][1].transpose(0, 1).flatten(1, 2)
+        for i in range(rows):
+            v = x[:, :length - rows + i + 1].repeat_interleave(hq // h, 0)
+            want, size = v.mean(1), v.abs().mean(1)
+            # weights and values to fp16 (those 2^-30 below go under: 2^-24 of the largest),
+            # the output's own rounding, fp32's sums
+            tol = (2 ** -10 + 2 ** -17) * size + 2 ** -24 * v.abs().amax((1, 2))[:, None]
+            tol = tol + O.half_step(dt) * (want.abs() + tol)
+            assert ((out[i].double().cpu() - want).abs() <= tol).all()
