@@ -501,13 +501,6 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
       }
     }
   }
-  // The last products' commits arrive on their own: not after the CTA has gone.
-  for (uint32_t back = FP16 ? 1 : 2; back > 0; --back) {
-    if (step_no < back) continue;
-    const uint32_t no = step_no - back, slot = slot_of<FP16>(no, seg >> 1);
-    if (!KVS_WAIT(&C->k_empty[slot], phase_of<FP16>(no))) return;
-    if (!KVS_WAIT(&C->v_empty[slot], phase_of<FP16>(no))) return;
-  }
 }
 
 // ------------------------------------------------------ matrix instructions
@@ -585,6 +578,11 @@ KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, int x, uint32_
     // the last half's scores were taken, too: one phase of s_free a half
     if (QK && !idle && !KVS_WAIT(&C->s_free[x], (half_no - 1) & 1)) return;
     step_no += p.steps;
+  }
+  // The last products' commits arrive on their own: not after the CTA has gone.
+  for (uint32_t back = 1; back < 3 && step_no >= (FP16 ? 1 : back); ++back) {
+    const uint32_t no = step_no - (FP16 ? 1 : back), slot = slot_of<FP16>(no, back & 1);
+    if (!KVS_WAIT(QK ? &C->k_empty[slot] : &C->v_empty[slot], phase_of<FP16>(no))) return;
   }
 }
 
@@ -726,37 +724,41 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         bool raise;
         const bool huge = fmaxf(said_up[0], said_up[1]) > up_most;
         if (t0 + 64 > plain_to || flag != 0 || huge) {  // hidden scores become -inf
+          if (flag & kWideK || huge) {
+#pragma unroll
+            for (int sg = 0; sg < 2; ++sg) {
+              const float* const up = C->k_tok[ring] + 32 * (seg0 + sg);
+              if (C->flags[ring][seg0 + sg] & kWideK) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  v[sg][k] = __float_as_uint(__uint_as_float(v[sg][k]) * (f * up[k]));
+                fs[sg] = 1.f;
+              } else if (huge) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  v[sg][k] = __float_as_uint(__fmul_rn(__uint_as_float(v[sg][k]), fs[sg]));
+                fs[sg] = 1.f;
+              }
+            }
+          }
 #pragma unroll
           for (int sg = 0; sg < 2; ++sg) {
-            const uint32_t vis = visible(sg), what = flag ? C->flags[ring][seg0 + sg] : 0u;
-            if (what & kWideK) {
-              const float* const up = C->k_tok[ring] + 32 * (seg0 + sg);
-#pragma unroll
-              for (int k = 0; k < 32; ++k)
-                v[sg][k] = __float_as_uint(__uint_as_float(v[sg][k]) * (f * up[k]));
-              fs[sg] = 1.f;
-            } else if (huge) {
-#pragma unroll
-              for (int k = 0; k < 32; ++k)
-                v[sg][k] = __float_as_uint(__fmul_rn(__uint_as_float(v[sg][k]), fs[sg]));
-              fs[sg] = 1.f;
-            }
+            const uint32_t vis = visible(sg);
 #pragma unroll
             for (int k = 0; k < 32; ++k) v[sg][k] = vis >> k & 1u ? v[sg][k] : 0xFF800000u;
+            // values that the row does not see have no say in its units
+            if (vis == 0) v_exp[sg] = kLowestExp;
             if (flag) {
 #pragma unroll
               for (int gr = 0; gr < NG; ++gr)
                 if (C->bad[ring][seg0 + sg][gr] & vis) poison |= 1u << gr;
-            }
-            // values that the row does not see have no say in its units
-            if (what & kWideV) {
-              float most = 0.f;
+              if (C->flags[ring][seg0 + sg] & kWideV) {
+                float most = 0.f;
 #pragma unroll 4
-              for (int k = 0; k < 32; ++k)
-                if (vis >> k & 1u) most = fmaxf(most, C->v_tok[ring][32 * (seg0 + sg) + k]);
-              v_exp[sg] = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, kLowestExp);
-            } else if (vis == 0) {
-              v_exp[sg] = kLowestExp;
+                for (int k = 0; k < 32; ++k)
+                  if (vis >> k & 1u) most = fmaxf(most, C->v_tok[ring][32 * (seg0 + sg) + k]);
+                v_exp[sg] = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, kLowestExp);
+              }
             }
           }
         }
