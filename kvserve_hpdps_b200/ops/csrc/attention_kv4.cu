@@ -695,23 +695,24 @@ Grid grid_of(const Attn4Launch* L) {
   return g;
 }
 
-// Whether a call goes to attention_kv4_tile.cu: many rows a kv head, and enough of them.
-// Measured, us here / there, bf16, groups of 64: 32 sequences of 2000 tokens, 8 heads: 48
-// rows 98 / 103, 52 rows 121 / 104; 16 of 2000: 48 rows 58 / 59, 64 rows 71 / 61, 96 rows
-// 97 / 64; 8 of 8000, 4 heads: 42 rows 51 / 53, 56 rows 63 / 54; 64 of 1000, 4 heads: 42 rows
-// 70 / 72, 56 rows 85 / 74.
+// Whether a call goes to attention_kv4_tile.cu: many rows a kv head, and enough of them by what the
+// host knows (max_query_len, and the tokens that the table has room for; tables as wide as the
+// sequences below).  fp16 caches, whose tiles take twice the conversion there, from more rows on.
+// Measured, us here / there for bf16 and for fp16, groups of 64: 32 sequences of 2000 tokens,
+// 8 heads: 48 rows 99 / 97 and 99 / 175, 80 rows 153 / 103 and 153 / 178; 16 of 2000: 64 rows
+// 72 / 58 and 72 / 93, 96 rows 99 / 62 and 99 / 96; 8 of 8000, 4 heads: 56 rows 61 / 51 and 61 / 80,
+// 84 rows 86 / 55 and 86 / 82; 64 of 1000, 4 heads: 84 rows 122 / 78 and 123 / 114.
 // With little to do the tiles' fixed cost decides (Mi rows times tokens times heads): one of
-// 1024 tokens, 4 heads: 448 rows (1.8 Mi) 22 / 35, 896 rows (3.5 Mi) 31 / 39, 1792 rows (7 Mi)
-// 41 / 41; one of 4000, 8 heads: 128 rows (3.9 Mi) 27 / 33, 192 rows (5.9 Mi) 41 / 41; 4 of
-// 2000: 64 rows (3.9 Mi) 29 / 29, 96 rows (5.9 Mi) 37 / 33; 8 of 2000: 52 rows (6.3 Mi) 44 / 39.
-// Many short ones lose a little there: 64 of 200, 8 heads: 64 rows (6.2 Mi) 58 / 63.
-constexpr int kManyRows = 48;
+// 1024 tokens, 4 heads: 1792 rows (7 Mi) 43 / 37 and 43 / 40; 8 of 2000, 8 heads: 52 rows (6.3 Mi)
+// 43 / 37; 4 of 2000: 96 rows (5.9 Mi) 36 / 32 and 36 / 40.  One long sequence on many heads
+// loses there: one of 4000, 8 heads: 192 rows (5.9 Mi) 32 / 40 and 32 / 44.
+constexpr int kManyRows = 48, kManyRowsFp16 = 80;
 constexpr long long kMuchWork = 5ll << 20;
 bool many_rows(const Attn4Launch* L) {
   const long long rows = static_cast<long long>(L->max_q) * (L->q_heads / L->heads);
   const double work = static_cast<double>(rows) * L->seqs * L->heads * L->table_cols *
                       L->block_size;
-  return rows > kManyRows && work > static_cast<double>(kMuchWork);
+  return rows > (L->fp16 ? kManyRowsFp16 : kManyRows) && work > static_cast<double>(kMuchWork);
 }
 
 template <bool FP16, int NG, int NT>
