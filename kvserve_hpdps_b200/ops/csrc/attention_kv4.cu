@@ -12,10 +12,17 @@
 // (and a shift for every second pair): the integer pipe, which has half the
 // rate, shares the work with the floating-point one.  Products with the
 // power-of-two scaled query are then exact and sums are fp32, so scores are
-// as good as fp32's.  For the output the one rounding is that of w to fp16,
-// relative 2^-11.  (Codes taken as fp16 subnormals by the AND alone cost one
+// as good as fp32's.  (Codes taken as fp16 subnormals by the AND alone cost one
 // instruction less, but sums are aligned to the operands' exponent fields, so
 // they lose the bits that a subnormal has in front of its first one.)
+//
+// The one rounding to fewer bits is that of w to fp16, the matrix
+// instructions' type: 2^-11 relative, an eighth of a bf16 output's own.  An fp16
+// output would lose by it (errors 1.1 to 1.55 times those of fp32 arithmetic), so for fp16
+// caches w is two fp16 parts and V's product is taken with both (16 x 5 rows
+// 54 -> 61 us, 48 ragged sequences 67 -> 74).  Weights share a row's exponent: a
+// channel group whose steps are 2^-14 of the largest step or mid that the row
+// has seen is in fp16's subnormals and keeps 2^-25 of that one.
 //
 // Why mma.sync and not tcgen05 for few query rows: tcgen05 reads its operands
 // from shared or tensor memory, so every code would be written there as 16
@@ -531,7 +538,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
         for (int gr = 0; gr < NG; ++gr) {
           const float s0 = h2f<FP16>(vm[hf][0][gr] & 0xFFFFu), z0 = h2f<FP16>(vm[hf][0][gr] >> 16);
           const float s1 = h2f<FP16>(vm[hf][1][gr] & 0xFFFFu), z1 = h2f<FP16>(vm[hf][1][gr] >> 16);
-          uint32_t b0[NT], b1[NT];
+          uint32_t b0[NT], b1[NT], rest0[NT], rest1[NT];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float w[4];
@@ -547,8 +554,15 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
                 ms = fmaf(p[nt][i], i < 2 ? z0 : z1, ms);
               }
             }
-            b0[nt] = transpose8(half2_bits(w[0], w[1]));
-            b1[nt] = transpose8(half2_bits(w[2], w[3]));
+            const uint32_t lo = half2_bits(w[0], w[1]), hi = half2_bits(w[2], w[3]);
+            b0[nt] = transpose8(lo);
+            b1[nt] = transpose8(hi);
+            if constexpr (FP16) {  // what the rounding leaves over
+              rest0[nt] = transpose8(half2_bits(w[0] - h2f<true>(lo & 0xFFFFu),
+                                                w[1] - h2f<true>(lo >> 16)));
+              rest1[nt] = transpose8(half2_bits(w[2] - h2f<true>(hi & 0xFFFFu),
+                                                w[3] - h2f<true>(hi >> 16)));
+            }
           }
 #pragma unroll
           for (int q = gr * 4 / NG; q < (gr + 1) * 4 / NG; ++q) {
@@ -564,6 +578,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
               mma16816(acc[2 * q + 1][nt], u[1], u[3], v[1], v[3], b0[nt], b1[nt]);
+            if constexpr (FP16) {
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816(acc[2 * q][nt], u[0], u[2], v[0], v[2], rest0[nt], rest1[nt]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816(acc[2 * q + 1][nt], u[1], u[3], v[1], v[3], rest0[nt], rest1[nt]);
+            }
           }
         }
       }

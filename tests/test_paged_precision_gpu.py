@@ -69,3 +69,38 @@ def test_scores_are_those_of_fp32(dt, g_size, mids, size):
         # add up to less than the output's own; twice half a step leaves room for both
         off = (got - want).norm() / want.norm()
         assert off <= 2 * O.half_step(dt)
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("g_size", [32, 64, 128])
+@pytest.mark.parametrize("rows,length", [(1, 900), (1, 40), (7, 500)])
+def test_few_rows_weights(dt, g_size, rows, length):
+    """The kernel for few rows: in bf16 caches weights times steps are fp16, 2^-11 of p |v - mid|; in
+    fp16 ones two parts of fp16, which leave 2^-22 at most."""
+    g = torch.Generator().manual_seed(g_size + rows)
+    hq, h, bs, ng = 8, 2, 16, 128 // g_size
+    nb = -(-length // bs)
+    codes = torch.randint(0, 16, (2, nb, h, bs, 128), generator=g)
+    step = (0.1 + 0.1 * torch.rand((2, nb, h, bs, ng), generator=g)).to(dt)
+    mid = (0.1 * torch.randn((2, nb, h, bs, ng), generator=g)).to(dt)
+    cache = O.pack(codes, step, mid)
+    table = torch.randperm(nb, generator=g).int()[None]
+    q = torch.randn((rows, hq, 128), generator=g).to(dt)
+    out, lse = P.attention_kv4(q.cuda(), cache.cuda(), table.cuda(),
+                               torch.tensor([length]).int().cuda(),
+                               torch.tensor([0, rows]).int().cuda(), rows, return_lse=True)
+    torch.cuda.synchronize()
+    K.check_device_error(out.device)
+    x, mids, _ = O.values(cache, dt)
+    x, mids = (y[:, table[0].long()].permute(0, 2, 1, 3, 4).flatten(2, 3) for y in (x, mids))
+    seen = length - rows + 1 + torch.arange(rows)
+    for head in range(hq):
+        k, v = x[0, head // 4, :length], x[1, head // 4, :length]
+        want, z, pv, werr = one_head(q[:, head], k, v, seen, 1 / math.sqrt(128))
+        dev = one_head(q[:, head], k, v - mids[1, head // 4, :length], seen, 1 / math.sqrt(128))[2]
+        got, l = out[:, head].double().cpu(), lse[:, head].double().cpu()
+        assert ((l - z).abs() <= werr + 2 ** -20 * (1 + z.abs())).all()
+        tol = (2 ** -11 * dev if dt == BF else 2 ** -22 * dev) + (2 ** -17 + 2 * werr[:, None]) * pv
+        # steps far below the largest, 2^-24 of it times 8 a weight: none here
+        tol = tol + O.half_step(dt) * (want.abs() + tol) + 2 ** -25
+        assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
