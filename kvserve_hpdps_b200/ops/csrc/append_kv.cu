@@ -12,7 +12,10 @@
 //   step = T((max - min) (1 / 15)), mid = T(min + 8 step),
 //   code = clamp(floor((x - mid) * (1 / step) + 8.5), 0, 15),
 // T being the 16-bit type.  Codes are taken against the rounded (step, mid):
-// the pair that readers use.
+// the pair that readers use.  The product with the rounded 1 / 15 is within
+// 2^-23 of the quotient, where a division is within 2^-24; T's own half step is
+// 2^-11 (fp16) or 2^-8 (bf16) of it, and a division by the number 15 in torch on
+// the device is that product too, so that the bytes are those of the formula there.
 //
 // Eight lanes hold one row: lane l the 16-byte chunks l and l + 8, so a row
 // is read with two 16-byte loads a lane, the two halves of a full rotation
@@ -152,9 +155,9 @@ KVS_DEV void store_row4(const AppendLaunch& L, uint8_t* rec, int value, int off,
 
 // Rows of a token: q_heads query rows, then key rows, then value rows.
 // 16-bit caches: bound by memory, 16384 tokens of 32 + 8 heads in 71 us, 5.7 TB/s or 87% of the
-// copy rate.  4-bit caches: by the quantisation's instructions, about 780 a warp for four rows
-// (4097 tokens of 28 + 4 heads 20 us, three CTAs an SM; 24 us with two).  A decode step of
-// either is one launch, 4.3 us.
+// copy rate.  4-bit caches: by the quantisation's instructions and the loads in front of them, about
+// 780 a warp for four rows in 59% of the issue slots (4097 tokens of 28 + 4 heads 20 us, three CTAs
+// an SM; 24 us with two).  A decode step of either is one launch, 4.3 us.
 template <bool FP16, int MODE, bool FOUR, int EACH>
 __global__ void __launch_bounds__(kThreads, 3)
     k_append_kv(const __grid_constant__ AppendLaunch L, const __grid_constant__ Spread S) {

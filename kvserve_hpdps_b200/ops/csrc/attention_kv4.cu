@@ -30,11 +30,11 @@
 // rate (23 bytes a clock and SM) that is above what shared memory moves.
 // mma.sync takes the operands from the registers that unpack them.
 //
-// What bounds it: instructions.  32 tokens of one head and up to 8 rows take a warp about 760,
-// 304 of them to unpack 8192 codes; 63% of the issue slots and half of the integer pipe are
-// used with 12 warps an SM.  48 ragged sequences of up to 8192 tokens, 32/8 heads, groups of 64
-// (230 MB): 69 us, 3.3 TB/s, where HBM would allow 35.  Not faster there: 16 warps with 128
-// registers (71 us), 64 tokens a step (70), 16 tokens a step (84).
+// What bounds it: instructions and their latency.  32 tokens of one head and up to 8 rows take a
+// warp about 780, 304 of them to unpack 8192 codes; 12 warps an SM fill 63% of the issue slots
+// and half of the integer pipe.  48 ragged sequences of up to 8192 tokens, 32/8 heads, groups of
+// 64 (230 MB): 69 to 72 us, 3.2 TB/s, where HBM would allow 35.  Not faster there: 16 warps with
+// 128 registers (71 us against 69), 64 tokens a step (70), 16 tokens a step (87).
 #include <type_traits>
 
 #include "attention_kv4.cuh"
@@ -721,13 +721,15 @@ Grid grid_of(const Attn4Launch* L) {
 // host knows (max_query_len, and the tokens that the table has room for; tables as wide as the
 // sequences below).  fp16 caches, whose tiles take twice the conversion there, from more rows on.
 // Measured, us here / there for bf16 and for fp16, groups of 64: 32 sequences of 2000 tokens,
-// 8 heads: 48 rows 99 / 97 and 99 / 175, 80 rows 153 / 103 and 153 / 178; 16 of 2000: 64 rows
-// 72 / 58 and 72 / 93, 96 rows 99 / 62 and 99 / 96; 8 of 8000, 4 heads: 56 rows 61 / 51 and 61 / 80,
-// 84 rows 86 / 55 and 86 / 82; 64 of 1000, 4 heads: 84 rows 122 / 78 and 123 / 114.
+// 8 heads: 48 rows 99 / 97 and 114 / 174, 80 rows 153 / 103 and 179 / 178; 16 of 2000: 64 rows
+// 72 / 58 and 81 / 93, 96 rows 99 / 62 and 113 / 96; 8 of 8000, 4 heads: 56 rows 61 / 51 and
+// 71 / 80, 84 rows 86 / 55 and 100 / 82; 64 of 1000, 4 heads: 84 rows 122 / 78 and 143 / 114.
 // With little to do the tiles' fixed cost decides (Mi rows times tokens times heads): one of
-// 1024 tokens, 4 heads: 1792 rows (7 Mi) 43 / 37 and 43 / 40; 8 of 2000, 8 heads: 52 rows (6.3 Mi)
-// 43 / 37; 4 of 2000: 96 rows (5.9 Mi) 36 / 32 and 36 / 40.  One long sequence on many heads
-// loses there: one of 4000, 8 heads: 192 rows (5.9 Mi) 32 / 40 and 32 / 44.
+// 1024 tokens, 4 heads: 1792 rows (7 Mi) 43 / 37 and 49 / 40; 8 of 2000, 8 heads: 52 rows (6.3 Mi)
+// 43 / 37; 4 of 2000: 96 rows (5.9 Mi) 36 / 32 and 39 / 40.  One long sequence on many heads
+// loses there: one of 4000, 8 heads: 192 rows (5.9 Mi) 32 / 40 and 36 / 44.  A call goes there as
+// a whole: one of 512 rows over 4096 tokens beside 48 sequences of one row, 32/8 heads, takes
+// 327 us, the two kinds in calls of their own 149.
 constexpr int kManyRows = 48, kManyRowsFp16 = 80;
 constexpr long long kMuchWork = 5ll << 20;
 bool many_rows(const Attn4Launch* L) {

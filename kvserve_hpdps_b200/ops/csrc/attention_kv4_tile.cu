@@ -37,8 +37,9 @@
 //
 // What bounds it: the softmax warps' chain of barriers, tensor memory and exponentials, about
 // 2400 clocks for 64 tokens of both tiles, of which the exponentials' rate (16 a clock and SM)
-// is 1024 and the products take 1320.  2 x 2048 tokens over up to 8193, 28/4 heads (361 GFLOP):
-// 464 us, 778 TFLOP/s; on mma.sync, a warp 16 rows, it was 2000 us.
+// is 1024 and the products take 1320 (fp16 caches: 2560, and twice the conversion).  2 x 2048
+// tokens over up to 8193, 28/4 heads (361 GFLOP), bf16: 472 us in a captured graph, 489 in calls
+// of their own, 738 TFLOP/s; on mma.sync, a warp 16 rows, it was 2000 us.
 //
 // The work is dealt out as in attention_kv4.cu, here by the number of visible
 // keys a tile has, so that causal tiles of a long chunk load all SMs alike.
@@ -64,9 +65,9 @@ constexpr float kApart = 0x1p-8f;
 constexpr uint32_t kHides = 1, kWideK = 2, kWideV = 4;
 constexpr int kFar = 60;
 // A score is a factor times 128 products of less than 2^15 and 2^11.  Where the factor lets it pass
-// 2^27, the product is rounded before the maximum is taken off: the fused multiply-add leaves the
-// maximum's own rounding over, up to 2^-25 of it, and weights are 2 to that from where they should be
-// (the same for all of a row's, so that 2^4 does no harm).
+// 2^27, or tokens have a scale each, the product is rounded before the maximum is taken off: the
+// fused multiply-add leaves the maximum's own rounding over, up to 2^-25 of it, and weights are 2 to
+// that from where they should be (the same for all of a row's, so that 2^4 does no harm).
 constexpr float kHuge = 0x1p-6f;
 
 struct Ctrl {
@@ -91,6 +92,7 @@ struct Ctrl {
 constexpr int kMidTile = 4096;
 constexpr int kMidAt = 12 * kHalfTile, kCtrlAt = kMidAt + 4 * kMidTile;
 constexpr int kSmem = 1024 + kCtrlAt + static_cast<int>(sizeof(Ctrl));
+static_assert(kSmem <= 227 * 1024);
 
 // Instruction descriptors: fp16 x fp16 -> fp32, M = 128; N = 64 tokens with B K-major, N = 128
 // channels with B MN-major.
@@ -112,9 +114,9 @@ KVS_DEV uint32_t k_desc(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
 KVS_DEV uint32_t mn_desc(uint32_t saddr) {
   return (saddr >> 4) | (static_cast<uint32_t>(kHalfTile >> 4) << 16);
 }
-// The value of lane 0 in a uniform register, where the matrix instructions want their operands:
-// from there each takes one uniform addition, from a vector register four moves (736 us at 2 x
-// 2048 tokens against 536: the issuing warp was what the kernel waited for).
+// A value that all lanes of the warp share, as a reduction over it: the compiler then keeps it where
+// the matrix instructions want their operands (536 us at 2 x 2048 tokens against 736 without, when
+// one warp issued them all).
 KVS_DEV uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }
 KVS_DEV bool elected() {
   uint32_t p;
@@ -721,10 +723,9 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
           const uint32_t v = n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
           return v & ~C->gone[ring][seg0 + sg];
         };
-        bool raise;
-        const bool huge = fmaxf(said_up[0], said_up[1]) > up_most;
+        const bool huge = fmaxf(said_up[0], said_up[1]) > up_most || (flag & kWideK) != 0;
         if (t0 + 64 > plain_to || flag != 0 || huge) {  // hidden scores become -inf
-          if (flag & kWideK || huge) {
+          if (huge) {
 #pragma unroll
             for (int sg = 0; sg < 2; ++sg) {
               const float* const up = C->k_tok[ring] + 32 * (seg0 + sg);
@@ -733,7 +734,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
                 for (int k = 0; k < 32; ++k)
                   v[sg][k] = __float_as_uint(__uint_as_float(v[sg][k]) * (f * up[k]));
                 fs[sg] = 1.f;
-              } else if (huge) {
+              } else {
 #pragma unroll
                 for (int k = 0; k < 32; ++k)
                   v[sg][k] = __float_as_uint(__fmul_rn(__uint_as_float(v[sg][k]), fs[sg]));
@@ -762,7 +763,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
             }
           }
         }
-        raise = __any_sync(0xFFFFFFFFu, max(v_exp[0], v_exp[1]) > E);
+        const bool raise = __any_sync(0xFFFFFFFFu, max(v_exp[0], v_exp[1]) > E);
         // Against the reference that there is, the scores only pass through once; a row
         // whose weights' sum has passed kMostSum, or larger values, make the warp find the maximum,
         // rescale and take the scores again (the first half always does).

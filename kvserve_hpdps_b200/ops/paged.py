@@ -151,6 +151,10 @@ def attention_kv4(query: torch.Tensor, cache: torch.Tensor, block_table: torch.T
     r.  ``Hq`` is a multiple of the cache's heads (consecutive query heads
     share one).  ``scale`` defaults to 1/sqrt(128).
 
+    ``max_query_len`` and the room in the table choose the kernel, for the call as a whole: give
+    sequences of one or a few rows and prefill chunks calls of their own (48 decodes
+    beside a chunk of 512: 327 us together, 149 apart), each with its own bound.
+
     Returns the output in the query's dtype (``out`` when given) and with
     ``return_lse`` also the fp32 logarithm of each row's sum of exponentials
     ``[T, Hq]``.  A row that sees no token is zeros with -inf.  A sequence
