@@ -160,8 +160,8 @@ def attention_kv4(query: torch.Tensor, cache: torch.Tensor, block_table: torch.T
     ``[T, Hq]``.  A row that sees no token is zeros with -inf.  A sequence
     whose extents do not fit the arrays records an error and is left out; so is
     a block id outside the cache, with its tokens.  Rows of no sequence and of
-    one left out keep what a given ``out`` holds, without one they are zeros;
-    their logarithm is -inf.  Scratch is allocated per call from torch's
+    one left out keep what a given ``out`` holds (which saves writing them, in a
+    batch padded far), without one they are zeros; their logarithm is -inf.  Scratch is allocated per call from torch's
     allocator, so captured graphs do not share it.
     """
     args = (query, cache, block_table, seq_lens, query_start, max_query_len, scale, out,
