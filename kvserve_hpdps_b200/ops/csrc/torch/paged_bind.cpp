@@ -25,6 +25,8 @@ using std::optional;
 extern "C" {
 int kvs_append_kv(const kvs::AppendLaunch* L, void* stream);
 int kvs_read_kv4(const kvs::Read4Launch* L, void* stream);
+int kvs_append_kv8(const kvs::AppendLaunch* L, void* stream);
+int kvs_read_kv8(const kvs::Read4Launch* L, void* stream);
 long long kvs_attn4_scratch_bytes(const kvs::Attn4Launch* L);
 int kvs_attention_kv4(const kvs::Attn4Launch* L, void* stream);
 const char* kvs_last_error_string(void);
@@ -106,6 +108,26 @@ int groups4(const Tensor& cache) {
   return static_cast<int>((rb - 128) / 8);
 }
 
+// Whether a cache is one of 8 bits; the other uint8 caches are taken for 4-bit ones.
+bool is_kv8(const Tensor& cache) {
+  return cache.scalar_type() == at::kByte && cache.dim() == 4 && cache.size(3) == kDim;
+}
+// The block size of an 8-bit cache.
+int64_t block8(const Tensor& cache) {
+  TORCH_CHECK_TYPE(cache.scalar_type() == at::kByte && cache.dim() == 4,
+                   "an 8-bit cache is a uint8 [blocks, heads, 2 * block_size + 1, 128] tensor");
+  const int64_t rows = cache.size(2), bs = (rows - 1) / 2;
+  TORCH_CHECK_VALUE(cache.size(3) == kDim && rows % 2 == 1 && bs > 0 && bs % 16 == 0 && bs <= 1024,
+                    "an 8-bit cache is [blocks, heads, 2 * block_size + 1, 128] with a block_size "
+                    "that is a multiple of 16 up to 1024, got ", cache.sizes());
+  TORCH_CHECK_VALUE(cache.stride(3) == 1 && cache.stride(2) == kDim && cache.stride(0) % 16 == 0 &&
+                        cache.stride(1) % 16 == 0 && aligned16(cache),
+                    "an 8-bit cache's records must be contiguous and 16-byte aligned, got strides ",
+                    cache.strides());
+  TORCH_CHECK_VALUE(cache.size(0) < (1ll << 31), "an 8-bit cache has at most 2^31 blocks");
+  return bs;
+}
+
 void on_device(const char* what, const at::Device& dev, std::initializer_list<const Tensor*> ts) {
   TORCH_CHECK_VALUE(dev.is_cuda(), what, " needs CUDA tensors");
   for (const Tensor* t : ts)
@@ -148,7 +170,11 @@ optional<Tensor> append_kv(const Tensor& cache, const Tensor& key_in, const Tens
   TORCH_CHECK_VALUE(n <= T, n, " slots for ", T, " tokens");
   kvs::AppendLaunch L = {};
   int64_t nb, bs, hc;
-  if (cache.scalar_type() == at::kByte) {
+  const bool eight = is_kv8(cache);
+  if (eight) {
+    bs = block8(cache), nb = cache.size(0), hc = cache.size(1);
+    L.block_stride = cache.stride(0), L.head_stride = cache.stride(1);
+  } else if (cache.scalar_type() == at::kByte) {
     L.groups = groups4(cache);
     nb = cache.size(0), hc = cache.size(1), bs = cache.size(2);
     L.block_stride = cache.stride(0), L.head_stride = cache.stride(1);
@@ -224,24 +250,29 @@ optional<Tensor> append_kv(const Tensor& cache, const Tensor& key_in, const Tens
   }
   if (n == 0 || H + L.q_heads == 0) return query_out;
   L.err = g_err[dev.index()];
-  launched(kvs_append_kv(&L, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "append_kv");
+  void* const stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  launched(eight ? kvs_append_kv8(&L, stream) : kvs_append_kv(&L, stream), "append_kv");
   return query_out;
 }
 
-Tensor read_kv4(const Tensor& cache, const Tensor& slot_mapping, at::ScalarType dt,
-                const optional<Tensor>& out_in) {
-  const int groups = groups4(cache);
+// Rows of a 4-bit or (EIGHT) 8-bit cache.
+template <bool EIGHT>
+Tensor read_rows(const Tensor& cache, const Tensor& slot_mapping, at::ScalarType dt,
+                 const optional<Tensor>& out_in) {
+  const char* const what = EIGHT ? "read_kv8" : "read_kv4";
+  const int groups = EIGHT ? 0 : groups4(cache);
+  const int64_t bs = EIGHT ? block8(cache) : cache.size(2);
   TORCH_CHECK_TYPE(dt == at::kBFloat16 || dt == at::kHalf, "dtype must be bf16 or fp16, got ", dt);
   const Tensor slots = index("slot_mapping", slot_mapping);
   const at::Device dev = cache.device();
-  const int64_t nb = cache.size(0), H = cache.size(1), bs = cache.size(2), n = slots.size(0);
+  const int64_t nb = cache.size(0), H = cache.size(1), n = slots.size(0);
   const int64_t shape[4] = {2, n, H, kDim};
   if (out_in.has_value())
     TORCH_CHECK_VALUE(out_in->sizes() == at::IntArrayRef(shape) && out_in->scalar_type() == dt &&
                           out_in->is_contiguous() && aligned16(*out_in),
                       "out must be a contiguous ", dt, " tensor of ", at::IntArrayRef(shape));
-  no_gradient("read_kv4", {opt(out_in)});
-  on_device("read_kv4", dev, {&slot_mapping, opt(out_in)});
+  no_gradient(what, {opt(out_in)});
+  on_device(what, dev, {&slot_mapping, opt(out_in)});
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor out = out_in.has_value() ? *out_in : at::empty(shape, cache.options().dtype(dt));
   if (n == 0 || H == 0) return out;
@@ -252,7 +283,8 @@ Tensor read_kv4(const Tensor& cache, const Tensor& slot_mapping, at::ScalarType 
   L.block_size = static_cast<int>(bs), L.groups = groups;
   L.fp16 = dt == at::kHalf, L.slots64 = slots.scalar_type() == at::kLong;
   L.err = g_err[dev.index()];
-  launched(kvs_read_kv4(&L, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "read_kv4");
+  void* const stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  launched(EIGHT ? kvs_read_kv8(&L, stream) : kvs_read_kv4(&L, stream), what);
   return out;
 }
 
@@ -337,7 +369,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("append_kv", &append_kv);
   m.def("read_kv4", [](const Tensor& cache, const Tensor& slots, py::object dtype,
                        const optional<Tensor>& out) {
-    return read_kv4(cache, slots, torch::python::detail::py_object_to_dtype(dtype), out);
+    return read_rows<false>(cache, slots, torch::python::detail::py_object_to_dtype(dtype), out);
+  });
+  m.def("read_kv8", [](const Tensor& cache, const Tensor& slots, py::object dtype,
+                       const optional<Tensor>& out) {
+    return read_rows<true>(cache, slots, torch::python::detail::py_object_to_dtype(dtype), out);
   });
   m.def("attention_kv4", &attention_kv4);
 }

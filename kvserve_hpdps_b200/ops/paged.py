@@ -1,12 +1,13 @@
 """Operators on the paged KV caches of a serving step.
 
 * :func:`append_kv`: a step's new keys and values into a paged cache (16-bit,
-  or held in 4 bits), the position rotation of keys and queries applied in the
-  same launch;
-* :func:`attention_kv4`: attention over a 4-bit cache without unpacking it
-  first (one token, several draft tokens or a prefill chunk per sequence);
-* :func:`read_kv4`: rows of a 4-bit cache as 16-bit values, e.g. to hand them
-  to the paths that take 16-bit KV.
+  or held in 8 or 4 bits), the position rotation of keys and queries applied in
+  the same launch;
+* :func:`attention_kv8`, :func:`attention_kv4`: attention over an 8-bit or 4-bit
+  cache without unpacking it first (one token, several draft tokens or a
+  prefill chunk per sequence; over 8 bits also cross attention);
+* :func:`read_kv8`, :func:`read_kv4`: rows of such a cache as 16-bit values, e.g.
+  to hand them to the paths that take 16-bit KV.
 
 A 4-bit cache of one layer is a uint8 tensor ``[num_blocks, heads, block_size,
 row_bytes]`` (:func:`kv4_cache`), ``row_bytes = 128 + 1024 / group_size``: 64
@@ -18,6 +19,14 @@ each part over the block's tokens (``csrc/kv4.cuh`` has the order of the
 codes in a row), so a block's record is contiguous and can be moved whole.  The metadata
 has the dtype of the keys, values and queries the cache is used with: one
 dtype for the life of a cache.
+
+An 8-bit cache of one layer is a uint8 tensor ``[num_blocks, heads, 2 * block_size + 1,
+128]`` (:func:`kv8_cache`): in each (block, head) ``block_size`` rows of key codes, as
+many of value codes and a row of scales, contiguous too.  Codes are e4m3 numbers
+(``cache[:, :, :block_size].view(torch.float8_e4m3fn)``).  Each unit of 16 tokens has two
+bytes in the last row, for its keys and its values; a channel's value is
+``code * 2 ** (byte - 127)``.  It has no dtype: keys of either 16-bit type can be
+appended and queries of either can attend.
 
 All functions run on the current CUDA stream and never synchronise the host.
 They have no backward pass and refuse tensors that require a gradient outside
@@ -92,6 +101,15 @@ def kv4_cache(num_blocks: int, num_heads: int, block_size: int = 16, group_size:
                        dtype=torch.uint8, device=device)
 
 
+def kv8_cache(num_blocks: int, num_heads: int, block_size: int = 16,
+              device="cuda") -> torch.Tensor:
+    """A zeroed 8-bit cache of one layer (every row reads as zeros)."""
+    if block_size <= 0 or block_size % 16 or block_size > 1024:
+        raise ValueError("block_size must be a multiple of 16 up to 1024")
+    return torch.zeros((num_blocks, num_heads, 2 * block_size + 1, HEAD_DIM), dtype=torch.uint8,
+                       device=device)
+
+
 # ------------------------------------------------------------------- append
 def append_kv(cache: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
               slot_mapping: torch.Tensor, positions: Optional[torch.Tensor] = None,
@@ -102,12 +120,21 @@ def append_kv(cache: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
 
     ``cache``: a 16-bit layer ``[2, nb, bs, H, 128]`` or ``[nb, 2, bs, H, 128]``
     (any block, slot and head strides, so token-major and head-major blocks)
-    in the keys' dtype, or a 4-bit cache (:func:`kv4_cache`).
+    in the keys' dtype, an 8-bit cache (:func:`kv8_cache`) or a 4-bit one
+    (:func:`kv4_cache`).
     ``key`` / ``value``: ``[T, H, 128]`` bf16 or fp16, any token and head
     strides.  ``slot_mapping`` ``[n <= T]``: slot of each token
     (``block * block_size + offset``); a negative slot's token is not appended,
     rows of ``key`` behind ``n`` are not read.  Slots of one call are distinct
-    (of two tokens with one slot either may be kept, in parts).
+    (of two tokens with one slot either may be kept, in parts; in an 8-bit cache the
+    slot's unit of 16 may hold anything).
+
+    In an 8-bit cache the 16 tokens of a unit share a scale, keys and values apart, per head: the
+    smallest power of two that holds the largest of them in e4m3.  It grows as tokens
+    come, and the codes of those before are moved to it (exact but for what falls into
+    e4m3's subnormals).  A call that has the token at offset 0 of a unit begins the unit anew:
+    the unit's slots that the call does not name lose what they held.  An infinity or NaN
+    is held as NaN and has no say in the scale.
 
     With ``positions`` ``[>= n]`` and ``cos_sin`` ``[max_position, rotary_dim]``
     (cosines, then sines; fp32 or the keys' dtype) the first ``rotary_dim``
@@ -133,6 +160,16 @@ def read_kv4(cache: torch.Tensor, slot_mapping: torch.Tensor, dtype: torch.dtype
     rounded to it once.  A negative slot reads zeros."""
     args = (cache, slot_mapping, dtype, out)
     return _call("read_kv4", cache, args)
+
+
+def read_kv8(cache: torch.Tensor, slot_mapping: torch.Tensor, dtype: torch.dtype,
+             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rows of an 8-bit cache: ``[2, n, H, 128]`` keys and values at the slots.
+
+    ``dtype``: bf16 or fp16; the values are rounded to it once (bf16 holds all of
+    them), those past its largest number to that.  A negative slot reads zeros."""
+    args = (cache, slot_mapping, dtype, out)
+    return _call("read_kv8", cache, args)
 
 
 # ---------------------------------------------------------------- attention
