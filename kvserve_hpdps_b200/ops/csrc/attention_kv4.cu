@@ -51,19 +51,6 @@ constexpr int kOver = 2;              // what starting and ending an item costs,
 // kSpread CTAs: short chains against few parts to join (kFew and kLeast alone: one sequence of
 // 2000 tokens, 8 heads, 11.5 and 12.5 us; of 32768, 4 heads, 22.8 and 20.7).
 constexpr int kLeast = 4, kFew = 2, kSpread = 148;
-KVS_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                      uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// Transposes an 8x8 matrix of 16-bit elements held two to a lane.
-KVS_DEV uint32_t transpose8(uint32_t a) {
-  uint32_t d;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
-  return d;
-}
 KVS_DEV void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -105,16 +92,6 @@ KVS_DEV void lds_meta(const uint8_t* a, uint32_t (&m)[NG]) {
 // two: one for an item that began before its share, one for an item that
 // goes on behind it) and k_attn4_combine joins an item's parts in order, so
 // results do not depend on timing.
-// CTA b's share of a line of length U dealt to B: [begin(b), begin(b + 1)).
-struct Deal {
-  int each, more;  // U / B, U % B
-  KVS_DEV int begin(int b) const { return each * b + min(b, more); }
-  KVS_DEV int owner(int x) const {
-    const int wide = more * (each + 1);
-    return x < wide ? x / (each + 1) : more + (x - wide) / each;
-  }
-};
-
 struct Work {
   int units;       // a sequence's share of the line
   int tiles, per;  // row tiles a head, units an item

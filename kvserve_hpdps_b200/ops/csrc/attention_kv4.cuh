@@ -1,5 +1,5 @@
-// What the attention kernels over a 4-bit cache share: the sequences' extents,
-// codes as fp16, the running softmax's constants and the join of partial results.
+// What the attention kernels over 4-bit and 8-bit caches share: the sequences' extents, 4-bit codes
+// as fp16, the running softmax's constants, how work is dealt out and the join of partial results.
 #pragma once
 
 #include "kv4.cuh"
@@ -142,6 +142,29 @@ KVS_DEV uint32_t max_u16x2(uint32_t a, uint32_t b) {
   asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+KVS_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                      uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transposes an 8x8 matrix of 16-bit elements held two to a lane.
+KVS_DEV uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+// CTA b's share of a line of length U dealt to B: [begin(b), begin(b + 1)).
+struct Deal {
+  int each, more;  // U / B, U % B
+  KVS_DEV int begin(int b) const { return each * b + min(b, more); }
+  KVS_DEV int owner(int x) const {
+    const int wide = more * (each + 1);
+    return x < wide ? x / (each + 1) : more + (x - wide) / each;
+  }
+};
+
 // Partial results of items that several CTAs share.  A CTA leaves at most two: one for an item
 // that began before its share, one for an item that goes on behind it.
 struct Parts {

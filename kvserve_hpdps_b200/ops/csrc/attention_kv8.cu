@@ -1,0 +1,648 @@
+// Attention over a paged KV cache held in 8 bits (kv8.cuh has the layout).
+//
+// With n query rows of a sequence whose cache holds `len` tokens, row i sees keys
+// j < len - n + i + 1 (all `len` of them without causal limits).  With the scales a_u, b_u of
+// token j's unit u, and codes k, v,
+//   s_j = scale a_u (q . k_j),   o = [ sum_j p_j b_u v_j ] / sum_j p_j,   p_j = exp(s_j - M).
+// A row that sees no key returns zeros and lse = -inf.
+//
+// Codes become fp16 exactly (one conversion for two), the query row is scaled by a power of two so
+// that fp16 holds it exactly, products are summed in fp32: scores are as good as fp32's.  The scales
+// are powers of two, constant over a matrix fragment of 16 tokens, and go into the softmax's factor
+// (keys) and into the weights (values).
+//
+// The one rounding to fewer bits is that of the weights w = p b_u 2^-k to fp16, 2^-11 relative, an
+// eighth of a bf16 output's own; fp16 outputs would lose by it, so for them w is two fp16 parts.  k
+// is the row's own: the largest w that it has seen is near 2^7, so a token keeps fp16's
+// precision down to 2^-21 of the row's largest contribution, whatever scales its tokens have and
+// whatever tokens that it does not see hold.
+//
+// Work for few query rows is mma.sync's: scores are computed transposed, tokens x rows, so that the
+// rows fill the narrow side of the instruction; what tcgen05 would save in products it would cost in
+// codes written to shared memory again as 16 bits.  Rows of a tile beyond 16 go to more warps
+// of the CTA, which read the same codes from shared memory: HBM delivers them once for up to 64.
+#include <type_traits>
+
+#include "attention_kv8.cuh"
+
+namespace kvs {
+
+namespace {
+
+constexpr int kWarps = 4;           // a CTA
+constexpr int kStep = 32;           // tokens a warp takes at a time
+constexpr int kStage = 2 * kStep * 128;  // bytes of codes: keys, then values
+constexpr int kStages = 8;          // of a CTA's rings together
+constexpr int kOver = 256;          // what starting and ending an item costs, in tokens
+// A CTA's share of the line is no shorter than kLeast tokens, or kFew while that takes no more than
+// kSpread CTAs.
+constexpr int kLeast = 512, kFew = 256, kSpread = 148;
+// Largest weights are 2^kAbove when their row's units are set, and may come to 2^kMost.
+constexpr float kAbove = 7.f, kMost = 15.f;
+
+struct Work {
+  int units;       // a sequence's share of the line
+  int tiles, per;  // row tiles a head, units an item
+};
+template <int UNIT>
+KVS_DEV Work work_of(const Attn4Launch& L, const Seq& s, int rows, int group) {
+  Work w;
+  w.tiles = (s.n * group + rows - 1) / rows;
+  w.per = s.len > 0 && !L.whole ? (s.len + UNIT - 1) / UNIT : 1;
+  w.units = w.tiles * L.heads * (w.per + kOver / UNIT);
+  return w;
+}
+
+constexpr int kSmem = 1024 + kStages * kStage;
+
+// A warp takes NT * 8 rows; RG warps side by side the rows of a tile, the 4 / RG such groups of
+// a CTA every (4 / RG)th 32 tokens.  Fragments (lane = 4 g + c): K is the A operand, row m = token m,
+// lane c's channels 32 c + 4 ks + 0..3 in product ks; the scores' transposed fragments (movmatrix) are
+// the B operand of V^T P^T, whose A operand joins the bytes of two tokens: lane g's channels
+// 16 g + 0..15, lane c's tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9.  With the copy engine's swizzle both
+// are read in 16-byte pieces without bank conflicts.
+template <bool FP16, int NT, int RG>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
+    k_attn8(const __grid_constant__ Attn4Launch L, const __grid_constant__ CUtensorMap map) {
+  constexpr int ROWS = 8 * NT * RG, TS = kWarps / RG, ST = kStages / TS, UNIT = TS * kStep;
+  constexpr int AHEAD = RG == 1 ? ST : ST - 1;  // steps that are asked for ahead
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+  __shared__ __align__(16) uint8_t s_scale[kStages][2][16];
+  __shared__ uint64_t s_full[kStages], s_empty[kStages];
+  __shared__ uint32_t s_note[kStages];  // halves that are there, and where their scales are
+  __shared__ int s_scan[kWarps], s_begin, s_seq;
+  __shared__ float2 s_ml[TS][ROWS];
+  __shared__ int2 s_named[kWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+  const int split = warp / RG, rg = warp % RG;
+  const int group = L.q_heads / L.heads;
+  const int B = gridDim.x, b = blockIdx.x;
+  const Parts P = parts(L.scratch, B, ROWS);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---- this CTA's share [pos, end) and the sequence that it begins in
+  if (tid == 0) {
+    P.desc[b] = make_int4(-1, 0, 0, 0);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], RG);
+    }
+    fence_mbar_init();
+  }
+  int U = 0, mine = 0;
+  Named named;
+  for (int r = tid; r < L.seqs; r += kWarps * 32) {
+    const Seq s = sequence(L, r, b == 0);
+    named.take(L, s, r);
+    mine = work_of<UNIT>(L, s, ROWS, group).units;
+    U += mine;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) U += __shfl_xor_sync(0xFFFFFFFFu, U, o);
+  if (lane == 0) s_scan[warp] = U;
+  named.leave(L, s_named);
+  __syncthreads();
+  named.clear<kWarps>(L, s_named);
+  U = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) U += s_scan[w];
+  constexpr int kLeastUnits = kLeast / UNIT, kFewUnits = kFew / UNIT, kOverUnits = kOver / UNIT;
+  const int used = min(B, L.whole ? U / (1 + kOverUnits)  // an item a CTA
+                                  : max((U + kLeastUnits - 1) / kLeastUnits,
+                                        min(kSpread, (U + kFewUnits - 1) / kFewUnits)));
+  if (b >= used) return;
+  const Deal deal{U / used, U % used};
+  int pos = deal.begin(b), base = 0;
+  const int end = deal.begin(b + 1);
+  for (int r0 = 0; r0 < L.seqs; r0 += kWarps * 32) {
+    const int r = r0 + tid;
+    if (L.seqs > kWarps * 32)  // else `mine` is it
+      mine = r < L.seqs ? work_of<UNIT>(L, sequence(L, r, false), ROWS, group).units : 0;
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    __syncthreads();
+    if (lane == 31) s_scan[warp] = inc;
+    __syncthreads();
+    int before = base;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += s_scan[w];
+      base += s_scan[w];
+    }
+    if (before + inc - mine <= pos && pos < before + inc) {
+      s_seq = r;
+      s_begin = before + inc - mine;
+    }
+    if (pos < base) break;  // the same for every thread
+  }
+  __syncthreads();
+  int r = s_seq;
+  int begin = s_begin;  // of sequence r on the line
+
+  const int stage0 = split * ST;
+  uint32_t asked = 0, taken = 0;  // steps of this ring
+  bool lost = false;              // a copy did not come: nothing is waited for any more
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (!lost && !mbar_wait(bar, parity, L.err, ERR_MBAR_TIMEOUT)) lost = true;
+  };
+  // fragment addresses inside a unit's 16 rows of keys and of values
+  uint32_t k_at[2], v_at[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) k_at[i] = g * 128 + (((2 * c + i) ^ g) << 4);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) v_at[i] = (2 * c + i) * 128 + ((g ^ (2 * c + i)) << 4);
+  v_at[2] = v_at[0] + 1024;
+  v_at[3] = v_at[1] + 1024;
+
+  while (pos < end) {
+    const Seq s = sequence(L, r, false);
+    const Work wk = work_of<UNIT>(L, s, ROWS, group);
+    if (pos >= begin + wk.units) {  // on to the next sequence that has work
+      begin += wk.units;
+      ++r;
+      continue;
+    }
+    const int cost = wk.per + kOverUnits;
+    const int item = (pos - begin) / cost;
+    const int from0 = pos - begin - item * cost;
+    const int share = min(end - pos, cost - from0);
+    // an item's overhead lies in front of its units
+    const int unit0 = max(0, from0 - kOverUnits);
+    const int units = max(0, from0 + share - kOverUnits) - unit0;
+    pos += share;
+    if (units <= 0) continue;
+    const int h = item / wk.tiles, ti = item - h * wk.tiles;
+    // low and high tiles in turn: with causal limits, neighbours add up to alike work
+    const int tile = (ti & 1) ? wk.tiles - 1 - (ti >> 1) : ti >> 1;
+    const int nrows = s.n * group;
+    const int last_row = min(nrows, (tile + 1) * ROWS) - 1;
+    const int min_seen = max(0, seen_by(L, s, tile * ROWS / group));
+    const int limit = max(0, seen_by(L, s, last_row / group));
+    const int row0 = tile * ROWS + rg * 8 * NT;  // of this warp
+
+    // ---- this warp's steps: tokens first + UNIT k + [0, 32)
+    const int first = unit0 * UNIT + split * kStep;
+    const int stop = L.whole ? limit : min(limit, (unit0 + units) * UNIT);
+    const int steps = first < stop ? (stop - first + UNIT - 1) / UNIT : 0;
+    const int32_t* const table = L.table + r * L.table_stride;
+    int ids = -1, offs = 0;  // of step k % 16 = lane / 2, half lane % 2
+    auto ask = [&](int k) {  // by one warp of a ring
+      const uint32_t slot = asked % ST;
+      if (RG > 1 && asked >= ST) wait(&s_empty[stage0 + slot], (asked / ST - 1) & 1);
+      ++asked;
+      if ((k & 15) == 0) {
+        const int tok = first + (k + (lane >> 1)) * UNIT + 16 * (lane & 1);
+        ids = -1;
+        if (tok < stop) {
+          const int page = tok / L.block_size;
+          offs = tok - page * L.block_size;
+          ids = table[page];
+          if (ids < 0 || ids >= L.num_blocks) {
+            record_error(L.err, ERR_BOUNDS);
+            ids = -1;
+          }
+        }
+      }
+      // lanes 0..2: keys, values and scales of the first half; 3..5: of the second
+      const int hf = lane >= 3 ? 1 : 0, from = 2 * (k & 15) + hf;
+      const int id = __shfl_sync(0xFFFFFFFFu, ids, from);
+      const int off = __shfl_sync(0xFFFFFFFFu, offs, from);
+      const uint32_t there = __ballot_sync(0xFFFFFFFFu, id >= 0 && lane < 6);
+      const uint32_t had = (there & 1u) | (there >> 2 & 2u);
+      const int other = __shfl_sync(0xFFFFFFFFu, off, 3);
+      if (lane == 0) {
+        s_note[stage0 + slot] = had | (off >> 3 & 14) << 8 | (other >> 3 & 14) << 16;
+        mbar_arrive_expect_tx(&s_full[stage0 + slot], __popc(had) * (4096 + 16));
+      }
+      __syncwarp();
+      if (lane < 6 && id >= 0) {
+        const int what = lane - 3 * hf;
+        if (what < 2) {
+          load_rows(smem_u32(smem) + (stage0 + slot) * kStage + what * 4096 + hf * 2048, &map,
+                    what * L.block_size + off, h, id, &s_full[stage0 + slot]);
+        } else {
+          const uint8_t* const rec =
+              static_cast<const uint8_t*>(L.cache) + id * L.block_stride + h * L.head_stride;
+          bulk_load(s_scale[stage0 + slot][hf], rec + 256ll * L.block_size + (off >> 3 & ~15), 16,
+                    &s_full[stage0 + slot]);
+        }
+      }
+    };
+    if (rg == 0)
+      for (int k = 0; k < AHEAD && k < steps; ++k) ask(k);
+
+    // ---- query fragments: fp16, each row scaled by a power of two so that its largest
+    // element is in [2^14, 2^15); exact unless 2^-31 of the largest
+    uint32_t qf[NT][8][2];
+    float f[NT][2];  // of this lane's columns 2c, 2c + 1
+    int seen[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      uint4 raw[4];
+      const int row = row0 + nt * 8 + g;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) raw[q] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < nrows) {
+        const uint16_t* qp = static_cast<const uint16_t*>(L.q) +
+                             (s.row0 + row / group) * L.q_ts +
+                             (h * group + row % group) * L.q_hs + 32 * c;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) raw[q] = *reinterpret_cast<const uint4*>(qp + 8 * q);
+      }
+      float x[4][8], top = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        unpack8<FP16>(raw[q], x[q]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[q][i]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+      int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+      e = top == 0.f ? 0 : max(kLowestExp, min(e, 100));
+      const float up = pow2(14 - e) * (L.scale < 0.f ? -1.f : 1.f);
+      const float fr = fabsf(L.scale) * 1.4426950408889634f * pow2(e - 14);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float* const y = &x[q][4 * i];
+          qf[nt][2 * q + i][0] = half2_bits(y[0] * up, y[1] * up);
+          qf[nt][2 * q + i][1] = half2_bits(y[2] * up, y[3] * up);
+        }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        f[nt][j] = __shfl_sync(0xFFFFFFFFu, fr, (2 * c + j) * 4);
+        const int cr = row0 + nt * 8 + 2 * c + j;
+        seen[nt][j] = cr < nrows ? seen_by(L, s, cr / group) : 0x7FFFFFFF;
+      }
+    }
+
+    float acc[8][NT][4], l[NT][2], M[NT][2], K[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][nt][i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        l[nt][j] = 0.f;
+        M[nt][j] = kLowest;
+        K[nt][j] = -120.f;  // weights are in units of 2^K, and 2^-K is a normal number
+      }
+    }
+
+    auto step = [&](auto tag, int t0, const uint8_t* st, uint32_t stage, uint32_t note) {
+      constexpr bool MASKED = decltype(tag)::value;
+      float sc[2][NT][4], ev[2], fv[2], top[2][NT][2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const uint32_t two = *reinterpret_cast<const uint16_t*>(
+            &s_scale[stage][hf][note >> (8 + 8 * hf) & 14]);
+        const float fk = __uint_as_float((two & 0xFFu) << 23);
+        fv[hf] = __uint_as_float(two >> 8 << 23);
+        ev[hf] = static_cast<float>(static_cast<int>(two >> 8) - 127);
+        float a[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[nt][i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 ka = *reinterpret_cast<const uint4*>(st + 2048 * hf + k_at[i]);
+          const uint4 kb = *reinterpret_cast<const uint4*>(st + 2048 * hf + k_at[i] + 1024);
+          const uint32_t u[4] = {ka.x, ka.y, ka.z, ka.w}, v[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t a0 = half2_low8(u[q]), a1 = half2_low8(v[q]), a2 = half2_high8(u[q]),
+                           a3 = half2_high8(v[q]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816(a[nt], a0, a1, a2, a3, qf[nt][4 * i + q][0], qf[nt][4 * i + q][1]);
+          }
+        }
+        const bool had = note >> hf & 1u;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float fs = f[nt][j] * fk;
+#pragma unroll
+            for (int i = j; i < 4; i += 2) {
+              // rounded before the maximum is taken off: a fused multiply-add would leave the
+              // maximum's rounding over, which grows with the score
+              float& x = sc[hf][nt][i];
+              x = __fmul_rn(a[nt][i], fs);
+              if (MASKED) {
+                const int tok = t0 + 16 * hf + g + (i < 2 ? 0 : 8);
+                if (!had || tok >= seen[nt][j]) x = -INFINITY;
+              }
+            }
+            top[hf][nt][j] = fmaxf(sc[hf][nt][j], sc[hf][nt][j + 2]);
+          }
+      }
+      // ---- a row's running maximum M, passed by up to 2^kLazy before it is moved, and the
+      // exponent K of its weights' units
+      bool move = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const float d = top[hf][nt][j] - M[nt][j];
+            move |= d > kLazy || d + ev[hf] > K[nt][j] + kMost;
+          }
+      if (__any_sync(0xFFFFFFFFu, move)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float x[2] = {top[0][nt][j], top[1][nt][j]};
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1)
+#pragma unroll
+              for (int hf = 0; hf < 2; ++hf)
+                x[hf] = fmaxf(x[hf], __shfl_xor_sync(0xFFFFFFFFu, x[hf], o));
+            const float old = M[nt][j], m = fmaxf(old, fmaxf(x[0], x[1])), less = old - m;
+            const float k = fmaxf(fmaxf(floorf(K[nt][j] + less), -120.f),
+                                  ceilf(fmaxf(x[0] - m + ev[0], x[1] - m + ev[1])) - kAbove);
+            const float k1 = ex2(less), k2 = ex2(less + (K[nt][j] - k));
+            M[nt][j] = m;
+            K[nt][j] = k;
+            l[nt][j] *= k1;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+              acc[d][nt][j] *= k2;
+              acc[d][nt][j + 2] *= k2;
+            }
+          }
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        uint4 raw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          raw[i] = *reinterpret_cast<const uint4*>(st + 4096 + 2048 * hf + v_at[i]);
+        uint32_t w0[NT], w1[NT], rest0[NT], rest1[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float w[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            // 2^(ev - K); the minimum is for rows that see none of these tokens
+            const float unit = fminf(fv[hf] * pow2(-static_cast<int>(K[nt][j])), 3e38f);
+#pragma unroll
+            for (int i = j; i < 4; i += 2) {
+              const float p = ex2(sc[hf][nt][i] - M[nt][j]);
+              l[nt][j] += p;
+              w[i] = p * unit;
+            }
+          }
+          const uint32_t lo = half2_bits(w[0], w[1]), hi = half2_bits(w[2], w[3]);
+          w0[nt] = transpose8(lo);
+          w1[nt] = transpose8(hi);
+          if constexpr (FP16) {  // what the rounding leaves over
+            rest0[nt] = transpose8(half2_bits(w[0] - h2f<true>(lo & 0xFFFFu),
+                                              w[1] - h2f<true>(lo >> 16)));
+            rest1[nt] = transpose8(half2_bits(w[2] - h2f<true>(hi & 0xFFFFu),
+                                              w[3] - h2f<true>(hi >> 16)));
+          }
+        }
+        uint32_t v[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[i][0] = raw[i].x, v[i][1] = raw[i].y, v[i][2] = raw[i].z, v[i][3] = raw[i].w;
+        if (MASKED) {
+          // what no row of the tile sees counts as zeros, whatever its bytes are
+          uint32_t nan = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int tok = t0 + 16 * hf + 2 * c + (i & 1) + 8 * (i >> 1);
+            const bool keep = (note >> hf & 1u) && tok < limit;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              v[i][q] = keep ? v[i][q] : 0u;
+              nan |= (v[i][q] & 0x7F7F7F7Fu) + 0x01010101u;
+            }
+          }
+          if (__any_sync(0xFFFFFFFFu, nan & 0x80808080u)) {
+            // Not a number, in tokens that some rows see: zeros in the product, which would
+            // carry them to the others, and NaN where a row sees one, by a product of marks.
+            uint32_t s0[NT], s1[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              auto mark = [&](int i) { return sc[hf][nt][i] == -INFINITY ? 0.f : 1.f; };
+              s0[nt] = transpose8(half2_bits(mark(0), mark(1)));
+              s1[nt] = transpose8(half2_bits(mark(2), mark(3)));
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t is[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                is[i] = ((v[i][q] & 0x7F7F7F7Fu) + 0x01010101u) >> 7 & 0x01010101u;
+                v[i][q] &= ~(is[i] * 0xFFu);
+                is[i] *= 0x38u;  // e4m3's 1
+              }
+#pragma unroll
+              for (int o = 0; o < 2; ++o) {
+                const uint32_t pick = o ? 0x7362u : 0x5140u;
+                const uint32_t x = __byte_perm(is[0], is[1], pick),
+                               y = __byte_perm(is[2], is[3], pick);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  float n[4] = {0.f, 0.f, 0.f, 0.f};
+                  mma16816(n, half2_low8(x), half2_high8(x), half2_low8(y), half2_high8(y), s0[nt],
+                           s1[nt]);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    if (n[i] > 0.f) acc[2 * q + o][nt][i] = __uint_as_float(0x7FC00000u);
+                }
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {  // channels 16 g + 4 q + 2 o + 0, 1
+            const uint32_t pick = o ? 0x7362u : 0x5140u;
+            const uint32_t x = __byte_perm(v[0][q], v[1][q], pick),
+                           y = __byte_perm(v[2][q], v[3][q], pick);
+            const uint32_t a0 = half2_low8(x), a1 = half2_high8(x), a2 = half2_low8(y),
+                           a3 = half2_high8(y);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816(acc[2 * q + o][nt], a0, a1, a2, a3, w0[nt], w1[nt]);
+            if constexpr (FP16) {
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816(acc[2 * q + o][nt], a0, a1, a2, a3, rest0[nt], rest1[nt]);
+            }
+          }
+      }
+    };
+    for (int k = 0; k < steps; ++k) {
+      const uint32_t slot = taken % ST, stage = stage0 + slot;
+      wait(&s_full[stage], (taken / ST) & 1);
+      ++taken;
+      const int t0 = first + k * UNIT;
+      const uint32_t note = s_note[stage];
+      if (row0 < nrows) {
+        if ((note & 3u) != 3u || t0 + kStep > min_seen)
+          step(std::true_type{}, t0, smem + stage * kStage, stage, note);
+        else
+          step(std::false_type{}, t0, smem + stage * kStage, stage, note);
+      }
+      __syncwarp();  // the stage may be overwritten
+      if (RG > 1 && lane == 0) mbar_arrive(&s_empty[stage]);
+      if (rg == 0 && k + AHEAD < steps) ask(k + AHEAD);
+    }
+    // ---- join the warps' results
+    __syncthreads();  // the rings are empty: they hold the results
+    float* const s_o = reinterpret_cast<float*>(smem);  // [TS][ROWS][128]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = rg * 8 * NT + nt * 8 + 2 * c + j;
+        float ls = l[nt][j];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) ls += __shfl_xor_sync(0xFFFFFFFFu, ls, o);
+        if (g == 0) s_ml[split][row] = make_float2(M[nt][j], ls);
+        const float unit = pow2(static_cast<int>(K[nt][j]));
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<float4*>(s_o + (split * ROWS + row) * 128 + 16 * g + 4 * q) =
+              make_float4(acc[2 * q][nt][j] * unit, acc[2 * q][nt][j + 2] * unit,
+                          acc[2 * q + 1][nt][j] * unit, acc[2 * q + 1][nt][j + 2] * unit);
+      }
+    __syncthreads();
+    const bool whole = unit0 == 0 && units == wk.per;
+    const int slot = 2 * b + (unit0 == 0 ? 1 : 0);
+#pragma unroll 4
+    for (int it = 0; it < ROWS / kWarps; ++it) {  // a warp a row, four channels a lane
+      const int row = it * kWarps + warp, rr = tile * ROWS + row;
+      if (rr >= nrows) break;
+      float m = kLowest, ls = 0.f;
+      float2 ml[TS];
+#pragma unroll
+      for (int w = 0; w < TS; ++w) {
+        ml[w] = s_ml[w][row];
+        m = fmaxf(m, ml[w].x);
+      }
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < TS; ++w) {
+        const float k2 = ex2(ml[w].x - m);
+        const float4 x =
+            *reinterpret_cast<const float4*>(s_o + (w * ROWS + row) * 128 + lane * 4);
+        ls = fmaf(ml[w].y, k2, ls);
+        o.x = fmaf(x.x, k2, o.x);
+        o.y = fmaf(x.y, k2, o.y);
+        o.z = fmaf(x.z, k2, o.z);
+        o.w = fmaf(x.w, k2, o.w);
+      }
+      if (whole) {
+        const long long tq = s.row0 + rr / group;
+        const int hq = h * group + rr % group;
+        const float inv = ls == 0.f ? 0.f : __fdividef(1.f, ls);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + tq * L.o_ts + hq * L.o_hs +
+                                  lane * 4) =
+            make_uint2(f2h2<FP16>(o.x * inv, o.y * inv), f2h2<FP16>(o.z * inv, o.w * inv));
+        if (L.lse != nullptr && lane == 0)
+          L.lse[tq * L.q_heads + hq] =
+              ls == 0.f ? -INFINITY : (m + log2f(ls)) * 0.69314718055994531f;
+      } else {
+        *reinterpret_cast<float4*>(
+            P.o + (static_cast<long long>(slot) * ROWS + row) * 128 + lane * 4) = o;
+        if (lane == 0) P.ml[slot * ROWS + row] = make_float2(m, ls);
+      }
+    }
+    if (!whole && unit0 == 0 && tid == 0)  // parts: up to the CTA that holds the item's end
+      P.desc[b] = make_int4(r, h, tile, deal.owner(begin + (item + 1) * cost - 1) - b + 1);
+    fence_proxy_async_smem();  // the copy engine writes there next
+    __syncthreads();
+  }
+}
+
+struct Grid {
+  int ctas, rows;
+  bool fits;   // the line's length is an int
+  bool split;  // whether items may be split
+};
+
+// Tables of at most so many tokens are not split: the launch that joins the parts takes longer
+// than a second step.
+constexpr int kWholeTokens = 256;
+
+Grid grid_of(const Attn4Launch* L) {
+  Grid g;
+  const int group = L->q_heads / L->heads;
+  const long long rows = static_cast<long long>(L->max_q) * group;
+  g.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  const int unit = g.rows <= 16 ? 128 : g.rows == 32 ? 64 : 32;
+  const long long room = static_cast<long long>(L->table_cols) * L->block_size;
+  const long long per = (room + unit - 1) / unit;
+  const long long items = static_cast<long long>(L->seqs) * L->heads *
+                          ((rows + g.rows - 1) / g.rows);
+  g.split = room > kWholeTokens;
+  const long long units = items * (g.split ? per : 1);
+  g.fits = items < (1ll << 31) && items * (per + 1 + kOver / unit) < (1ll << 31);
+  const long long most = 148ll * (g.rows == 8 ? 3 : 2);  // resident at once
+  g.ctas = static_cast<int>(units < most ? units : most);
+  return g;
+}
+
+template <bool FP16, int NT, int RG>
+cudaError_t launch(const Attn4Launch& L, const Grid& g, const CUtensorMap& map, cudaStream_t s) {
+  cudaError_t e = cudaFuncSetAttribute(k_attn8<FP16, NT, RG>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  k_attn8<FP16, NT, RG><<<g.ctas, kWarps * 32, kSmem, s>>>(L, map);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || !g.split) return e;
+  return launch_combine<FP16, NT * RG, 4>(L, g.ctas, s);
+}
+template <bool FP16>
+cudaError_t launch_rows(const Attn4Launch& L, const Grid& g, const CUtensorMap& map,
+                        cudaStream_t s) {
+  return g.rows == 8    ? launch<FP16, 1, 1>(L, g, map, s)
+         : g.rows == 16 ? launch<FP16, 2, 1>(L, g, map, s)
+         : g.rows == 32 ? launch<FP16, 2, 2>(L, g, map, s)
+                        : launch<FP16, 2, 4>(L, g, map, s);
+}
+
+}  // namespace
+}  // namespace kvs
+
+using namespace kvs;
+
+extern "C" {
+
+long long kvs_attn8_scratch_bytes(const Attn4Launch* L) {
+  const Grid g = grid_of(L);
+  return 16ll * g.ctas + 2ll * g.ctas * g.rows * (8 + 512);
+}
+
+int kvs_attention_kv8(const Attn4Launch* L, void* stream) {
+  if (L->seqs <= 0 || L->max_q <= 0 || L->tokens <= 0 || L->heads <= 0) return 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const Grid g = grid_of(L);
+  if (!g.fits) return -2;
+  Attn4Launch A = *L;
+  A.whole = !g.split;
+  CUtensorMap map;
+  if (!record_map(A, &map)) return -3;
+  const cudaError_t e = L->fp16 ? launch_rows<true>(A, g, map, s) : launch_rows<false>(A, g, map, s);
+  return e == cudaSuccess ? 0 : -1;
+}
+
+}  // extern "C"

@@ -32,6 +32,7 @@
 //  * engine 1: thread-per-row loads and an in-register fp32 butterfly.
 #include "common.cuh"
 #include "kvs_types.h"
+#include "tensor_map.h"
 
 namespace kvs {
 
@@ -2492,24 +2493,6 @@ __global__ void k_init_key_stats(uint32_t* kstat, long long n_pairs) {
 }
 
 // ----------------------------------------------------------------- host
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (fn == nullptr) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  }
-  return fn;
-}
-
 // Persistent grid: two CTAs per SM (the shared-memory limit), never more
 // CTAs than jobs.
 static int persistent_grid(const LayerLaunch& L) {

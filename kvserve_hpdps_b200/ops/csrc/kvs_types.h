@@ -111,18 +111,18 @@ struct AppendLaunch {
   void* cache;
   uint32_t* err;
   long long key_ts, key_hs, val_ts, val_hs, q_ts, q_hs, qo_ts, qo_hs;  // token, head
-  // 16-bit cache: element strides of (block, plane, slot, head).  4-bit cache:
+  // 16-bit cache: element strides of (block, plane, slot, head).  4-bit and 8-bit caches:
   // block_stride and head_stride are the bytes between records.
   long long block_stride, kv_stride, slot_stride, head_stride;
   long long num_slots, max_pos, table_stride;
   int tokens, heads, q_heads, block_size, rotary, interleaved;
   int fp16;        // 0: bf16, 1: fp16
   int slots64, pos64, table32;  // index widths; fp32 table (else the 16-bit type)
-  int groups;      // 4-bit cache: channel groups a row (1, 2, 4); 0: 16-bit cache
+  int groups;      // 4-bit cache: channel groups a row (1, 2, 4); 0: 16-bit or 8-bit cache
   int pad_;
 };
 
-// Rows of a 4-bit cache read as 16-bit values: out [2][tokens][heads][128].
+// Rows of a 4-bit or 8-bit cache read as 16-bit values: out [2][tokens][heads][128].
 struct Read4Launch {
   const void* cache;
   const void* slots;
@@ -132,7 +132,7 @@ struct Read4Launch {
   int tokens, heads, block_size, groups, fp16, slots64;
 };
 
-// Attention of `tokens` query rows over a 4-bit cache.
+// Attention of `tokens` query rows over a 4-bit or 8-bit cache.
 struct Attn4Launch {
   const void* q;
   void* out;
@@ -148,6 +148,7 @@ struct Attn4Launch {
   float scale;
   int whole;  // set by the launcher: tables so short that items are not split
   int clear;  // rows of no sequence become zeros, too (their lse is -inf either way)
+  int causal; // 8-bit cache: a sequence's query rows are its last tokens; 0: each sees all of them
 };
 
 }  // namespace kvs

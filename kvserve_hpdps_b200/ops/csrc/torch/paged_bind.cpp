@@ -29,6 +29,8 @@ int kvs_append_kv8(const kvs::AppendLaunch* L, void* stream);
 int kvs_read_kv8(const kvs::Read4Launch* L, void* stream);
 long long kvs_attn4_scratch_bytes(const kvs::Attn4Launch* L);
 int kvs_attention_kv4(const kvs::Attn4Launch* L, void* stream);
+long long kvs_attn8_scratch_bytes(const kvs::Attn4Launch* L);
+int kvs_attention_kv8(const kvs::Attn4Launch* L, void* stream);
 const char* kvs_last_error_string(void);
 }
 
@@ -124,7 +126,12 @@ int64_t block8(const Tensor& cache) {
                         cache.stride(1) % 16 == 0 && aligned16(cache),
                     "an 8-bit cache's records must be contiguous and 16-byte aligned, got strides ",
                     cache.strides());
-  TORCH_CHECK_VALUE(cache.size(0) < (1ll << 31), "an 8-bit cache has at most 2^31 blocks");
+  for (int d = 0; d < 2; ++d)  // the copy engine's limits
+    TORCH_CHECK_VALUE(cache.size(d) < (1ll << 31) &&
+                          (cache.size(d) <= 1 ||
+                           (cache.stride(d) > 0 && cache.stride(d) < (1ll << 40))),
+                      "an 8-bit cache's records do not overlap and are at most 2^40 bytes apart, "
+                      "got strides ", cache.strides());
   return bs;
 }
 
@@ -147,6 +154,7 @@ const Tensor* opt(const optional<Tensor>& t) { return t.has_value() ? &*t : null
 
 void launched(int rc, const char* what) {
   TORCH_CHECK(rc != -2, what, ": the call is too large for one launch");
+  TORCH_CHECK(rc != -3, what, ": the driver makes no tensor map of this cache");
   TORCH_CHECK(rc == 0, what, " failed: ", kvs_last_error_string());
 }
 
@@ -288,12 +296,16 @@ Tensor read_rows(const Tensor& cache, const Tensor& slot_mapping, at::ScalarType
   return out;
 }
 
-std::pair<Tensor, optional<Tensor>> attention_kv4(
+// Attention over a 4-bit or (EIGHT) 8-bit cache.
+template <bool EIGHT>
+std::pair<Tensor, optional<Tensor>> attention(
     const Tensor& query, const Tensor& cache, const Tensor& block_table, const Tensor& seq_lens,
     const optional<Tensor>& query_start, int64_t max_query_len, optional<double> scale,
-    const optional<Tensor>& out_in, bool return_lse) {
+    const optional<Tensor>& out_in, bool return_lse, bool causal) {
+  const char* const what = EIGHT ? "attention_kv8" : "attention_kv4";
   check_heads("query", query, query.scalar_type());
-  const int groups = groups4(cache);
+  const int groups = EIGHT ? 0 : groups4(cache);
+  const int64_t bs = EIGHT ? block8(cache) : cache.size(2);
   const at::Device dev = query.device();
   TORCH_CHECK_TYPE(block_table.scalar_type() == at::kInt && block_table.dim() == 2,
                    "block_table must be an int32 [sequences, columns] tensor");
@@ -314,8 +326,8 @@ std::pair<Tensor, optional<Tensor>> attention_kv4(
   const double sc = scale.has_value() ? *scale : 0.08838834764831845;  // 1 / sqrt(128)
   TORCH_CHECK_VALUE(std::isfinite(sc) && sc != 0.0, "scale must be finite and not zero, got ", sc);
   if (out_in.has_value()) check_out("out", *out_in, query);
-  no_gradient("attention_kv4", {&query, opt(out_in)});
-  on_device("attention_kv4", dev,
+  no_gradient(what, {&query, opt(out_in)});
+  on_device(what, dev,
             {&cache, &block_table, &seq_lens, opt(query_start), opt(out_in)});
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor out = out_in.has_value() ? *out_in : at::empty(query.sizes(), query.options());
@@ -340,20 +352,20 @@ std::pair<Tensor, optional<Tensor>> attention_kv4(
   L.seqs = int_of("sequences", R), L.tokens = int_of("rows", T);
   L.num_blocks = static_cast<int>(cache.size(0));
   L.q_heads = int_of("query heads", Hq), L.heads = int_of("heads", H);
-  L.block_size = static_cast<int>(cache.size(2)), L.groups = groups;
+  L.block_size = static_cast<int>(bs), L.groups = groups, L.causal = causal;
   L.fp16 = query.scalar_type() == at::kHalf;
   L.max_q = static_cast<int>(std::min(max_query_len, T));
   L.scale = static_cast<float>(sc);
   L.clear = !out_in.has_value();
   L.err = g_err[dev.index()];
-  const long long bytes = kvs_attn4_scratch_bytes(&L);
+  const long long bytes = EIGHT ? kvs_attn8_scratch_bytes(&L) : kvs_attn4_scratch_bytes(&L);
   Tensor scratch;  // from the caching allocator: a captured graph has its own
   if (bytes > 0) {
     scratch = at::empty({bytes}, query.options().dtype(at::kByte));
     L.scratch = scratch.data_ptr();
   }
-  launched(kvs_attention_kv4(&L, at::cuda::getCurrentCUDAStream(dev.index()).stream()),
-           "attention_kv4");
+  void* const stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  launched(EIGHT ? kvs_attention_kv8(&L, stream) : kvs_attention_kv4(&L, stream), what);
   return {out, lse};
 }
 
@@ -375,5 +387,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                        const optional<Tensor>& out) {
     return read_rows<true>(cache, slots, torch::python::detail::py_object_to_dtype(dtype), out);
   });
-  m.def("attention_kv4", &attention_kv4);
+  m.def("attention_kv4", &attention<false>);
+  m.def("attention_kv8", &attention<true>);
 }

@@ -202,6 +202,24 @@ def attention_kv4(query: torch.Tensor, cache: torch.Tensor, block_table: torch.T
     allocator, so captured graphs do not share it.
     """
     args = (query, cache, block_table, seq_lens, query_start, max_query_len, scale, out,
-            return_lse)
+            return_lse, True)
     out, lse = _call("attention_kv4", query, args)
+    return (out, lse) if return_lse else out
+
+
+def attention_kv8(query: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
+                  seq_lens: torch.Tensor, query_start: Optional[torch.Tensor] = None,
+                  max_query_len: int = 1, scale: Optional[float] = None,
+                  out: Optional[torch.Tensor] = None, return_lse: bool = False, *,
+                  causal: bool = True):
+    """Attention of ``query`` ``[T, Hq, 128]`` (bf16 or fp16) over an 8-bit cache.
+
+    Arguments, results and errors are :func:`attention_kv4`'s.  With ``causal=False``
+    every query row sees all ``seq_lens[r]`` tokens of its sequence: cross attention to an
+    encoder's states, whose keys and values :func:`append_kv` has put into the cache (without
+    positions) and whose number has nothing to do with that of the query rows.
+    """
+    args = (query, cache, block_table, seq_lens, query_start, max_query_len, scale, out,
+            return_lse, causal)
+    out, lse = _call("attention_kv8", query, args)
     return (out, lse) if return_lse else out

@@ -97,3 +97,62 @@ def read(cache, slots):
 
 
 half_step = O.half_step
+
+
+def random_cache(g, nb, h, bs, spread=2):
+    """Rows like N(0, 1) with outlier key channels, under scales a few powers of two apart (CPU)."""
+    x = torch.randn((nb, h, 2 * bs, D), generator=g, dtype=torch.float64) * 40
+    x[:, :, :bs, :3] *= 4
+    cache = torch.zeros((nb, h, 2 * bs + 1, D), dtype=torch.uint8)
+    cache[:, :, :2 * bs] = codes(x.clamp(-448, 448))
+    cache[:, :, 2 * bs] = torch.randint(121 - spread, 122 + spread, (nb, h, D), generator=g,
+                                        dtype=torch.uint8)
+    return cache
+
+
+def attend(q, cache, table, lens, start, scale=None, causal=True, one_part=None):
+    """fp64 (out, lse, tolerance, lse's tolerance) of attention over an 8-bit cache (CPU); NaN rows
+    where no sequence has a row.  The tolerance, element by element, of an implementation that takes
+    products and sums in fp32 and weights in fp16, before the output's own rounding:
+      scores: 128 products summed in fp32, 2^-23 of the sum of their magnitudes an addition and 24 of
+        them in a chain (rounded up: 2^-18), which moves each weight by that share;
+      weights p 2^e (e the values' exponent): fp16's half step, 2^-11, of p |v|, or 2^-21 where fp16
+        takes two parts (fp16 outputs, unless ``one_part``); below fp16's normal range half of
+        2^-24 of a unit that is at most 2^-6 of the row's largest weight, times |code|;
+      exponentials, sums and the division: 2^-18 of p |v| together.
+    """
+    q64, table, lens = q.double(), table.long(), lens.long()
+    T, hq, _ = q.shape
+    bs, h = (cache.shape[2] - 1) // 2, cache.shape[1]
+    G = hq // h
+    scale = 1 / math.sqrt(D) if scale is None else scale
+    part = 2 ** -11 if (q.dtype == torch.bfloat16 if one_part is None else one_part) else 2 ** -21
+    starts = list(range(len(lens) + 1)) if start is None else start.tolist()
+    out = torch.full((T, hq, D), math.nan, dtype=torch.float64)
+    lse = torch.full((T, hq), math.nan, dtype=torch.float64)
+    tol, ltol = torch.zeros_like(out), torch.zeros_like(lse)
+    for r, n in enumerate(lens.tolist()):
+        a, b = starts[r], starts[r + 1]
+        t = torch.arange(n)
+        kv = read(cache, table[r][t // bs] * bs + t % bs).transpose(1, 2)  # [2, H, n, D]
+        k, v = kv[0], kv[1]
+        e = cache[table[r][t // bs], :, 2 * bs, 2 * (t % bs // UNIT) + 1].double().T - 127  # [H, n]
+        for i in range(b - a):
+            seen = max(0, n - (b - a) + i + 1) if causal else n
+            if seen == 0:
+                out[a + i], lse[a + i] = 0.0, -math.inf
+                continue
+            qi = q64[a + i].view(h, G, D)
+            w = torch.einsum("hgd,hld->hgl", qi, k[:, :seen]) * scale
+            werr = torch.einsum("hgd,hld->hgl", qi.abs(), k[:, :seen].abs()) * abs(scale) * 2 ** -18
+            z = torch.logsumexp(w, -1, keepdim=True)
+            p = torch.exp(w - z)
+            out[a + i] = torch.einsum("hgl,hld->hgd", p, v[:, :seen]).reshape(hq, D)
+            lse[a + i] = z.reshape(hq)
+            share = 2 * werr.amax(-1, keepdim=True) + 2 ** -18 + part
+            most = (p * 2.0 ** e[:, None, :seen]).amax(-1)
+            mag = (v[:, :seen] * 2.0 ** -e[:, :seen, None]).abs().sum(1)  # of the codes
+            tol[a + i] = (torch.einsum("hgl,hld->hgd", p * share, v[:, :seen].abs())
+                          + 2 ** -31 * most[..., None] * mag[:, None]).reshape(hq, D)
+            ltol[a + i] = (2 * werr.amax(-1) + 2 ** -18 + 2 ** -22 * z[..., 0].abs()).reshape(hq)
+    return out, lse, tol, ltol
