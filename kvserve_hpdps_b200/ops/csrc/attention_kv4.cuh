@@ -43,6 +43,11 @@ KVS_DEV Seq sequence(const Attn4Launch& L, int r, bool report) {
   return s;
 }
 
+// Tokens that row i of a sequence's query rows sees.
+KVS_DEV int seen_by(const Attn4Launch& L, const Seq& s, int i) {
+  return L.causal ? s.len - s.n + i + 1 : s.len;
+}
+
 // Rows [from, to) have no result: 16 bytes `at`, at + by, ... of them.  Called, not inlined: inside
 // the kernels it costs the registers of calls that clear nothing (drafts 55.7 us against 54.1).
 __device__ __noinline__ void clear_rows(const Attn4Launch& L, long long from, long long to, long long at,

@@ -601,6 +601,17 @@ Grid grid_of(const Attn4Launch* L) {
   return g;
 }
 
+// Whether a call goes to attention_kv8_tile.cu: many rows a kv head, and enough of them by what the
+// host knows (max_query_len, and the tokens that the table has room for).
+constexpr int kManyRows = 64;
+constexpr long long kMuchWork = 5ll << 20;
+bool many_rows(const Attn4Launch* L) {
+  const long long rows = static_cast<long long>(L->max_q) * (L->q_heads / L->heads);
+  const double work = static_cast<double>(rows) * L->seqs * L->heads * L->table_cols *
+                      L->block_size;
+  return rows > kManyRows && work > static_cast<double>(kMuchWork);
+}
+
 template <bool FP16, int NT, int RG>
 cudaError_t launch(const Attn4Launch& L, const Grid& g, const CUtensorMap& map, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(k_attn8<FP16, NT, RG>,
@@ -628,6 +639,7 @@ using namespace kvs;
 extern "C" {
 
 long long kvs_attn8_scratch_bytes(const Attn4Launch* L) {
+  if (many_rows(L)) return attn8_tile_scratch(*L);
   const Grid g = grid_of(L);
   return 16ll * g.ctas + 2ll * g.ctas * g.rows * (8 + 512);
 }
@@ -635,6 +647,7 @@ long long kvs_attn8_scratch_bytes(const Attn4Launch* L) {
 int kvs_attention_kv8(const Attn4Launch* L, void* stream) {
   if (L->seqs <= 0 || L->max_q <= 0 || L->tokens <= 0 || L->heads <= 0) return 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (many_rows(L)) return attn8_tile_launch(*L, s) == cudaSuccess ? 0 : -1;
   const Grid g = grid_of(L);
   if (!g.fits) return -2;
   Attn4Launch A = *L;

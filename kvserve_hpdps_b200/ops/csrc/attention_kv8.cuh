@@ -9,11 +9,6 @@ namespace kvs {
 
 namespace {
 
-// Tokens that row i of a sequence's query rows sees.
-KVS_DEV int seen_by(const Attn4Launch& L, const Seq& s, int i) {
-  return L.causal ? s.len - s.n + i + 1 : s.len;
-}
-
 // Rows of records as the copy engine sees them: 128 bytes, 2 bs + 1 rows, heads, blocks; boxes of
 // one unit, 16-byte chunks swizzled by the row.
 inline bool record_map(const Attn4Launch& L, CUtensorMap* map) {
@@ -42,5 +37,9 @@ KVS_DEV void load_rows(uint32_t dst, const CUtensorMap* map, int row, int head, 
 }
 
 }  // namespace
+
+// attention_kv8_tile.cu: many query rows a sequence.
+cudaError_t attn8_tile_launch(const Attn4Launch& L, cudaStream_t s);
+long long attn8_tile_scratch(const Attn4Launch& L);
 
 }  // namespace kvs

@@ -64,6 +64,18 @@ def _problem(seqs, hq, h, bs, dt, seed, spare_rows=0, cols_more=2, spread=2):
     return q, cache, table, lens, start
 
 
+def _tiles(table, rows, hq, h, bs):
+    """Whether a call takes the kernel for many rows, going by what the host knows: rows a kv
+    head, and rows times tokens that the table has room for."""
+    rows *= hq // h
+    return rows > 64 and rows * h * table.numel() * bs > 5 << 20
+
+
+def _wide(rows, seqs, hq, h, bs=16):
+    """Table columns that take a call of few tokens there all the same."""
+    return (6 << 20) // (rows * (hq // h) * h * seqs * bs) + 1
+
+
 def _attend(q, cache, table, lens, start=None, most=1, **kw):
     got = P.attention_kv8(q.cuda(), cache.cuda(), table.cuda(), lens.cuda(),
                           None if start is None else start.cuda(), most, return_lse=True, **kw)
@@ -98,13 +110,21 @@ SEVERAL = [
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("hq,h,seqs", SEVERAL)
 @pytest.mark.parametrize("causal", [True, False])
-def test_several_rows(dt, hq, h, seqs, causal):
+@pytest.mark.parametrize("wide", [False, True])
+def test_several_rows(dt, hq, h, seqs, causal, wide):
     most = max(n for n, _ in seqs)
-    q, cache, table, lens, start = _problem(seqs, hq, h, 16, dt, hq * 7, spare_rows=3)
+    if wide and most * (hq // h) <= 64:
+        pytest.skip("too few rows for the other kernel")
+    q, cache, table, lens, start = _problem(
+        seqs, hq, h, 16, dt, hq * 7, spare_rows=3,
+        cols_more=_wide(most, len(seqs), hq, h) if wide else 2)
+    tiles = _tiles(table, most, hq, h, 16)
+    assert tiles or not wide
     out = torch.full_like(q, 9.0).cuda()
     got, lse = _attend(q, cache, table, lens, start, most, out=out, causal=causal)
     assert got is out
-    _check(out, lse, O8.attend(q, cache, table, lens, start, causal=causal), dt)
+    ref = O8.attend(q, cache, table, lens, start, causal=causal, one_part=tiles or None)
+    _check(out, lse, ref, dt)
     assert (out[int(start[-1]):] == 9.0).all()  # rows of no sequence
     got, lse = _attend(q, cache, table, lens, start, most, causal=causal)
     assert not got[int(start[-1]):].any() and (lse[int(start[-1]):] == -math.inf).all()
@@ -112,37 +132,44 @@ def test_several_rows(dt, hq, h, seqs, causal):
 
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("hq,h,rows,n", [(28, 4, 1, 9001), (8, 8, 1, 5003), (28, 4, 4, 7000),
-                                         (8, 1, 7, 6007), (4, 4, 3, 8192)])
+                                         (8, 1, 7, 6007), (4, 4, 3, 8192), (28, 4, 150, 5000)])
 def test_long_sequences_are_split(dt, hq, h, rows, n):
     q, cache, table, lens, start = _problem([(rows, n), (1, 40), (rows, 3000)], hq, h, 32, dt, n)
-    ref = O8.attend(q, cache, table, lens, start)
+    tiles = _tiles(table, rows, hq, h, 32)
+    ref = O8.attend(q, cache, table, lens, start, one_part=tiles or None)
     first = _attend(q, cache, table, lens, start, rows)
     _check(*first, ref, dt)
     again = _attend(q, cache, table, lens, start, rows)  # nothing depends on timing
     assert all(torch.equal(a, b) for a, b in zip(first, again))
 
 
-@pytest.mark.parametrize("rows", [1, 5, 20])
+@pytest.mark.parametrize("rows", [1, 5, 20, 40])
 @pytest.mark.parametrize("dt", DTYPES)
 def test_scales_far_apart(dt, rows):
     """Units whose scales are up to 2^40 apart: a row's weight may lie on small ones, beside
     others that it sees with none and others that it does not see at all."""
     g = torch.Generator().manual_seed(rows)
-    q, cache, table, lens, start = _problem([(rows, 300), (rows, 200)], 8, 2, 16, dt, 91)
+    q, cache, table, lens, start = _problem([(rows, 300), (rows, 200)], 8, 2, 16, dt, 91,
+                                            cols_more=_wide(40, 2, 8, 2))
+    tiles = _tiles(table, rows, 8, 2, 16)
+    assert tiles == (rows == 40)
     up = torch.randint(-20, 20, (cache.shape[0], 2), generator=g)
     cache[:, :, 32, 1] = (cache[:, :, 32, 1] + up).to(torch.uint8)
     big = int(table[0, 18])  # the last tokens of sequence 0: only some rows see them
     cache[big, :, 32, 1] = 160
     huge = int(table[1, 2])  # keys that no row has weight on, with huge values
     cache[huge, :, :16] = torch.where(cache[huge, :, :16] >= 128, cache[huge, :, :16], 0)
-    ref = O8.attend(q, cache, table, lens, start)
+    ref = O8.attend(q, cache, table, lens, start, one_part=tiles or None)
     _check(*_attend(q, cache, table, lens, start, rows), ref, dt)
 
 
-def test_weight_on_small_scales():
+@pytest.mark.parametrize("rows", [1, 30])
+def test_weight_on_small_scales(rows):
     """All of a row's weight on a unit of tiny values, beside one of large ones without any."""
     dt = torch.bfloat16
-    q, cache, table, lens, _ = _problem([(1, 96)], 4, 1, 16, dt, 92)
+    q, cache, table, lens, start = _problem([(rows, 96)], 4, 1, 16, dt, 92,
+                                            cols_more=_wide(30, 1, 4, 1))
+    assert _tiles(table, rows, 4, 1, 16) == (rows == 30)
     q[:] = 1
     blocks = table[0][:6].long()
     cache[blocks, :, :16] = 0x28 + 0x80           # keys: a small negative number
@@ -150,30 +177,51 @@ def test_weight_on_small_scales():
     cache[blocks, :, 32, 0] = 130
     cache[blocks, :, 32, 1] = 127 + 15
     cache[blocks[3], :, 32, 1] = 127 - 15
-    ref = O8.attend(q, cache, table, lens, None)
-    _check(*_attend(q, cache, table, lens), ref, dt)
+    ref = O8.attend(q, cache, table, lens, start)
+    _check(*_attend(q, cache, table, lens, start, rows), ref, dt)
 
 
-@pytest.mark.parametrize("mag", [1e-30, 1e-6, 1e6, 1e30])
-def test_magnitudes_and_scale(mag):
+@pytest.mark.parametrize("rows", [1, 40])
+def test_values_of_zero_count_in_the_sum(rows):
+    """Units never written or of zeros, next to large ones: their tokens weigh as others do."""
     dt = torch.bfloat16
-    q, cache, table, lens, start = _problem([(9, 300), (2, 20)], 4, 2, 16, dt, 31)
+    q, cache, table, lens, start = _problem([(rows, 150), (rows, rows)], 8, 2, 16, dt, 44,
+                                            cols_more=_wide(40, 2, 8, 2))
+    assert _tiles(table, rows, 8, 2, 16) == (rows == 40)
+    cache[:, :, 32, 1] += 40
+    zero = table[0][2:9].long()  # tokens 32 to 143 of sequence 0
+    cache[zero, :, 16:32] = 0
+    cache[zero, :, 32, 1] = 17
+    cache[zero[3]] = 0
+    for scale in (0.1, 1e-37):
+        ref = O8.attend(q, cache, table, lens, start, scale=scale)
+        _check(*_attend(q, cache, table, lens, start, rows, scale=scale), ref, dt)
+
+
+@pytest.mark.parametrize("rows", [9, 90])
+@pytest.mark.parametrize("mag", [1e-30, 1e-6, 1e6, 1e30])
+def test_magnitudes_and_scale(mag, rows):
+    dt = torch.bfloat16
+    q, cache, table, lens, start = _problem([(rows, 300), (2, 20)], 4, 2, 16, dt, 31,
+                                            cols_more=_wide(90, 2, 4, 2))
+    assert _tiles(table, rows, 4, 2, 16) == (rows == 90)
     byte = round(math.log2(mag))
     cache[:, :, 32, 0::2] = (cache[:, :, 32, 0::2].int() - byte).clamp(17, 247).to(torch.uint8)
     cache[:, :, 32, 1::2] = (cache[:, :, 32, 1::2].int() + byte).clamp(17, 247).to(torch.uint8)
     q = (q.double() * mag).to(dt)
     for scale in (-0.11, 0.3):
         ref = O8.attend(q, cache, table, lens, start, scale=scale)
-        _check(*_attend(q, cache, table, lens, start, 9, scale=scale), ref, dt)
+        _check(*_attend(q, cache, table, lens, start, rows, scale=scale), ref, dt)
 
 
-@pytest.mark.parametrize("rows", [1, 9, 30])
+@pytest.mark.parametrize("rows", [1, 9, 30, 64])
 def test_not_a_number_reaches_those_that_see_it(rows):
     """NaN codes behind the length, in blocks of no sequence and behind a row's own position
     change nothing; one in a value that a row sees is NaN in that channel, one in a key in all."""
     dt, hq, h = torch.bfloat16, 8, 2
     q, cache, table, lens, start = _problem([(rows, 203), (rows, 100), (rows, 64)], hq, h, 16, dt,
-                                            rows + 50)
+                                            rows + 50, cols_more=_wide(30, 3, hq, h))
+    assert _tiles(table, rows, hq, h, 16) == (rows >= 30)
     used = torch.zeros(cache.shape[0], dtype=torch.bool)
     for r, n in enumerate(lens.tolist()):
         used[table[r, :(n + 15) // 16].long()] = True
@@ -235,10 +283,11 @@ def test_bad_blocks_and_extents():
 
 def test_more_sequences_than_threads():
     g = torch.Generator().manual_seed(3)
-    for first in (1, 6):
+    for first in (1, 6, 30):
         seqs = [(int(n > 0), n) for n in torch.randint(0, 60, (700,), generator=g).tolist()]
         seqs[3], seqs[650] = (0, 25), (first, 77)
         q, cache, table, lens, start = _problem(seqs, 4, 1, 16, torch.bfloat16, first)
+        assert _tiles(table, first, 4, 1, 16) == (first == 30)
         ref = O8.attend(q, cache, table, lens, start)
         _check(*_attend(q, cache, table, lens, start, first), ref, torch.bfloat16)
 
