@@ -647,12 +647,15 @@ long long kvs_attn8_scratch_bytes(const Attn4Launch* L) {
 int kvs_attention_kv8(const Attn4Launch* L, void* stream) {
   if (L->seqs <= 0 || L->max_q <= 0 || L->tokens <= 0 || L->heads <= 0) return 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (many_rows(L)) return attn8_tile_launch(*L, s) == cudaSuccess ? 0 : -1;
+  CUtensorMap map;
+  if (many_rows(L)) {
+    if (!record_map(*L, &map)) return -3;
+    return attn8_tile_launch(*L, map, s) == cudaSuccess ? 0 : -1;
+  }
   const Grid g = grid_of(L);
   if (!g.fits) return -2;
   Attn4Launch A = *L;
   A.whole = !g.split;
-  CUtensorMap map;
   if (!record_map(A, &map)) return -3;
   const cudaError_t e = L->fp16 ? launch_rows<true>(A, g, map, s) : launch_rows<false>(A, g, map, s);
   return e == cudaSuccess ? 0 : -1;

@@ -39,7 +39,7 @@ KVS_DEV void load_rows(uint32_t dst, const CUtensorMap* map, int row, int head, 
 }  // namespace
 
 // attention_kv8_tile.cu: many query rows a sequence.
-cudaError_t attn8_tile_launch(const Attn4Launch& L, cudaStream_t s);
+cudaError_t attn8_tile_launch(const Attn4Launch& L, const CUtensorMap& map, cudaStream_t s);
 long long attn8_tile_scratch(const Attn4Launch& L);
 
 }  // namespace kvs

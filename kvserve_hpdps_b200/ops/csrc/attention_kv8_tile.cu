@@ -1,14 +1,18 @@
 // Attention over a paged 8-bit cache for many query rows (prefill chunks, prompts' cross attention).
 //
 // The mathematics is attention_kv8.cu's; here 2 x 128 query rows (several tokens times the query
-// heads of one kv head) share each key, so the codes are turned into fp16 tiles once, for tcgen05:
-//   S = Q K^T, O += P V, fp16 products of 128 rows and 64 tokens into tensor memory.
-// fp16 holds every code exactly, so the tiles lose nothing whatever the scales of their tokens: a
+// heads of one kv head) share each key, on tcgen05:
+//   S = Q K^T, O += P V, products of 128 rows and 64 tokens into tensor memory.
+// K's codes are matrix operands as they are (kind::f8f6f4, fp32 sums: measured off by at most 2^-21.9 of
+// the sum of magnitudes).  A query row, scaled by a power of two to at most 448, is taken in e4m3
+// parts that add up to it: two for bf16 (4 + 4 bits), three for fp16, which is exact but for
+// elements below 2^-9 of the row's largest; those are off by 2^-10 where the largest is above 224.
+// V's codes become fp16 tiles, which hold every code exactly.  The scales stay out of the products: a
 // unit's key scale goes into the softmax's factor, its value scale b = 2^e into the weights,
 //   w = 2^(s - M + e - K),  l += 2^(K - e) w,  o = 2^K O / l,
 // M near the row's running maximum of s and K such that the largest w was 2^kAbove when it was set.
 //
-// The one rounding to fewer bits than fp32's is that of the weights to fp16, 2^-11, as the matrix
+// The other rounding to fewer bits than fp32's is that of the weights to fp16, 2^-11, as the matrix
 // instructions' A operand has to be of V's type; their sum is taken before that.  An fp16 output's
 // error grows by a third, a bf16 output's does not change; two parts of the weights would need
 // half as many products again and tensor memory, of which none is left.
@@ -16,11 +20,12 @@
 // Roles of a CTA (one an SM, 16 warps whose registers are dealt out anew):
 //   warps 0-3, 4-7   softmax of query tile 0, 1: a thread a row, which it reads from tensor memory
 //                    and writes back as fp16 weights, the A operand of O += P V
-//   warps 8-11       codes to fp16 tiles in shared memory, a warp two units, eight lanes a row
+//   warps 8-11       value codes to fp16 tiles in shared memory, a warp a unit of each half; warp 8
+//                    also asks the copy engine for all codes, ahead
 //   warps 12-15      issue the matrix instructions: S of tile 0, 1, O of tile 0, 1
-// The softmax warps take 64 tokens' scores at a time into registers, so that the next ones are
-// computed while they work.  O stays in tensor memory; it is rescaled by the softmax warps when 64
-// weights of a row sum up to more than kMostSum, which after the first tiles is rare.
+// All go by halves of 64 tokens.  The softmax warps take a half's scores into registers, so that the
+// next ones are computed while they work.  O stays in tensor memory; it is rescaled by the softmax
+// warps when 64 weights of a row sum up to more than kMostSum, which after the first tiles is rare.
 #include "attention_kv8.cuh"
 #include "attention_tile.cuh"
 
@@ -28,205 +33,288 @@ namespace kvs {
 
 namespace {
 
-constexpr uint32_t kHides = 1;
 // Units whose scale is less than 2^-kFar of K's weigh nothing beside it in fp16, but count in the sum.
 constexpr float kFar = 60.f;
-// A score is a factor times 128 products of less than 2^15 and 2^9.  Where the factor lets it pass
+// A score is a factor times 128 products of at most 2^9 and 2^9.  Where the factor lets it pass
 // 2^27, the product is rounded before the maximum is taken off: the fused multiply-add leaves the
 // maximum's own rounding over, up to 2^-25 of it, and weights are 2 to that from where they should
 // be (the same for all of a row's, so that 2^4 does no harm).
-constexpr float kHuge = 0x1p-4f;
+constexpr float kHuge = 0x1p2f;
+
+constexpr int kHalf = 64;                  // tokens
+constexpr int kCodes = kHalf * 128;        // bytes of a half's key or value codes
+constexpr int kValues = 2 * kHalf * 128;   // of its values as fp16
+constexpr int kPart = 128 * 128;           // of a part of a query tile
+constexpr int kNotes = 16;                 // halves that something is known of
+
+// RING halves' key codes and value codes are there or on their way, four halves' values as fp16.
+template <bool FP16>
+struct Room {
+  static constexpr int PARTS = FP16 ? 3 : 2, RING = FP16 ? 3 : 4;
+};
+constexpr int kTiles = 4;
 
 struct Ctrl {
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2][2], e_full[4];  // [tile][buffer]
+  uint64_t q_full[2], k_full[4], k_empty[4], v_came[4], v_taken[4], v_full[kTiles], v_empty[kTiles];
+  uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2][2], done[2], e_full[kNotes];
   uint32_t tmem;
-  // What the converting warps say of a step (ring of four):
-  float4 k_up[4][2];       // by halves, its four units: the keys' scale
-  float4 v_exp[4][2];      // and the exponent of the values'
-  uint32_t gone[4][4];     // by 32 tokens: those whose block does not exist
-  uint32_t bad[4][4];      // those with a value that is not a number
-  uint32_t flags[4][4];    // kHides: any of the two is set
-  uint4 poison[kRows];     // channels of a row that are not numbers
+  uint32_t any_bad;         // some half of this CTA had values that are not numbers
+  // What is known of a half, by units:
+  float4 k_up[kNotes];      // the keys' scale
+  float4 v_exp[kNotes];     // the exponent of the values'
+  uint32_t there[kNotes];   // bit u: the unit's block exists, bit 4 + u: it does not
+  uint16_t bad[kNotes][4];  // tokens with a value that is not a number
+  uint4 poison[kRows];      // channels of a row that are not numbers
   long long scan[kThreads / 32];
   int2 named[kThreads / 32];
   long long begin;
   int seq;
 };
 
-constexpr int kCtrlAt = 12 * kHalfTile;
-constexpr int kSmem = 1024 + kCtrlAt + static_cast<int>(sizeof(Ctrl));
-static_assert(kSmem <= 227 * 1024);
+template <bool FP16>
+struct Layout {
+  static constexpr int keys = 2 * Room<FP16>::PARTS * kPart, codes = keys + Room<FP16>::RING * kCodes,
+                       values = codes + Room<FP16>::RING * kCodes, ctrl = values + kTiles * kValues,
+                       bytes = 1024 + ctrl + static_cast<int>(sizeof(Ctrl));
+  static_assert(bytes <= 227 * 1024);
+};
+
+// A slot of a ring and the phase of its barriers.
+template <int N>
+struct Turn {
+  uint32_t slot = 0, phase = 0;
+  KVS_DEV void next() {
+    if (++slot == N) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// [rows][128 bytes], 16-byte chunks swizzled by the row.
+KVS_DEV uint32_t at128(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+
+// Bytes of a word that are not numbers: 1 in each.
+KVS_DEV uint32_t not_numbers(uint32_t w) {
+  return ((w & 0x7F7F7F7Fu) + 0x01010101u) >> 7 & 0x01010101u;
+}
 
 // ------------------------------------------------------------ codes to tiles
-// Tiles have two slots of 128 tokens, a step in each in turn.  A warp takes the 32 tokens of its
-// segment, four rows at a time: lane 8 i + c the 16 codes of chunk c, which become two chunks of fp16.
-KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* k_tile,
-                          uint8_t* v_tile, Ctrl* C) {
-  const int lane = threadIdx.x & 31, seg = (threadIdx.x >> 5) & 3, sub = lane >> 3, c = lane & 7;
-  uint32_t step_no = 0;
+template <bool FP16>
+KVS_DEV void convert_role(const Attn4Launch& L, const CUtensorMap* map, Walk walk, int group,
+                          uint8_t* smem, Ctrl* C) {
+  constexpr int RING = Room<FP16>::RING, AHEAD = RING - 1;
+  const int lane = threadIdx.x & 31, unit = (threadIdx.x >> 5) & 3, sub = lane >> 3, c = lane & 7;
+  Turn<RING> asks, comes;
+  Turn<kTiles> fills;
+  uint32_t asked = 0, half_no = 0;
   Piece p;
   // of the two fp16 chunks 2 c and 2 c + 1 the one whose place leaves no bank conflict goes first
-  const int swap = c >> 2;
+  const bool swap = c >= 4;
   while (walk.next(L, group, p)) {
     const uint8_t* const head = static_cast<const uint8_t*>(L.cache) + p.h * L.head_stride;
     const int32_t* const table = L.table + p.r * L.table_stride;
-    const uint8_t* rec[2] = {nullptr, nullptr};  // of a unit's first row; none: not there
-    uint32_t scale[2] = {0x7F7Fu, 0x7F7Fu};
-    uint32_t gone = 0;
-    int left = 0;  // tokens of the segment up to `stop`
-    auto locate = [&](int j) {
-      const int tok = p.start + j * kTile + 32 * seg;
-      left = p.stop - tok;
-      gone = 0;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        rec[u] = nullptr;
-        scale[u] = 0x7F7Fu;
-        if (left <= 16 * u) continue;
-        const int page = (tok + 16 * u) / L.block_size;
-        const int off = tok + 16 * u - page * L.block_size;
-        const int id = table[page];
+    // Blocks, places and scales of eight halves' units: of half lane / 4, unit lane % 4; and of the
+    // next eight's.
+    int id = -1, off = 0, id2 = -1, off2 = 0;
+    uint32_t scale = 0x7F7Fu, scale2 = 0x7F7Fu;
+    auto look = [&](int i, int& id, int& off) {  // from half i on
+      const int tok = p.start + (i + (lane >> 2)) * kHalf + kUnit8 * (lane & 3);
+      id = -1;
+      if (tok < p.stop) {
+        const int page = tok / L.block_size;
+        off = tok - page * L.block_size;
+        id = table[page];
         if (id < 0 || id >= L.num_blocks) {
-          if (lane == 0) record_error(L.err, ERR_BOUNDS);
-          gone |= 0xFFFFu << (16 * u);
-        } else {
-          const uint8_t* const at = head + id * L.block_stride;
-          scale[u] = *reinterpret_cast<const uint16_t*>(at + 256ll * L.block_size + (off >> 3));
-          rec[u] = at + off * 128;
+          record_error(L.err, ERR_BOUNDS);
+          id = -2;
         }
       }
     };
-    uint4 code[2][8];
-    auto load_codes = [&](int v) {
-      const long long plane = v ? 128ll * L.block_size : 0;
-#pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const int row = 4 * it + sub;
-        code[v][it] = make_uint4(0u, 0u, 0u, 0u);
-        if (rec[it >> 2] != nullptr && row < left)
-          code[v][it] = *reinterpret_cast<const uint4*>(rec[it >> 2] + plane +
-                                                        (row & 15) * 128 + 16 * c);
-      }
+    auto look_scale = [&](int id, int off, uint32_t& scale) {
+      scale = 0x7F7Fu;
+      if (id >= 0)
+        scale = *reinterpret_cast<const uint16_t*>(head + id * L.block_stride +
+                                                   256ll * L.block_size + (off >> 3));
     };
-    if (p.steps > 0) {
-      locate(0);
-      load_codes(0);
-      load_codes(1);
-    }
-    for (int j = 0; j < p.steps; ++j, ++step_no) {
-      // ---- values that are not numbers: zeros in the tile; rows that see them are marked
-      uint32_t nan = 0, bad = 0;
+    auto ask = [&](int i) -> bool {  // by warp 8: all codes of a half
+      const int at = i & 7;
+      if (i == 0) {
+        look(0, id, off);
+        look_scale(id, off, scale);
+      } else if (at == 0) {
+        id = id2;
+        off = off2;
+        scale = scale2;
+      } else if (at == 2) {
+        look(i + 6, id2, off2);
+      } else if (at == 5) {
+        look_scale(id2, off2, scale2);
+      }
+      if (asked >= RING && (!wait_phase(&C->k_empty[asks.slot], asks.phase ^ 1, L.err) ||
+                            !wait_phase(&C->v_taken[asks.slot], asks.phase ^ 1, L.err)))
+        return false;
+      // lane 4 v + u: unit u's keys (v = 0) or values
+      const int from = 4 * at + (lane & 3), v = lane >> 2 & 1;
+      const int block = __shfl_sync(0xFFFFFFFFu, id, from);
+      const int place = __shfl_sync(0xFFFFFFFFu, off, from);
+      const uint32_t sc = __shfl_sync(0xFFFFFFFFu, scale, from);
+      const uint32_t has = __ballot_sync(0xFFFFFFFFu, block >= 0) & 15u;
+      const uint32_t lost = __ballot_sync(0xFFFFFFFFu, block == -2) & 15u;
+      const uint32_t note = asked % kNotes;
+      if (lane < 4) {
+        reinterpret_cast<float*>(&C->k_up[note])[lane] = __uint_as_float((sc & 0xFFu) << 23);
+        reinterpret_cast<float*>(&C->v_exp[note])[lane] =
+            static_cast<float>(static_cast<int>(sc >> 8) - 127);
+        C->bad[note][lane] = 0;
+      }
+      if (lane == 0) C->there[note] = has | lost << 4;
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&C->k_full[asks.slot], __popc(has) * (kUnit8 * 128));
+        mbar_arrive_expect_tx(&C->v_came[asks.slot], __popc(has) * (kUnit8 * 128));
+        mbar_arrive(&C->e_full[note]);
+      }
+      __syncwarp();
+      if (lane < 8 && block >= 0)
+        load_rows(smem_u32(smem) + (v ? Layout<FP16>::codes : Layout<FP16>::keys) +
+                      asks.slot * kCodes + (lane & 3) * (kUnit8 * 128),
+                  map, v * L.block_size + place, p.h, block,
+                  v ? &C->v_came[asks.slot] : &C->k_full[asks.slot]);
+      asks.next();
+      ++asked;
+      return true;
+    };
+    if (unit == 0)
+      for (int i = 0; i < AHEAD && i < p.halves; ++i)
+        if (!ask(i)) return;
+    for (int i = 0; i < p.halves; ++i, ++half_no) {
+      if (unit == 0 && i + AHEAD < p.halves && !ask(i + AHEAD)) return;
+      if (!wait_phase(&C->v_came[comes.slot], comes.phase, L.err)) return;
+      const int left = p.stop - (p.start + i * kHalf + kUnit8 * unit);
+      const bool there = C->there[half_no % kNotes] >> unit & 1u;
+      uint4 w[4];
+      uint32_t nan = 0;
 #pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const uint4& w = code[1][it];
-        nan |= (w.x & 0x7F7F7F7Fu) + 0x01010101u;
-        nan |= (w.y & 0x7F7F7F7Fu) + 0x01010101u;
-        nan |= (w.z & 0x7F7F7F7Fu) + 0x01010101u;
-        nan |= (w.w & 0x7F7F7F7Fu) + 0x01010101u;
+      for (int it = 0; it < 4; ++it) {
+        const int row = 4 * it + sub;
+        w[it] = make_uint4(0u, 0u, 0u, 0u);
+        if (there && row < left)
+          w[it] = *reinterpret_cast<const uint4*>(smem + Layout<FP16>::codes + comes.slot * kCodes +
+                                                  at128(kUnit8 * unit + row, c));
+        nan |= (w[it].x & 0x7F7F7F7Fu) + 0x01010101u;
+        nan |= (w[it].y & 0x7F7F7F7Fu) + 0x01010101u;
+        nan |= (w[it].z & 0x7F7F7F7Fu) + 0x01010101u;
+        nan |= (w[it].w & 0x7F7F7F7Fu) + 0x01010101u;
       }
       if (__any_sync(0xFFFFFFFFu, nan & 0x80808080u)) {
+        // values that are not numbers: zeros in the tile; rows that see them are marked
+        uint32_t bad = 0;
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          uint32_t w[4] = {code[1][it].x, code[1][it].y, code[1][it].z, code[1][it].w}, any = 0;
+        for (int it = 0; it < 4; ++it) {
+          uint32_t y[4] = {w[it].x, w[it].y, w[it].z, w[it].w}, any = 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t is = ((w[i] & 0x7F7F7F7Fu) + 0x01010101u) >> 7 & 0x01010101u;
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t is = not_numbers(y[k]);
             any |= is;
-            w[i] &= ~(is * 0xFFu);
+            y[k] &= ~(is * 0xFFu);
           }
-          code[1][it] = make_uint4(w[0], w[1], w[2], w[3]);
+          w[it] = make_uint4(y[0], y[1], y[2], y[3]);
           const uint32_t rows = __ballot_sync(0xFFFFFFFFu, any != 0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (rows >> (8 * i) & 0xFFu) bad |= 1u << (4 * it + i);
+          for (int k = 0; k < 4; ++k)
+            if (rows >> (8 * k) & 0xFFu) bad |= 1u << (4 * it + k);
+        }
+        if (lane == 0) {
+          C->bad[half_no % kNotes][unit] = static_cast<uint16_t>(bad);
+          C->any_bad = 1;
         }
       }
-      const int ring = step_no & 3;
-      if (lane == 0) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&C->v_taken[comes.slot]);
+      comes.next();
+      if (half_no >= kTiles && !wait_phase(&C->v_empty[fills.slot], fills.phase ^ 1, L.err)) return;
+      uint8_t* const dst = smem + Layout<FP16>::values + fills.slot * kValues;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          reinterpret_cast<float*>(C->k_up[ring])[2 * seg + u] =
-              __uint_as_float((scale[u] & 0xFFu) << 23);
-          reinterpret_cast<float*>(C->v_exp[ring])[2 * seg + u] =
-              static_cast<float>(static_cast<int>(scale[u] >> 8) - 127);
-        }
-        C->gone[ring][seg] = gone;
-        C->bad[ring][seg] = bad;
-        C->flags[ring][seg] = gone | bad ? kHides : 0u;
-        mbar_arrive(&C->e_full[ring]);
+      for (int it = 0; it < 4; ++it) {
+        const uint32_t a0 = swap ? w[it].z : w[it].x, a1 = swap ? w[it].w : w[it].y,
+                       b0 = swap ? w[it].x : w[it].z, b1 = swap ? w[it].y : w[it].w;
+        // channels 64 (c / 4) + ...: two blocks of 64 channels, rows of 128 bytes
+        uint8_t* const block = dst + (c >> 2) * (kHalf * 128);
+        const int row = kUnit8 * unit + 4 * it + sub, chunk = 2 * (c & 3);
+        *reinterpret_cast<uint4*>(block + at128(row, chunk + swap)) =
+            make_uint4(half2_low8(a0), half2_high8(a0), half2_low8(a1), half2_high8(a1));
+        *reinterpret_cast<uint4*>(block + at128(row, chunk + 1 - swap)) =
+            make_uint4(half2_low8(b0), half2_high8(b0), half2_low8(b1), half2_high8(b1));
       }
-      if (j + 1 < p.steps) locate(j + 1);  // its loads go out as registers become free
-      const uint32_t slot = step_no & 1, again = (step_no >> 1 & 1) ^ 1;
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        uint64_t* const empty = v ? &C->v_empty[slot] : &C->k_empty[slot];
-        if (!wait_phase(empty, again, L.err)) return;
-        uint8_t* const dst = (v ? v_tile : k_tile) + slot * 2 * kHalfTile;
-#pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          const uint4 w = code[v][it];
-          const uint4 lo = make_uint4(half2_low8(w.x), half2_high8(w.x), half2_low8(w.y),
-                                      half2_high8(w.y)),
-                      hi = make_uint4(half2_low8(w.z), half2_high8(w.z), half2_low8(w.w),
-                                      half2_high8(w.w));
-          const int row = 32 * seg + 4 * it + sub;
-          *reinterpret_cast<uint4*>(dst + chunk_at(row, 2 * c + swap)) = swap ? hi : lo;
-          *reinterpret_cast<uint4*>(dst + chunk_at(row, 2 * c + 1 - swap)) = swap ? lo : hi;
-        }
-        if (j + 1 < p.steps) load_codes(v);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(v ? &C->v_full[slot] : &C->k_full[slot]);
-      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&C->v_full[fills.slot]);
+      fills.next();
     }
   }
 }
 
 // ------------------------------------------------------ matrix instructions
-// Four warps issue them, one a query tile x and product, each on a scheduler of its own: all
-// from one warp, its scheduler's two softmax warps were a third slower than the others.
+KVS_DEV void mma_codes(uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%1, %4};\n\tmov.b64 y, {%2, %4};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], x, y, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(kIdescQK), "n"(kDescHigh), "r"(accumulate)  // e4m3's number is fp16's, 0
+      : "memory");
+}
+// Values: 64 channels a block, blocks 8 KB apart (leading offset).
+KVS_DEV uint32_t values_desc(uint32_t saddr) {
+  return (saddr >> 4) | (static_cast<uint32_t>(kHalf * 128 >> 4) << 16);
+}
+
+// Four warps issue them, one a query tile x and product, each on a scheduler of its own.
 //
 // Scores of half i + 1 are asked for as soon as the softmax warps have those of half i in their
 // registers, so they find them ready when they are through; the weights have two buffers of
-// their own.  A stage is free when both tiles' products with it are done; without a second tile
+// their own.  A slot is free when both tiles' products with it are done; without a second tile
 // its warps only say so.
-template <bool QK>
-KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, int x, uint32_t q_tile,
-                      uint32_t kv_tile, uint32_t tmem, Ctrl* C) {
-  uint32_t step_no = 0, piece_no = 0, half_no = 0;
+template <bool FP16, bool QK>
+KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, int x, uint32_t smem,
+                      uint32_t tmem, Ctrl* C) {
+  constexpr int PARTS = Room<FP16>::PARTS, N = QK ? Room<FP16>::RING : kTiles;
+  uint32_t piece_no = 0, half_no = 0, all = 0;
+  Turn<N> turn;
   Piece p;
-  const uint32_t qd = uniform(k_desc(q_tile) + x * (2 * kHalfTile >> 4)),
-                 kvd = uniform(QK ? k_desc(kv_tile) : mn_desc(kv_tile)),
+  const uint32_t qd = uniform(k_desc(smem + x * PARTS * kPart)),
+                 kvd = uniform(QK ? k_desc(smem + Layout<FP16>::keys)
+                                  : values_desc(smem + Layout<FP16>::values)),
                  scores = uniform(tmem + 64 * x), weights = uniform(tmem + kWeightsAt + 64 * x),
                  result = uniform(tmem + kOutAt + 128 * x);
+  uint64_t *const fulls = QK ? C->k_full : C->v_full, *const empties = QK ? C->k_empty : C->v_empty;
   while (walk.next(L, group, p)) {
     if (p.steps == 0) continue;
     const int H = static_cast<int>(uniform(p.halves));
     const bool idle = x == 1 && !p.two;
     if (QK && !idle && !KVS_WAIT(&C->q_full[x], piece_no++ & 1)) return;
-    uint64_t *const fulls = QK ? C->k_full : C->v_full, *const empties = QK ? C->k_empty : C->v_empty;
-    for (int i = 0; i < H; ++i) {
-      const uint32_t no = step_no + (i >> 1), slot = no & 1;
-      const bool last = (i & 1) || i == H - 1;  // half of the slot
-      if (!(i & 1) && !KVS_WAIT(&fulls[slot], (no >> 1) & 1)) return;
-      uint64_t* const empty = &empties[slot];
+    for (int i = 0; i < H; ++i, ++all) {
+      if (!KVS_WAIT(&fulls[turn.slot], turn.phase)) return;
+      uint64_t* const empty = &empties[turn.slot];
+      const uint32_t b = kvd + turn.slot * ((QK ? kCodes : kValues) >> 4);
+      turn.next();
       if (idle) {
-        if (last && (threadIdx.x & 31) == 0) mbar_arrive(empty);
+        if ((threadIdx.x & 31) == 0) mbar_arrive(empty);
         continue;
       }
-      const uint32_t b = kvd + slot * (2 * kHalfTile >> 4) + (i & 1) * (8192 >> 4);
       if constexpr (QK) {
         if (i > 0 && !KVS_WAIT(&C->s_free[x], (half_no - 1) & 1)) return;
         tc_fence_after();
         if (elected()) {
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks) {
-            const uint32_t off = ((ks >> 2) * kHalfTile + (ks & 3) * 32) >> 4;
-            mma_qk<kDescHigh>(scores, qd + off, b + off, ks > 0 ? 1u : 0u);
-          }
+          for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              mma_codes(scores, qd + ((part * kPart + ks * 32) >> 4), b + (ks * 32 >> 4),
+                        part + ks > 0 ? 1u : 0u);
           umma_commit(&C->s_full[x]);
-          if (last) umma_commit(empty);
+          umma_commit(empty);
         }
       } else {
         const uint32_t buf = half_no & 1;
@@ -234,41 +322,44 @@ KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, int x, uint32_
         tc_fence_after();
         if (elected()) {
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {  // 16 tokens: two groups of eight rows, 8 columns of P
+          for (int ks = 0; ks < 4; ++ks)  // 16 tokens: two groups of eight rows, 8 columns of P
             mma_pv(result, weights + 32 * buf + 8 * ks, b + ks * (2048 >> 4),
                    ks > 0 || i > 0 ? 1u : 0u);
-          }
           umma_commit(&C->pv_done[x][buf]);
-          if (last) umma_commit(empty);
+          umma_commit(empty);
         }
       }
       __syncwarp();
       ++half_no;
     }
-    // the last half's scores were taken, too: one phase of s_free a half
-    if (QK && !idle && !KVS_WAIT(&C->s_free[x], (half_no - 1) & 1)) return;
-    step_no += p.steps;
+    // The last half's scores were taken, too: one phase of s_free a half.  And not on to pieces without
+    // this tile, which free slots as they come, before its softmax has read what is known of this one's.
+    if (QK && !idle && (!KVS_WAIT(&C->s_free[x], (half_no - 1) & 1) ||
+                        !KVS_WAIT(&C->done[x], (piece_no - 1) & 1)))
+      return;
   }
   // The last products' commits arrive on their own: not after the CTA has gone.
-  for (uint32_t back = 1; back < 3 && step_no >= back; ++back) {
-    const uint32_t no = step_no - back, slot = no & 1;
-    if (!KVS_WAIT(QK ? &C->k_empty[slot] : &C->v_empty[slot], (no >> 1) & 1)) return;
+  for (int back = 0; back < N && all > 0; ++back, --all) {
+    turn.slot = turn.slot == 0 ? N - 1 : turn.slot - 1;
+    if (turn.slot == N - 1) turn.phase ^= 1;
+    if (!KVS_WAIT(&empties[turn.slot], turn.phase)) return;
   }
 }
 
 // ------------------------------------------------------------------ softmax
 template <bool FP16>
-KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q_tile,
+KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* smem,
                           uint32_t tmem, const Parts& P, Ctrl* C) {
   const int x = threadIdx.x >> 7, row = threadIdx.x & 127;
   const uint32_t lanes = static_cast<uint32_t>((threadIdx.x >> 5) & 3) << 21;  // a warp's 32
   const uint32_t S = tmem + 64 * x + lanes, O = tmem + kOutAt + 128 * x + lanes;
-  uint8_t* const qt = q_tile + x * 2 * kHalfTile;
-  uint32_t step_no = 0, half_no = 0;
+  constexpr int PARTS = Room<FP16>::PARTS;
+  uint8_t* const qt = smem + x * PARTS * kPart;
+  uint32_t notes = 0, half_no = 0;  // halves before this piece; this tile's
   Piece p;
   while (walk.next(L, group, p)) {
     if (x == 1 && !p.two) {
-      step_no += p.steps;
+      notes += p.halves;
       continue;
     }
     const int rr = p.tile * kRows + x * 128 + row;
@@ -279,7 +370,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
     float m = kLowest, l = 0.f, f = 0.f, K = -120.f;
     bool poisoned = false;
     if (p.steps > 0) {
-      // ---- the row as fp16, scaled by a power of two: largest element in [2^14, 2^15)
+      // ---- the row scaled by a power of two, its largest element in (224, 448], in e4m3 parts
       uint4 raw[16] = {};
       if (mine) {
         const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(L.q) +
@@ -295,19 +386,32 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
 #pragma unroll
         for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(y[k]));
       }
-      int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-      e = top == 0.f ? 0 : max(kLowestExp, min(e, 100));
-      const float up = pow2(14 - e) * (L.scale < 0.f ? -1.f : 1.f);
-      f = fabsf(L.scale) * 1.4426950408889634f * pow2(e - 14);
+      const int e = min(scale_exponent(__float_as_uint(top)), 120);
+      // an infinite element makes the row what is not a number
+      const float up = top < INFINITY ? pow2(-e) * (L.scale < 0.f ? -1.f : 1.f)
+                                      : __uint_as_float(0x7FC00000u);
+      f = fabsf(L.scale) * 1.4426950408889634f * pow2(e);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float y[8];
-        unpack8<FP16>(raw[i], y);
+      for (int i = 0; i < 8; ++i) {  // 16 channels
+        float y[16];
+        unpack8<FP16>(raw[2 * i], *reinterpret_cast<float(*)[8]>(y));
+        unpack8<FP16>(raw[2 * i + 1], *reinterpret_cast<float(*)[8]>(y + 8));
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] *= up;
-        *reinterpret_cast<uint4*>(qt + chunk_at(row, i)) =
-            make_uint4(half2_bits(y[0], y[1]), half2_bits(y[2], y[3]), half2_bits(y[4], y[5]),
-                       half2_bits(y[6], y[7]));
+        for (int k = 0; k < 16; ++k) y[k] *= up;
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          uint32_t four[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            four[k] = codes8x4(y + 4 * k);
+            float z[4];
+            values8x4(four[k], z);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) y[4 * k + n] -= z[n];  // what the part leaves over, exactly
+          }
+          *reinterpret_cast<uint4*>(qt + part * kPart + at128(row, i)) =
+              make_uint4(four[0], four[1], four[2], four[3]);
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -318,29 +422,58 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
       // tokens that every row of this warp sees
       const int all_see = __reduce_min_sync(0xFFFFFFFFu, mine ? max(seen, 0) : 0x7FFFFFFF);
       const int plain_to = min(all_see, p.stop);
-      // what the converting warps say of half i's tokens, read a half ahead
+      // what is known of half i's tokens, read a half ahead
       struct {
-        uint32_t flag;
+        uint32_t there, any_bad;
         float4 v_exp, k_up;
       } said;
       auto listen = [&](int i) {
-        const uint32_t ring = (step_no + (i >> 1)) & 3, half = i & 1;
-        said.flag = C->flags[ring][2 * half] | C->flags[ring][2 * half + 1];
-        said.v_exp = C->v_exp[ring][half];
-        said.k_up = C->k_up[ring][half];
+        const uint32_t note = (notes + i) % kNotes;
+        said.there = C->there[note];
+        said.any_bad = C->any_bad;
+        said.v_exp = C->v_exp[note];
+        said.k_up = C->k_up[note];
       };
-      // The first scores' barrier before the converting warps' one: tile 1 walks past pieces
-      // without a second tile and waits for nothing there, so it can be many steps ahead, and a
-      // parity cannot tell the phase wanted from the one two before it.  Once the scores are there,
-      // e_full is past this step and cannot be a phase further.
+      auto visible = [&](int i, int u, uint32_t there) {  // of a unit's tokens, by this row
+        const int n = min(seen, p.stop) - p.start - kHalf * i - kUnit8 * u;
+        return n <= 0 || (there >> (4 + u) & 1u) ? 0u : n >= 16 ? 0xFFFFu : (1u << n) - 1u;
+      };
+      // The row sees tokens of half i with values that are not numbers: which, from their codes.
+      auto mark = [&](int i) {
+        const uint32_t note = (notes + i) % kNotes;
+        for (int u = 0; u < 4; ++u) {
+          for (uint32_t b = C->bad[note][u] & visible(i, u, C->there[note]); b != 0; b &= b - 1) {
+            const int tok = p.start + kHalf * i + kUnit8 * u + __ffs(b) - 1;
+            const int page = tok / L.block_size;
+            const uint32_t* const codes = reinterpret_cast<const uint32_t*>(
+                static_cast<const uint8_t*>(L.cache) +
+                L.table[p.r * L.table_stride + page] * L.block_stride + p.h * L.head_stride +
+                (L.block_size + tok - page * L.block_size) * 128ll);
+            uint32_t* const to = reinterpret_cast<uint32_t*>(&C->poison[x * 128 + row]);
+#pragma unroll 1
+            for (int w = 0; w < 4; ++w) {
+              uint32_t bits = poisoned ? to[w] : 0u;
+#pragma unroll 1
+              for (int k = 0; k < 8; ++k)
+                bits |= (not_numbers(codes[8 * w + k]) * 0x01020408u >> 24 & 15u) << (4 * k);
+              to[w] = bits;
+            }
+            poisoned = true;
+          }
+        }
+      };
+      // The first scores' barrier before the notes' one: tile 1 walks past pieces without a second
+      // tile and waits for nothing there, so it can be many halves ahead, and a parity cannot
+      // tell the phase wanted from the one two before it.  Once the scores are there, e_full
+      // is past this half and cannot be a phase further.
       if (!KVS_WAIT(&C->s_full[x], half_no & 1)) return;
-      if (!KVS_WAIT(&C->e_full[step_no & 3], (step_no >> 2) & 1)) return;
+      if (!KVS_WAIT(&C->e_full[notes % kNotes], (notes / kNotes) & 1)) return;
       listen(0);
       uint32_t s_ready = 1;
       for (int i = 0; i < p.halves; ++i, ++half_no) {
-        const int ring = (step_no + (i >> 1)) & 3, seg0 = 2 * (i & 1), t0 = p.start + 64 * i;
+        const int t0 = p.start + kHalf * i;
         const uint32_t buf = half_no & 1, W = tmem + kWeightsAt + 64 * x + 32 * buf + lanes;
-        const uint32_t flag = said.flag;
+        const uint32_t there = said.there, any_bad = said.any_bad;
         const float ev[4] = {said.v_exp.x, said.v_exp.y, said.v_exp.z, said.v_exp.w};
         const float up4[4] = {said.k_up.x, said.k_up.y, said.k_up.z, said.k_up.w};
         float fs[4];
@@ -354,58 +487,27 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         tmem_ld32_start(S + 32, v[1]);
         // Asked long before the answers are needed: a wait costs 140 clocks even when it is over.
         const bool next = i + 1 < p.halves;
-        const uint32_t no = step_no + ((i + 1) >> 1);  // of the next half
+        const uint32_t no = notes + i + 1;  // of the next half
         const uint32_t ahead =
             peek_phase(&C->pv_done[x][buf], ((half_no >> 1) & 1) ^ 1) &
-            ((i & 1) && next ? peek_phase(&C->e_full[no & 3], (no >> 2) & 1) : 1u);
+            (next ? peek_phase(&C->e_full[no % kNotes], (no / kNotes) & 1) : 1u);
         tmem_arrived(v[0]);
         tmem_arrived(v[1]);
         tc_fence_before();
         __syncwarp();
         if ((threadIdx.x & 31) == 0) mbar_arrive(&C->s_free[x]);
         const bool huge = fmaxf(fmaxf(up4[0], up4[1]), fmaxf(up4[2], up4[3])) > up_most;
-        if (t0 + 64 > plain_to || flag != 0 || huge) {  // hidden scores become -inf
-          if (huge) {
+        if (t0 + kHalf > plain_to || there >> 4 != 0 || huge) {  // hidden scores become -inf
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+          for (int u = 0; u < 4; ++u) {
+            const uint32_t vis = visible(i, u, there);
 #pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                uint32_t& y = v[u >> 1][16 * (u & 1) + k];
-                y = __float_as_uint(__fmul_rn(__uint_as_float(y), fs[u]));
-              }
-              fs[u] = 1.f;
+            for (int k = 0; k < 16; ++k) {
+              uint32_t& y = v[u >> 1][16 * (u & 1) + k];
+              if (huge) y = __float_as_uint(__fmul_rn(__uint_as_float(y), fs[u]));
+              y = vis >> k & 1u ? y : 0xFF800000u;
             }
-          }
-#pragma unroll
-          for (int sg = 0; sg < 2; ++sg) {
-            const int n = min(seen, p.stop) - t0 - 32 * sg;
-            uint32_t vis = n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
-            vis &= ~C->gone[ring][seg0 + sg];
-#pragma unroll
-            for (int k = 0; k < 32; ++k) v[sg][k] = vis >> k & 1u ? v[sg][k] : 0xFF800000u;
-            if (flag) {
-              for (uint32_t b = C->bad[ring][seg0 + sg] & vis; b != 0; b &= b - 1) {
-                // the row sees a token with values that are not numbers: which, from its codes
-                const int tok = t0 + 32 * sg + __ffs(b) - 1, page = tok / L.block_size;
-                const uint4* const codes = reinterpret_cast<const uint4*>(
-                    static_cast<const uint8_t*>(L.cache) +
-                    L.table[p.r * L.table_stride + page] * L.block_stride + p.h * L.head_stride +
-                    (L.block_size + tok - page * L.block_size) * 128ll);
-                uint32_t* const to = reinterpret_cast<uint32_t*>(&C->poison[x * 128 + row]);
-#pragma unroll 1
-                for (int w = 0; w < 4; ++w) {
-                  uint32_t bits = poisoned ? to[w] : 0u;
-#pragma unroll 1
-                  for (int k = 0; k < 8; ++k) {
-                    const uint32_t four = reinterpret_cast<const uint32_t*>(codes)[8 * w + k];
-                    const uint32_t is = ((four & 0x7F7F7F7Fu) + 0x01010101u) >> 7 & 0x01010101u;
-                    bits |= ((is * 0x01020408u) >> 24 & 15u) << (4 * k);
-                  }
-                  to[w] = bits;
-                }
-                poisoned = true;
-              }
-            }
+            if (huge) fs[u] = 1.f;
           }
         }
         // Against the reference that there is, the scores only pass through once; a row whose
@@ -495,9 +597,10 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         if (!ready) {
           // the products with the weights two halves ago; what is said of the next half
           if (!KVS_WAIT(&C->pv_done[x][buf], ((half_no >> 1) & 1) ^ 1)) return;
-          if ((i & 1) && next && !KVS_WAIT(&C->e_full[no & 3], (no >> 2) & 1)) return;
+          if (next && !KVS_WAIT(&C->e_full[no % kNotes], (no / kNotes) & 1)) return;
         }
         tc_fence_after();
+        if (any_bad && i >= 3) mark(i - 3);  // whose values were converted when any_bad was read
         if (next) listen(i + 1);
         s_ready = next ? peek_phase(&C->s_full[x], (half_no + 1) & 1) : 0u;
         tmem_st16(W, h[0]);
@@ -507,12 +610,16 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
         __syncwarp();
         if ((threadIdx.x & 31) == 0) mbar_arrive(&C->p_full[x][half_no & 1]);
       }
-      step_no += p.steps;
       for (int back = p.halves > 1 ? 2 : 1; back > 0; --back) {  // both buffers' last products
         const uint32_t no = half_no - back;
         if (!KVS_WAIT(&C->pv_done[x][no & 1], (no >> 1) & 1)) return;
       }
       tc_fence_after();
+      if (C->any_bad)
+        for (int i = max(0, p.halves - 3); i < p.halves; ++i) mark(i);
+      notes += p.halves;
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&C->done[x]);
     }
     // ---- the result, or this part of it
     const float unit = p.steps > 0 ? pow2(static_cast<int>(K)) : 0.f;
@@ -571,13 +678,11 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
 }
 
 template <bool FP16>
-__global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constant__ Attn4Launch L) {
+__global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constant__ Attn4Launch L, const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t *const q_tile = smem, *const k_tile = smem + 4 * kHalfTile,
-                 *const v_tile = smem + 8 * kHalfTile;
-  Ctrl* const C = reinterpret_cast<Ctrl*>(smem + kCtrlAt);
+  Ctrl* const C = reinterpret_cast<Ctrl*>(smem + Layout<FP16>::ctrl);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = L.q_heads / L.heads, B = gridDim.x, b = blockIdx.x;
   const Parts P = parts(L.scratch, B, kRows);
@@ -586,18 +691,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constan
     P.desc[b] = make_int4(-1, 0, 0, 0);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&C->q_full[i], 4);
-      mbar_init(&C->k_full[i], 4);
-      mbar_init(&C->k_empty[i], 2);
-      mbar_init(&C->v_full[i], 4);
-      mbar_init(&C->v_empty[i], 2);
       mbar_init(&C->s_full[i], 1);
       mbar_init(&C->s_free[i], 4);
+      mbar_init(&C->done[i], 4);
       for (int k = 0; k < 2; ++k) {
         mbar_init(&C->p_full[i][k], 4);
         mbar_init(&C->pv_done[i][k], 1);
       }
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&C->e_full[i], 4);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&C->k_full[i], 1);
+      mbar_init(&C->k_empty[i], 2);
+      mbar_init(&C->v_came[i], 1);
+      mbar_init(&C->v_taken[i], 4);
+      mbar_init(&C->v_full[i], 4);
+      mbar_init(&C->v_empty[i], 2);
+    }
+    for (int i = 0; i < kNotes; ++i) mbar_init(&C->e_full[i], 1);
+    C->any_bad = 0;
     fence_mbar_init();
   }
   if (warp == 12) tmem_alloc(&C->tmem, 512);
@@ -659,19 +770,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constan
     __syncthreads();
     walk.r = C->seq;
     walk.begin = C->begin;
-    // 256 x 168 + 128 x 104 + 128 x 72 = the 512 x 128 registers of the launch
+    // 256 x 184 + 256 x 72 = the 512 x 128 registers of the launch
     if (warp < 8) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-      softmax_role<FP16>(L, walk, group, q_tile, tmem, P, C);
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+      softmax_role<FP16>(L, walk, group, smem, tmem, P, C);
     } else if (warp < 12) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-      convert_role(L, walk, group, k_tile, v_tile, C);
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+      convert_role<FP16>(L, &map, walk, group, smem, C);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
       if (warp < 14)
-        mma_role<true>(L, walk, group, warp & 1, smem_u32(q_tile), smem_u32(k_tile), tmem, C);
+        mma_role<FP16, true>(L, walk, group, warp & 1, smem_u32(smem), tmem, C);
       else
-        mma_role<false>(L, walk, group, warp & 1, smem_u32(q_tile), smem_u32(v_tile), tmem, C);
+        mma_role<FP16, false>(L, walk, group, warp & 1, smem_u32(smem), tmem, C);
     }
   }
   __syncwarp();
@@ -682,20 +793,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constan
 }
 
 template <bool FP16>
-cudaError_t launch(const Attn4Launch& L, cudaStream_t s) {
+cudaError_t launch(const Attn4Launch& L, const CUtensorMap& map, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(k_attn8_tile<FP16>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<FP16>::bytes);
   if (e != cudaSuccess) return e;
   const int ctas = tile_ctas(L);
-  k_attn8_tile<FP16><<<ctas, kThreads, kSmem, s>>>(L);
+  k_attn8_tile<FP16><<<ctas, kThreads, Layout<FP16>::bytes, s>>>(L, map);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   return launch_combine<FP16, kRows / 8, 1>(L, ctas, s);
 }
 
 }  // namespace
 
-cudaError_t attn8_tile_launch(const Attn4Launch& L, cudaStream_t s) {
-  return L.fp16 ? launch<true>(L, s) : launch<false>(L, s);
+cudaError_t attn8_tile_launch(const Attn4Launch& L, const CUtensorMap& map, cudaStream_t s) {
+  return L.fp16 ? launch<true>(L, map, s) : launch<false>(L, map, s);
 }
 
 long long attn8_tile_scratch(const Attn4Launch& L) {
