@@ -20,8 +20,8 @@
 // Roles of a CTA (one an SM, 16 warps whose registers are dealt out anew):
 //   warps 0-3, 4-7   softmax of query tile 0, 1: a thread a row, which it reads from tensor memory
 //                    and writes back as fp16 weights, the A operand of O += P V
-//   warps 8-11       value codes to fp16 tiles in shared memory, a warp a unit of each half; warp 8
-//                    also asks the copy engine for all codes, ahead
+//   warps 8-11       ask the copy engine for codes, ahead, and turn the values' into fp16 tiles in
+//                    shared memory, a warp a unit of each half
 //   warps 12-15      issue the matrix instructions: S of tile 0, 1, O of tile 0, 1
 // All go by halves of 64 tokens.  The softmax warps take a half's scores into registers, so that the
 // next ones are computed while they work.  O stays in tensor memory; it is rescaled by the softmax
@@ -55,14 +55,14 @@ struct Room {
 constexpr int kTiles = 4;
 
 struct Ctrl {
-  uint64_t q_full[2], k_full[4], k_empty[4], v_came[4], v_taken[4], v_full[kTiles], v_empty[kTiles];
-  uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2][2], done[2], e_full[kNotes];
+  uint64_t q_full[2], k_full[4], k_empty[4], v_came[4][4], v_full[kTiles], v_empty[kTiles];
+  uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2][2], done[2];
   uint32_t tmem;
   uint32_t any_bad;         // some half of this CTA had values that are not numbers
   // What is known of a half, by units:
   float4 k_up[kNotes];      // the keys' scale
   float4 v_exp[kNotes];     // the exponent of the values'
-  uint32_t there[kNotes];   // bit u: the unit's block exists, bit 4 + u: it does not
+  uint32_t gone[kNotes];    // a byte a unit: 1 if its block does not exist
   uint16_t bad[kNotes][4];  // tokens with a value that is not a number
   uint4 poison[kRows];      // channels of a row that are not numbers
   long long scan[kThreads / 32];
@@ -107,19 +107,18 @@ KVS_DEV void convert_role(const Attn4Launch& L, const CUtensorMap* map, Walk wal
   const int lane = threadIdx.x & 31, unit = (threadIdx.x >> 5) & 3, sub = lane >> 3, c = lane & 7;
   Turn<RING> asks, comes;
   Turn<kTiles> fills;
-  uint32_t asked = 0, half_no = 0;
+  uint32_t asked = 0, half_no = 0, has = 0;  // has: slots that hold codes
   Piece p;
   // of the two fp16 chunks 2 c and 2 c + 1 the one whose place leaves no bank conflict goes first
   const bool swap = c >= 4;
   while (walk.next(L, group, p)) {
     const uint8_t* const head = static_cast<const uint8_t*>(L.cache) + p.h * L.head_stride;
     const int32_t* const table = L.table + p.r * L.table_stride;
-    // Blocks, places and scales of eight halves' units: of half lane / 4, unit lane % 4; and of the
-    // next eight's.
+    // Blocks, places and scales of this warp's unit in 32 halves, a lane each; and in the next 32.
     int id = -1, off = 0, id2 = -1, off2 = 0;
     uint32_t scale = 0x7F7Fu, scale2 = 0x7F7Fu;
     auto look = [&](int i, int& id, int& off) {  // from half i on
-      const int tok = p.start + (i + (lane >> 2)) * kHalf + kUnit8 * (lane & 3);
+      const int tok = p.start + (i + lane) * kHalf + kUnit8 * unit;
       id = -1;
       if (tok < p.stop) {
         const int page = tok / L.block_size;
@@ -137,8 +136,8 @@ KVS_DEV void convert_role(const Attn4Launch& L, const CUtensorMap* map, Walk wal
         scale = *reinterpret_cast<const uint16_t*>(head + id * L.block_stride +
                                                    256ll * L.block_size + (off >> 3));
     };
-    auto ask = [&](int i) -> bool {  // by warp 8: all codes of a half
-      const int at = i & 7;
+    auto ask = [&](int i) -> bool {  // for the unit's codes in half i
+      const int at = i & 31;
       if (i == 0) {
         look(0, id, off);
         look_scale(id, off, scale);
@@ -146,53 +145,44 @@ KVS_DEV void convert_role(const Attn4Launch& L, const CUtensorMap* map, Walk wal
         id = id2;
         off = off2;
         scale = scale2;
-      } else if (at == 2) {
-        look(i + 6, id2, off2);
-      } else if (at == 5) {
+      } else if (at == 16) {
+        look(i + 16, id2, off2);
+      } else if (at == 24) {
         look_scale(id2, off2, scale2);
       }
-      if (asked >= RING && (!wait_phase(&C->k_empty[asks.slot], asks.phase ^ 1, L.err) ||
-                            !wait_phase(&C->v_taken[asks.slot], asks.phase ^ 1, L.err)))
-        return false;
-      // lane 4 v + u: unit u's keys (v = 0) or values
-      const int from = 4 * at + (lane & 3), v = lane >> 2 & 1;
-      const int block = __shfl_sync(0xFFFFFFFFu, id, from);
-      const int place = __shfl_sync(0xFFFFFFFFu, off, from);
-      const uint32_t sc = __shfl_sync(0xFFFFFFFFu, scale, from);
-      const uint32_t has = __ballot_sync(0xFFFFFFFFu, block >= 0) & 15u;
-      const uint32_t lost = __ballot_sync(0xFFFFFFFFu, block == -2) & 15u;
-      const uint32_t note = asked % kNotes;
-      if (lane < 4) {
-        reinterpret_cast<float*>(&C->k_up[note])[lane] = __uint_as_float((sc & 0xFFu) << 23);
-        reinterpret_cast<float*>(&C->v_exp[note])[lane] =
+      if (asked >= RING && !wait_phase(&C->k_empty[asks.slot], asks.phase ^ 1, L.err)) return false;
+      const int block = __shfl_sync(0xFFFFFFFFu, id, at);
+      const int place = __shfl_sync(0xFFFFFFFFu, off, at);
+      const uint32_t sc = __shfl_sync(0xFFFFFFFFu, scale, at);
+      const uint32_t note = asked % kNotes, bytes = block >= 0 ? kUnit8 * 128 : 0;
+      if (elected()) {
+        uint64_t *const k_bar = &C->k_full[asks.slot], *const v_bar = &C->v_came[unit][asks.slot];
+        reinterpret_cast<float*>(&C->k_up[note])[unit] = __uint_as_float((sc & 0xFFu) << 23);
+        reinterpret_cast<float*>(&C->v_exp[note])[unit] =
             static_cast<float>(static_cast<int>(sc >> 8) - 127);
-        C->bad[note][lane] = 0;
+        reinterpret_cast<uint8_t*>(&C->gone[note])[unit] = block == -2 ? 1 : 0;
+        C->bad[note][unit] = 0;
+        mbar_arrive_expect_tx(k_bar, bytes);
+        mbar_arrive_expect_tx(v_bar, bytes);
+        if (block >= 0) {
+          const uint32_t at = smem_u32(smem) + asks.slot * kCodes + unit * (kUnit8 * 128);
+          load_rows(at + Layout<FP16>::keys, map, place, p.h, block, k_bar);
+          load_rows(at + Layout<FP16>::codes, map, L.block_size + place, p.h, block, v_bar);
+        }
       }
-      if (lane == 0) C->there[note] = has | lost << 4;
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&C->k_full[asks.slot], __popc(has) * (kUnit8 * 128));
-        mbar_arrive_expect_tx(&C->v_came[asks.slot], __popc(has) * (kUnit8 * 128));
-        mbar_arrive(&C->e_full[note]);
-      }
-      __syncwarp();
-      if (lane < 8 && block >= 0)
-        load_rows(smem_u32(smem) + (v ? Layout<FP16>::codes : Layout<FP16>::keys) +
-                      asks.slot * kCodes + (lane & 3) * (kUnit8 * 128),
-                  map, v * L.block_size + place, p.h, block,
-                  v ? &C->v_came[asks.slot] : &C->k_full[asks.slot]);
+      has = (has & ~(1u << asks.slot)) | (block >= 0 ? 1u : 0u) << asks.slot;
       asks.next();
       ++asked;
       return true;
     };
-    if (unit == 0)
-      for (int i = 0; i < AHEAD && i < p.halves; ++i)
-        if (!ask(i)) return;
+    for (int i = 0; i < AHEAD && i < p.halves; ++i)
+      if (!ask(i)) return;
     for (int i = 0; i < p.halves; ++i, ++half_no) {
-      if (unit == 0 && i + AHEAD < p.halves && !ask(i + AHEAD)) return;
-      if (!wait_phase(&C->v_came[comes.slot], comes.phase, L.err)) return;
+      if (i + AHEAD < p.halves && !ask(i + AHEAD)) return;
+      if (!wait_phase(&C->v_came[unit][comes.slot], comes.phase, L.err)) return;
       const int left = p.stop - (p.start + i * kHalf + kUnit8 * unit);
-      const bool there = C->there[half_no % kNotes] >> unit & 1u;
+      const bool there = has >> comes.slot & 1u;
       uint4 w[4];
       uint32_t nan = 0;
 #pragma unroll
@@ -230,8 +220,7 @@ KVS_DEV void convert_role(const Attn4Launch& L, const CUtensorMap* map, Walk wal
           C->any_bad = 1;
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&C->v_taken[comes.slot]);
+      __syncwarp();  // the slot is free
       comes.next();
       if (half_no >= kTiles && !wait_phase(&C->v_empty[fills.slot], fills.phase ^ 1, L.err)) return;
       uint8_t* const dst = smem + Layout<FP16>::values + fills.slot * kValues;
@@ -422,27 +411,15 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* s
       // tokens that every row of this warp sees
       const int all_see = __reduce_min_sync(0xFFFFFFFFu, mine ? max(seen, 0) : 0x7FFFFFFF);
       const int plain_to = min(all_see, p.stop);
-      // what is known of half i's tokens, read a half ahead
-      struct {
-        uint32_t there, any_bad;
-        float4 v_exp, k_up;
-      } said;
-      auto listen = [&](int i) {
-        const uint32_t note = (notes + i) % kNotes;
-        said.there = C->there[note];
-        said.any_bad = C->any_bad;
-        said.v_exp = C->v_exp[note];
-        said.k_up = C->k_up[note];
-      };
-      auto visible = [&](int i, int u, uint32_t there) {  // of a unit's tokens, by this row
+      auto visible = [&](int i, int u, uint32_t gone) {  // of a unit's tokens, by this row
         const int n = min(seen, p.stop) - p.start - kHalf * i - kUnit8 * u;
-        return n <= 0 || (there >> (4 + u) & 1u) ? 0u : n >= 16 ? 0xFFFFu : (1u << n) - 1u;
+        return n <= 0 || (gone >> (8 * u) & 1u) ? 0u : n >= 16 ? 0xFFFFu : (1u << n) - 1u;
       };
       // The row sees tokens of half i with values that are not numbers: which, from their codes.
       auto mark = [&](int i) {
         const uint32_t note = (notes + i) % kNotes;
         for (int u = 0; u < 4; ++u) {
-          for (uint32_t b = C->bad[note][u] & visible(i, u, C->there[note]); b != 0; b &= b - 1) {
+          for (uint32_t b = C->bad[note][u] & visible(i, u, C->gone[note]); b != 0; b &= b - 1) {
             const int tok = p.start + kHalf * i + kUnit8 * u + __ffs(b) - 1;
             const int page = tok / L.block_size;
             const uint32_t* const codes = reinterpret_cast<const uint32_t*>(
@@ -462,45 +439,38 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* s
           }
         }
       };
-      // The first scores' barrier before the notes' one: tile 1 walks past pieces without a second
-      // tile and waits for nothing there, so it can be many halves ahead, and a parity cannot
-      // tell the phase wanted from the one two before it.  Once the scores are there, e_full
-      // is past this half and cannot be a phase further.
       if (!KVS_WAIT(&C->s_full[x], half_no & 1)) return;
-      if (!KVS_WAIT(&C->e_full[notes % kNotes], (notes / kNotes) & 1)) return;
-      listen(0);
       uint32_t s_ready = 1;
       for (int i = 0; i < p.halves; ++i, ++half_no) {
         const int t0 = p.start + kHalf * i;
         const uint32_t buf = half_no & 1, W = tmem + kWeightsAt + 64 * x + 32 * buf + lanes;
-        const uint32_t there = said.there, any_bad = said.any_bad;
-        const float ev[4] = {said.v_exp.x, said.v_exp.y, said.v_exp.z, said.v_exp.w};
-        const float up4[4] = {said.k_up.x, said.k_up.y, said.k_up.z, said.k_up.w};
-        float fs[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)  // not zero: a hidden score is -inf times it
-          fs[u] = fmaxf(f * up4[u], 1.17549435e-38f);
         if (!__all_sync(0xFFFFFFFFu, s_ready) && !KVS_WAIT(&C->s_full[x], half_no & 1)) return;
         tc_fence_after();
         uint32_t v[2][32];
         tmem_ld32_start(S, v[0]);
         tmem_ld32_start(S + 32, v[1]);
-        // Asked long before the answers are needed: a wait costs 140 clocks even when it is over.
+        // what is known of the half was written before its codes were asked for
+        const uint32_t note = (notes + i) % kNotes, gone = C->gone[note], any_bad = C->any_bad;
+        const float4 v_exp = C->v_exp[note], k_up = C->k_up[note];
+        const float ev[4] = {v_exp.x, v_exp.y, v_exp.z, v_exp.w};
+        const float up4[4] = {k_up.x, k_up.y, k_up.z, k_up.w};
+        float fs[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)  // not zero: a hidden score is -inf times it
+          fs[u] = fmaxf(f * up4[u], 1.17549435e-38f);
+        // Asked long before the answer is needed: a wait costs 140 clocks even when it is over.
         const bool next = i + 1 < p.halves;
-        const uint32_t no = notes + i + 1;  // of the next half
-        const uint32_t ahead =
-            peek_phase(&C->pv_done[x][buf], ((half_no >> 1) & 1) ^ 1) &
-            (next ? peek_phase(&C->e_full[no % kNotes], (no / kNotes) & 1) : 1u);
+        const uint32_t ahead = peek_phase(&C->pv_done[x][buf], ((half_no >> 1) & 1) ^ 1);
         tmem_arrived(v[0]);
         tmem_arrived(v[1]);
         tc_fence_before();
         __syncwarp();
         if ((threadIdx.x & 31) == 0) mbar_arrive(&C->s_free[x]);
         const bool huge = fmaxf(fmaxf(up4[0], up4[1]), fmaxf(up4[2], up4[3])) > up_most;
-        if (t0 + kHalf > plain_to || there >> 4 != 0 || huge) {  // hidden scores become -inf
+        if (t0 + kHalf > plain_to || gone != 0 || huge) {  // hidden scores become -inf
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const uint32_t vis = visible(i, u, there);
+            const uint32_t vis = visible(i, u, gone);
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               uint32_t& y = v[u >> 1][16 * (u & 1) + k];
@@ -594,14 +564,10 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* s
           if (ready || !__any_sync(0xFFFFFFFFu, all > kMostSum)) break;
         }
         l += sum;
-        if (!ready) {
-          // the products with the weights two halves ago; what is said of the next half
-          if (!KVS_WAIT(&C->pv_done[x][buf], ((half_no >> 1) & 1) ^ 1)) return;
-          if (next && !KVS_WAIT(&C->e_full[no % kNotes], (no / kNotes) & 1)) return;
-        }
+        // the products with the weights two halves ago
+        if (!ready && !KVS_WAIT(&C->pv_done[x][buf], ((half_no >> 1) & 1) ^ 1)) return;
         tc_fence_after();
         if (any_bad && i >= 3) mark(i - 3);  // whose values were converted when any_bad was read
-        if (next) listen(i + 1);
         s_ready = next ? peek_phase(&C->s_full[x], (half_no + 1) & 1) : 0u;
         tmem_st16(W, h[0]);
         tmem_st16(W + 16, h[1]);
@@ -700,14 +666,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constan
       }
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&C->k_full[i], 1);
+      mbar_init(&C->k_full[i], 4);
       mbar_init(&C->k_empty[i], 2);
-      mbar_init(&C->v_came[i], 1);
-      mbar_init(&C->v_taken[i], 4);
+      for (int k = 0; k < 4; ++k) mbar_init(&C->v_came[i][k], 1);
       mbar_init(&C->v_full[i], 4);
       mbar_init(&C->v_empty[i], 2);
     }
-    for (int i = 0; i < kNotes; ++i) mbar_init(&C->e_full[i], 1);
     C->any_bad = 0;
     fence_mbar_init();
   }
