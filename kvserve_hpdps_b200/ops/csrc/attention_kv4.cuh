@@ -160,6 +160,16 @@ KVS_DEV uint32_t transpose8(uint32_t a) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
+// One lane of a whole warp.
+KVS_DEV bool elected() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
+}
 // CTA b's share of a line of length U dealt to B: [begin(b), begin(b + 1)).
 struct Deal {
   int each, more;  // U / B, U % B

@@ -69,9 +69,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  __shared__ __align__(16) uint8_t s_scale[kStages][2][16];
   __shared__ uint64_t s_full[kStages], s_empty[kStages];
-  __shared__ uint32_t s_note[kStages];  // halves that are there, and where their scales are
+  __shared__ uint2 s_note[kStages];  // the two units' scale bytes; bit 0, 1: the unit is there
   __shared__ int s_scan[kWarps], s_begin, s_seq;
   __shared__ float2 s_ml[TS][ROWS];
   __shared__ int2 s_named[kWarps];
@@ -91,6 +90,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     }
     fence_mbar_init();
   }
+  if (tid == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)));
   int U = 0, mine = 0;
   Named named;
   for (int r = tid; r < L.seqs; r += kWarps * 32) {
@@ -99,53 +99,67 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     mine = work_of<UNIT>(L, s, ROWS, group).units;
     U += mine;
   }
+  auto scan = [&](int x) {  // the sum of the warp's up to this lane
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) U += __shfl_xor_sync(0xFFFFFFFFu, U, o);
-  if (lane == 0) s_scan[warp] = U;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+      if (lane >= o) x += y;
+    }
+    return x;
+  };
+  int inc = scan(U);
+  if (lane == 31) s_scan[warp] = inc;
   named.leave(L, s_named);
   __syncthreads();
   named.clear<kWarps>(L, s_named);
   U = 0;
+  int before = inc;  // of the line up to this thread's sequence (if there are no more than threads)
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) U += s_scan[w];
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += s_scan[w];
+    U += s_scan[w];
+  }
   constexpr int kLeastUnits = kLeast / UNIT, kFewUnits = kFew / UNIT, kOverUnits = kOver / UNIT;
   const int used = min(B, L.whole ? U / (1 + kOverUnits)  // an item a CTA
                                   : max((U + kLeastUnits - 1) / kLeastUnits,
                                         min(kSpread, (U + kFewUnits - 1) / kFewUnits)));
   if (b >= used) return;
   const Deal deal{U / used, U % used};
-  int pos = deal.begin(b), base = 0;
+  int pos = deal.begin(b);
   const int end = deal.begin(b + 1);
-  for (int r0 = 0; r0 < L.seqs; r0 += kWarps * 32) {
-    const int r = r0 + tid;
-    if (L.seqs > kWarps * 32)  // else `mine` is it
+  if (L.seqs <= kWarps * 32) {
+    if (before - mine <= pos && pos < before) {
+      s_seq = tid;
+      s_begin = before - mine;
+    }
+  } else {
+    int base = 0;
+    for (int r0 = 0; r0 < L.seqs; r0 += kWarps * 32) {
+      const int r = r0 + tid;
       mine = r < L.seqs ? work_of<UNIT>(L, sequence(L, r, false), ROWS, group).units : 0;
-    int inc = mine;
+      inc = scan(mine);
+      __syncthreads();
+      if (lane == 31) s_scan[warp] = inc;
+      __syncthreads();
+      before = base + inc;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-      if (lane >= o) inc += x;
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += s_scan[w];
+        base += s_scan[w];
+      }
+      if (before - mine <= pos && pos < before) {
+        s_seq = r;
+        s_begin = before - mine;
+      }
+      if (pos < base) break;  // the same for every thread
     }
-    __syncthreads();
-    if (lane == 31) s_scan[warp] = inc;
-    __syncthreads();
-    int before = base;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += s_scan[w];
-      base += s_scan[w];
-    }
-    if (before + inc - mine <= pos && pos < before + inc) {
-      s_seq = r;
-      s_begin = before + inc - mine;
-    }
-    if (pos < base) break;  // the same for every thread
   }
   __syncthreads();
   int r = s_seq;
   int begin = s_begin;  // of sequence r on the line
 
   const int stage0 = split * ST;
+  const bool wide = L.block_size % kStep == 0;  // the tensor map's boxes are of 32 rows
   uint32_t asked = 0, taken = 0;  // steps of this ring
   bool lost = false;              // a copy did not come: nothing is waited for any more
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -191,48 +205,74 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     const int stop = L.whole ? limit : min(limit, (unit0 + units) * UNIT);
     const int steps = first < stop ? (stop - first + UNIT - 1) / UNIT : 0;
     const int32_t* const table = L.table + r * L.table_stride;
-    int ids = -1, offs = 0;  // of step k % 16 = lane / 2, half lane % 2
+    const uint8_t* const head = static_cast<const uint8_t*>(L.cache) + h * L.head_stride;
+    // Blocks, places and scales of 16 steps' units: of step lane / 2, half lane % 2; and of the next 16's.
+    int ids = -1, ids2 = -1, offs = 0, offs2 = 0;
+    uint32_t scale = 0, scale2 = 0;
+    auto look = [&](int k, int& ids, int& offs) {  // from step k on
+      const int tok = first + (k + (lane >> 1)) * UNIT + kUnit8 * (lane & 1);
+      ids = -1;
+      if (tok < stop) {
+        const int page = tok / L.block_size;
+        offs = tok - page * L.block_size;
+        ids = table[page];
+        if (ids < 0 || ids >= L.num_blocks) {
+          record_error(L.err, ERR_BOUNDS);
+          ids = -1;
+        }
+      }
+    };
+    auto look_scale = [&](int ids, int offs, uint32_t& scale) {
+      if (ids >= 0)
+        scale = *reinterpret_cast<const uint16_t*>(head + ids * L.block_stride +
+                                                   256ll * L.block_size + (offs >> 3));
+    };
     auto ask = [&](int k) {  // by one warp of a ring
       const uint32_t slot = asked % ST;
       if (RG > 1 && asked >= ST) wait(&s_empty[stage0 + slot], (asked / ST - 1) & 1);
       ++asked;
-      if ((k & 15) == 0) {
-        const int tok = first + (k + (lane >> 1)) * UNIT + 16 * (lane & 1);
-        ids = -1;
-        if (tok < stop) {
-          const int page = tok / L.block_size;
-          offs = tok - page * L.block_size;
-          ids = table[page];
-          if (ids < 0 || ids >= L.num_blocks) {
-            record_error(L.err, ERR_BOUNDS);
-            ids = -1;
-          }
-        }
+      const int step = k & 15;
+      if (k == 0) {
+        look(0, ids, offs);
+        look_scale(ids, offs, scale);
+      } else if (step == 0) {
+        ids = ids2;
+        offs = offs2;
+        scale = scale2;
+      } else if (step == 8) {
+        look(k + 8, ids2, offs2);
+      } else if (step == 12) {
+        look_scale(ids2, offs2, scale2);
       }
-      // lanes 0..2: keys, values and scales of the first half; 3..5: of the second
-      const int hf = lane >= 3 ? 1 : 0, from = 2 * (k & 15) + hf;
-      const int id = __shfl_sync(0xFFFFFFFFu, ids, from);
-      const int off = __shfl_sync(0xFFFFFFFFu, offs, from);
-      const uint32_t there = __ballot_sync(0xFFFFFFFFu, id >= 0 && lane < 6);
-      const uint32_t had = (there & 1u) | (there >> 2 & 2u);
-      const int other = __shfl_sync(0xFFFFFFFFu, off, 3);
-      if (lane == 0) {
-        s_note[stage0 + slot] = had | (off >> 3 & 14) << 8 | (other >> 3 & 14) << 16;
-        mbar_arrive_expect_tx(&s_full[stage0 + slot], __popc(had) * (4096 + 16));
+      uint64_t* const bar = &s_full[stage0 + slot];
+      const int id0 = __shfl_sync(0xFFFFFFFFu, ids, 2 * step);
+      const int id1 = __shfl_sync(0xFFFFFFFFu, ids, 2 * step + 1);
+      const int off0 = __shfl_sync(0xFFFFFFFFu, offs, 2 * step);
+      const int off1 = __shfl_sync(0xFFFFFFFFu, offs, 2 * step + 1);
+      if (elected()) {  // one lane: copies by several are issued one after the other, 200 clocks each
+        const uint32_t to = smem_u32(smem) + (stage0 + slot) * kStage;
+        // with wide boxes both units are in one block; a second one behind the end hides itself
+        const int halves = wide ? 2 * (id0 >= 0) : (id0 >= 0) + (id1 >= 0);
+        mbar_expect_tx(bar, halves * (kStage / 2));
+        if (id0 >= 0) {
+          load_rows(to, &map, off0, h, id0, bar);
+          load_rows(to + 4096, &map, L.block_size + off0, h, id0, bar);
+        }
+        if (id1 >= 0 && !wide) {
+          load_rows(to + 2048, &map, off1, h, id1, bar);
+          load_rows(to + 6144, &map, L.block_size + off1, h, id1, bar);
+        }
       }
       __syncwarp();
-      if (lane < 6 && id >= 0) {
-        const int what = lane - 3 * hf;
-        if (what < 2) {
-          load_rows(smem_u32(smem) + (stage0 + slot) * kStage + what * 4096 + hf * 2048, &map,
-                    what * L.block_size + off, h, id, &s_full[stage0 + slot]);
-        } else {
-          const uint8_t* const rec =
-              static_cast<const uint8_t*>(L.cache) + id * L.block_stride + h * L.head_stride;
-          bulk_load(s_scale[stage0 + slot][hf], rec + 256ll * L.block_size + (off >> 3 & ~15), 16,
-                    &s_full[stage0 + slot]);
-        }
+      // the scales, which an item's first copies need not wait for
+      const uint32_t sc0 = __shfl_sync(0xFFFFFFFFu, scale, 2 * step);
+      const uint32_t sc1 = __shfl_sync(0xFFFFFFFFu, scale, 2 * step + 1);
+      if (elected()) {
+        s_note[stage0 + slot] =
+            make_uint2(sc0 | sc1 << 16, (id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u));
+        mbar_arrive(bar);
       }
+      __syncwarp();
     };
     if (rg == 0)
       for (int k = 0; k < AHEAD && k < steps; ++k) ask(k);
@@ -299,13 +339,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       }
     }
 
-    auto step = [&](auto tag, int t0, const uint8_t* st, uint32_t stage, uint32_t note) {
+    auto step = [&](auto tag, int t0, const uint8_t* st, uint32_t scales, uint32_t note) {
       constexpr bool MASKED = decltype(tag)::value;
       float sc[2][NT][4], ev[2], fv[2], top[2][NT][2];
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const uint32_t two = *reinterpret_cast<const uint16_t*>(
-            &s_scale[stage][hf][note >> (8 + 8 * hf) & 14]);
+        const uint32_t two = scales >> (16 * hf) & 0xFFFFu;
         const float fk = __uint_as_float((two & 0xFFu) << 23);
         fv[hf] = __uint_as_float(two >> 8 << 23);
         ev[hf] = static_cast<float>(static_cast<int>(two >> 8) - 127);
@@ -494,12 +533,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       wait(&s_full[stage], (taken / ST) & 1);
       ++taken;
       const int t0 = first + k * UNIT;
-      const uint32_t note = s_note[stage];
+      const uint2 note = s_note[stage];
       if (row0 < nrows) {
-        if ((note & 3u) != 3u || t0 + kStep > min_seen)
-          step(std::true_type{}, t0, smem + stage * kStage, stage, note);
+        if (note.y != 3u || t0 + kStep > min_seen)
+          step(std::true_type{}, t0, smem + stage * kStage, note.x, note.y);
         else
-          step(std::false_type{}, t0, smem + stage * kStage, stage, note);
+          step(std::false_type{}, t0, smem + stage * kStage, note.x, note.y);
       }
       __syncwarp();  // the stage may be overwritten
       if (RG > 1 && lane == 0) mbar_arrive(&s_empty[stage]);
@@ -649,14 +688,14 @@ int kvs_attention_kv8(const Attn4Launch* L, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   CUtensorMap map;
   if (many_rows(L)) {
-    if (!record_map(*L, &map)) return -3;
+    if (!record_map(*L, kUnit8, &map)) return -3;
     return attn8_tile_launch(*L, map, s) == cudaSuccess ? 0 : -1;
   }
   const Grid g = grid_of(L);
   if (!g.fits) return -2;
   Attn4Launch A = *L;
   A.whole = !g.split;
-  if (!record_map(A, &map)) return -3;
+  if (!record_map(A, A.block_size % kStep == 0 ? kStep : kUnit8, &map)) return -3;
   const cudaError_t e = L->fp16 ? launch_rows<true>(A, g, map, s) : launch_rows<false>(A, g, map, s);
   return e == cudaSuccess ? 0 : -1;
 }

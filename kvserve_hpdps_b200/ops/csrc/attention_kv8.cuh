@@ -10,8 +10,8 @@ namespace kvs {
 namespace {
 
 // Rows of records as the copy engine sees them: 128 bytes, 2 bs + 1 rows, heads, blocks; boxes of
-// one unit, 16-byte chunks swizzled by the row.
-inline bool record_map(const Attn4Launch& L, CUtensorMap* map) {
+// `rows` rows, 16-byte chunks swizzled by the row.
+inline bool record_map(const Attn4Launch& L, unsigned rows, CUtensorMap* map) {
   const EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return false;
   const cuuint64_t record = 128ull * (2 * L.block_size + 1);
@@ -21,10 +21,16 @@ inline bool record_map(const Attn4Launch& L, CUtensorMap* map) {
   const cuuint64_t strides[3] = {128,
                                  L.heads > 1 ? static_cast<cuuint64_t>(L.head_stride) : record,
                                  L.num_blocks > 1 ? static_cast<cuuint64_t>(L.block_stride) : record};
-  const cuuint32_t box[4] = {128, kUnit8, 1, 1}, step[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {128, rows, 1, 1}, step[4] = {1, 1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(L.cache), dims, strides, box,
             step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Bytes that a phase waits for, beside its arrivals.
+KVS_DEV void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+               "r"(bytes)
+               : "memory");
 }
 KVS_DEV void load_rows(uint32_t dst, const CUtensorMap* map, int row, int head, int block,
                        uint64_t* bar) {

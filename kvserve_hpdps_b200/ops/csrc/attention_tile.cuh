@@ -43,15 +43,6 @@ KVS_DEV uint32_t mn_desc(uint32_t saddr) {
 // the matrix instructions want their operands (536 us at 2 x 2048 tokens against 736 without, when
 // one warp issued them all).
 KVS_DEV uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }
-KVS_DEV bool elected() {
-  uint32_t p;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xFFFFFFFF;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(p));
-  return p != 0;
-}
 KVS_DEV uint32_t chunk_at(int row, int chunk) {
   return (chunk >> 3) * kHalfTile + (row >> 3) * 1024 + (row & 7) * 128 +
          (((chunk & 7) ^ (row & 7)) << 4);
