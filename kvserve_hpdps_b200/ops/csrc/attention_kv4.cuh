@@ -160,6 +160,10 @@ KVS_DEV uint32_t transpose8(uint32_t a) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
+// Whether all lanes saw the phase end.
+KVS_DEV bool wait_phase(uint64_t* bar, uint32_t parity, uint32_t* err) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, err, ERR_MBAR_TIMEOUT));
+}
 // One lane of a whole warp.
 KVS_DEV bool elected() {
   uint32_t p;

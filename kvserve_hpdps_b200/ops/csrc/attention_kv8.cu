@@ -29,13 +29,13 @@ namespace kvs {
 
 namespace {
 
-constexpr int kWarps = 4;           // a CTA
+constexpr int kWarps = 4;           // a team
 constexpr int kStep = 32;           // tokens a warp takes at a time
 constexpr int kStage = 2 * kStep * 128;  // bytes of codes: keys, then values
-constexpr int kStages = 8;          // of a CTA's rings together
+constexpr int kStages = 8;          // of a team's rings together
 constexpr int kOver = 256;          // what starting and ending an item costs, in tokens
-// A CTA's share of the line is no shorter than kLeast tokens, or kFew while that takes no more than
-// kSpread CTAs.
+// A team's share of the line is no shorter than kLeast tokens, or kFew while that takes no more than
+// kSpread teams.
 constexpr int kLeast = 512, kFew = 256, kSpread = 148;
 // Largest weights are 2^kAbove when their row's units are set, and may come to 2^kMost.
 constexpr float kAbove = 7.f, kMost = 15.f;
@@ -53,166 +53,97 @@ KVS_DEV Work work_of(const Attn4Launch& L, const Seq& s, int rows, int group) {
   return w;
 }
 
-constexpr int kSmem = 1024 + kStages * kStage;
+// A CTA (one an SM) is TEAMS teams of four warps, each with a share of its own, and four more warps
+// of which one fetches for each team: it walks through the team's items ahead of it, so that the
+// copies of the next item are on their way while this one's results are joined.
+template <int NT>
+struct Shape {
+  static constexpr int TEAMS = NT == 1 ? 3 : 2, THREADS = (TEAMS + 1) * kWarps * 32;
+  static constexpr int CH = NT == 1 ? 64 : 128;  // channels that are joined at a time
+  // registers of the launch, of the teams and of the other four warps
+  static constexpr int REGS = NT == 1 ? 128 : 168, TEAM = NT == 1 ? 152 : 208,
+                       OTHER = NT == 1 ? 56 : 88;
+  static_assert(TEAMS * TEAM + OTHER == (TEAMS + 1) * REGS);
+  static constexpr int RESULT = kWarps * 8 * NT * CH * 4;  // bytes of a team's results
+  static constexpr int SMEM = 1024 + TEAMS * (kStages * kStage + RESULT);
+  static_assert(SMEM <= 224 * 1024);
+};
 
-// A warp takes NT * 8 rows; RG warps side by side the rows of a tile, the 4 / RG such groups of
-// a CTA every (4 / RG)th 32 tokens.  Fragments (lane = 4 g + c): K is the A operand, row m = token m,
-// lane c's channels 32 c + 4 ks + 0..3 in product ks; the scores' transposed fragments (movmatrix) are
-// the B operand of V^T P^T, whose A operand joins the bytes of two tokens: lane g's channels
-// 16 g + 0..15, lane c's tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9.  With the copy engine's swizzle both
-// are read in 16-byte pieces without bank conflicts.
-template <bool FP16, int NT, int RG>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
-    k_attn8(const __grid_constant__ Attn4Launch L, const __grid_constant__ CUtensorMap map) {
-  constexpr int ROWS = 8 * NT * RG, TS = kWarps / RG, ST = kStages / TS, UNIT = TS * kStep;
-  constexpr int AHEAD = RG == 1 ? ST : ST - 1;  // steps that are asked for ahead
-  extern __shared__ uint8_t raw_smem[];
-  uint8_t* const smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  __shared__ uint64_t s_full[kStages], s_empty[kStages];
-  __shared__ uint2 s_note[kStages];  // the two units' scale bytes; bit 0, 1: the unit is there
-  __shared__ int s_scan[kWarps], s_begin, s_seq;
-  __shared__ float2 s_ml[TS][ROWS];
-  __shared__ int2 s_named[kWarps];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
-  const int split = warp / RG, rg = warp % RG;
-  const int group = L.q_heads / L.heads;
-  const int B = gridDim.x, b = blockIdx.x;
-  const Parts P = parts(L.scratch, B, ROWS);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+KVS_DEV void team_sync(int team) {
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(kWarps * 32) : "memory");
+}
 
-  // ---- this CTA's share [pos, end) and the sequence that it begins in
-  if (tid == 0) {
-    P.desc[b] = make_int4(-1, 0, 0, 0);
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], RG);
-    }
-    fence_mbar_init();
-  }
-  if (tid == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)));
-  int U = 0, mine = 0;
-  Named named;
-  for (int r = tid; r < L.seqs; r += kWarps * 32) {
-    const Seq s = sequence(L, r, b == 0);
-    named.take(L, s, r);
-    mine = work_of<UNIT>(L, s, ROWS, group).units;
-    U += mine;
-  }
-  auto scan = [&](int x) {  // the sum of the warp's up to this lane
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xFFFFFFFFu, x, o);
-      if (lane >= o) x += y;
-    }
-    return x;
-  };
-  int inc = scan(U);
-  if (lane == 31) s_scan[warp] = inc;
-  named.leave(L, s_named);
-  __syncthreads();
-  named.clear<kWarps>(L, s_named);
-  U = 0;
-  int before = inc;  // of the line up to this thread's sequence (if there are no more than threads)
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s_scan[w];
-    U += s_scan[w];
-  }
-  constexpr int kLeastUnits = kLeast / UNIT, kFewUnits = kFew / UNIT, kOverUnits = kOver / UNIT;
-  const int used = min(B, L.whole ? U / (1 + kOverUnits)  // an item a CTA
-                                  : max((U + kLeastUnits - 1) / kLeastUnits,
-                                        min(kSpread, (U + kFewUnits - 1) / kFewUnits)));
-  if (b >= used) return;
-  const Deal deal{U / used, U % used};
-  int pos = deal.begin(b);
-  const int end = deal.begin(b + 1);
-  if (L.seqs <= kWarps * 32) {
-    if (before - mine <= pos && pos < before) {
-      s_seq = tid;
-      s_begin = before - mine;
-    }
-  } else {
-    int base = 0;
-    for (int r0 = 0; r0 < L.seqs; r0 += kWarps * 32) {
-      const int r = r0 + tid;
-      mine = r < L.seqs ? work_of<UNIT>(L, sequence(L, r, false), ROWS, group).units : 0;
-      inc = scan(mine);
-      __syncthreads();
-      if (lane == 31) s_scan[warp] = inc;
-      __syncthreads();
-      before = base + inc;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s_scan[w];
-        base += s_scan[w];
+// What a team does next: item (sequence r, head h, tile) from unit0 on, `units` of them.
+struct Job {
+  Seq s;
+  Work wk;
+  int r, h, tile, unit0, units, nrows, min_seen, limit, stop, item_end;
+};
+// A team's share [pos, end) of the line; `begin`: of sequence r on it.
+template <int UNIT, int ROWS>
+struct Share {
+  int pos, end, begin, r;
+  KVS_DEV bool next(const Attn4Launch& L, int group, Job& j) {
+    constexpr int kOverUnits = kOver / UNIT;
+    while (pos < end) {
+      j.s = sequence(L, r, false);
+      j.wk = work_of<UNIT>(L, j.s, ROWS, group);
+      if (pos >= begin + j.wk.units) {  // on to the next sequence that has work
+        begin += j.wk.units;
+        ++r;
+        continue;
       }
-      if (before - mine <= pos && pos < before) {
-        s_seq = r;
-        s_begin = before - mine;
-      }
-      if (pos < base) break;  // the same for every thread
+      const int cost = j.wk.per + kOverUnits;
+      const int item = (pos - begin) / cost;
+      const int from0 = pos - begin - item * cost;
+      const int share = min(end - pos, cost - from0);
+      // an item's overhead lies in front of its units
+      j.unit0 = max(0, from0 - kOverUnits);
+      j.units = max(0, from0 + share - kOverUnits) - j.unit0;
+      pos += share;
+      if (j.units <= 0) continue;
+      j.r = r;
+      j.h = item / j.wk.tiles;
+      const int ti = item - j.h * j.wk.tiles;
+      // low and high tiles in turn: with causal limits, neighbours add up to alike work
+      j.tile = (ti & 1) ? j.wk.tiles - 1 - (ti >> 1) : ti >> 1;
+      j.nrows = j.s.n * group;
+      const int last_row = min(j.nrows, (j.tile + 1) * ROWS) - 1;
+      j.min_seen = max(0, seen_by(L, j.s, j.tile * ROWS / group));
+      j.limit = max(0, seen_by(L, j.s, last_row / group));
+      j.stop = L.whole ? j.limit : min(j.limit, (j.unit0 + j.units) * UNIT);
+      j.item_end = begin + (item + 1) * cost - 1;
+      return true;
     }
+    return false;
   }
-  __syncthreads();
-  int r = s_seq;
-  int begin = s_begin;  // of sequence r on the line
+};
 
-  const int stage0 = split * ST;
+struct Bars {
+  uint64_t full[kStages], empty[kStages];
+  uint2 note[kStages];  // the two units' scale bytes; bit 0, 1: the unit is there
+};
+
+// Fetches a team's codes: 32 tokens a stage, in turn for its TS rings.
+template <int TS, int ROWS>
+KVS_DEV void fetch_role(const Attn4Launch& L, const CUtensorMap* map,
+                        Share<TS * kStep, ROWS> share, int group, uint32_t stages, Bars* bars) {
+  constexpr int ST = kStages / TS;
+  const int lane = threadIdx.x & 31;
   const bool wide = L.block_size % kStep == 0;  // the tensor map's boxes are of 32 rows
-  uint32_t asked = 0, taken = 0;  // steps of this ring
-  bool lost = false;              // a copy did not come: nothing is waited for any more
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (!lost && !mbar_wait(bar, parity, L.err, ERR_MBAR_TIMEOUT)) lost = true;
-  };
-  // fragment addresses inside a unit's 16 rows of keys and of values
-  uint32_t k_at[2], v_at[4];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) k_at[i] = g * 128 + (((2 * c + i) ^ g) << 4);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) v_at[i] = (2 * c + i) * 128 + ((g ^ (2 * c + i)) << 4);
-  v_at[2] = v_at[0] + 1024;
-  v_at[3] = v_at[1] + 1024;
-
-  while (pos < end) {
-    const Seq s = sequence(L, r, false);
-    const Work wk = work_of<UNIT>(L, s, ROWS, group);
-    if (pos >= begin + wk.units) {  // on to the next sequence that has work
-      begin += wk.units;
-      ++r;
-      continue;
-    }
-    const int cost = wk.per + kOverUnits;
-    const int item = (pos - begin) / cost;
-    const int from0 = pos - begin - item * cost;
-    const int share = min(end - pos, cost - from0);
-    // an item's overhead lies in front of its units
-    const int unit0 = max(0, from0 - kOverUnits);
-    const int units = max(0, from0 + share - kOverUnits) - unit0;
-    pos += share;
-    if (units <= 0) continue;
-    const int h = item / wk.tiles, ti = item - h * wk.tiles;
-    // low and high tiles in turn: with causal limits, neighbours add up to alike work
-    const int tile = (ti & 1) ? wk.tiles - 1 - (ti >> 1) : ti >> 1;
-    const int nrows = s.n * group;
-    const int last_row = min(nrows, (tile + 1) * ROWS) - 1;
-    const int min_seen = max(0, seen_by(L, s, tile * ROWS / group));
-    const int limit = max(0, seen_by(L, s, last_row / group));
-    const int row0 = tile * ROWS + rg * 8 * NT;  // of this warp
-
-    // ---- this warp's steps: tokens first + UNIT k + [0, 32)
-    const int first = unit0 * UNIT + split * kStep;
-    const int stop = L.whole ? limit : min(limit, (unit0 + units) * UNIT);
-    const int steps = first < stop ? (stop - first + UNIT - 1) / UNIT : 0;
-    const int32_t* const table = L.table + r * L.table_stride;
-    const uint8_t* const head = static_cast<const uint8_t*>(L.cache) + h * L.head_stride;
-    // Blocks, places and scales of 16 steps' units: of step lane / 2, half lane % 2; and of the next 16's.
+  uint32_t asked[TS] = {};  // of each ring
+  Job job;
+  while (share.next(L, group, job)) {
+    const int from = job.unit0 * (TS * kStep);
+    const int32_t* const table = L.table + job.r * L.table_stride;
+    const uint8_t* const head = static_cast<const uint8_t*>(L.cache) + job.h * L.head_stride;
+    // Blocks, places and scales of 16 stages' units, a lane each; and of the next 16's.
     int ids = -1, ids2 = -1, offs = 0, offs2 = 0;
     uint32_t scale = 0, scale2 = 0;
-    auto look = [&](int k, int& ids, int& offs) {  // from step k on
-      const int tok = first + (k + (lane >> 1)) * UNIT + kUnit8 * (lane & 1);
+    auto look = [&](int k, int& ids, int& offs) {  // from stage k of the item on
+      const int tok = from + k * kStep + kUnit8 * lane;
       ids = -1;
-      if (tok < stop) {
+      if (tok < job.stop) {
         const int page = tok / L.block_size;
         offs = tok - page * L.block_size;
         ids = table[page];
@@ -227,55 +158,93 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
         scale = *reinterpret_cast<const uint16_t*>(head + ids * L.block_stride +
                                                    256ll * L.block_size + (offs >> 3));
     };
-    auto ask = [&](int k) {  // by one warp of a ring
-      const uint32_t slot = asked % ST;
-      if (RG > 1 && asked >= ST) wait(&s_empty[stage0 + slot], (asked / ST - 1) & 1);
-      ++asked;
-      const int step = k & 15;
-      if (k == 0) {
-        look(0, ids, offs);
-        look_scale(ids, offs, scale);
-      } else if (step == 0) {
-        ids = ids2;
-        offs = offs2;
-        scale = scale2;
-      } else if (step == 8) {
-        look(k + 8, ids2, offs2);
-      } else if (step == 12) {
-        look_scale(ids2, offs2, scale2);
-      }
-      uint64_t* const bar = &s_full[stage0 + slot];
-      const int id0 = __shfl_sync(0xFFFFFFFFu, ids, 2 * step);
-      const int id1 = __shfl_sync(0xFFFFFFFFu, ids, 2 * step + 1);
-      const int off0 = __shfl_sync(0xFFFFFFFFu, offs, 2 * step);
-      const int off1 = __shfl_sync(0xFFFFFFFFu, offs, 2 * step + 1);
-      if (elected()) {  // one lane: copies by several are issued one after the other, 200 clocks each
-        const uint32_t to = smem_u32(smem) + (stage0 + slot) * kStage;
-        // with wide boxes both units are in one block; a second one behind the end hides itself
-        const int halves = wide ? 2 * (id0 >= 0) : (id0 >= 0) + (id1 >= 0);
-        mbar_expect_tx(bar, halves * (kStage / 2));
-        if (id0 >= 0) {
-          load_rows(to, &map, off0, h, id0, bar);
-          load_rows(to + 4096, &map, L.block_size + off0, h, id0, bar);
+    const int all = job.stop > from ? (job.stop - from + kStep - 1) / kStep : 0;
+    for (int k0 = 0; k0 < all; k0 += TS) {
+#pragma unroll
+      for (int ring = 0; ring < TS; ++ring) {
+        const int k = k0 + ring, step = k & 15;
+        if (k >= all) break;
+        const uint32_t slot = asked[ring] % ST, at = ring * ST + slot;
+        if (k == 0) {
+          look(0, ids, offs);
+          look_scale(ids, offs, scale);
+        } else if (step == 0) {
+          ids = ids2;
+          offs = offs2;
+          scale = scale2;
+        } else if (step == 4) {
+          look(k + 12, ids2, offs2);
+        } else if (step == 10) {
+          look_scale(ids2, offs2, scale2);
         }
-        if (id1 >= 0 && !wide) {
-          load_rows(to + 2048, &map, off1, h, id1, bar);
-          load_rows(to + 6144, &map, L.block_size + off1, h, id1, bar);
+        if (asked[ring] >= ST && !wait_phase(&bars->empty[at], (asked[ring] / ST - 1) & 1, L.err))
+          return;
+        ++asked[ring];
+        uint64_t* const bar = &bars->full[at];
+        const int id0 = __shfl_sync(0xFFFFFFFFu, ids, 2 * step);
+        const int id1 = __shfl_sync(0xFFFFFFFFu, ids, 2 * step + 1);
+        const int off0 = __shfl_sync(0xFFFFFFFFu, offs, 2 * step);
+        const int off1 = __shfl_sync(0xFFFFFFFFu, offs, 2 * step + 1);
+        if (elected()) {  // one lane: copies by several are issued one after the other anyway
+          const uint32_t to = stages + at * kStage;
+          // with wide boxes both units are in one block; a second one behind the end hides itself
+          const int halves = wide ? 2 * (id0 >= 0) : (id0 >= 0) + (id1 >= 0);
+          mbar_expect_tx(bar, halves * (kStage / 2));
+          if (id0 >= 0) {
+            load_rows(to, map, off0, job.h, id0, bar);
+            load_rows(to + 4096, map, L.block_size + off0, job.h, id0, bar);
+          }
+          if (id1 >= 0 && !wide) {
+            load_rows(to + 2048, map, off1, job.h, id1, bar);
+            load_rows(to + 6144, map, L.block_size + off1, job.h, id1, bar);
+          }
         }
+        __syncwarp();
+        // the scales, which an item's first copies need not wait for
+        const uint32_t sc0 = __shfl_sync(0xFFFFFFFFu, scale, 2 * step);
+        const uint32_t sc1 = __shfl_sync(0xFFFFFFFFu, scale, 2 * step + 1);
+        if (elected()) {
+          bars->note[at] = make_uint2(sc0 | sc1 << 16, (id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u));
+          mbar_arrive(bar);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      // the scales, which an item's first copies need not wait for
-      const uint32_t sc0 = __shfl_sync(0xFFFFFFFFu, scale, 2 * step);
-      const uint32_t sc1 = __shfl_sync(0xFFFFFFFFu, scale, 2 * step + 1);
-      if (elected()) {
-        s_note[stage0 + slot] =
-            make_uint2(sc0 | sc1 << 16, (id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u));
-        mbar_arrive(bar);
-      }
-      __syncwarp();
-    };
-    if (rg == 0)
-      for (int k = 0; k < AHEAD && k < steps; ++k) ask(k);
+    }
+  }
+}
+
+// A warp takes NT * 8 rows; RG warps side by side the rows of a tile, the TS = 4 / RG such groups of
+// a team every TS-th 32 tokens.  Fragments (lane = 4 g + c): K is the A operand, row m = token m,
+// lane c's channels 32 c + 4 ks + 0..3 in product ks; the scores' transposed fragments (movmatrix) are
+// the B operand of V^T P^T, whose A operand joins the bytes of two tokens: lane g's channels
+// 16 g + 0..15, lane c's tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9.  With the copy engine's swizzle both
+// are read in 16-byte pieces without bank conflicts.
+template <bool FP16, int NT, int RG>
+KVS_DEV void team_role(const Attn4Launch& L, Share<kWarps / RG * kStep, 8 * NT * RG> share, int group,
+                       const Deal& deal, const Parts& P, int b, int team, const uint8_t* stages,
+                       float* s_o, float2 (*s_ml)[8 * NT * RG], Bars* bars) {
+  constexpr int ROWS = 8 * NT * RG, TS = kWarps / RG, ST = kStages / TS, UNIT = TS * kStep;
+  const int tid = threadIdx.x & 127, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+  const int split = warp / RG, rg = warp % RG, stage0 = split * ST;
+  uint32_t taken = 0;  // steps of this ring
+  bool lost = false;   // a copy did not come: nothing is waited for any more
+  // fragment addresses inside a unit's 16 rows of keys and of values
+  uint32_t k_at[2], v_at[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) k_at[i] = g * 128 + (((2 * c + i) ^ g) << 4);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) v_at[i] = (2 * c + i) * 128 + ((g ^ (2 * c + i)) << 4);
+  v_at[2] = v_at[0] + 1024;
+  v_at[3] = v_at[1] + 1024;
+
+  Job job;
+  while (share.next(L, group, job)) {
+    const Seq& s = job.s;
+    const int h = job.h, nrows = job.nrows, limit = job.limit;
+    const int row0 = job.tile * ROWS + rg * 8 * NT;  // of this warp
+    // this warp's steps: tokens first + UNIT k + [0, 32)
+    const int first = job.unit0 * UNIT + split * kStep;
+    const int steps = first < job.stop ? (job.stop - first + UNIT - 1) / UNIT : 0;
 
     // ---- query fragments: fp16, each row scaled by a power of two so that its largest
     // element is in [2^14, 2^15); exact unless 2^-31 of the largest
@@ -529,91 +498,310 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       }
     };
     for (int k = 0; k < steps; ++k) {
-      const uint32_t slot = taken % ST, stage = stage0 + slot;
-      wait(&s_full[stage], (taken / ST) & 1);
+      const uint32_t stage = stage0 + taken % ST;
+      if (!lost && !mbar_wait(&bars->full[stage], (taken / ST) & 1, L.err, ERR_MBAR_TIMEOUT))
+        lost = true;
       ++taken;
       const int t0 = first + k * UNIT;
-      const uint2 note = s_note[stage];
+      const uint2 note = bars->note[stage];
       if (row0 < nrows) {
-        if (note.y != 3u || t0 + kStep > min_seen)
-          step(std::true_type{}, t0, smem + stage * kStage, note.x, note.y);
+        if (note.y != 3u || t0 + kStep > job.min_seen)
+          step(std::true_type{}, t0, stages + stage * kStage, note.x, note.y);
         else
-          step(std::false_type{}, t0, smem + stage * kStage, note.x, note.y);
+          step(std::false_type{}, t0, stages + stage * kStage, note.x, note.y);
       }
       __syncwarp();  // the stage may be overwritten
-      if (RG > 1 && lane == 0) mbar_arrive(&s_empty[stage]);
-      if (rg == 0 && k + AHEAD < steps) ask(k + AHEAD);
+      if (lane == 0) mbar_arrive(&bars->empty[stage]);
     }
-    // ---- join the warps' results
-    __syncthreads();  // the rings are empty: they hold the results
-    float* const s_o = reinterpret_cast<float*>(smem);  // [TS][ROWS][128]
+
+    // ---- join the warps' results, CH channels at a time: s_o is [TS][ROWS][CH]
+    constexpr int CH = Shape<NT>::CH, ACROSS = CH / 4;  // lanes a row
+    const bool whole = job.unit0 == 0 && job.units == job.wk.per;
+    const int slot = 2 * b + (job.unit0 == 0 ? 1 : 0);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int row = rg * 8 * NT + nt * 8 + 2 * c + j;
         float ls = l[nt][j];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) ls += __shfl_xor_sync(0xFFFFFFFFu, ls, o);
-        if (g == 0) s_ml[split][row] = make_float2(M[nt][j], ls);
-        const float unit = pow2(static_cast<int>(K[nt][j]));
+        if (g == 0) s_ml[split][rg * 8 * NT + nt * 8 + 2 * c + j] = make_float2(M[nt][j], ls);
+      }
+#pragma unroll 1
+    for (int c0 = 0; c0 < 128; c0 += CH) {
+      if (16 * g >= c0 && 16 * g < c0 + CH) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<float4*>(s_o + (split * ROWS + row) * 128 + 16 * g + 4 * q) =
-              make_float4(acc[2 * q][nt][j] * unit, acc[2 * q][nt][j + 2] * unit,
-                          acc[2 * q + 1][nt][j] * unit, acc[2 * q + 1][nt][j + 2] * unit);
-      }
-    __syncthreads();
-    const bool whole = unit0 == 0 && units == wk.per;
-    const int slot = 2 * b + (unit0 == 0 ? 1 : 0);
-#pragma unroll 4
-    for (int it = 0; it < ROWS / kWarps; ++it) {  // a warp a row, four channels a lane
-      const int row = it * kWarps + warp, rr = tile * ROWS + row;
-      if (rr >= nrows) break;
-      float m = kLowest, ls = 0.f;
-      float2 ml[TS];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int w = 0; w < TS; ++w) {
-        ml[w] = s_ml[w][row];
-        m = fmaxf(m, ml[w].x);
-      }
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int j = 0; j < 2; ++j) {
+            const int row = rg * 8 * NT + nt * 8 + 2 * c + j;
+            const float unit = pow2(static_cast<int>(K[nt][j]));
 #pragma unroll
-      for (int w = 0; w < TS; ++w) {
-        const float k2 = ex2(ml[w].x - m);
-        const float4 x =
-            *reinterpret_cast<const float4*>(s_o + (w * ROWS + row) * 128 + lane * 4);
-        ls = fmaf(ml[w].y, k2, ls);
-        o.x = fmaf(x.x, k2, o.x);
-        o.y = fmaf(x.y, k2, o.y);
-        o.z = fmaf(x.z, k2, o.z);
-        o.w = fmaf(x.w, k2, o.w);
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<float4*>(s_o + (split * ROWS + row) * CH + 16 * g - c0 + 4 * q) =
+                  make_float4(acc[2 * q][nt][j] * unit, acc[2 * q][nt][j + 2] * unit,
+                              acc[2 * q + 1][nt][j] * unit, acc[2 * q + 1][nt][j + 2] * unit);
+          }
       }
-      if (whole) {
-        const long long tq = s.row0 + rr / group;
-        const int hq = h * group + rr % group;
-        const float inv = ls == 0.f ? 0.f : __fdividef(1.f, ls);
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + tq * L.o_ts + hq * L.o_hs +
-                                  lane * 4) =
-            make_uint2(f2h2<FP16>(o.x * inv, o.y * inv), f2h2<FP16>(o.z * inv, o.w * inv));
-        if (L.lse != nullptr && lane == 0)
-          L.lse[tq * L.q_heads + hq] =
-              ls == 0.f ? -INFINITY : (m + log2f(ls)) * 0.69314718055994531f;
-      } else {
-        *reinterpret_cast<float4*>(
-            P.o + (static_cast<long long>(slot) * ROWS + row) * 128 + lane * 4) = o;
-        if (lane == 0) P.ml[slot * ROWS + row] = make_float2(m, ls);
+      team_sync(team);
+      const int ch = tid % ACROSS * 4;
+#pragma unroll 2
+      for (int row = tid / ACROSS; row < ROWS; row += kWarps * 32 / ACROSS) {
+        const int rr = job.tile * ROWS + row;
+        if (rr >= nrows) break;
+        float m = kLowest, ls = 0.f;
+        float2 ml[TS];
+#pragma unroll
+        for (int w = 0; w < TS; ++w) {
+          ml[w] = s_ml[w][row];
+          m = fmaxf(m, ml[w].x);
+        }
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < TS; ++w) {
+          const float k2 = ex2(ml[w].x - m);
+          const float4 x = *reinterpret_cast<const float4*>(s_o + (w * ROWS + row) * CH + ch);
+          ls = fmaf(ml[w].y, k2, ls);
+          o.x = fmaf(x.x, k2, o.x);
+          o.y = fmaf(x.y, k2, o.y);
+          o.z = fmaf(x.z, k2, o.z);
+          o.w = fmaf(x.w, k2, o.w);
+        }
+        if (whole) {
+          const long long tq = s.row0 + rr / group;
+          const int hq = h * group + rr % group;
+          const float inv = ls == 0.f ? 0.f : __fdividef(1.f, ls);
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + tq * L.o_ts + hq * L.o_hs + c0 +
+                                    ch) =
+              make_uint2(f2h2<FP16>(o.x * inv, o.y * inv), f2h2<FP16>(o.z * inv, o.w * inv));
+          if (L.lse != nullptr && c0 + ch == 0)
+            L.lse[tq * L.q_heads + hq] =
+                ls == 0.f ? -INFINITY : (m + log2f(ls)) * 0.69314718055994531f;
+        } else {
+          *reinterpret_cast<float4*>(
+              P.o + (static_cast<long long>(slot) * ROWS + row) * 128 + c0 + ch) = o;
+          if (c0 + ch == 0) P.ml[slot * ROWS + row] = make_float2(m, ls);
+        }
       }
+      team_sync(team);  // the next results take their place
     }
-    if (!whole && unit0 == 0 && tid == 0)  // parts: up to the CTA that holds the item's end
-      P.desc[b] = make_int4(r, h, tile, deal.owner(begin + (item + 1) * cost - 1) - b + 1);
-    fence_proxy_async_smem();  // the copy engine writes there next
-    __syncthreads();
+    if (!whole && job.unit0 == 0 && tid == 0)  // parts: up to the team that holds the item's end
+      P.desc[b] = make_int4(job.r, h, job.tile, deal.owner(job.item_end) - b + 1);
   }
 }
 
+template <bool FP16, int NT, int RG>
+__global__ void __launch_bounds__(Shape<NT>::THREADS, 1)
+    k_attn8(const __grid_constant__ Attn4Launch L, const __grid_constant__ CUtensorMap map) {
+  using S = Shape<NT>;
+  constexpr int ROWS = 8 * NT * RG, TS = kWarps / RG, UNIT = TS * kStep, TEAMS = S::TEAMS;
+  constexpr int WARPS = S::THREADS / 32;
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+  __shared__ Bars s_bars[TEAMS];
+  __shared__ int s_scan[WARPS], s_begin[TEAMS], s_seq[TEAMS];
+  __shared__ float2 s_ml[TEAMS][TS][ROWS];
+  __shared__ int2 s_named[WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int group = L.q_heads / L.heads;
+  // Teams are numbered across the SMs first: few of them get an SM each.
+  const int B = gridDim.x * TEAMS;
+  const Parts P = parts(L.scratch, B, ROWS);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---- the teams' shares [pos, end) and the sequences that they begin in
+  if (tid == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)));
+    for (int t = 0; t < TEAMS; ++t) {
+      P.desc[t * gridDim.x + blockIdx.x] = make_int4(-1, 0, 0, 0);
+      for (int i = 0; i < kStages; ++i) {
+        mbar_init(&s_bars[t].full[i], 1);
+        mbar_init(&s_bars[t].empty[i], RG);
+      }
+    }
+    fence_mbar_init();
+  }
+  int U = 0, mine = 0;
+  Named named;
+  for (int r = tid; r < L.seqs; r += S::THREADS) {
+    const Seq s = sequence(L, r, blockIdx.x == 0);
+    named.take(L, s, r);
+    mine = work_of<UNIT>(L, s, ROWS, group).units;
+    U += mine;
+  }
+  auto scan = [&](int x) {  // the sum of the warp's up to this lane
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+      if (lane >= o) x += y;
+    }
+    return x;
+  };
+  int inc = scan(U);
+  if (lane == 31) s_scan[warp] = inc;
+  named.leave(L, s_named);
+  __syncthreads();
+  named.clear<WARPS>(L, s_named);
+  U = 0;
+  int before = inc;  // of the line up to this thread's sequence (if there are no more than threads)
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) before += s_scan[w];
+    U += s_scan[w];
+  }
+  constexpr int kLeastUnits = kLeast / UNIT, kFewUnits = kFew / UNIT, kOverUnits = kOver / UNIT;
+  const int used = min(B, L.whole ? U / (1 + kOverUnits)  // an item a team
+                                  : max((U + kLeastUnits - 1) / kLeastUnits,
+                                        min(kSpread, (U + kFewUnits - 1) / kFewUnits)));
+  const Deal deal{U / max(used, 1), U % max(used, 1)};
+  auto found = [&](int r, int from, int to) {  // sequence r has [from, to) of the line
+#pragma unroll
+    for (int t = 0; t < TEAMS; ++t) {
+      const int b = t * gridDim.x + blockIdx.x, pos = deal.begin(b);
+      if (b < used && from <= pos && pos < to) {
+        s_seq[t] = r;
+        s_begin[t] = from;
+      }
+    }
+  };
+  if (L.seqs <= S::THREADS) {
+    found(tid, before - mine, before);
+  } else {
+    int base = 0;
+    for (int r0 = 0; r0 < L.seqs; r0 += S::THREADS) {
+      const int r = r0 + tid;
+      mine = r < L.seqs ? work_of<UNIT>(L, sequence(L, r, false), ROWS, group).units : 0;
+      inc = scan(mine);
+      __syncthreads();
+      if (lane == 31) s_scan[warp] = inc;
+      __syncthreads();
+      before = base + inc;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) before += s_scan[w];
+        base += s_scan[w];
+      }
+      found(r, before - mine, before);
+    }
+  }
+  __syncthreads();
+  const bool fetches = warp >= TEAMS * kWarps;
+  const int team = fetches ? warp - TEAMS * kWarps : warp / kWarps;
+  const int b = team * gridDim.x + blockIdx.x;
+  Share<UNIT, ROWS> share{0, 0, 0, 0};
+  if (team < TEAMS && b < used) share = {deal.begin(b), deal.begin(b + 1), s_begin[team], s_seq[team]};
+  uint8_t* const stages = smem + min(team, TEAMS - 1) * (kStages * kStage);
+  if (!fetches) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::TEAM));
+    team_role<FP16, NT, RG>(L, share, group, deal, P, b, team, stages,
+                            reinterpret_cast<float*>(smem + TEAMS * kStages * kStage +
+                                                     team * S::RESULT),
+                            s_ml[team], &s_bars[team]);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::OTHER));
+    fetch_role<TS, ROWS>(L, &map, share, group, smem_u32(stages), &s_bars[min(team, TEAMS - 1)]);
+  }
+}
+
+// Joins the parts of the items that several teams share.  A part's weights are relative to its own
+// maximum; they are added up in order, so results do not depend on timing.
+//
+// Few parts an item (many items): CTA b takes the item that begins with team b and goes on, if one
+// does, a warp a row.  Many parts (DEEP; few items, which the host knows): the CTAs of column i look for
+// the i-th of them and take a row each, 16 warps every 16th part.  One sequence of 49157 tokens, 4
+// heads, 97 parts each: 17 us with four warps a row and a CTA a team, of which most found nothing.
+template <bool FP16, int ROWS, bool DEEP>
+__global__ void __launch_bounds__(DEEP ? 512 : 256)
+    k_attn8_join(const __grid_constant__ Attn4Launch L, int B) {
+  constexpr int WARPS = DEEP ? 16 : 8;
+  __shared__ int s_count[WARPS], s_b;
+  __shared__ float2 s_ml[DEEP ? WARPS : 1];
+  __shared__ float4 s_o[DEEP ? WARPS : 1][32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Parts P = parts(L.scratch, B, ROWS);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int b = blockIdx.x;
+  if constexpr (DEEP) {
+    int base = 0;  // items found
+    for (int b0 = 0; b0 < B; b0 += 32 * WARPS) {
+      const bool is = b0 + tid < B && P.desc[b0 + tid].x >= 0;
+      const uint32_t mask = __ballot_sync(0xFFFFFFFFu, is);
+      if (tid == 0) s_b = -1;
+      if (lane == 0) s_count[warp] = __popc(mask);
+      __syncthreads();
+      int before = base;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) before += s_count[w];
+        base += s_count[w];
+      }
+      if (is && before + __popc(mask & ((1u << lane) - 1)) == static_cast<int>(blockIdx.x))
+        s_b = b0 + tid;
+      __syncthreads();
+      b = s_b;
+      if (b >= 0) break;
+      __syncthreads();
+    }
+    if (b < 0) return;
+  }
+  const int4 d = P.desc[b];
+  if (d.x < 0) return;
+  const int group = L.q_heads / L.heads, np = d.w;
+  const Seq s = sequence(L, d.x, false);
+  const int rows = min(ROWS, s.n * group - d.z * ROWS);  // of this tile
+  const int row = DEEP ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * 8 + warp;
+  if (row >= rows) return;
+  // part 0 is in team b's second slot, the others in the first ones of the next teams
+  auto slot = [&](int i) { return (i == 0 ? 2 * b + 1 : 2 * (b + i)) * ROWS + row; };
+  float m = kLowest, ls = 0.f;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float m2, float l2, const float4& x) {
+    const float top = fmaxf(m, m2), k1 = ex2(m - top), k2 = ex2(m2 - top);
+    m = top;
+    ls = fmaf(ls, k1, l2 * k2);
+    a.x = fmaf(a.x, k1, x.x * k2);
+    a.y = fmaf(a.y, k1, x.y * k2);
+    a.z = fmaf(a.z, k1, x.z * k2);
+    a.w = fmaf(a.w, k1, x.w * k2);
+  };
+  for (int i0 = DEEP ? warp : 0; i0 < np; i0 += DEEP ? 4 * WARPS : 4) {  // four loads together
+    float2 ml[4];
+    float4 x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + (DEEP ? WARPS : 1) * u;
+      ml[u] = make_float2(kLowest, 0.f);
+      x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < np) {
+        ml[u] = P.ml[slot(i)];
+        x[u] = *reinterpret_cast<const float4*>(P.o + slot(i) * 128ll + lane * 4);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) add(ml[u].x, ml[u].y, x[u]);
+  }
+  if constexpr (DEEP) {
+    s_o[warp][lane] = a;
+    if (lane == 0) s_ml[warp] = make_float2(m, ls);
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll 4
+    for (int w = 1; w < WARPS; ++w) add(s_ml[w].x, s_ml[w].y, s_o[w][lane]);
+  }
+  const int rr = d.z * ROWS + row;
+  const long long tq = s.row0 + rr / group;
+  const int hq = d.y * group + rr % group;
+  const float inv = ls == 0.f ? 0.f : __fdividef(1.f, ls);
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + tq * L.o_ts + hq * L.o_hs + lane * 4) =
+      make_uint2(f2h2<FP16>(a.x * inv, a.y * inv), f2h2<FP16>(a.z * inv, a.w * inv));
+  if (L.lse != nullptr && lane == 0)
+    L.lse[tq * L.q_heads + hq] = ls == 0.f ? -INFINITY : (m + log2f(ls)) * 0.69314718055994531f;
+}
+
 struct Grid {
-  int ctas, rows;
+  int ctas, teams, rows;
+  long long items;
   bool fits;   // the line's length is an int
   bool split;  // whether items may be split
 };
@@ -634,9 +822,10 @@ Grid grid_of(const Attn4Launch* L) {
                           ((rows + g.rows - 1) / g.rows);
   g.split = room > kWholeTokens;
   const long long units = items * (g.split ? per : 1);
+  g.items = items;
   g.fits = items < (1ll << 31) && items * (per + 1 + kOver / unit) < (1ll << 31);
-  const long long most = 148ll * (g.rows == 8 ? 3 : 2);  // resident at once
-  g.ctas = static_cast<int>(units < most ? units : most);
+  g.ctas = static_cast<int>(units < 148 ? units : 148);
+  g.teams = g.ctas * (g.rows == 8 ? Shape<1>::TEAMS : Shape<2>::TEAMS);
   return g;
 }
 
@@ -654,12 +843,24 @@ bool many_rows(const Attn4Launch* L) {
 template <bool FP16, int NT, int RG>
 cudaError_t launch(const Attn4Launch& L, const Grid& g, const CUtensorMap& map, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(k_attn8<FP16, NT, RG>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<NT>::SMEM);
   if (e != cudaSuccess) return e;
-  k_attn8<FP16, NT, RG><<<g.ctas, kWarps * 32, kSmem, s>>>(L, map);
+  k_attn8<FP16, NT, RG><<<g.ctas, Shape<NT>::THREADS, Shape<NT>::SMEM, s>>>(L, map);
   e = cudaGetLastError();
   if (e != cudaSuccess || !g.split) return e;
-  return launch_combine<FP16, NT * RG, 4>(L, g.ctas, s);
+  constexpr int ROWS = 8 * NT * RG;
+  const bool deep = 8 * g.items <= g.teams;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = deep ? dim3(static_cast<unsigned>(g.items), ROWS) : dim3(g.teams, ROWS / 8);
+  cfg.blockDim = dim3(deep ? 512 : 256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr = {};  // it may start while the attention kernel ends
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return deep ? cudaLaunchKernelEx(&cfg, k_attn8_join<FP16, ROWS, true>, L, g.teams)
+              : cudaLaunchKernelEx(&cfg, k_attn8_join<FP16, ROWS, false>, L, g.teams);
 }
 template <bool FP16>
 cudaError_t launch_rows(const Attn4Launch& L, const Grid& g, const CUtensorMap& map,
@@ -680,7 +881,7 @@ extern "C" {
 long long kvs_attn8_scratch_bytes(const Attn4Launch* L) {
   if (many_rows(L)) return attn8_tile_scratch(*L);
   const Grid g = grid_of(L);
-  return 16ll * g.ctas + 2ll * g.ctas * g.rows * (8 + 512);
+  return 16ll * g.teams + 2ll * g.teams * g.rows * (8 + 512);
 }
 
 int kvs_attention_kv8(const Attn4Launch* L, void* stream) {

@@ -193,9 +193,6 @@ struct Walk {
   }
 };
 
-KVS_DEV bool wait_phase(uint64_t* bar, uint32_t parity, uint32_t* err) {
-  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, err, ERR_MBAR_TIMEOUT));
-}
 #define KVS_WAIT(bar, parity) wait_phase(bar, parity, L.err)
 // Whether the phase is over; nothing waits for the answer before it is used.
 KVS_DEV uint32_t peek_phase(uint64_t* bar, uint32_t parity) {
