@@ -66,7 +66,7 @@ struct Shape {
   static_assert(TEAMS * TEAM + OTHER == (TEAMS + 1) * REGS);
   static constexpr int RESULT = kWarps * 8 * NT * CH * 4;  // bytes of a team's results
   static constexpr int SMEM = 1024 + TEAMS * (kStages * kStage + RESULT);
-  static_assert(SMEM <= 224 * 1024);
+  static_assert(SMEM <= 224 * 1024 && TEAMS * (kStages + 1) < 31);
 };
 
 KVS_DEV void team_sync(int team) {
@@ -83,14 +83,15 @@ struct Job {
 template <int UNIT, int ROWS>
 struct Share {
   int pos, end, begin, r;
+  Seq own;  // sequence r's extents
   KVS_DEV bool next(const Attn4Launch& L, int group, Job& j) {
     constexpr int kOverUnits = kOver / UNIT;
     while (pos < end) {
-      j.s = sequence(L, r, false);
+      j.s = own;
       j.wk = work_of<UNIT>(L, j.s, ROWS, group);
       if (pos >= begin + j.wk.units) {  // on to the next sequence that has work
         begin += j.wk.units;
-        ++r;
+        own = sequence(L, ++r, false);
         continue;
       }
       const int cost = j.wk.per + kOverUnits;
@@ -586,7 +587,8 @@ KVS_DEV void team_role(const Attn4Launch& L, Share<kWarps / RG * kStep, 8 * NT *
       team_sync(team);  // the next results take their place
     }
     if (!whole && job.unit0 == 0 && tid == 0)  // parts: up to the team that holds the item's end
-      P.desc[b] = make_int4(job.r, h, job.tile, deal.owner(job.item_end) - b + 1);
+      P.desc[b] = make_int4(s.row0, h, job.tile, (deal.owner(job.item_end) - b + 1) |
+                                                      min(ROWS, nrows - job.tile * ROWS) << 16);
   }
 }
 
@@ -601,6 +603,7 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1)
       (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
   __shared__ Bars s_bars[TEAMS];
   __shared__ int s_scan[WARPS], s_begin[TEAMS], s_seq[TEAMS];
+  __shared__ Seq s_own[TEAMS];
   __shared__ float2 s_ml[TEAMS][TS][ROWS];
   __shared__ int2 s_named[WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -611,23 +614,24 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- the teams' shares [pos, end) and the sequences that they begin in
-  if (tid == 0) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)));
-    for (int t = 0; t < TEAMS; ++t) {
-      P.desc[t * gridDim.x + blockIdx.x] = make_int4(-1, 0, 0, 0);
-      for (int i = 0; i < kStages; ++i) {
-        mbar_init(&s_bars[t].full[i], 1);
-        mbar_init(&s_bars[t].empty[i], RG);
-      }
+  if (warp == WARPS - 1) {
+    if (lane < TEAMS * kStages) {
+      mbar_init(&s_bars[lane / kStages].full[lane % kStages], 1);
+      mbar_init(&s_bars[lane / kStages].empty[lane % kStages], RG);
+      fence_mbar_init();
+    } else if (lane < TEAMS * (kStages + 1)) {
+      P.desc[(lane - TEAMS * kStages) * gridDim.x + blockIdx.x] = make_int4(-1, 0, 0, 0);
+    } else if (lane == 31) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)));
     }
-    fence_mbar_init();
   }
   int U = 0, mine = 0;
+  Seq own = {};
   Named named;
   for (int r = tid; r < L.seqs; r += S::THREADS) {
-    const Seq s = sequence(L, r, blockIdx.x == 0);
-    named.take(L, s, r);
-    mine = work_of<UNIT>(L, s, ROWS, group).units;
+    own = sequence(L, r, blockIdx.x == 0);
+    named.take(L, own, r);
+    mine = work_of<UNIT>(L, own, ROWS, group).units;
     U += mine;
   }
   auto scan = [&](int x) {  // the sum of the warp's up to this lane
@@ -662,6 +666,7 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1)
       if (b < used && from <= pos && pos < to) {
         s_seq[t] = r;
         s_begin[t] = from;
+        s_own[t] = own;
       }
     }
   };
@@ -671,7 +676,9 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1)
     int base = 0;
     for (int r0 = 0; r0 < L.seqs; r0 += S::THREADS) {
       const int r = r0 + tid;
-      mine = r < L.seqs ? work_of<UNIT>(L, sequence(L, r, false), ROWS, group).units : 0;
+      own = {};
+      if (r < L.seqs) own = sequence(L, r, false);
+      mine = r < L.seqs ? work_of<UNIT>(L, own, ROWS, group).units : 0;
       inc = scan(mine);
       __syncthreads();
       if (lane == 31) s_scan[warp] = inc;
@@ -689,8 +696,9 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1)
   const bool fetches = warp >= TEAMS * kWarps;
   const int team = fetches ? warp - TEAMS * kWarps : warp / kWarps;
   const int b = team * gridDim.x + blockIdx.x;
-  Share<UNIT, ROWS> share{0, 0, 0, 0};
-  if (team < TEAMS && b < used) share = {deal.begin(b), deal.begin(b + 1), s_begin[team], s_seq[team]};
+  Share<UNIT, ROWS> share{};
+  if (team < TEAMS && b < used)
+    share = {deal.begin(b), deal.begin(b + 1), s_begin[team], s_seq[team], s_own[team]};
   uint8_t* const stages = smem + min(team, TEAMS - 1) * (kStages * kStage);
   if (!fetches) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::TEAM));
@@ -745,15 +753,28 @@ __global__ void __launch_bounds__(DEEP ? 512 : 256)
     }
     if (b < 0) return;
   }
-  const int4 d = P.desc[b];
-  if (d.x < 0) return;
-  const int group = L.q_heads / L.heads, np = d.w;
-  const Seq s = sequence(L, d.x, false);
-  const int rows = min(ROWS, s.n * group - d.z * ROWS);  // of this tile
   const int row = DEEP ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * 8 + warp;
-  if (row >= rows) return;
   // part 0 is in team b's second slot, the others in the first ones of the next teams
   auto slot = [&](int i) { return (i == 0 ? 2 * b + 1 : 2 * (b + i)) * ROWS + row; };
+  float2 ml[4];
+  float4 x[4];
+  auto load = [&](int u, int i, bool is) {
+    ml[u] = make_float2(kLowest, 0.f);
+    x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (is) {
+      ml[u] = P.ml[slot(i)];
+      x[u] = *reinterpret_cast<const float4*>(P.o + slot(i) * 128ll + lane * 4);
+    }
+  };
+  // most items have two parts: theirs come together with what says so
+  if constexpr (!DEEP) {
+    load(0, 0, true);
+    load(1, 1, b + 1 < B);
+  }
+  const int4 d = P.desc[b];
+  if (d.x < 0) return;
+  const int group = L.q_heads / L.heads, np = d.w & 0xFFFF;
+  if (row >= d.w >> 16) return;
   float m = kLowest, ls = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](float m2, float l2, const float4& x) {
@@ -765,18 +786,15 @@ __global__ void __launch_bounds__(DEEP ? 512 : 256)
     a.z = fmaf(a.z, k1, x.z * k2);
     a.w = fmaf(a.w, k1, x.w * k2);
   };
-  for (int i0 = DEEP ? warp : 0; i0 < np; i0 += DEEP ? 4 * WARPS : 4) {  // four loads together
-    float2 ml[4];
-    float4 x[4];
+  if constexpr (!DEEP) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) add(ml[u].x, ml[u].y, x[u]);
+  }
+  for (int i0 = DEEP ? warp : 2; i0 < np; i0 += DEEP ? 4 * WARPS : 4) {  // four loads together
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int i = i0 + (DEEP ? WARPS : 1) * u;
-      ml[u] = make_float2(kLowest, 0.f);
-      x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (i < np) {
-        ml[u] = P.ml[slot(i)];
-        x[u] = *reinterpret_cast<const float4*>(P.o + slot(i) * 128ll + lane * 4);
-      }
+      load(u, i, i < np);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) add(ml[u].x, ml[u].y, x[u]);
@@ -790,7 +808,7 @@ __global__ void __launch_bounds__(DEEP ? 512 : 256)
     for (int w = 1; w < WARPS; ++w) add(s_ml[w].x, s_ml[w].y, s_o[w][lane]);
   }
   const int rr = d.z * ROWS + row;
-  const long long tq = s.row0 + rr / group;
+  const long long tq = d.x + rr / group;
   const int hq = d.y * group + rr % group;
   const float inv = ls == 0.f ? 0.f : __fdividef(1.f, ls);
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + tq * L.o_ts + hq * L.o_hs + lane * 4) =
