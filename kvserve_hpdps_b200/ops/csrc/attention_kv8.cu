@@ -56,14 +56,15 @@ KVS_DEV Work work_of(const Attn4Launch& L, const Seq& s, int rows, int group) {
 // A CTA (one an SM) is TEAMS teams of four warps, each with a share of its own, and four more warps
 // of which one fetches for each team: it walks through the team's items ahead of it, so that the
 // copies of the next item are on their way while this one's results are joined.
-template <int NT>
+// Calls for which a team an SM is enough take CTAs of one team, which start sooner.
+template <int NT, bool ONE>
 struct Shape {
-  static constexpr int TEAMS = NT == 1 ? 3 : 2, THREADS = (TEAMS + 1) * kWarps * 32;
+  static constexpr int TEAMS = ONE ? 1 : NT == 1 ? 3 : 2, THREADS = (TEAMS + 1) * kWarps * 32;
   static constexpr int CH = NT == 1 ? 64 : 128;  // channels that are joined at a time
   // registers of the launch, of the teams and of the other four warps
   static constexpr int REGS = NT == 1 ? 128 : 168, TEAM = NT == 1 ? 152 : 208,
                        OTHER = NT == 1 ? 56 : 88;
-  static_assert(TEAMS * TEAM + OTHER == (TEAMS + 1) * REGS);
+  static_assert(ONE || TEAMS * TEAM + OTHER == (TEAMS + 1) * REGS);
   static constexpr int RESULT = kWarps * 8 * NT * CH * 4;  // bytes of a team's results
   static constexpr int SMEM = 1024 + TEAMS * (kStages * kStage + RESULT);
   static_assert(SMEM <= 224 * 1024 && TEAMS * (kStages + 1) < 31);
@@ -516,7 +517,7 @@ KVS_DEV void team_role(const Attn4Launch& L, Share<kWarps / RG * kStep, 8 * NT *
     }
 
     // ---- join the warps' results, CH channels at a time: s_o is [TS][ROWS][CH]
-    constexpr int CH = Shape<NT>::CH, ACROSS = CH / 4;  // lanes a row
+    constexpr int CH = Shape<NT, false>::CH, ACROSS = CH / 4;  // lanes a row
     const bool whole = job.unit0 == 0 && job.units == job.wk.per;
     const int slot = 2 * b + (job.unit0 == 0 ? 1 : 0);
 #pragma unroll
@@ -592,10 +593,10 @@ KVS_DEV void team_role(const Attn4Launch& L, Share<kWarps / RG * kStep, 8 * NT *
   }
 }
 
-template <bool FP16, int NT, int RG>
-__global__ void __launch_bounds__(Shape<NT>::THREADS, 1)
+template <bool FP16, int NT, int RG, bool ONE>
+__global__ void __launch_bounds__(Shape<NT, ONE>::THREADS, 1)
     k_attn8(const __grid_constant__ Attn4Launch L, const __grid_constant__ CUtensorMap map) {
-  using S = Shape<NT>;
+  using S = Shape<NT, ONE>;
   constexpr int ROWS = 8 * NT * RG, TS = kWarps / RG, UNIT = TS * kStep, TEAMS = S::TEAMS;
   constexpr int WARPS = S::THREADS / 32;
   extern __shared__ uint8_t raw_smem[];
@@ -701,13 +702,13 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1)
     share = {deal.begin(b), deal.begin(b + 1), s_begin[team], s_seq[team], s_own[team]};
   uint8_t* const stages = smem + min(team, TEAMS - 1) * (kStages * kStage);
   if (!fetches) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::TEAM));
+    if constexpr (!ONE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::TEAM));
     team_role<FP16, NT, RG>(L, share, group, deal, P, b, team, stages,
                             reinterpret_cast<float*>(smem + TEAMS * kStages * kStage +
                                                      team * S::RESULT),
                             s_ml[team], &s_bars[team]);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::OTHER));
+    if constexpr (!ONE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::OTHER));
     fetch_role<TS, ROWS>(L, &map, share, group, smem_u32(stages), &s_bars[min(team, TEAMS - 1)]);
   }
 }
@@ -822,6 +823,7 @@ struct Grid {
   long long items;
   bool fits;   // the line's length is an int
   bool split;  // whether items may be split
+  bool one;    // a team a CTA
 };
 
 // Tables of at most so many tokens are not split: the launch that joins the parts takes longer
@@ -843,7 +845,8 @@ Grid grid_of(const Attn4Launch* L) {
   g.items = items;
   g.fits = items < (1ll << 31) && items * (per + 1 + kOver / unit) < (1ll << 31);
   g.ctas = static_cast<int>(units < 148 ? units : 148);
-  g.teams = g.ctas * (g.rows == 8 ? Shape<1>::TEAMS : Shape<2>::TEAMS);
+  g.one = units <= 148;
+  g.teams = g.ctas * (g.one ? 1 : g.rows == 8 ? Shape<1, false>::TEAMS : Shape<2, false>::TEAMS);
   return g;
 }
 
@@ -858,13 +861,19 @@ bool many_rows(const Attn4Launch* L) {
   return rows > kManyRows && work > static_cast<double>(kMuchWork);
 }
 
+template <bool FP16, int NT, int RG, bool ONE>
+cudaError_t launch_shape(const Attn4Launch& L, const Grid& g, const CUtensorMap& map, cudaStream_t s) {
+  using S = Shape<NT, ONE>;
+  const cudaError_t e = cudaFuncSetAttribute(
+      k_attn8<FP16, NT, RG, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+  if (e != cudaSuccess) return e;
+  k_attn8<FP16, NT, RG, ONE><<<g.ctas, S::THREADS, S::SMEM, s>>>(L, map);
+  return cudaGetLastError();
+}
 template <bool FP16, int NT, int RG>
 cudaError_t launch(const Attn4Launch& L, const Grid& g, const CUtensorMap& map, cudaStream_t s) {
-  cudaError_t e = cudaFuncSetAttribute(k_attn8<FP16, NT, RG>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<NT>::SMEM);
-  if (e != cudaSuccess) return e;
-  k_attn8<FP16, NT, RG><<<g.ctas, Shape<NT>::THREADS, Shape<NT>::SMEM, s>>>(L, map);
-  e = cudaGetLastError();
+  const cudaError_t e = g.one ? launch_shape<FP16, NT, RG, true>(L, g, map, s)
+                              : launch_shape<FP16, NT, RG, false>(L, g, map, s);
   if (e != cudaSuccess || !g.split) return e;
   constexpr int ROWS = 8 * NT * RG;
   const bool deep = 8 * g.items <= g.teams;
