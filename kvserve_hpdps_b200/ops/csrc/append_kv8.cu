@@ -10,11 +10,12 @@
 //
 // A unit's scale needs all of the call's tokens in it, wherever they stand in slot_mapping.  The
 // first of them (the leader) takes all 16 slots: so no two CTAs write one unit, there is no second
-// launch and no atomic, and results do not depend on timing.  A CTA looks for leaders among
-// a window of tokens.  Tokens of a unit mostly stand next to each other, so it first looks at the 15
-// tokens around; a unit that it finds there whole is settled.  Only for the others (both ends of
-// a sequence's new tokens, a decode step's) all slots of the call are looked through, by
-// 256 threads: 2 us for 16384.  In any order at all that is quadratic, and still 60 us for 16384.
+// launch and no atomic on the cache, and results do not depend on timing.  A CTA looks for leaders
+// among a window of tokens.  Tokens of a unit mostly stand next to each other: every warp looks at
+// the 15 tokens before and behind by itself, and a unit that it finds there whole, and not begun
+// before, is settled without another word.  Only for the others (both ends of a sequence's
+// new tokens, a decode step's) all slots of the call are looked through, by 256 threads.  In any
+// order at all that is quadratic: 16384 shuffled tokens take four times as long as in order.
 #include "append_kv.cuh"
 #include "kv8.cuh"
 
@@ -22,21 +23,10 @@ namespace kvs {
 
 namespace {
 
-constexpr int kWarps8 = kThreads / 32;
-constexpr int kManyTokens = 4096;  // from here on a CTA takes 16 tokens instead of one
-
-// Where a token goes; false: nowhere.
-KVS_DEV bool place(const AppendLaunch& L, int i, bool report, long long& slot) {
-  slot = load_index(L.slots, i, L.slots64);
-  if (slot < 0) return false;
-  bool ok = slot < L.num_slots;
-  if (ok && L.pos != nullptr) {
-    const long long pos = load_index(L.pos, i, L.pos64);
-    ok = pos >= 0 && pos < L.max_pos;
-  }
-  if (!ok && report) record_error(L.err, ERR_BOUNDS);
-  return ok;
-}
+constexpr int kWarps8 = kThreads / 32, kJobs = kWarps8 / 2;  // heads' keys or values at once
+// A CTA takes one token up to kFewTokens (decode steps: every token has a unit of its own), else 16;
+// up to kSomeTokens there are four CTAs for a window's units that are not whole.
+constexpr int kFewTokens = 512, kSomeTokens = 4096;
 
 // Rows of queries, eight lanes each, as k_append_kv deals them out.
 template <bool FP16, int MODE, int EACH>
@@ -85,36 +75,40 @@ KVS_DEV void rotate_queries(const AppendLaunch& L, const Spread& S, int x, int y
 }
 
 struct Units {
-  long long id[kUnit8];         // of a window token that is the first of its unit there; else -1
-  int member[kUnit8][kUnit8];   // [window token][offset] the call's last token there, or -1
+  int id[kUnit8];               // units to be looked for, or -1
+  int member[kUnit8][kUnit8];   // [unit][offset] the call's last token there, or -1
   int first[kUnit8];            // the call's first token in the unit
-  int count[kUnit8];            // tokens found around the window
-  int open;                     // some unit has to be looked for everywhere
 };
 
-// One unit's keys or values of one head, a warp: four rows at a time, eight lanes each.
+// One unit's keys or values of one head, two warps, eight rows each (16 in one warp's registers do
+// not fit beside a rotation's angles): four at a time, eight lanes a row.  This warp's row
+// 4 it + sub is token tok[it] at position pos[it], or is not the call's (-1).
 template <bool FP16, int MODE>
-KVS_DEV void append_unit(const AppendLaunch& L, const int (&member)[kUnit8], long long unit, int h,
-                         int value) {
-  const int lane = threadIdx.x & 31, l = lane & 7, sub = lane >> 3;
-  const int per = L.block_size / kUnit8;
-  const long long blk = L.num_slots < (1ll << 31)
-                            ? static_cast<long long>(static_cast<uint32_t>(unit) /
-                                                     static_cast<uint32_t>(per))
-                            : unit / per;
-  const int u = static_cast<int>(unit - blk * per);
-  uint8_t* const rec = static_cast<uint8_t*>(L.cache) + blk * L.block_stride + h * L.head_stride;
-  uint8_t* const rows = rec + (value * L.block_size + u * kUnit8) * 128ll;
+KVS_DEV void append_unit(const AppendLaunch& L, const int (&tok)[2], const long long (&pos)[2],
+                         bool begins, bool whole, int unit, int h, int value,
+                         uint32_t* s_top) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & 7, sub = lane >> 3;
+  // the largest of both warps'
+  auto both = [&](uint32_t top) {
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    if (lane == 0) s_top[warp] = top;
+    asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp >> 1)) : "memory");
+    top = max(top, s_top[warp ^ 1]);
+    asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp >> 1)) : "memory");
+    return top;
+  };
+  const uint32_t per = static_cast<uint32_t>(L.block_size) / kUnit8;
+  const uint32_t blk = static_cast<uint32_t>(unit) / per;
+  const int u = static_cast<int>(static_cast<uint32_t>(unit) - blk * per);
+  uint8_t* const rec = static_cast<uint8_t*>(L.cache) + static_cast<long long>(blk) * L.block_stride + h * L.head_stride;
+  uint8_t* const rows = rec + (value * L.block_size + u * kUnit8 + 8 * (warp & 1)) * 128ll;
   uint8_t* const byte = rec + 256ll * L.block_size + 2 * u + value;
-  const int was = *byte;
-  const bool begins = member[0] >= 0;
-  int tok[4];
-  float y[4][2][8];
+  const int was = whole ? 0 : *byte;
+  float y[2][2][8];
   uint32_t top = 0;
-  uint4 raw[4][2], partner[4][2];
+  uint4 raw[2][2], partner[2][2];
 #pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    tok[it] = member[4 * it + sub];
+  for (int it = 0; it < 2; ++it) {
     raw[it][0] = raw[it][1] = make_uint4(0u, 0u, 0u, 0u);
     if (tok[it] < 0) continue;
     const uint16_t* src = value ? static_cast<const uint16_t*>(L.value) + tok[it] * L.val_ts + h * L.val_hs
@@ -131,24 +125,24 @@ KVS_DEV void append_unit(const AppendLaunch& L, const int (&member)[kUnit8], lon
     }
   }
 #pragma unroll
-  for (int it = 0; it < 4; ++it) {
+  for (int it = 0; it < 2; ++it) {
     unpack8<FP16>(raw[it][0], y[it][0]);
     unpack8<FP16>(raw[it][1], y[it][1]);
     if (!value && L.pos != nullptr && tok[it] >= 0) {
       float co[2][8], si[2][8];
-      load_angles<FP16, MODE>(L, load_index(L.pos, tok[it], L.pos64), l, co, si);
+      load_angles<FP16, MODE>(L, pos[it], l, co, si);
       rotate<FP16, MODE>(L.rotary, l, partner[it], co, si, y[it]);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       top = max(top, __float_as_uint(y[it][i >> 3][i & 7]) & 0x7FFFFFFFu);
   }
-  top = __reduce_max_sync(0xFFFFFFFFu, top);
+  top = both(top);
   constexpr uint32_t kInf = 0x7F800000u;
   if (top >= kInf) {  // the largest that is finite; infinities become what is not a number
     top = 0;
 #pragma unroll
-    for (int it = 0; it < 4; ++it)
+    for (int it = 0; it < 2; ++it)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float& x = y[it][i >> 3][i & 7];
@@ -158,14 +152,14 @@ KVS_DEV void append_unit(const AppendLaunch& L, const int (&member)[kUnit8], lon
         else
           x = __uint_as_float(0x7FC00000u);
       }
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    top = both(top);
   }
   // a byte that no append writes is a cache's that was never cleared: it has no say
   const int old = was > kTopByte ? kLowScale : max(was - 127, kLowScale);
   const int need = scale_exponent(top), e = begins ? need : max(need, old);
   const float down = pow2(-e);
 #pragma unroll
-  for (int it = 0; it < 4; ++it) {
+  for (int it = 0; it < 2; ++it) {
     uint8_t* const row = rows + (4 * it + sub) * 128;
     if (tok[it] >= 0) {
 #pragma unroll
@@ -188,79 +182,120 @@ KVS_DEV void append_unit(const AppendLaunch& L, const int (&member)[kUnit8], lon
       }
     }
   }
-  __syncwarp();
-  if (lane == 0) *byte = static_cast<uint8_t>(e + 127);
+  if (lane == 0 && !(warp & 1)) *byte = static_cast<uint8_t>(e + 127);
 }
 
-// Blocks [0, kv): window x / parts, heads of part x % parts.  Behind them the queries.
+// Blocks [0, kv): of window x / (parts * subs) the heads of part x / subs % parts; units that are not
+// whole are dealt out to the subs.  Behind them the queries.
 template <bool FP16, int MODE, int WINDOW, int EACH>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 3)
     k_append_kv8(const __grid_constant__ AppendLaunch L, const __grid_constant__ Spread S, int kv,
-                 int parts) {
+                 int parts, int subs) {
   if (static_cast<int>(blockIdx.x) >= kv) {
     const unsigned q = blockIdx.x - kv;
     rotate_queries<FP16, MODE, EACH>(L, S, static_cast<int>(q % S.x), static_cast<int>(q / S.x));
     return;
   }
   __shared__ Units U;
-  const int tid = threadIdx.x, warp = tid >> 5;
-  const int part = static_cast<int>(blockIdx.x) % parts;
-  const int i0 = static_cast<int>(blockIdx.x) / parts * WINDOW;
-  const int lo = max(0, i0 - 15), hi = min(L.tokens, i0 + WINDOW + 15);
-  // ---- the window's units
-  if (tid < 32) {
-    long long unit = -1;
-    if (tid < WINDOW && i0 + tid < L.tokens) {
-      long long slot;
-      if (place(L, i0 + tid, part == 0, slot)) unit = slot / kUnit8;
+  __shared__ int8_t s_from[kWarps8][kUnit8];
+  __shared__ uint32_t s_top[kWarps8];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane >> 3;
+  const int x = static_cast<int>(blockIdx.x), mine = x % subs, part = x / subs % parts;
+  const int i0 = x / subs / parts * WINDOW;
+  // This pair of warps' heads' keys or values, keys and values in turn.
+  const int jobs = 2 * L.heads;
+  auto each = [&](auto f) {
+#pragma unroll 1
+    for (int n = part, j; (j = n * kJobs + (warp >> 1)) < jobs; n += parts) f(j >> 1, (j + n) & 1);
+  };
+  const int row0 = 8 * (warp & 1) + sub;  // of this lane in a unit; 4 further on the second
+  // ---- the window's tokens, the 15 behind them and the 15 before
+  long long slot = -1, slot_b = -1, pos = 0, pos_b = 0;
+  const int ia = i0 + lane, ib = i0 - 15 + lane;
+  const bool in = lane < WINDOW + 15 && ia < L.tokens, in_b = lane < 15 && ib >= 0;
+  if (in) slot = load_index(L.slots, ia, L.slots64);
+  if (in_b) slot_b = load_index(L.slots, ib, L.slots64);
+  if (L.pos != nullptr) {
+    if (in) pos = load_index(L.pos, ia, L.pos64);
+    if (in_b) pos_b = load_index(L.pos, ib, L.pos64);
+  }
+  auto fine = [&](long long slot, long long pos) {
+    return slot >= 0 && slot < L.num_slots && (L.pos == nullptr || (pos >= 0 && pos < L.max_pos));
+  };
+  if (lane < WINDOW && slot >= 0 && !fine(slot, pos) && part + mine + warp == 0)
+    record_error(L.err, ERR_BOUNDS);
+  const int unit = fine(slot, pos) ? static_cast<int>(slot / kUnit8) : -1;
+  const int unit_b = fine(slot_b, pos_b) ? static_cast<int>(slot_b / kUnit8) : -2;
+  const int off = static_cast<int>(slot) & (kUnit8 - 1);
+  const uint32_t same = __match_any_sync(0xFFFFFFFFu, unit);
+  uint32_t todo = __ballot_sync(0xFFFFFFFFu, lane < WINDOW && unit >= 0 && __ffs(same) - 1 == lane);
+  uint32_t open = 0;  // window tokens whose units have to be looked for everywhere
+  for (; todo != 0; todo &= todo - 1) {
+    const int k = __ffs(todo) - 1;
+    const int u = __shfl_sync(0xFFFFFFFFu, unit, k);
+    if (__any_sync(0xFFFFFFFFu, unit_b == u)) continue;  // begun before: another window's
+    const bool is = unit == u;
+    const uint32_t found = __ballot_sync(0xFFFFFFFFu, is);
+    const uint32_t offs = __reduce_or_sync(0xFFFFFFFFu, is ? 1u << off : 0u);
+    if (__popc(found) != kUnit8 || offs != 0xFFFFu) {
+      open |= 1u << k;
+      continue;
     }
-    const uint32_t same = __match_any_sync(0xFFFFFFFFu, unit);
-    if (unit >= 0 && __ffs(same) - 1 != tid) unit = -1;
-    if (tid < WINDOW) {
-      U.id[tid] = unit;
-      U.first[tid] = 0x7FFFFFFF;
-      U.count[tid] = 0;
+    if (mine != 0) continue;
+    if (is) s_from[warp][off] = static_cast<int8_t>(lane);
+    __syncwarp();
+    int tok[2];
+    long long at[2];
+#pragma unroll
+    for (int it = 0; it < 2; ++it) {
+      const int from = s_from[warp][row0 + 4 * it];
+      tok[it] = i0 + from;
+      at[it] = __shfl_sync(0xFFFFFFFFu, pos, from);
     }
-    if (tid == 0) U.open = 0;
+    each([&](int h, int value) {
+      append_unit<FP16, MODE>(L, tok, at, true, true, u, h, value, s_top);
+    });
+    __syncwarp();
+  }
+  if (open == 0) return;  // the same for all warps
+  // ---- the others: the tokens of the call that are in them, wherever they stand
+  if (warp == 0 && lane < WINDOW) {
+    U.id[lane] = open >> lane & 1u ? unit : -1;
+    U.first[lane] = 0x7FFFFFFF;
   }
   for (int i = tid; i < WINDOW * kUnit8; i += kThreads) U.member[i / kUnit8][i % kUnit8] = -1;
   __syncthreads();
-  auto take = [&](int i) {
+  for (int i = tid; i < L.tokens; i += kThreads) {
     const long long slot = load_index(L.slots, i, L.slots64);
-    if (slot < 0 || slot >= L.num_slots) return;
+    if (slot < 0 || slot >= L.num_slots) continue;
 #pragma unroll
     for (int k = 0; k < WINDOW; ++k) {
       if (U.id[k] == slot / kUnit8) {
-        long long again;
-        if (!place(L, i, false, again)) return;
-        atomicMax(&U.member[k][slot % kUnit8], i);
-        atomicMin(&U.first[k], i);
-        atomicAdd(&U.count[k], 1);
+        if (fine(slot, L.pos != nullptr ? load_index(L.pos, i, L.pos64) : 0)) {
+          atomicMax(&U.member[k][slot % kUnit8], i);
+          atomicMin(&U.first[k], i);
+        }
+        break;
       }
     }
-  };
-  // ---- the tokens around it, then all others where a unit is not found whole
-  if (lo + tid < hi) take(lo + tid);
-  __syncthreads();
-  if (tid < WINDOW && U.id[tid] >= 0 && (lo > 0 || hi < L.tokens)) {
-    bool whole = U.count[tid] == kUnit8;
-#pragma unroll
-    for (int k = 0; k < kUnit8; ++k) whole &= U.member[tid][k] >= 0;
-    if (!whole && U.first[tid] >= i0) U.open = 1;
   }
   __syncthreads();
-  if (U.open) {
-    for (int i = tid; i < lo; i += kThreads) take(i);
-    for (int i = hi + tid; i < L.tokens; i += kThreads) take(i);
-    __syncthreads();
-  }
-  // ---- a warp a head's keys or values
-  const int job = part * kWarps8 + warp;
-  if (job >= 2 * L.heads) return;
+  int turn = 0;
 #pragma unroll 1
-  for (int k = 0; k < WINDOW; ++k)
-    if (U.id[k] >= 0 && U.first[k] >= i0)
-      append_unit<FP16, MODE>(L, U.member[k], U.id[k], job >> 1, job & 1);
+  for (; open != 0; open &= open - 1) {
+    const int k = __ffs(open) - 1;
+    if (turn++ % subs != mine || U.first[k] < i0) continue;
+    int tok[2];
+    long long at[2];
+#pragma unroll
+    for (int it = 0; it < 2; ++it) {
+      tok[it] = U.member[k][row0 + 4 * it];
+      at[it] = tok[it] >= 0 && L.pos != nullptr ? load_index(L.pos, tok[it], L.pos64) : 0;
+    }
+    each([&](int h, int value) {
+      append_unit<FP16, MODE>(L, tok, at, U.member[k][0] >= 0, false, U.id[k], h, value, s_top);
+    });
+  }
 }
 
 // Eight lanes read one row: key rows of a token, then value rows; slot < 0 reads zeros.
@@ -326,19 +361,24 @@ template <bool FP16, int MODE, int WINDOW>
 int append(const AppendLaunch& L, cudaStream_t s) {
   const Spread S = spread_of(L.tokens, L.q_heads);
   const long long windows = (L.tokens + WINDOW - 1) / WINDOW;
-  const int parts = (2 * L.heads + kWarps8 - 1) / kWarps8;
-  const long long kv = windows * parts, q = L.q_heads > 0 ? static_cast<long long>(S.x) * S.y : 0;
-  if (kv + q >= (1ll << 31)) return -2;
+  // all heads in one CTA when there are windows enough: finding its units takes as long as a job
+  const int most = (2 * L.heads + kJobs - 1) / kJobs;
+  const int parts = windows >= 592 ? (most > 0) : most;
+  const int subs = WINDOW > 1 && L.tokens <= kSomeTokens ? 4 : 1;
+  const long long kv = windows * parts * subs;
+  const long long q = L.q_heads > 0 ? static_cast<long long>(S.x) * S.y : 0;
+  if (kv + q >= (1ll << 31) || L.num_slots / kUnit8 >= (1ll << 31)) return -2;
   const unsigned grid = static_cast<unsigned>(kv + q);
+  const int kv_ctas = static_cast<int>(kv);
   if (S.each == 4)
-    k_append_kv8<FP16, MODE, WINDOW, 4><<<grid, kThreads, 0, s>>>(L, S, static_cast<int>(kv), parts);
+    k_append_kv8<FP16, MODE, WINDOW, 4><<<grid, kThreads, 0, s>>>(L, S, kv_ctas, parts, subs);
   else
-    k_append_kv8<FP16, MODE, WINDOW, 1><<<grid, kThreads, 0, s>>>(L, S, static_cast<int>(kv), parts);
+    k_append_kv8<FP16, MODE, WINDOW, 1><<<grid, kThreads, 0, s>>>(L, S, kv_ctas, parts, subs);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 template <bool FP16, int MODE>
 int append_window(const AppendLaunch& L, cudaStream_t s) {
-  return L.tokens <= kManyTokens ? append<FP16, MODE, 1>(L, s) : append<FP16, MODE, kUnit8>(L, s);
+  return L.tokens <= kFewTokens ? append<FP16, MODE, 1>(L, s) : append<FP16, MODE, kUnit8>(L, s);
 }
 template <bool FP16>
 int append_mode(const AppendLaunch& L, cudaStream_t s) {
