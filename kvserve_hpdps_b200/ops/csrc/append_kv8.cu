@@ -26,7 +26,7 @@ namespace {
 constexpr int kWarps8 = kThreads / 32, kJobs = kWarps8 / 2;  // heads' keys or values at once
 // A CTA takes one token up to kFewTokens (decode steps: every token has a unit of its own), else 16;
 // up to kSomeTokens there are four CTAs for a window's units that are not whole.
-constexpr int kFewTokens = 512, kSomeTokens = 4096;
+constexpr int kFewTokens = 256, kSomeTokens = 1024;
 
 // Rows of queries, eight lanes each, as k_append_kv deals them out.
 template <bool FP16, int MODE, int EACH>
@@ -82,12 +82,14 @@ struct Units {
 
 // One unit's keys or values of one head, two warps, eight rows each (16 in one warp's registers do
 // not fit beside a rotation's angles): four at a time, eight lanes a row.  This warp's row
-// 4 it + sub is token tok[it] at position pos[it], or is not the call's (-1).
+// 4 it + sub is token tok<it> at position pos<it>, or is not the call's (-1).
 template <bool FP16, int MODE>
-KVS_DEV void append_unit(const AppendLaunch& L, const int (&tok)[2], const long long (&pos)[2],
-                         bool begins, bool whole, int unit, int h, int value,
+KVS_DEV void append_unit(const AppendLaunch& L, int tok0, int tok1, long long pos0, long long pos1,
+                                         bool begins, bool whole, int unit, int h, int value,
                          uint32_t* s_top) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & 7, sub = lane >> 3;
+  const int tok[2] = {tok0, tok1};
+  const long long pos[2] = {pos0, pos1};
   // the largest of both warps'
   auto both = [&](uint32_t top) {
     top = __reduce_max_sync(0xFFFFFFFFu, top);
@@ -188,7 +190,7 @@ KVS_DEV void append_unit(const AppendLaunch& L, const int (&tok)[2], const long 
 // Blocks [0, kv): of window x / (parts * subs) the heads of part x / subs % parts; units that are not
 // whole are dealt out to the subs.  Behind them the queries.
 template <bool FP16, int MODE, int WINDOW, int EACH>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, WINDOW == 1 ? 2 : 3)
     k_append_kv8(const __grid_constant__ AppendLaunch L, const __grid_constant__ Spread S, int kv,
                  int parts, int subs) {
   if (static_cast<int>(blockIdx.x) >= kv) {
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 3)
     return;
   }
   __shared__ Units U;
-  __shared__ int8_t s_from[kWarps8][kUnit8];
+  __shared__ int s_from[kWarps8][kUnit8];
   __shared__ uint32_t s_top[kWarps8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane >> 3;
   const int x = static_cast<int>(blockIdx.x), mine = x % subs, part = x / subs % parts;
@@ -209,6 +211,48 @@ __global__ void __launch_bounds__(kThreads, 3)
     for (int n = part, j; (j = n * kJobs + (warp >> 1)) < jobs; n += parts) f(j >> 1, (j + n) & 1);
   };
   const int row0 = 8 * (warp & 1) + sub;  // of this lane in a unit; 4 further on the second
+  auto fine = [&](long long slot, long long pos) {
+    return slot >= 0 && slot < L.num_slots && (L.pos == nullptr || (pos >= 0 && pos < L.max_pos));
+  };
+  auto position = [&](int i) { return L.pos != nullptr ? load_index(L.pos, i, L.pos64) : 0; };
+  if constexpr (WINDOW == 1) {
+    // ---- few tokens: every warp looks through all slots, which it asks for with its own token's
+    long long at[kFewTokens / 32];
+#pragma unroll
+    for (int n = 0; n < kFewTokens / 32; ++n)
+      at[n] = lane + 32 * n < L.tokens ? load_index(L.slots, lane + 32 * n, L.slots64) : -1;
+    const long long slot = load_index(L.slots, i0, L.slots64), pos = position(i0);
+    if (!fine(slot, pos)) {
+      if (slot >= 0 && part + tid == 0) record_error(L.err, ERR_BOUNDS);
+      return;
+    }
+    if (lane < kUnit8) s_from[warp][lane] = -1;
+    __syncwarp();
+    int first = i0;
+#pragma unroll
+    for (int n = 0; n < kFewTokens / 32; ++n) {
+      const int i = lane + 32 * n;
+      if (at[n] / kUnit8 == slot / kUnit8 && at[n] >= 0 && (i == i0 || fine(at[n], position(i)))) {
+        atomicMax(&s_from[warp][at[n] % kUnit8], i);
+        first = min(first, i);
+      }
+    }
+    __syncwarp();
+    if (__reduce_min_sync(0xFFFFFFFFu, first) < i0) return;
+    const uint32_t has = __ballot_sync(0xFFFFFFFFu, lane < kUnit8 && s_from[warp][lane & 15] >= 0);
+    int tok[2];
+    long long where[2];
+#pragma unroll
+    for (int it = 0; it < 2; ++it) {
+      tok[it] = s_from[warp][row0 + 4 * it];
+      where[it] = tok[it] < 0 || tok[it] == i0 ? pos : position(tok[it]);
+    }
+    each([&](int h, int value) {
+      append_unit<FP16, MODE>(L, tok[0], tok[1], where[0], where[1], has & 1u, has == 0xFFFFu,
+                              static_cast<int>(slot / kUnit8), h, value, s_top);
+    });
+    return;
+  }
   // ---- the window's tokens, the 15 behind them and the 15 before
   long long slot = -1, slot_b = -1, pos = 0, pos_b = 0;
   const int ia = i0 + lane, ib = i0 - 15 + lane;
@@ -219,9 +263,6 @@ __global__ void __launch_bounds__(kThreads, 3)
     if (in) pos = load_index(L.pos, ia, L.pos64);
     if (in_b) pos_b = load_index(L.pos, ib, L.pos64);
   }
-  auto fine = [&](long long slot, long long pos) {
-    return slot >= 0 && slot < L.num_slots && (L.pos == nullptr || (pos >= 0 && pos < L.max_pos));
-  };
   if (lane < WINDOW && slot >= 0 && !fine(slot, pos) && part + mine + warp == 0)
     record_error(L.err, ERR_BOUNDS);
   const int unit = fine(slot, pos) ? static_cast<int>(slot / kUnit8) : -1;
@@ -242,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 3)
       continue;
     }
     if (mine != 0) continue;
-    if (is) s_from[warp][off] = static_cast<int8_t>(lane);
+    if (is) s_from[warp][off] = lane;
     __syncwarp();
     int tok[2];
     long long at[2];
@@ -253,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 3)
       at[it] = __shfl_sync(0xFFFFFFFFu, pos, from);
     }
     each([&](int h, int value) {
-      append_unit<FP16, MODE>(L, tok, at, true, true, u, h, value, s_top);
+      append_unit<FP16, MODE>(L, tok[0], tok[1], at[0], at[1], true, true, u, h, value, s_top);
     });
     __syncwarp();
   }
@@ -265,14 +306,28 @@ __global__ void __launch_bounds__(kThreads, 3)
   }
   for (int i = tid; i < WINDOW * kUnit8; i += kThreads) U.member[i / kUnit8][i % kUnit8] = -1;
   __syncthreads();
-  for (int i = tid; i < L.tokens; i += kThreads) {
-    const long long slot = load_index(L.slots, i, L.slots64);
-    if (slot < 0 || slot >= L.num_slots) continue;
+  // Eight slots a thread at a time, whose loads are in flight together: one after the other they
+  // took 40 us for 16384.
+  const bool wanted = lane < WINDOW && (open >> lane & 1u);
+  const int low = __reduce_min_sync(0xFFFFFFFFu, wanted ? unit : 0x7FFFFFFF),
+            high = __reduce_max_sync(0xFFFFFFFFu, wanted ? unit : -1);
+  for (int from = tid; from < L.tokens; from += 8 * kThreads) {
+    long long at[8];
 #pragma unroll
-    for (int k = 0; k < WINDOW; ++k) {
-      if (U.id[k] == slot / kUnit8) {
-        if (fine(slot, L.pos != nullptr ? load_index(L.pos, i, L.pos64) : 0)) {
-          atomicMax(&U.member[k][slot % kUnit8], i);
+    for (int n = 0; n < 8; ++n) {
+      const int i = from + n * kThreads;
+      at[n] = i < L.tokens ? load_index(L.slots, i, L.slots64) : -1;
+    }
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      if (at[n] < 0 || at[n] >= L.num_slots) continue;
+      const int in_unit = static_cast<int>(at[n] / kUnit8), i = from + n * kThreads;
+      if (in_unit < low || in_unit > high) continue;
+#pragma unroll 1
+      for (int k = 0; k < WINDOW; ++k) {
+        if (U.id[k] != in_unit) continue;
+        if (fine(at[n], position(i))) {
+          atomicMax(&U.member[k][at[n] % kUnit8], i);
           atomicMin(&U.first[k], i);
         }
         break;
@@ -290,10 +345,11 @@ __global__ void __launch_bounds__(kThreads, 3)
 #pragma unroll
     for (int it = 0; it < 2; ++it) {
       tok[it] = U.member[k][row0 + 4 * it];
-      at[it] = tok[it] >= 0 && L.pos != nullptr ? load_index(L.pos, tok[it], L.pos64) : 0;
+      at[it] = tok[it] >= 0 ? position(tok[it]) : 0;
     }
     each([&](int h, int value) {
-      append_unit<FP16, MODE>(L, tok, at, U.member[k][0] >= 0, false, U.id[k], h, value, s_top);
+      append_unit<FP16, MODE>(L, tok[0], tok[1], at[0], at[1], U.member[k][0] >= 0, false,
+                              U.id[k], h, value, s_top);
     });
   }
 }
