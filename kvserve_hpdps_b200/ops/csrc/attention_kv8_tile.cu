@@ -153,22 +153,26 @@ KVS_DEV void convert_role(const Attn4Launch& L, const CUtensorMap* map, Walk wal
       if (asked >= RING && !wait_phase(&C->k_empty[asks.slot], asks.phase ^ 1, L.err)) return false;
       const int block = __shfl_sync(0xFFFFFFFFu, id, at);
       const int place = __shfl_sync(0xFFFFFFFFu, off, at);
+      uint64_t *const k_bar = &C->k_full[asks.slot], *const v_bar = &C->v_came[unit][asks.slot];
+      if (elected() && block >= 0) {
+        const uint32_t to = smem_u32(smem) + asks.slot * kCodes + unit * (kUnit8 * 128);
+        mbar_expect_tx(k_bar, kUnit8 * 128);
+        load_rows(to + Layout<FP16>::keys, map, place, p.h, block, k_bar);
+        mbar_expect_tx(v_bar, kUnit8 * 128);
+        load_rows(to + Layout<FP16>::codes, map, L.block_size + place, p.h, block, v_bar);
+      }
+      __syncwarp();
+      // the scales, which a piece's first copies need not wait for
       const uint32_t sc = __shfl_sync(0xFFFFFFFFu, scale, at);
-      const uint32_t note = asked % kNotes, bytes = block >= 0 ? kUnit8 * 128 : 0;
+      const uint32_t note = asked % kNotes;
       if (elected()) {
-        uint64_t *const k_bar = &C->k_full[asks.slot], *const v_bar = &C->v_came[unit][asks.slot];
         reinterpret_cast<float*>(&C->k_up[note])[unit] = __uint_as_float((sc & 0xFFu) << 23);
         reinterpret_cast<float*>(&C->v_exp[note])[unit] =
             static_cast<float>(static_cast<int>(sc >> 8) - 127);
         reinterpret_cast<uint8_t*>(&C->gone[note])[unit] = block == -2 ? 1 : 0;
         C->bad[note][unit] = 0;
-        mbar_arrive_expect_tx(k_bar, bytes);
-        mbar_arrive_expect_tx(v_bar, bytes);
-        if (block >= 0) {
-          const uint32_t at = smem_u32(smem) + asks.slot * kCodes + unit * (kUnit8 * 128);
-          load_rows(at + Layout<FP16>::keys, map, place, p.h, block, k_bar);
-          load_rows(at + Layout<FP16>::codes, map, L.block_size + place, p.h, block, v_bar);
-        }
+        mbar_arrive(k_bar);
+        mbar_arrive(v_bar);
       }
       __syncwarp();
       has = (has & ~(1u << asks.slot)) | (block >= 0 ? 1u : 0u) << asks.slot;
@@ -336,6 +340,12 @@ KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, int x, uint32_
 }
 
 // ------------------------------------------------------------------ softmax
+// A pointer that another lane has.
+KVS_DEV const uint8_t* of_lane(const uint8_t* p, int lane) {
+  return reinterpret_cast<const uint8_t*>(
+      __shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(p), lane));
+}
+
 template <bool FP16>
 KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* smem,
                           uint32_t tmem, const Parts& P, Ctrl* C) {
@@ -344,6 +354,10 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* s
   const uint32_t S = tmem + 64 * x + lanes, O = tmem + kOutAt + 128 * x + lanes;
   constexpr int PARTS = Room<FP16>::PARTS;
   uint8_t* const qt = smem + x * PARTS * kPart;
+  // Two places of 32 rows of 128 bytes, 16 KB apart: the warp's own queries', where rows and results
+  // change from a thread a row to whole lines.
+  const int lane = threadIdx.x & 31;
+  uint8_t* const area = qt + (row - lane) * 128;
   uint32_t notes = 0, half_no = 0;  // halves before this piece; this tile's
   Piece p;
   while (walk.next(L, group, p)) {
@@ -353,6 +367,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* s
     }
     const int rr = p.tile * kRows + x * 128 + row;
     const bool mine = rr < p.nrows;
+    const uint32_t has = __ballot_sync(0xFFFFFFFFu, mine);
     const long long tq = p.s.row0 + rr / group;
     const int hq = p.h * group + rr % group;
     const int seen = mine ? seen_by(L, p.s, rr / group) : 0;
@@ -360,13 +375,27 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* s
     bool poisoned = false;
     if (p.steps > 0) {
       // ---- the row scaled by a power of two, its largest element in (224, 448], in e4m3 parts
-      uint4 raw[16] = {};
-      if (mine) {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(L.q) +
-                                                          tq * L.q_ts + hq * L.q_hs);
+      uint4 raw[16];
+      // a row that is not there is read from the first one: with a load each behind a condition of
+      // its own the 16 came one after the other (11000 clocks a piece against 3800)
+      const uint8_t* const src = reinterpret_cast<const uint8_t*>(
+          static_cast<const uint16_t*>(L.q) + (mine ? tq * L.q_ts + hq * L.q_hs : 0));
 #pragma unroll
-        for (int i = 0; i < 16; ++i) raw[i] = src[i];
+      for (int i = 0; i < 16; ++i) {  // half a warp a row: whole lines, where a thread's own row is 16
+        const int r = 2 * i + (lane >> 4);
+        const uint8_t* const from = of_lane(src, r);
+        raw[i] = *reinterpret_cast<const uint4*>(from + 16 * (lane & 15));
+        if (!(has >> r & 1u)) raw[i] = make_uint4(0u, 0u, 0u, 0u);
       }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        *reinterpret_cast<uint4*>(area + (lane >> 3 & 1) * kPart +
+                                  at128(2 * i + (lane >> 4), lane & 7)) = raw[i];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        raw[i] = *reinterpret_cast<const uint4*>(area + (i >> 3) * kPart + at128(lane, i & 7));
+      __syncwarp();  // the parts take their place
       float top = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -591,11 +620,29 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* s
     const float unit = p.steps > 0 ? pow2(static_cast<int>(K)) : 0.f;
     const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
     const int slot = 2 * static_cast<int>(blockIdx.x) + (p.begins ? 1 : 0);
-    uint16_t* const out = static_cast<uint16_t*>(L.out) + tq * L.o_ts + hq * L.o_hs;
-    float* const part = P.o + (static_cast<long long>(slot) * kRows + x * 128 + row) * 128;
+    uint8_t* const out = reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(L.out) + tq * L.o_ts +
+                                                    hq * L.o_hs);
+    uint8_t* const part = reinterpret_cast<uint8_t*>(
+        P.o + (static_cast<long long>(slot) * kRows + x * 128 + row) * 128);
+    // 128 bytes of each row, from a thread a row
+    auto flush = [&](const uint4 (&w)[8], uint8_t* at, uint8_t* to) {
 #pragma unroll
-    for (int cg = 0; cg < 4; ++cg) {
-      float v[32];
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(at + at128(lane, i)) = w[i];
+      __syncwarp();
+      uint4 y[8];
+      uint8_t* dst[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        y[i] = *reinterpret_cast<const uint4*>(at + at128(r, lane & 7));
+        dst[i] = const_cast<uint8_t*>(of_lane(to, r)) + 16 * (lane & 7);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (has >> (4 * i + (lane >> 3)) & 1u) *reinterpret_cast<uint4*>(dst[i]) = y[i];
+    };
+    // 32 channels of the output, in loops: what runs once a piece is not in the instruction cache
+    auto channels = [&](int cg, float (&v)[32]) {
       if (p.steps > 0) {
         tmem_ld32(O + 32 * cg, v);
       } else {
@@ -608,25 +655,37 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* s
         for (int i = 0; i < 32; ++i)
           if (bits >> i & 1u) v[i] = __uint_as_float(0x7FC00000u);
       }
-      if (!mine) continue;
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] *= unit;
-      if (p.whole) {
+    };
+    if (p.whole) {
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        uint4 w[8];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] *= inv;
-      }
+        for (int cg = 0; cg < 2; ++cg) {
+          float v[32];
+          channels(2 * half + cg, v);
 #pragma unroll
-      for (int ch = 0; ch < 4; ++ch) {
-        float y[8];
+          for (int i = 0; i < 32; ++i) v[i] *= inv;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = v[8 * ch + i];
-        if (p.whole) {
-          *reinterpret_cast<uint4*>(out + 32 * cg + 8 * ch) = pack8<FP16>(y);
-        } else {
-          float4* d = reinterpret_cast<float4*>(part + 32 * cg + 8 * ch);
-          d[0] = make_float4(y[0], y[1], y[2], y[3]);
-          d[1] = make_float4(y[4], y[5], y[6], y[7]);
+          for (int i = 0; i < 4; ++i)
+            w[4 * cg + i] = pack8<FP16>(*reinterpret_cast<const float(*)[8]>(v + 8 * i));
         }
+        flush(w, area + half * kPart, out + 128 * half);
+      }
+    } else {
+#pragma unroll 1
+      for (int cg = 0; cg < 4; ++cg) {
+        float v[32];
+        channels(cg, v);
+        uint4 w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          w[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
+                            __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+        flush(w, area + (cg & 1) * kPart, part + 128 * cg);
+        __syncwarp();
       }
     }
     if (mine) {

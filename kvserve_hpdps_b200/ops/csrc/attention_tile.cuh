@@ -107,6 +107,11 @@ KVS_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: 
 // A tile's cost is linear in its number: with n rows' worth of queries and `len` tokens,
 // tile t's last row sees about len - n + (256 t + 255) / group + 1 of them (all without causal
 // limits).  In units of 1 / group tokens: cost(t) = first + more t, which sums up in closed form.
+// a / b of numbers that mostly have 32 bits (a 64-bit division is some 150 instructions).
+KVS_DEV long long div64(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
 struct TileWork {
   int tiles, more;        // what each tile costs more than the one before it
   long long first, head;  // cost of tile 0; of a head's tiles together
@@ -136,7 +141,7 @@ struct Piece {
 struct Walk {
   long long U, pos, end, begin;
   int r, used, b;
-  KVS_DEV long long share(int i) const { return U * i / used; }
+  KVS_DEV long long share(int i) const { return div64(U * i, used); }
   KVS_DEV bool next(const Attn4Launch& L, int group, Piece& p) {
     const long long unit = static_cast<long long>(kTile) * group;
     while (pos < end) {
@@ -148,7 +153,7 @@ struct Walk {
         continue;
       }
       long long off = pos - begin;
-      const int h = static_cast<int>(off / w.head);
+      const int h = static_cast<int>(div64(off, w.head));
       off -= h * w.head;
       int lo = 0, hi = w.tiles - 1;  // the last tile that begins at or before off
       while (lo < hi) {
@@ -167,7 +172,7 @@ struct Walk {
       auto step_of = [&](long long x) {
         if (x >= item + cost) return all;
         if (x <= body) return 0;
-        const long long k = (x - body) / unit;
+        const long long k = div64(x - body, unit);
         return static_cast<int>(k < all ? k : all);
       };
       const int u0 = step_of(pos), u1 = step_of(to);
@@ -185,7 +190,7 @@ struct Walk {
       p.whole = u0 == 0 && u1 == all;
       if (p.begins && !p.whole) {  // the last part is the CTA's whose share reaches the last step
         const long long x = min(item + cost, body + all * unit) - 1;
-        p.parts = static_cast<int>(((x + 1) * used + U - 1) / U - 1) - b + 1;
+        p.parts = static_cast<int>(div64((x + 1) * used + U - 1, U) - 1) - b + 1;
       }
       return true;
     }
