@@ -696,7 +696,8 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* s
             l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
     }
     if (!p.whole && p.begins && threadIdx.x == 0)
-      P.desc[blockIdx.x] = make_int4(p.r, p.h, p.tile, p.parts);
+      P.desc[blockIdx.x] = make_int4(p.s.row0, p.h, p.tile,
+                                     p.parts | min(kRows, p.nrows - p.tile * kRows) << 16);
     tc_fence_before();
     __syncwarp();
   }
@@ -823,7 +824,9 @@ cudaError_t launch(const Attn4Launch& L, const CUtensorMap& map, cudaStream_t s)
   const int ctas = tile_ctas(L);
   k_attn8_tile<FP16><<<ctas, kThreads, Layout<FP16>::bytes, s>>>(L, map);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  return launch_combine<FP16, kRows / 8, 1>(L, ctas, s);
+  const long long rows = static_cast<long long>(L.max_q) * (L.q_heads / L.heads);
+  return launch_join<FP16, kRows>(L, ctas, static_cast<long long>(L.seqs) * L.heads *
+                                               ((rows + kRows - 1) / kRows), s);
 }
 
 }  // namespace

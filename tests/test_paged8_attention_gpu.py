@@ -68,12 +68,12 @@ def _tiles(table, rows, hq, h, bs):
     """Whether a call takes the kernel for many rows, going by what the host knows: rows a kv
     head, and rows times tokens that the table has room for."""
     rows *= hq // h
-    return rows > 64 and rows * h * table.numel() * bs > 5 << 20
+    return rows > 64 and rows * h * table.numel() * bs > 3 << 20
 
 
 def _wide(rows, seqs, hq, h, bs=16):
     """Table columns that take a call of few tokens there all the same."""
-    return (6 << 20) // (rows * (hq // h) * h * seqs * bs) + 1
+    return (4 << 20) // (rows * (hq // h) * h * seqs * bs) + 1
 
 
 def _attend(q, cache, table, lens, start=None, most=1, **kw):
