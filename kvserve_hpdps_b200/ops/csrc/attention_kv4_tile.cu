@@ -51,6 +51,7 @@ namespace {
 
 // Tokens (of 32) with scales less than kApart of the largest take a scale each: a row may see only
 // the small ones, or need their bits.
+constexpr int kOverTile = 2;     // an item's own cost, in steps
 constexpr float kApart = 0x1p-8f;
 constexpr uint32_t kHides = 1, kWideK = 2, kWideV = 4;
 constexpr int kFar = 60;
@@ -120,7 +121,7 @@ KVS_DEV uint32_t phase_of(uint32_t step) {  // of its slot's barriers
 constexpr int kRestAt = 2 * kHalfTile;
 
 template <bool FP16, int NG>
-KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q_tile,
+KVS_DEV void convert_role(const Attn4Launch& L, Walk<kOverTile> walk, int group, uint8_t* q_tile,
                           uint8_t* k_tile, uint8_t* v_tile, Ctrl* C) {
   const int lane = threadIdx.x & 31, seg = (threadIdx.x >> 5) & 3, row = seg * 32 + lane;
   constexpr uint32_t kInf = FP16 ? 0x7C00u : 0x7F80u;
@@ -306,7 +307,7 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q
 // their own.  A stage is free when both tiles' products with it are done; without a second tile
 // its warps only say so.
 template <bool FP16, bool QK>
-KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, int x, uint32_t q_tile,
+KVS_DEV void mma_role(const Attn4Launch& L, Walk<kOverTile> walk, int group, int x, uint32_t q_tile,
                       uint32_t kv_tile, uint32_t tmem, Ctrl* C) {
   uint32_t step_no = 0, piece_no = 0, half_no = 0;
   Piece p;
@@ -382,7 +383,7 @@ KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, int x, uint32_
 
 // ------------------------------------------------------------------ softmax
 template <bool FP16, int NG>
-KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* q_tile,
+KVS_DEV void softmax_role(const Attn4Launch& L, Walk<kOverTile> walk, int group, uint8_t* q_tile,
                           uint32_t tmem, const Parts& P, Ctrl* C) {
   const int x = threadIdx.x >> 7, row = threadIdx.x & 127;
   const uint32_t lanes = static_cast<uint32_t>((threadIdx.x >> 5) & 3) << 21;  // a warp's 32
@@ -764,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
   for (int r = tid; r < L.seqs; r += kThreads) {
     const Seq s = sequence(L, r, b == 0);
     named.take(L, s, r);
-    mine = tile_work(L, s, group).head * L.heads;
+    mine = tile_work<kOverTile>(L, s, group).head * L.heads;
     total += mine;
   }
 #pragma unroll
@@ -779,7 +780,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) total += C->scan[w];
   const long long least = static_cast<long long>(kLeastTile) * kTile * group;
-  Walk walk;
+  Walk<kOverTile> walk;
   walk.U = total;
   walk.b = b;
   walk.used = static_cast<int>(min(static_cast<long long>(B), (total + least - 1) / least));
@@ -790,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
     for (int r0 = 0; r0 < L.seqs; r0 += kThreads) {
       const int r = r0 + tid;
       if (L.seqs > kThreads)  // else `mine` is it
-        mine = r < L.seqs ? tile_work(L, sequence(L, r, false), group).head * L.heads : 0;
+        mine = r < L.seqs ? tile_work<kOverTile>(L, sequence(L, r, false), group).head * L.heads : 0;
       long long inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -841,7 +842,7 @@ cudaError_t launch(const Attn4Launch& L, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(k_attn4_tile<FP16, NG>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  const int ctas = tile_ctas(L);
+  const int ctas = tile_ctas<kOverTile>(L);
   k_attn4_tile<FP16, NG><<<ctas, kThreads, kSmem, s>>>(L);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   return launch_combine<FP16, kRows / 8, 1>(L, ctas, s);
@@ -858,7 +859,7 @@ cudaError_t attn4_tile_launch(const Attn4Launch& L, cudaStream_t s) {
 }
 
 long long attn4_tile_scratch(const Attn4Launch& L) {
-  return 16ll * tile_ctas(L) + 2ll * tile_ctas(L) * kRows * (8 + 512);
+  return 16ll * tile_ctas<kOverTile>(L) + 2ll * tile_ctas<kOverTile>(L) * kRows * (8 + 512);
 }
 
 }  // namespace kvs

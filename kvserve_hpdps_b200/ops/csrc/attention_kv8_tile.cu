@@ -20,9 +20,9 @@
 // Roles of a CTA (one an SM, 16 warps whose registers are dealt out anew):
 //   warps 0-3, 4-7   softmax of query tile 0, 1: a thread a row, which it reads from tensor memory
 //                    and writes back as fp16 weights, the A operand of O += P V
-//   warps 8-11       ask the copy engine for codes, ahead, and turn the values' into fp16 tiles in
-//                    shared memory, a warp a unit of each half
-//   warps 12-15      issue the matrix instructions: S of tile 0, 1, O of tile 0, 1
+//   warps 8-11       turn the values' codes into fp16 tiles in shared memory, a warp a unit of each half
+//   warps 12, 13, 14 issue the matrix instructions: S of tile 0, 1, O of both
+//   warp 15          deals out the pieces of the CTA's share and asks the copy engine for codes, ahead
 // All go by halves of 64 tokens.  The softmax warps take a half's scores into registers, so that the
 // next ones are computed while they work.  O stays in tensor memory; it is rescaled by the softmax
 // warps when 64 weights of a row sum up to more than kMostSum, which after the first tiles is rare.
@@ -41,11 +41,16 @@ constexpr float kFar = 60.f;
 // be (the same for all of a row's, so that 2^4 does no harm).
 constexpr float kHuge = 0x1p2f;
 
+// An item's own cost in steps of 128 tokens: the share is what a CTA's pieces take, 18000 clocks each
+// and 4600 a step (2 x 2048 rows: 396 us with 2, 393 with 3 and 4, 396 with 6).
+constexpr int kOverTile = 3;
 constexpr int kHalf = 64;                  // tokens
 constexpr int kCodes = kHalf * 128;        // bytes of a half's key or value codes
 constexpr int kValues = 2 * kHalf * 128;   // of its values as fp16
 constexpr int kPart = 128 * 128;           // of a part of a query tile
 constexpr int kNotes = 16;                 // halves that something is known of
+constexpr int kPieces = 4;                 // pieces that are dealt out ahead
+constexpr int kReaders = 15;               // warps that take them
 
 // RING halves' key codes and value codes are there or on their way, four halves' values as fp16.
 template <bool FP16>
@@ -55,8 +60,10 @@ struct Room {
 constexpr int kTiles = 4;
 
 struct Ctrl {
-  uint64_t q_full[2], k_full[4], k_empty[4], v_came[4][4], v_full[kTiles], v_empty[kTiles];
+  uint64_t q_full[2], k_full[4], k_empty[4], v_came[4], v_taken[4], v_full[kTiles], v_empty[kTiles];
   uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2][2], done[2];
+  uint64_t piece_full[kPieces], piece_empty[kPieces];
+  Piece piece[kPieces];
   uint32_t tmem;
   uint32_t any_bad;         // some half of this CTA had values that are not numbers
   // What is known of a half, by units:
@@ -99,26 +106,46 @@ KVS_DEV uint32_t not_numbers(uint32_t w) {
   return ((w & 0x7F7F7F7Fu) + 0x01010101u) >> 7 & 0x01010101u;
 }
 
-// ------------------------------------------------------------ codes to tiles
+// ---------------------------------------------------------- pieces and codes
+// The next piece, as the fetching warp left it; false behind the last one.
+KVS_DEV bool take_piece(const Attn4Launch& L, Ctrl* C, Turn<kPieces>& at, Piece& p) {
+  if (!wait_phase(&C->piece_full[at.slot], at.phase, L.err)) return false;
+  p = C->piece[at.slot];
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&C->piece_empty[at.slot]);
+  at.next();
+  return p.r >= 0;
+}
+
+// One warp walks through the CTA's share, ahead of all others, and asks the copy engine for codes.
 template <bool FP16>
-KVS_DEV void convert_role(const Attn4Launch& L, const CUtensorMap* map, Walk walk, int group,
-                          uint8_t* smem, Ctrl* C) {
-  constexpr int RING = Room<FP16>::RING, AHEAD = RING - 1;
-  const int lane = threadIdx.x & 31, unit = (threadIdx.x >> 5) & 3, sub = lane >> 3, c = lane & 7;
-  Turn<RING> asks, comes;
-  Turn<kTiles> fills;
-  uint32_t asked = 0, half_no = 0, has = 0;  // has: slots that hold codes
-  Piece p;
-  // of the two fp16 chunks 2 c and 2 c + 1 the one whose place leaves no bank conflict goes first
-  const bool swap = c >= 4;
-  while (walk.next(L, group, p)) {
+KVS_DEV void fetch_role(const Attn4Launch& L, const CUtensorMap* map, Walk<kOverTile> walk, int group,
+                        uint32_t smem, Ctrl* C) {
+  constexpr int RING = Room<FP16>::RING;
+  const int lane = threadIdx.x & 31;
+  Turn<RING> asks;
+  Turn<kPieces> to;
+  uint32_t asked = 0, told = 0;
+  for (bool more = true; more;) {
+    Piece p;
+    more = walk.next(L, group, p);
+    if (told >= kPieces && !wait_phase(&C->piece_empty[to.slot], to.phase ^ 1, L.err)) return;
+    if (elected()) {
+      if (!more) p.r = -1;
+      C->piece[to.slot] = p;
+      mbar_arrive(&C->piece_full[to.slot]);
+    }
+    __syncwarp();
+    to.next();
+    ++told;
+    if (!more) return;
     const uint8_t* const head = static_cast<const uint8_t*>(L.cache) + p.h * L.head_stride;
     const int32_t* const table = L.table + p.r * L.table_stride;
-    // Blocks, places and scales of this warp's unit in 32 halves, a lane each; and in the next 32.
+    // Blocks, places and scales of 8 halves' units, a lane each; and of the next 8's.
     int id = -1, off = 0, id2 = -1, off2 = 0;
     uint32_t scale = 0x7F7Fu, scale2 = 0x7F7Fu;
     auto look = [&](int i, int& id, int& off) {  // from half i on
-      const int tok = p.start + (i + lane) * kHalf + kUnit8 * unit;
+      const int tok = p.start + i * kHalf + kUnit8 * lane;
       id = -1;
       if (tok < p.stop) {
         const int page = tok / L.block_size;
@@ -136,8 +163,8 @@ KVS_DEV void convert_role(const Attn4Launch& L, const CUtensorMap* map, Walk wal
         scale = *reinterpret_cast<const uint16_t*>(head + id * L.block_stride +
                                                    256ll * L.block_size + (off >> 3));
     };
-    auto ask = [&](int i) -> bool {  // for the unit's codes in half i
-      const int at = i & 31;
+    for (int i = 0; i < p.halves; ++i, ++asked) {
+      const int at = i & 7;
       if (i == 0) {
         look(0, id, off);
         look_scale(id, off, scale);
@@ -145,55 +172,87 @@ KVS_DEV void convert_role(const Attn4Launch& L, const CUtensorMap* map, Walk wal
         id = id2;
         off = off2;
         scale = scale2;
-      } else if (at == 16) {
-        look(i + 16, id2, off2);
-      } else if (at == 24) {
+      } else if (at == 2) {
+        look(i + 6, id2, off2);
+      } else if (at == 5) {
         look_scale(id2, off2, scale2);
       }
-      if (asked >= RING && !wait_phase(&C->k_empty[asks.slot], asks.phase ^ 1, L.err)) return false;
-      const int block = __shfl_sync(0xFFFFFFFFu, id, at);
-      const int place = __shfl_sync(0xFFFFFFFFu, off, at);
-      uint64_t *const k_bar = &C->k_full[asks.slot], *const v_bar = &C->v_came[unit][asks.slot];
-      if (elected() && block >= 0) {
-        const uint32_t to = smem_u32(smem) + asks.slot * kCodes + unit * (kUnit8 * 128);
-        mbar_expect_tx(k_bar, kUnit8 * 128);
-        load_rows(to + Layout<FP16>::keys, map, place, p.h, block, k_bar);
-        mbar_expect_tx(v_bar, kUnit8 * 128);
-        load_rows(to + Layout<FP16>::codes, map, L.block_size + place, p.h, block, v_bar);
+      if (asked >= RING && (!wait_phase(&C->k_empty[asks.slot], asks.phase ^ 1, L.err) ||
+                            !wait_phase(&C->v_taken[asks.slot], asks.phase ^ 1, L.err)))
+        return;
+      uint64_t *const k_bar = &C->k_full[asks.slot], *const v_bar = &C->v_came[asks.slot];
+      int block[4], place[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        block[u] = __shfl_sync(0xFFFFFFFFu, id, 4 * at + u);
+        place[u] = __shfl_sync(0xFFFFFFFFu, off, 4 * at + u);
+      }
+      if (elected()) {  // one lane: copies by several are issued one after the other anyway
+        const uint32_t bytes = kUnit8 * 128 * ((block[0] >= 0) + (block[1] >= 0) +
+                                               (block[2] >= 0) + (block[3] >= 0));
+        mbar_expect_tx(k_bar, bytes);
+        mbar_expect_tx(v_bar, bytes);
+        const uint32_t dst = smem + asks.slot * kCodes;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (block[u] >= 0)
+            load_rows(dst + Layout<FP16>::keys + u * (kUnit8 * 128), map, place[u], p.h, block[u],
+                      k_bar);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (block[u] >= 0)
+            load_rows(dst + Layout<FP16>::codes + u * (kUnit8 * 128), map, L.block_size + place[u],
+                      p.h, block[u], v_bar);
       }
       __syncwarp();
       // the scales, which a piece's first copies need not wait for
-      const uint32_t sc = __shfl_sync(0xFFFFFFFFu, scale, at);
+      const int mine = __shfl_sync(0xFFFFFFFFu, id, 4 * at + (lane & 3));
+      const uint32_t sc = __shfl_sync(0xFFFFFFFFu, scale, 4 * at + (lane & 3));
       const uint32_t note = asked % kNotes;
-      if (elected()) {
-        reinterpret_cast<float*>(&C->k_up[note])[unit] = __uint_as_float((sc & 0xFFu) << 23);
-        reinterpret_cast<float*>(&C->v_exp[note])[unit] =
+      if (lane < 4) {
+        reinterpret_cast<float*>(&C->k_up[note])[lane] = __uint_as_float((sc & 0xFFu) << 23);
+        reinterpret_cast<float*>(&C->v_exp[note])[lane] =
             static_cast<float>(static_cast<int>(sc >> 8) - 127);
-        reinterpret_cast<uint8_t*>(&C->gone[note])[unit] = block == -2 ? 1 : 0;
-        C->bad[note][unit] = 0;
+        reinterpret_cast<uint8_t*>(&C->gone[note])[lane] = mine == -2 ? 1 : 0;
+        C->bad[note][lane] = 0;
+      }
+      __syncwarp();
+      if (elected()) {
         mbar_arrive(k_bar);
         mbar_arrive(v_bar);
       }
       __syncwarp();
-      has = (has & ~(1u << asks.slot)) | (block >= 0 ? 1u : 0u) << asks.slot;
       asks.next();
-      ++asked;
-      return true;
-    };
-    for (int i = 0; i < AHEAD && i < p.halves; ++i)
-      if (!ask(i)) return;
+    }
+  }
+}
+
+// Values' codes to fp16 tiles, a warp a unit of each half.
+template <bool FP16>
+KVS_DEV void convert_role(const Attn4Launch& L, uint8_t* smem, Ctrl* C) {
+  constexpr int RING = Room<FP16>::RING;
+  const int lane = threadIdx.x & 31, unit = (threadIdx.x >> 5) & 3, sub = lane >> 3, c = lane & 7;
+  Turn<RING> comes;
+  Turn<kTiles> fills;
+  Turn<kPieces> pieces;
+  uint32_t half_no = 0;
+  Piece p;
+  // of the two fp16 chunks 2 c and 2 c + 1 the one whose place leaves no bank conflict goes first
+  const bool swap = c >= 4;
+  while (take_piece(L, C, pieces, p)) {
     for (int i = 0; i < p.halves; ++i, ++half_no) {
-      if (i + AHEAD < p.halves && !ask(i + AHEAD)) return;
-      if (!wait_phase(&C->v_came[unit][comes.slot], comes.phase, L.err)) return;
-      const int left = p.stop - (p.start + i * kHalf + kUnit8 * unit);
-      const bool there = has >> comes.slot & 1u;
+      if (!wait_phase(&C->v_came[comes.slot], comes.phase, L.err)) return;
+      // rows of the unit that are there
+      const int left = C->gone[half_no % kNotes] >> (8 * unit) & 1u
+                           ? 0
+                           : p.stop - (p.start + i * kHalf + kUnit8 * unit);
       uint4 w[4];
       uint32_t nan = 0;
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
         const int row = 4 * it + sub;
         w[it] = make_uint4(0u, 0u, 0u, 0u);
-        if (there && row < left)
+        if (row < left)
           w[it] = *reinterpret_cast<const uint4*>(smem + Layout<FP16>::codes + comes.slot * kCodes +
                                                   at128(kUnit8 * unit + row, c));
         nan |= (w[it].x & 0x7F7F7F7Fu) + 0x01010101u;
@@ -224,7 +283,8 @@ KVS_DEV void convert_role(const Attn4Launch& L, const CUtensorMap* map, Walk wal
           C->any_bad = 1;
         }
       }
-      __syncwarp();  // the slot is free
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&C->v_taken[comes.slot]);
       comes.next();
       if (half_no >= kTiles && !wait_phase(&C->v_empty[fills.slot], fills.phase ^ 1, L.err)) return;
       uint8_t* const dst = smem + Layout<FP16>::values + fills.slot * kValues;
@@ -263,80 +323,106 @@ KVS_DEV uint32_t values_desc(uint32_t saddr) {
   return (saddr >> 4) | (static_cast<uint32_t>(kHalf * 128 >> 4) << 16);
 }
 
-// Four warps issue them, one a query tile x and product, each on a scheduler of its own.
+// Three warps issue them, on schedulers of their own: the scores of query tile 0, of tile 1, and both
+// tiles' output.
 //
 // Scores of half i + 1 are asked for as soon as the softmax warps have those of half i in their
 // registers, so they find them ready when they are through; the weights have two buffers of
-// their own.  A slot is free when both tiles' products with it are done; without a second tile
-// its warps only say so.
-template <bool FP16, bool QK>
-KVS_DEV void mma_role(const Attn4Launch& L, Walk walk, int group, int x, uint32_t smem,
-                      uint32_t tmem, Ctrl* C) {
-  constexpr int PARTS = Room<FP16>::PARTS, N = QK ? Room<FP16>::RING : kTiles;
+// their own, and their products time to wait for the other tile's.  A slot is free when both tiles'
+// products with it are done; without a second tile its warp only says so.
+//
+// The last products' commits arrive on their own: not after the CTA has gone.
+template <int N>
+KVS_DEV void last_commits(const Attn4Launch& L, uint64_t* empties, Turn<N> turn, uint32_t all) {
+  for (int back = 0; back < N && all > 0; ++back, --all) {
+    turn.slot = turn.slot == 0 ? N - 1 : turn.slot - 1;
+    if (turn.slot == N - 1) turn.phase ^= 1;
+    if (!KVS_WAIT(&empties[turn.slot], turn.phase)) return;
+  }
+}
+
+template <bool FP16>
+KVS_DEV void qk_role(const Attn4Launch& L, int x, uint32_t smem, uint32_t tmem, Ctrl* C) {
+  constexpr int PARTS = Room<FP16>::PARTS, RING = Room<FP16>::RING;
   uint32_t piece_no = 0, half_no = 0, all = 0;
-  Turn<N> turn;
+  Turn<RING> turn;
+  Turn<kPieces> pieces;
   Piece p;
   const uint32_t qd = uniform(k_desc(smem + x * PARTS * kPart)),
-                 kvd = uniform(QK ? k_desc(smem + Layout<FP16>::keys)
-                                  : values_desc(smem + Layout<FP16>::values)),
-                 scores = uniform(tmem + 64 * x), weights = uniform(tmem + kWeightsAt + 64 * x),
-                 result = uniform(tmem + kOutAt + 128 * x);
-  uint64_t *const fulls = QK ? C->k_full : C->v_full, *const empties = QK ? C->k_empty : C->v_empty;
-  while (walk.next(L, group, p)) {
-    if (p.steps == 0) continue;
+                 kd = uniform(k_desc(smem + Layout<FP16>::keys)), scores = uniform(tmem + 64 * x);
+  while (take_piece(L, C, pieces, p)) {
     const int H = static_cast<int>(uniform(p.halves));
+    if (H == 0) continue;
     const bool idle = x == 1 && !p.two;
-    if (QK && !idle && !KVS_WAIT(&C->q_full[x], piece_no++ & 1)) return;
+    if (!idle && !KVS_WAIT(&C->q_full[x], piece_no++ & 1)) return;
     for (int i = 0; i < H; ++i, ++all) {
-      if (!KVS_WAIT(&fulls[turn.slot], turn.phase)) return;
-      uint64_t* const empty = &empties[turn.slot];
-      const uint32_t b = kvd + turn.slot * ((QK ? kCodes : kValues) >> 4);
+      if (!KVS_WAIT(&C->k_full[turn.slot], turn.phase)) return;
+      uint64_t* const empty = &C->k_empty[turn.slot];
+      const uint32_t b = kd + turn.slot * (kCodes >> 4);
       turn.next();
       if (idle) {
         if ((threadIdx.x & 31) == 0) mbar_arrive(empty);
         continue;
       }
-      if constexpr (QK) {
-        if (i > 0 && !KVS_WAIT(&C->s_free[x], (half_no - 1) & 1)) return;
-        tc_fence_after();
-        if (elected()) {
+      if (i > 0 && !KVS_WAIT(&C->s_free[x], (half_no - 1) & 1)) return;
+      tc_fence_after();
+      if (elected()) {
 #pragma unroll
-          for (int part = 0; part < PARTS; ++part)
+        for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              mma_codes(scores, qd + ((part * kPart + ks * 32) >> 4), b + (ks * 32 >> 4),
-                        part + ks > 0 ? 1u : 0u);
-          umma_commit(&C->s_full[x]);
-          umma_commit(empty);
-        }
-      } else {
-        const uint32_t buf = half_no & 1;
-        if (!KVS_WAIT(&C->p_full[x][buf], (half_no >> 1) & 1)) return;
-        tc_fence_after();
-        if (elected()) {
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks)  // 16 tokens: two groups of eight rows, 8 columns of P
-            mma_pv(result, weights + 32 * buf + 8 * ks, b + ks * (2048 >> 4),
-                   ks > 0 || i > 0 ? 1u : 0u);
-          umma_commit(&C->pv_done[x][buf]);
-          umma_commit(empty);
-        }
+          for (int ks = 0; ks < 4; ++ks)
+            mma_codes(scores, qd + ((part * kPart + ks * 32) >> 4), b + (ks * 32 >> 4),
+                      part + ks > 0 ? 1u : 0u);
+        umma_commit(&C->s_full[x]);
+        umma_commit(empty);
       }
       __syncwarp();
       ++half_no;
     }
     // The last half's scores were taken, too: one phase of s_free a half.  And not on to pieces without
     // this tile, which free slots as they come, before its softmax has read what is known of this one's.
-    if (QK && !idle && (!KVS_WAIT(&C->s_free[x], (half_no - 1) & 1) ||
-                        !KVS_WAIT(&C->done[x], (piece_no - 1) & 1)))
+    if (!idle && (!KVS_WAIT(&C->s_free[x], (half_no - 1) & 1) ||
+                  !KVS_WAIT(&C->done[x], (piece_no - 1) & 1)))
       return;
   }
-  // The last products' commits arrive on their own: not after the CTA has gone.
-  for (int back = 0; back < N && all > 0; ++back, --all) {
-    turn.slot = turn.slot == 0 ? N - 1 : turn.slot - 1;
-    if (turn.slot == N - 1) turn.phase ^= 1;
-    if (!KVS_WAIT(&empties[turn.slot], turn.phase)) return;
+  last_commits(L, C->k_empty, turn, all);
+}
+
+template <bool FP16>
+KVS_DEV void pv_role(const Attn4Launch& L, uint32_t smem, uint32_t tmem, Ctrl* C) {
+  uint32_t halves_of[2] = {0, 0}, all = 0;  // of a tile, so far
+  Turn<kTiles> turn;
+  Turn<kPieces> pieces;
+  Piece p;
+  const uint32_t vd = uniform(values_desc(smem + Layout<FP16>::values)),
+                 weights = uniform(tmem + kWeightsAt), result = uniform(tmem + kOutAt);
+  while (take_piece(L, C, pieces, p)) {
+    const int H = static_cast<int>(uniform(p.halves));
+    const bool two = uniform(p.two) != 0;
+    for (int i = 0; i < H; ++i, ++all) {
+      if (!KVS_WAIT(&C->v_full[turn.slot], turn.phase)) return;
+      const uint32_t b = vd + turn.slot * (kValues >> 4);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (x == 1 && !two) continue;
+        const uint32_t buf = halves_of[x] & 1;
+        if (!KVS_WAIT(&C->p_full[x][buf], (halves_of[x] >> 1) & 1)) return;
+        tc_fence_after();
+        if (elected()) {
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)  // 16 tokens: two groups of eight rows, 8 columns of P
+            mma_pv(result + 128 * x, weights + 64 * x + 32 * buf + 8 * ks, b + ks * (2048 >> 4),
+                   ks > 0 || i > 0 ? 1u : 0u);
+          umma_commit(&C->pv_done[x][buf]);
+          if (x == 1 || !two) umma_commit(&C->v_empty[turn.slot]);
+        }
+        __syncwarp();
+        ++halves_of[x];
+      }
+      turn.next();
+    }
   }
+  last_commits(L, C->v_empty, turn, all);
 }
 
 // ------------------------------------------------------------------ softmax
@@ -347,8 +433,8 @@ KVS_DEV const uint8_t* of_lane(const uint8_t* p, int lane) {
 }
 
 template <bool FP16>
-KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* smem,
-                          uint32_t tmem, const Parts& P, Ctrl* C) {
+KVS_DEV void softmax_role(const Attn4Launch& L, int group, uint8_t* smem, uint32_t tmem,
+                          const Parts& P, Ctrl* C) {
   const int x = threadIdx.x >> 7, row = threadIdx.x & 127;
   const uint32_t lanes = static_cast<uint32_t>((threadIdx.x >> 5) & 3) << 21;  // a warp's 32
   const uint32_t S = tmem + 64 * x + lanes, O = tmem + kOutAt + 128 * x + lanes;
@@ -359,8 +445,9 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk walk, int group, uint8_t* s
   const int lane = threadIdx.x & 31;
   uint8_t* const area = qt + (row - lane) * 128;
   uint32_t notes = 0, half_no = 0;  // halves before this piece; this tile's
+  Turn<kPieces> pieces;
   Piece p;
-  while (walk.next(L, group, p)) {
+  while (take_piece(L, C, pieces, p)) {
     if (x == 1 && !p.two) {
       notes += p.halves;
       continue;
@@ -726,11 +813,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constan
       }
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&C->k_full[i], 4);
+      mbar_init(&C->k_full[i], 1);
       mbar_init(&C->k_empty[i], 2);
-      for (int k = 0; k < 4; ++k) mbar_init(&C->v_came[i][k], 1);
+      mbar_init(&C->v_came[i], 1);
+      mbar_init(&C->v_taken[i], 4);
       mbar_init(&C->v_full[i], 4);
-      mbar_init(&C->v_empty[i], 2);
+      mbar_init(&C->v_empty[i], 1);
+    }
+    for (int i = 0; i < kPieces; ++i) {
+      mbar_init(&C->piece_full[i], 1);
+      mbar_init(&C->piece_empty[i], kReaders);
     }
     C->any_bad = 0;
     fence_mbar_init();
@@ -744,7 +836,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constan
   for (int r = tid; r < L.seqs; r += kThreads) {
     const Seq s = sequence(L, r, b == 0);
     named.take(L, s, r);
-    mine = tile_work(L, s, group).head * L.heads;
+    mine = tile_work<kOverTile>(L, s, group).head * L.heads;
     total += mine;
   }
 #pragma unroll
@@ -759,7 +851,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constan
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) total += C->scan[w];
   const long long least = static_cast<long long>(kLeastTile) * kTile * group;
-  Walk walk;
+  Walk<kOverTile> walk;
   walk.U = total;
   walk.b = b;
   walk.used = static_cast<int>(min(static_cast<long long>(B), (total + least - 1) / least));
@@ -770,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constan
     for (int r0 = 0; r0 < L.seqs; r0 += kThreads) {
       const int r = r0 + tid;
       if (L.seqs > kThreads)  // else `mine` is it
-        mine = r < L.seqs ? tile_work(L, sequence(L, r, false), group).head * L.heads : 0;
+        mine = r < L.seqs ? tile_work<kOverTile>(L, sequence(L, r, false), group).head * L.heads : 0;
       long long inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -797,16 +889,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constan
     // 256 x 184 + 256 x 72 = the 512 x 128 registers of the launch
     if (warp < 8) {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-      softmax_role<FP16>(L, walk, group, smem, tmem, P, C);
+      softmax_role<FP16>(L, group, smem, tmem, P, C);
     } else if (warp < 12) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-      convert_role<FP16>(L, &map, walk, group, smem, C);
+      convert_role<FP16>(L, smem, C);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
       if (warp < 14)
-        mma_role<FP16, true>(L, walk, group, warp & 1, smem_u32(smem), tmem, C);
+        qk_role<FP16>(L, warp & 1, smem_u32(smem), tmem, C);
+      else if (warp == 14)
+        pv_role<FP16>(L, smem_u32(smem), tmem, C);
       else
-        mma_role<FP16, false>(L, walk, group, warp & 1, smem_u32(smem), tmem, C);
+        fetch_role<FP16>(L, &map, walk, group, smem_u32(smem), C);
     }
   }
   __syncwarp();
@@ -821,7 +915,7 @@ cudaError_t launch(const Attn4Launch& L, const CUtensorMap& map, cudaStream_t s)
   cudaError_t e = cudaFuncSetAttribute(k_attn8_tile<FP16>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<FP16>::bytes);
   if (e != cudaSuccess) return e;
-  const int ctas = tile_ctas(L);
+  const int ctas = tile_ctas<kOverTile>(L);
   k_attn8_tile<FP16><<<ctas, kThreads, Layout<FP16>::bytes, s>>>(L, map);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const long long rows = static_cast<long long>(L.max_q) * (L.q_heads / L.heads);
@@ -836,7 +930,7 @@ cudaError_t attn8_tile_launch(const Attn4Launch& L, const CUtensorMap& map, cuda
 }
 
 long long attn8_tile_scratch(const Attn4Launch& L) {
-  return 16ll * tile_ctas(L) + 2ll * tile_ctas(L) * kRows * (8 + 512);
+  return 16ll * tile_ctas<kOverTile>(L) + 2ll * tile_ctas<kOverTile>(L) * kRows * (8 + 512);
 }
 
 }  // namespace kvs

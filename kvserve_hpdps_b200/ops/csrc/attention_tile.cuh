@@ -11,7 +11,6 @@ namespace {
 constexpr int kRows = 256;       // an item's query rows, two tiles
 constexpr int kTile = 128;       // tokens a step
 constexpr int kThreads = 16 * 32;
-constexpr int kOverTile = 2;     // an item's own cost, in steps
 constexpr int kLeastTile = 2;    // steps a CTA takes at least
 // The largest weight is 2^kAbove at its maximum's time, so that those down to 2^-21 of it are normal
 // fp16 numbers (a first token often takes nearly all of the weight and has a small value).
@@ -117,11 +116,12 @@ struct TileWork {
   long long first, head;  // cost of tile 0; of a head's tiles together
   KVS_DEV long long before(long long t) const { return t * first + more * (t * (t - 1) / 2); }
 };
+template <int OVER>  // an item's own cost, in steps
 KVS_DEV TileWork tile_work(const Attn4Launch& L, const Seq& s, int group) {
   TileWork w;
   w.tiles = static_cast<int>((static_cast<long long>(s.n) * group + kRows - 1) / kRows);
   w.more = L.causal ? kRows : 0;
-  w.first = static_cast<long long>(group) * (kOverTile * kTile + 1 +
+  w.first = static_cast<long long>(group) * (OVER * kTile + 1 +
                                              (L.causal ? max(s.len - s.n, 0) : s.len)) +
             kRows - 1;
   w.head = w.before(w.tiles);
@@ -138,6 +138,7 @@ struct Piece {
 };
 
 // Walks the pieces of a CTA's share; every thread does the same.
+template <int OVER>
 struct Walk {
   long long U, pos, end, begin;
   int r, used, b;
@@ -146,7 +147,7 @@ struct Walk {
     const long long unit = static_cast<long long>(kTile) * group;
     while (pos < end) {
       p.s = sequence(L, r, false);
-      const TileWork w = tile_work(L, p.s, group);
+      const TileWork w = tile_work<OVER>(L, p.s, group);
       if (pos >= begin + w.head * L.heads) {
         begin += w.head * L.heads;
         ++r;
@@ -163,7 +164,7 @@ struct Walk {
       }
       const long long item = begin + h * w.head + w.before(lo);
       const long long cost = w.first + static_cast<long long>(w.more) * lo;
-      const long long body = item + kOverTile * unit;  // the steps lie behind the item's own cost
+      const long long body = item + OVER * unit;  // the steps lie behind the item's own cost
       const long long to = min(end, item + cost);
       p.nrows = p.s.n * group;
       const int last_row = min(p.nrows, (lo + 1) * kRows) - 1;
@@ -212,12 +213,13 @@ KVS_DEV uint32_t peek_phase(uint64_t* bar, uint32_t parity) {
   return done;
 }
 
+template <int OVER>
 int tile_ctas(const Attn4Launch& L) {
   const int group = L.q_heads / L.heads;
   const long long tiles = (static_cast<long long>(L.max_q) * group + kRows - 1) / kRows;
   const long long steps =
       (static_cast<long long>(L.table_cols) * L.block_size + kTile - 1) / kTile;
-  const long long most = static_cast<long long>(L.seqs) * L.heads * tiles * (steps + kOverTile + 1);
+  const long long most = static_cast<long long>(L.seqs) * L.heads * tiles * (steps + OVER + 1);
   return static_cast<int>(most < 148 ? (most > 0 ? most : 1) : 148);
 }
 
