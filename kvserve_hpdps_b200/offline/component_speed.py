@@ -28,7 +28,9 @@ are wall time.
 queries rotated too), ``append4`` (into a 4-bit cache), ``read4`` (its rows back
 as bf16), ``attn4_decode`` (one query token of each of ``--requests`` sequences
 over its ``--tokens`` cached ones) and ``attn4_chunk`` (the last ``--chunk``
-tokens of one sequence).  Their rates are GB/s of the bf16 KV that the stage
+tokens of one sequence); ``append8``, ``read8``, ``attn8_decode`` and ``attn8_chunk``
+are the same on an 8-bit cache, ``attn8_cross`` attends without causal limits, ``--chunk``
+query tokens of each of four requests over the others' length.  Their rates are GB/s of the bf16 KV that the stage
 writes, reads or attends over.
 
 Every fused-stage figure is CUDA-event time on the launching stream after warm-up,
@@ -55,7 +57,8 @@ import torch
 STAGES = ("quant", "dequant", "rans_enc", "rans_dec", "lc_enc", "lc_dec", "block_copy")
 PEER_STAGES = ("quant_peer", "rans_enc_peer")
 METHODS = ("custom", "kivi", "cachegen", "hadamard", "minmax")
-SERVING = ("append", "append4", "read4", "attn4_decode", "attn4_chunk")
+SERVING = ("append", "append4", "read4", "attn4_decode", "attn4_chunk", "append8", "read8",
+           "attn8_decode", "attn8_chunk", "attn8_cross")
 
 
 def _timeit(fn, iters: int, warmup: int = 3) -> float:
@@ -291,6 +294,7 @@ def run_serving(tokens: int = 8192, heads: int = 4, q_heads: int = 28, requests:
     cos_sin = torch.cat([angle.cos(), angle.sin()], 1).float()
     cache = torch.zeros((2, nb, block_size, heads, 128), dtype=torch.bfloat16, device="cuda")
     cache4 = P.kv4_cache(nb, heads, block_size, group_size)
+    cache8 = P.kv8_cache(nb, heads, block_size)
 
     def rows(n, h):
         return torch.randn((n, h, 128), generator=g, device="cuda").bfloat16()
@@ -300,10 +304,14 @@ def run_serving(tokens: int = 8192, heads: int = 4, q_heads: int = 28, requests:
     for r in range(requests):  # every request holds the same tokens at its own blocks
         slots = table[r].long()[place // block_size] * block_size + place % block_size
         P.append_kv(cache4, k, v, slots, place, cos_sin)
+        P.append_kv(cache8, k, v, slots, place, cos_sin)
     lens = torch.full((requests,), tokens, dtype=torch.int32, device="cuda")
     qd = rows(requests, q_heads)
     chunk = min(chunk, tokens)
     start = torch.tensor([0, chunk], dtype=torch.int32, device="cuda")
+    few = min(4, requests)
+    qc = rows(few * chunk, q_heads)
+    starts = torch.arange(0, few * chunk + 1, chunk, dtype=torch.int32, device="cuda")
     stages = {
         "append": (lambda: P.append_kv(cache, k, v, slots, place, cos_sin, q), 1),
         "append4": (lambda: P.append_kv(cache4, k, v, slots, place, cos_sin, q), 1),
@@ -311,6 +319,13 @@ def run_serving(tokens: int = 8192, heads: int = 4, q_heads: int = 28, requests:
         "attn4_decode": (lambda: P.attention_kv4(qd, cache4, table, lens), requests),
         "attn4_chunk": (lambda: P.attention_kv4(q[-chunk:], cache4, table[:1], lens[:1], start,
                                                 chunk), 1),
+        "append8": (lambda: P.append_kv(cache8, k, v, slots, place, cos_sin, q), 1),
+        "read8": (lambda: P.read_kv8(cache8, slots, torch.bfloat16), 1),
+        "attn8_decode": (lambda: P.attention_kv8(qd, cache8, table, lens), requests),
+        "attn8_chunk": (lambda: P.attention_kv8(q[-chunk:], cache8, table[:1], lens[:1], start,
+                                                chunk), 1),
+        "attn8_cross": (lambda: P.attention_kv8(qc, cache8, table[:few], lens[:few], starts, chunk,
+                                                causal=False), few),
     }
     out = []
     for stage in SERVING:
@@ -319,14 +334,20 @@ def run_serving(tokens: int = 8192, heads: int = 4, q_heads: int = 28, requests:
         out.append({"stage": stage, "ms": round(ms, 5),
                     "gbps": round(n * tokens * heads * 512 / ms / 1e6, 1), "tokens": tokens,
                     "heads": heads, "q_heads": q_heads, "requests": n, "group_size": group_size})
-        if stage == "attn4_chunk":
+        if "8" in stage:
+            del out[-1]["group_size"]
+        if stage in ("attn4_chunk", "attn8_chunk", "attn8_cross"):
             out[-1]["chunk"] = chunk
     from kvserve_hpdps_b200.ops import kernels as K
-    back = P.read_kv4(cache4, slots, torch.bfloat16)
-    err = K.kv_error(torch.stack([cache.flatten(1, 2)[p][slots] for p in range(2)]), back)
+    held = torch.stack([cache.flatten(1, 2)[p][slots] for p in range(2)])
+    err = K.kv_error(held, P.read_kv4(cache4, slots, torch.bfloat16))
+    err8 = K.kv_error(held, P.read_kv8(cache8, slots, torch.bfloat16))
+    bytes8 = 256 + 128 / block_size  # a record's last row is its scales
     out.append({"stage": "summary", "bytes_per_token_head": P.kv4_row_bytes(group_size),
                 "compression_ratio": round(512 / P.kv4_row_bytes(group_size), 3),
                 "rel_mse": err["rel_mse"], "cosine": err["cosine"],
+                "bytes_per_token_head_8bit": bytes8, "compression_ratio_8bit": round(512 / bytes8, 3),
+                "rel_mse_8bit": err8["rel_mse"], "cosine_8bit": err8["cosine"],
                 "device_error": K.read_device_error(cache.device)})
     return out
 

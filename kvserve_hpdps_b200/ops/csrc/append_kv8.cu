@@ -15,7 +15,11 @@
 // the 15 tokens before and behind by itself, and a unit that it finds there whole, and not begun
 // before, is settled without another word.  Only for the others (both ends of a sequence's
 // new tokens, a decode step's) all slots of the call are looked through, by 256 threads.  In any
-// order at all that is quadratic: 16384 shuffled tokens take four times as long as in order.
+// order at all that is quadratic: 16384 tokens of 8 heads take 45 us in order, 219 shuffled.
+//
+// What bounds it: for many tokens the instructions of rotating and encoding between the loads and the
+// stores (16379 tokens of 32+8 heads, 369 MB: 74 us, 76 % of the copy rate), for few the chain
+// slots, rows, codes (one token 3.7 us in a captured graph, 48 of as many sequences 4.1).
 #include "append_kv.cuh"
 #include "kv8.cuh"
 
@@ -24,9 +28,10 @@ namespace kvs {
 namespace {
 
 constexpr int kWarps8 = kThreads / 32, kJobs = kWarps8 / 2;  // heads' keys or values at once
-// A CTA takes one token up to kFewTokens (decode steps: every token has a unit of its own), else 16;
-// up to kSomeTokens there are four CTAs for a window's units that are not whole.
-constexpr int kFewTokens = 256, kSomeTokens = 1024;
+// A CTA takes one token up to kFewTokens (decode steps: every token has a unit of its own), else 16.
+// Measured, 32+8 heads, one a CTA / 16: 300 tokens of as many sequences 12.3 / 34.1 us, of one 9.2 /
+// 8.5; 500 tokens 15.0 / 37.7 and 12.3 / 9.2; 1000 tokens 36 / 45 and 26 / 10.
+constexpr int kFewTokens = 512;
 
 // Rows of queries, eight lanes each, as k_append_kv deals them out.
 template <bool FP16, int MODE, int EACH>
@@ -187,12 +192,11 @@ KVS_DEV void append_unit(const AppendLaunch& L, int tok0, int tok1, long long po
   if (lane == 0 && !(warp & 1)) *byte = static_cast<uint8_t>(e + 127);
 }
 
-// Blocks [0, kv): of window x / (parts * subs) the heads of part x / subs % parts; units that are not
-// whole are dealt out to the subs.  Behind them the queries.
+// Blocks [0, kv): of window x / parts the heads of part x % parts.  Behind them the queries.
 template <bool FP16, int MODE, int WINDOW, int EACH>
 __global__ void __launch_bounds__(kThreads, WINDOW == 1 ? 2 : 3)
     k_append_kv8(const __grid_constant__ AppendLaunch L, const __grid_constant__ Spread S, int kv,
-                 int parts, int subs) {
+                 int parts) {
   if (static_cast<int>(blockIdx.x) >= kv) {
     const unsigned q = blockIdx.x - kv;
     rotate_queries<FP16, MODE, EACH>(L, S, static_cast<int>(q % S.x), static_cast<int>(q / S.x));
@@ -202,8 +206,7 @@ __global__ void __launch_bounds__(kThreads, WINDOW == 1 ? 2 : 3)
   __shared__ int s_from[kWarps8][kUnit8];
   __shared__ uint32_t s_top[kWarps8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane >> 3;
-  const int x = static_cast<int>(blockIdx.x), mine = x % subs, part = x / subs % parts;
-  const int i0 = x / subs / parts * WINDOW;
+  const int x = static_cast<int>(blockIdx.x), part = x % parts, i0 = x / parts * WINDOW;
   // This pair of warps' heads' keys or values, keys and values in turn.
   const int jobs = 2 * L.heads;
   auto each = [&](auto f) {
@@ -219,8 +222,10 @@ __global__ void __launch_bounds__(kThreads, WINDOW == 1 ? 2 : 3)
     // ---- few tokens: every warp looks through all slots, which it asks for with its own token's
     long long at[kFewTokens / 32];
 #pragma unroll
-    for (int n = 0; n < kFewTokens / 32; ++n)
+    for (int n = 0; n < kFewTokens / 32; ++n) {
+      if (32 * n >= L.tokens) break;
       at[n] = lane + 32 * n < L.tokens ? load_index(L.slots, lane + 32 * n, L.slots64) : -1;
+    }
     const long long slot = load_index(L.slots, i0, L.slots64), pos = position(i0);
     if (!fine(slot, pos)) {
       if (slot >= 0 && part + tid == 0) record_error(L.err, ERR_BOUNDS);
@@ -231,6 +236,7 @@ __global__ void __launch_bounds__(kThreads, WINDOW == 1 ? 2 : 3)
     int first = i0;
 #pragma unroll
     for (int n = 0; n < kFewTokens / 32; ++n) {
+      if (32 * n >= L.tokens) break;
       const int i = lane + 32 * n;
       if (at[n] / kUnit8 == slot / kUnit8 && at[n] >= 0 && (i == i0 || fine(at[n], position(i)))) {
         atomicMax(&s_from[warp][at[n] % kUnit8], i);
@@ -263,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, WINDOW == 1 ? 2 : 3)
     if (in) pos = load_index(L.pos, ia, L.pos64);
     if (in_b) pos_b = load_index(L.pos, ib, L.pos64);
   }
-  if (lane < WINDOW && slot >= 0 && !fine(slot, pos) && part + mine + warp == 0)
+  if (lane < WINDOW && slot >= 0 && !fine(slot, pos) && part + warp == 0)
     record_error(L.err, ERR_BOUNDS);
   const int unit = fine(slot, pos) ? static_cast<int>(slot / kUnit8) : -1;
   const int unit_b = fine(slot_b, pos_b) ? static_cast<int>(slot_b / kUnit8) : -2;
@@ -282,7 +288,6 @@ __global__ void __launch_bounds__(kThreads, WINDOW == 1 ? 2 : 3)
       open |= 1u << k;
       continue;
     }
-    if (mine != 0) continue;
     if (is) s_from[warp][off] = lane;
     __syncwarp();
     int tok[2];
@@ -335,11 +340,10 @@ __global__ void __launch_bounds__(kThreads, WINDOW == 1 ? 2 : 3)
     }
   }
   __syncthreads();
-  int turn = 0;
 #pragma unroll 1
   for (; open != 0; open &= open - 1) {
     const int k = __ffs(open) - 1;
-    if (turn++ % subs != mine || U.first[k] < i0) continue;
+    if (U.first[k] < i0) continue;
     int tok[2];
     long long at[2];
 #pragma unroll
@@ -417,19 +421,20 @@ template <bool FP16, int MODE, int WINDOW>
 int append(const AppendLaunch& L, cudaStream_t s) {
   const Spread S = spread_of(L.tokens, L.q_heads);
   const long long windows = (L.tokens + WINDOW - 1) / WINDOW;
-  // all heads in one CTA when there are windows enough: finding its units takes as long as a job
+  // All heads in one CTA when there are windows enough: finding its units takes as long as a job.
+  // Measured, 32+8 heads, apart / in one CTA: one token a window, 64 tokens 4.8 / 6.8 us, 128 7.5 / 7.2,
+  // 256 12.6 / 8.5; 16 tokens a window, 3000 tokens 17.1 / 21.2, 4000 23.2 / 24.8, 6000 35.8 / 33.1.
   const int most = (2 * L.heads + kJobs - 1) / kJobs;
-  const int parts = windows >= 592 ? (most > 0) : most;
-  const int subs = WINDOW > 1 && L.tokens <= kSomeTokens ? 4 : 1;
-  const long long kv = windows * parts * subs;
+  const int parts = windows >= (WINDOW == 1 ? 128 : 256) ? (most > 0) : most;
+  const long long kv = windows * parts;
   const long long q = L.q_heads > 0 ? static_cast<long long>(S.x) * S.y : 0;
   if (kv + q >= (1ll << 31) || L.num_slots / kUnit8 >= (1ll << 31)) return -2;
   const unsigned grid = static_cast<unsigned>(kv + q);
   const int kv_ctas = static_cast<int>(kv);
   if (S.each == 4)
-    k_append_kv8<FP16, MODE, WINDOW, 4><<<grid, kThreads, 0, s>>>(L, S, kv_ctas, parts, subs);
+    k_append_kv8<FP16, MODE, WINDOW, 4><<<grid, kThreads, 0, s>>>(L, S, kv_ctas, parts);
   else
-    k_append_kv8<FP16, MODE, WINDOW, 1><<<grid, kThreads, 0, s>>>(L, S, kv_ctas, parts, subs);
+    k_append_kv8<FP16, MODE, WINDOW, 1><<<grid, kThreads, 0, s>>>(L, S, kv_ctas, parts);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 template <bool FP16, int MODE>

@@ -49,9 +49,9 @@ namespace kvs {
 
 namespace {
 
+constexpr int kOverTile = 2;  // an item's own cost, in steps
 // Tokens (of 32) with scales less than kApart of the largest take a scale each: a row may see only
 // the small ones, or need their bits.
-constexpr int kOverTile = 2;     // an item's own cost, in steps
 constexpr float kApart = 0x1p-8f;
 constexpr uint32_t kHides = 1, kWideK = 2, kWideV = 4;
 constexpr int kFar = 60;

@@ -26,6 +26,14 @@
 // All go by halves of 64 tokens.  The softmax warps take a half's scores into registers, so that the
 // next ones are computed while they work.  O stays in tensor memory; it is rescaled by the softmax
 // warps when 64 weights of a row sum up to more than kMostSum, which after the first tiles is rare.
+//
+// What bounds it: the softmax warps' chain, 2300 clocks for 64 tokens of both tiles, of which the
+// exponentials' rate (16 a clock and SM) is 1024 and the products take 1050 (fp16: 1320).
+// 2 x 2048 tokens over up to 8193, 28/4 heads (361 GFLOP), in a captured graph: bf16 390 us (926
+// TFLOP/s), fp16 401; 6 prompts of 389 tokens over up to 1501, 16 heads: 72 us, a third of it what
+// pieces cost beside their steps.  With K as fp16 tiles it was 633 us and 107.
+//
+// The work is dealt out as in attention_kv8.cu, here by the number of visible keys a tile has.
 #include "attention_kv8.cuh"
 #include "attention_tile.cuh"
 
@@ -886,15 +894,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constan
     __syncthreads();
     walk.r = C->seq;
     walk.begin = C->begin;
-    // 256 x 184 + 256 x 72 = the 512 x 128 registers of the launch
+    // 256 x 168 + 256 x 88 = the 512 x 128 registers of the launch
     if (warp < 8) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
       softmax_role<FP16>(L, group, smem, tmem, P, C);
     } else if (warp < 12) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
       convert_role<FP16>(L, smem, C);
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
       if (warp < 14)
         qk_role<FP16>(L, warp & 1, smem_u32(smem), tmem, C);
       else if (warp == 14)

@@ -223,3 +223,14 @@ def test_a_captured_append_reads_its_inputs_again():
     k.mul_(4)
     graph.replay()
     assert (P.read_kv8(cache, slots, torch.bfloat16) == 4).all()
+
+
+def test_component_speed_times_the_8bit_stages():
+    from kvserve_hpdps_b200.offline import component_speed as CS
+    rows = {r["stage"]: r for r in CS.run_serving(tokens=500, requests=5, chunk=40, q_heads=8,
+                                                  heads=2, iters=2, warmup=1)}
+    for stage in ("append8", "read8", "attn8_decode", "attn8_chunk", "attn8_cross"):
+        assert rows[stage]["ms"] > 0
+    # e4m3 below 448 2^e: half a step of 2^-4 at most, and exact powers of two between
+    assert rows["summary"]["cosine_8bit"] > 1 - 2 ** -8 and rows["summary"]["device_error"] == 0
+    assert rows["summary"]["rel_mse_8bit"] < rows["summary"]["rel_mse"]
