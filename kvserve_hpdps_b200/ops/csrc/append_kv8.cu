@@ -19,7 +19,9 @@
 //
 // What bounds it: for many tokens the instructions of rotating and encoding between the loads and the
 // stores (16379 tokens of 32+8 heads, 369 MB: 74 us, 76 % of the copy rate), for few the chain
-// slots, rows, codes (one token 3.7 us in a captured graph, 48 of as many sequences 4.1).
+// slots, rows, codes (one token 3.5 us in a captured graph, 48 of as many sequences 3.8).
+#include <type_traits>
+
 #include "append_kv.cuh"
 #include "kv8.cuh"
 
@@ -29,8 +31,8 @@ namespace {
 
 constexpr int kWarps8 = kThreads / 32, kJobs = kWarps8 / 2;  // heads' keys or values at once
 // A CTA takes one token up to kFewTokens (decode steps: every token has a unit of its own), else 16.
-// Measured, 32+8 heads, one a CTA / 16: 300 tokens of as many sequences 12.3 / 34.1 us, of one 9.2 /
-// 8.5; 500 tokens 15.0 / 37.7 and 12.3 / 9.2; 1000 tokens 36 / 45 and 26 / 10.
+// Measured, 32+8 heads, one a CTA / 16: 300 tokens of as many sequences 12.3 / 27.7 us, of one 9.6 /
+// 7.9; 500 tokens 15.4 / 30.7 and 12.3 / 7.9; 700 tokens 22.5 / 31.4 and 16.4 / 7.9.
 constexpr int kFewTokens = 512;
 
 // Rows of queries, eight lanes each, as k_append_kv deals them out.
@@ -193,8 +195,8 @@ KVS_DEV void append_unit(const AppendLaunch& L, int tok0, int tok1, long long po
 }
 
 // Blocks [0, kv): of window x / parts the heads of part x % parts.  Behind them the queries.
-template <bool FP16, int MODE, int WINDOW, int EACH>
-__global__ void __launch_bounds__(kThreads, WINDOW == 1 ? 2 : 3)
+template <bool FP16, int MODE, int WINDOW, int EACH, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS)
     k_append_kv8(const __grid_constant__ AppendLaunch L, const __grid_constant__ Spread S, int kv,
                  int parts) {
   if (static_cast<int>(blockIdx.x) >= kv) {
@@ -421,20 +423,34 @@ template <bool FP16, int MODE, int WINDOW>
 int append(const AppendLaunch& L, cudaStream_t s) {
   const Spread S = spread_of(L.tokens, L.q_heads);
   const long long windows = (L.tokens + WINDOW - 1) / WINDOW;
-  // All heads in one CTA when there are windows enough: finding its units takes as long as a job.
-  // Measured, 32+8 heads, apart / in one CTA: one token a window, 64 tokens 4.8 / 6.8 us, 128 7.5 / 7.2,
-  // 256 12.6 / 8.5; 16 tokens a window, 3000 tokens 17.1 / 21.2, 4000 23.2 / 24.8, 6000 35.8 / 33.1.
+  // All heads in one CTA when the windows fill the SMs: finding its units takes as long as a job.
+  // Measured, 32+8 heads, apart / in one CTA: one token a window, 64 tokens 4.1 / 6.2 us, 128 6.8 / 6.5,
+  // 256 13.3 / 8.5; 16 tokens a window, 2000 tokens 12.7 / 14.3, 3000 17.7 / 15.5, 4000 24.6 / 19.5.
   const int most = (2 * L.heads + kJobs - 1) / kJobs;
-  const int parts = windows >= (WINDOW == 1 ? 128 : 256) ? (most > 0) : most;
+  const int parts = windows > 148 ? (most > 0) : most;
   const long long kv = windows * parts;
   const long long q = L.q_heads > 0 ? static_cast<long long>(S.x) * S.y : 0;
   if (kv + q >= (1ll << 31) || L.num_slots / kUnit8 >= (1ll << 31)) return -2;
   const unsigned grid = static_cast<unsigned>(kv + q);
   const int kv_ctas = static_cast<int>(kv);
-  if (S.each == 4)
-    k_append_kv8<FP16, MODE, WINDOW, 4><<<grid, kThreads, 0, s>>>(L, S, kv_ctas, parts);
-  else
-    k_append_kv8<FP16, MODE, WINDOW, 1><<<grid, kThreads, 0, s>>>(L, S, kv_ctas, parts);
+  // Registers for two CTAs an SM, or for three whose windows are many: their loads cover one another's,
+  // and spilled registers cost less than that.  Measured, 32+8 heads, two / three: 700 tokens 7.5 / 9.2 us,
+  // 4096 20.1 / 26.3, 6000 30.7 / 32.1, 8192 41.3 / 41.0, 16379 83 / 74; rotated in part 16379 92 / 163.
+  auto start = [&](auto each, auto ctas) {
+    k_append_kv8<FP16, MODE, WINDOW, each.value, ctas.value>
+        <<<grid, kThreads, 0, s>>>(L, S, kv_ctas, parts);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Four = std::integral_constant<int, 4>;
+  using Two = std::integral_constant<int, 2>;
+  if constexpr (WINDOW > 1 && MODE != kPart) {
+    if (windows > 400) {
+      using Three = std::integral_constant<int, 3>;
+      S.each == 4 ? start(Four{}, Three{}) : start(One{}, Three{});
+      return cudaGetLastError() == cudaSuccess ? 0 : -1;
+    }
+  }
+  S.each == 4 ? start(Four{}, Two{}) : start(One{}, Two{});
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 template <bool FP16, int MODE>
