@@ -257,3 +257,20 @@ def test_read_out_of_range():
     with pytest.raises(RuntimeError):
         K.check_device_error(cache.device)
     assert not got[:, 0].any() and got[:, 1].all()
+
+
+@pytest.mark.parametrize("rd,inter", [(128, False), (64, False), (96, True)])
+@pytest.mark.parametrize("tokens", [148, 149, 512, 513, 2368, 2385, 6400, 6417])
+def test_append_where_the_work_is_dealt_otherwise(tokens, rd, inter):
+    """Both sides of the sizes at which windows, heads a CTA and registers change: three sequences,
+    their ends and starts inside units, in an order that goes on in the middle."""
+    g = _gen(tokens + rd)
+    bs, h, first = 32, 3, 5
+    nb = (tokens + 120) // bs + 2
+    blocks = torch.randperm(nb, generator=g)
+    i = torch.arange(tokens) + first + 37 * (torch.arange(tokens) // (tokens // 3 + 1))
+    slots = (blocks[i // bs] * bs + i % bs).roll(tokens // 2)
+    k, v = _rows(g, tokens, h, torch.bfloat16), _rows(g, tokens, h, torch.bfloat16)
+    q = _rows(g, tokens, 2, torch.bfloat16)
+    pos = torch.randint(0, 99, (tokens,), generator=g)
+    _check_append(_random_cache(g, nb, h, bs), k, v, slots, pos, _table(99, rd), inter, q)
