@@ -29,8 +29,8 @@
 //
 // What bounds it: the softmax warps' chain, 2300 clocks for 64 tokens of both tiles, of which the
 // exponentials' rate (16 a clock and SM) is 1024 and the products take 1050 (fp16: 1320).
-// 2 x 2048 tokens over up to 8193, 28/4 heads (361 GFLOP), in a captured graph: bf16 390 us (926
-// TFLOP/s), fp16 401; 6 prompts of 389 tokens over up to 1501, 16 heads: 72 us, a third of it what
+// 2 x 2048 tokens over up to 8193, 28/4 heads (361 GFLOP), in a captured graph: bf16 386 us (935
+// TFLOP/s), fp16 402; 6 prompts of 389 tokens over up to 1501, 16 heads: 72 us, a third of it what
 // pieces cost beside their steps.  With K as fp16 tiles it was 633 us and 107.
 //
 // The work is dealt out as in attention_kv8.cu, here by the number of visible keys a tile has.
@@ -542,7 +542,9 @@ KVS_DEV void softmax_role(const Attn4Launch& L, int group, uint8_t* smem, uint32
       // The row sees tokens of half i with values that are not numbers: which, from their codes.
       auto mark = [&](int i) {
         const uint32_t note = (notes + i) % kNotes;
+#pragma unroll 1
         for (int u = 0; u < 4; ++u) {
+#pragma unroll 1
           for (uint32_t b = C->bad[note][u] & visible(i, u, C->gone[note]); b != 0; b &= b - 1) {
             const int tok = p.start + kHalf * i + kUnit8 * u + __ffs(b) - 1;
             const int page = tok / L.block_size;
@@ -580,7 +582,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, int group, uint8_t* smem, uint32
         const float up4[4] = {k_up.x, k_up.y, k_up.z, k_up.w};
         float fs[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)  // not zero: a hidden score is -inf times it
+        for (int u = 0; u < 4; ++u)  // not zero: a maximum of -inf is taken times it
           fs[u] = fmaxf(f * up4[u], 1.17549435e-38f);
         // Asked long before the answer is needed: a wait costs 140 clocks even when it is over.
         const bool next = i + 1 < p.halves;
@@ -591,17 +593,16 @@ KVS_DEV void softmax_role(const Attn4Launch& L, int group, uint8_t* smem, uint32
         __syncwarp();
         if ((threadIdx.x & 31) == 0) mbar_arrive(&C->s_free[x]);
         const bool huge = fmaxf(fmaxf(up4[0], up4[1]), fmaxf(up4[2], up4[3])) > up_most;
-        if (t0 + kHalf > plain_to || gone != 0 || huge) {  // hidden scores become -inf
+        if (t0 + kHalf > plain_to || gone != 0 || huge) {  // hidden scores become -inf, others are rounded
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const uint32_t vis = visible(i, u, gone);
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               uint32_t& y = v[u >> 1][16 * (u & 1) + k];
-              if (huge) y = __float_as_uint(__fmul_rn(__uint_as_float(y), fs[u]));
-              y = vis >> k & 1u ? y : 0xFF800000u;
+              y = vis >> k & 1u ? __float_as_uint(__fmul_rn(__uint_as_float(y), fs[u])) : 0xFF800000u;
             }
-            if (huge) fs[u] = 1.f;
+            fs[u] = 1.f;
           }
         }
         // Against the reference that there is, the scores only pass through once; a row whose
