@@ -755,11 +755,12 @@ Grid grid_of(const Attn4Launch* L) {
 
 // Whether a call goes to attention_kv8_tile.cu: many rows a kv head, and enough of them by what the
 // host knows (max_query_len, and the tokens that the table has room for).  Measured, us here / there
-// (bf16; fp16 is alike, 5 to 15 % more on both sides): 32 sequences of 2000 tokens, 8 heads: 64 rows
-// 99 / 119, 96 rows 139 / 121; 16 of 2000: 64 rows 59 / 69, 96 rows 79 / 70; 8 of 8000, 4 heads: 56
-// rows 55 / 56, 84 rows 73 / 56; 64 of 1000, 4 heads: 84 rows 84 / 91.  With little to do (Mi rows
-// times tokens times heads): one of 1024 tokens, 4 heads: 448 rows (1.8 Mi) 22 / 29; one of 4000, 8
-// heads: 128 rows (3.9 Mi) 33 / 30, 512 rows 55 / 38; one of 16000, 4 heads: 112 rows (6.8 Mi) 39 / 33.
+// (bf16; fp16 is 10 to 16 % more here, 6 there): 32 sequences of 2000 tokens, 8 heads: 48 rows
+// 97 / 104, 64 rows 99 / 105 (fp16 114 / 112), 96 rows 138 / 106; 16 of 2000: 64 rows 58 / 61, 96 rows
+// 79 / 62; 8 of 8000, 4 heads: 56 rows 55 / 50, 84 rows 73 / 51; 64 of 1000, 4 heads: 84 rows 83 / 75.
+// With little to do (Mi rows times tokens times heads): one of 1024 tokens, 4 heads: 448 rows (1.8 Mi)
+// 22 / 26; one of 4000, 8 heads: 128 rows (3.9 Mi) 33 / 29, 512 rows 55 / 38; one of 16000, 4 heads:
+// 112 rows (6.8 Mi) 39 / 32.
 constexpr int kManyRows = 64;
 constexpr long long kMuchWork = 3ll << 20;
 bool many_rows(const Attn4Launch* L) {
