@@ -42,7 +42,10 @@ namespace kvs {
 namespace {
 
 // Units whose scale is less than 2^-kFar of K's weigh nothing beside it in fp16, but count in the sum.
+// Their weights, of 2^-kFar as it were, have to stay below fp16's 2^-25: a row's maximum moves on when
+// the sum of 64 passes 2^20 without their units, too (times kSumBefore that is kMostSum).
 constexpr float kFar = 60.f;
+constexpr float kSumBefore = kMostSum * 0x1p-20f;
 // A score is a factor times 128 products of at most 2^9 and 2^9.  Where the factor lets it pass
 // 2^27, the product is rounded before the maximum is taken off: the fused multiply-add leaves the
 // maximum's own rounding over, up to 2^-25 of it, and weights are 2 to that from where they should
@@ -606,8 +609,8 @@ KVS_DEV void softmax_role(const Attn4Launch& L, int group, uint8_t* smem, uint32
           }
         }
         // Against the reference that there is, the scores only pass through once; a row whose
-        // weights' sum has passed kMostSum makes the warp find the maximum, rescale and take the
-        // scores again (the first half always does).
+        // weights' sum has passed kMostSum (or 2^20 before the values' scales) makes the warp find the
+        // maximum, rescale and take the scores again (the first half always does).
         uint32_t h[2][16];
         float sum;
         bool ready = false;
@@ -685,8 +688,9 @@ KVS_DEV void softmax_role(const Attn4Launch& L, int group, uint8_t* smem, uint32
             sum = fmaf(s0, ex2(-d[u]), sum);
           }
           if (fresh) break;
-          ready = __all_sync(0xFFFFFFFFu, ahead != 0 && !(all > kMostSum));
-          if (ready || !__any_sync(0xFFFFFFFFu, all > kMostSum)) break;
+          const bool past = fmaxf(all, sum * kSumBefore) > kMostSum;
+          ready = __all_sync(0xFFFFFFFFu, ahead != 0 && !past);
+          if (ready || !__any_sync(0xFFFFFFFFu, past)) break;
         }
         l += sum;
         // the products with the weights two halves ago
