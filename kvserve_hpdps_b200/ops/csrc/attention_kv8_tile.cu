@@ -4,9 +4,12 @@
 // heads of one kv head) share each key, on tcgen05:
 //   S = Q K^T, O += P V, products of 128 rows and 64 tokens into tensor memory.
 // K's codes are matrix operands as they are (kind::f8f6f4, fp32 sums: measured off by at most 2^-21.9 of
-// the sum of magnitudes).  A query row, scaled by a power of two to at most 448, is taken in e4m3
-// parts that add up to it: two for bf16 (4 + 4 bits), three for fp16, which is exact but for
-// elements below 2^-9 of the row's largest; those are off by 2^-10 where the largest is above 224.
+// the sum of magnitudes).  A query row, scaled by a power of two to at most 448, is taken in 8-bit
+// parts that add up to it: one in e4m3 (4 bits) and one for bf16, two for fp16, in e5m2 (3 bits and a
+// sign each, down to 2^-16).  That is exact for elements down to 2^-6, which is less than 2^-13 of the
+// row's largest; those below are off by at most 2^-14 (bf16) and 2^-17 (fp16), 2^-21 and 2^-24 of it.  A
+// channel that a bias has made 1000 times the others leaves these as good as exact (parts in e4m3
+// alone end at 2^-10: the logarithms of the sums were off by 1e-2 then).
 // V's codes become fp16 tiles, which hold every code exactly.  The scales stay out of the products: a
 // unit's key scale goes into the softmax's factor, its value scale b = 2^e into the weights,
 //   w = 2^(s - M + e - K),  l += 2^(K - e) w,  o = 2^K O / l,
@@ -320,13 +323,15 @@ KVS_DEV void convert_role(const Attn4Launch& L, uint8_t* smem, Ctrl* C) {
 }
 
 // ------------------------------------------------------ matrix instructions
+// A: a part of the queries, e4m3 (number 0, which is also fp16's) or e5m2 (number 1).
+template <bool E5M2>
 KVS_DEV void mma_codes(uint32_t d, uint32_t a, uint32_t b, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
       "mov.b64 x, {%1, %4};\n\tmov.b64 y, {%2, %4};\n\t"
       "setp.ne.b32 p, %5, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], x, y, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "r"(b), "r"(kIdescQK), "n"(kDescHigh), "r"(accumulate)  // e4m3's number is fp16's, 0
+      "r"(a), "r"(b), "r"(kIdescQK | (E5M2 ? 1u << 7 : 0u)), "n"(kDescHigh), "r"(accumulate)
       : "memory");
 }
 // Values: 64 channels a block, blocks 8 KB apart (leading offset).
@@ -379,11 +384,13 @@ KVS_DEV void qk_role(const Attn4Launch& L, int x, uint32_t smem, uint32_t tmem, 
       tc_fence_after();
       if (elected()) {
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part)
+        for (int ks = 0; ks < 4; ++ks)
+          mma_codes<false>(scores, qd + (ks * 32 >> 4), b + (ks * 32 >> 4), ks > 0 ? 1u : 0u);
+#pragma unroll
+        for (int part = 1; part < PARTS; ++part)
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
-            mma_codes(scores, qd + ((part * kPart + ks * 32) >> 4), b + (ks * 32 >> 4),
-                      part + ks > 0 ? 1u : 0u);
+            mma_codes<true>(scores, qd + ((part * kPart + ks * 32) >> 4), b + (ks * 32 >> 4), 1u);
         umma_commit(&C->s_full[x]);
         umma_commit(empty);
       }
@@ -472,7 +479,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, int group, uint8_t* smem, uint32
     float m = kLowest, l = 0.f, f = 0.f, K = -120.f;
     bool poisoned = false;
     if (p.steps > 0) {
-      // ---- the row scaled by a power of two, its largest element in (224, 448], in e4m3 parts
+      // ---- the row scaled by a power of two, its largest element in (224, 448], in parts
       uint4 raw[16];
       // a row that is not there is read from the first one: with a load each behind a condition of
       // its own the 16 came one after the other (11000 clocks a piece against 3800)
@@ -519,9 +526,14 @@ KVS_DEV void softmax_role(const Attn4Launch& L, int group, uint8_t* smem, uint32
           uint32_t four[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            four[k] = codes8x4(y + 4 * k);
             float z[4];
-            values8x4(four[k], z);
+            if (part == 0) {
+              four[k] = codes8x4(y + 4 * k);
+              values8x4(four[k], z);
+            } else {
+              four[k] = codes52x4(y + 4 * k);
+              values52x4(four[k], z);
+            }
 #pragma unroll
             for (int n = 0; n < 4; ++n) y[4 * k + n] -= z[n];  // what the part leaves over, exactly
           }

@@ -60,5 +60,18 @@ KVS_DEV void values8x4(uint32_t w, float* x) {
   x[0] = h2f<true>(a & 0xFFFFu), x[1] = h2f<true>(a >> 16);
   x[2] = h2f<true>(b & 0xFFFFu), x[3] = h2f<true>(b >> 16);
 }
+// The same in e5m2, which is fp16's upper byte.
+KVS_DEV uint32_t codes52(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+KVS_DEV uint32_t codes52x4(const float* x) {
+  return codes52(x[0], x[1]) | codes52(x[2], x[3]) << 16;
+}
+KVS_DEV void values52x4(uint32_t w, float* x) {
+  x[0] = h2f<true>((w & 0xFFu) << 8), x[1] = h2f<true>(w & 0xFF00u);
+  x[2] = h2f<true>(w >> 8 & 0xFF00u), x[3] = h2f<true>(w >> 16 & 0xFF00u);
+}
 
 }  // namespace kvs

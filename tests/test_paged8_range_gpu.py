@@ -46,3 +46,31 @@ def test_small_values_under_scores_that_rise(rows, less):
         cache[block, :, 32, 1] = 127 - less
     ref = O8.attend(q, cache, table, lens, start)
     _check(*_attend(q, cache, table, lens, start, rows), ref, BF)
+
+
+@pytest.mark.parametrize("rows", [5, 40])
+@pytest.mark.parametrize("times", [300, 1000])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_a_query_channel_far_above_the_others(dt, times, rows):
+    """A bias makes one channel of the queries large, that channel is small in the keys: the scores
+    are the others'.  The kernel for many rows takes a row, scaled to at most 448, in parts that
+    are exact but for elements below 2^-6, which are off by 2^-14 (bf16) or 2^-17 (fp16) at most:
+    added to the tolerance, element by element."""
+    hq, h, scale = 8, 2, 1 / math.sqrt(128)
+    q, cache, table, lens, start = _one(rows, 300, dt, hq, h)
+    q[:, :, 5] = (q[:, :, 5].double() * times).to(dt)
+    cache[:, :, :16, 5] %= 5  # up to 2^-7, where the others are 40 in the mean
+    want, wlse, tol, ltol = O8.attend(q, cache, table, lens, start, scale, one_part=rows > 9 or None)
+    if rows > 9:
+        up = torch.ceil(torch.log2(q.double().abs().amax(-1, keepdim=True) / 448))
+        off = 2.0 ** up * (2 ** -14 if dt == BF else 2 ** -17)
+        off = off * (q.double().abs() < 2.0 ** (up - 6))            # [T, hq, 128]
+        t = torch.arange(300)
+        k = O8.read(cache, table[0].long()[t // 16] * 16 + t % 16)[0].abs()  # [300, h, 128]
+        move = 2 * scale * torch.einsum("thgd,lhd->thgl", off.view(rows, h, hq // h, 128), k)
+        move = move.amax(-1).reshape(rows, hq)                     # of a weight, at most
+        size = cache.clone()
+        size[:, :, 16:32] &= 0x7F
+        of_values = O8.attend(q, size, table, lens, start, scale)[0]  # sum of p |v|
+        tol, ltol = tol + move[..., None] * of_values, ltol + move
+    _check(*_attend(q, cache, table, lens, start, rows, scale=scale), (want, wlse, tol, ltol), dt)
