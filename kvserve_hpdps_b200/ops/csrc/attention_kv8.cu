@@ -284,7 +284,7 @@ KVS_DEV void team_role(const Attn4Launch& L, Share<kWarps / RG * kStep, 8 * NT *
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
       int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-      e = top == 0.f ? 0 : max(kLowestExp, min(e, 100));
+      e = top == 0.f ? 0 : max(kLowestExp, e);
       const float up = pow2(14 - e) * (L.scale < 0.f ? -1.f : 1.f);
       const float fr = fabsf(L.scale) * 1.4426950408889634f * pow2(e - 14);
 #pragma unroll

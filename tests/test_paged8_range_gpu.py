@@ -74,3 +74,15 @@ def test_a_query_channel_far_above_the_others(dt, times, rows):
         of_values = O8.attend(q, size, table, lens, start, scale)[0]  # sum of p |v|
         tol, ltol = tol + move[..., None] * of_values, ltol + move
     _check(*_attend(q, cache, table, lens, start, rows, scale=scale), (want, wlse, tol, ltol), dt)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("up", [101, 112, 125])
+def test_queries_near_the_largest_number(rows, up):
+    """bf16 queries of 2^101 and more over keys of 2^-100."""
+    q, cache, table, lens, start = _one(rows, 200)
+    q = (q.double().clamp(-3, 3) * 2.0 ** up).to(BF)
+    cache[:, :, 32, 0::2] = (cache[:, :, 32, 0::2].int() - 100).to(torch.uint8)
+    scale = 2.0 ** (100 - up - 8) / math.sqrt(128)
+    ref = O8.attend(q, cache, table, lens, start, scale)
+    _check(*_attend(q, cache, table, lens, start, rows, scale=scale), ref, BF)
