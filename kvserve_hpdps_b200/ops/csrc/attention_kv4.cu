@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
       int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-      e = top == 0.f ? 0 : max(kLowestExp, min(e, 100));
+      e = top == 0.f ? 0 : max(kLowestExp, e);
       const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23) *
                        (L.scale < 0.f ? -1.f : 1.f);
       // not zero: a hidden score is -inf times it

@@ -422,7 +422,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, Walk<kOverTile> walk, int group,
         for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(y[k]));
       }
       int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-      e = top == 0.f ? 0 : max(kLowestExp, min(e, 100));
+      e = top == 0.f ? 0 : max(kLowestExp, e);
       const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23) *
                        (L.scale < 0.f ? -1.f : 1.f);
       f = fabsf(L.scale) * 1.4426950408889634f *
