@@ -307,7 +307,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
       int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
       e = top == 0.f ? 0 : max(kLowestExp, e);
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23) *
+      // an infinite element makes the row what is not a number
+      const float up = __uint_as_float(top < INFINITY ? static_cast<uint32_t>(127 + 14 - e) << 23
+                                                      : 0x7FC00000u) *
                        (L.scale < 0.f ? -1.f : 1.f);
       // not zero: a hidden score is -inf times it
       const float fr = fmaxf(fabsf(L.scale) * 1.4426950408889634f *

@@ -285,7 +285,9 @@ KVS_DEV void team_role(const Attn4Launch& L, Share<kWarps / RG * kStep, 8 * NT *
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
       int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
       e = top == 0.f ? 0 : max(kLowestExp, e);
-      const float up = pow2(14 - e) * (L.scale < 0.f ? -1.f : 1.f);
+      // an infinite element makes the row what is not a number
+      const float up = top < INFINITY ? pow2(14 - e) * (L.scale < 0.f ? -1.f : 1.f)
+                                      : __uint_as_float(0x7FC00000u);
       const float fr = fabsf(L.scale) * 1.4426950408889634f * pow2(e - 14);
 #pragma unroll
       for (int q = 0; q < 4; ++q)

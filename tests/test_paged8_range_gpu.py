@@ -86,3 +86,21 @@ def test_queries_near_the_largest_number(rows, up):
     scale = 2.0 ** (100 - up - 8) / math.sqrt(128)
     ref = O8.attend(q, cache, table, lens, start, scale)
     _check(*_attend(q, cache, table, lens, start, rows, scale=scale), ref, BF)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_an_infinite_query_is_not_a_number(dt, rows):
+    """Whatever the keys' signs are in its channel: scores of -inf alone are no row without tokens."""
+    q, cache, table, lens, start = _one(rows, 100, dt)
+    cache[:, :, :16, 9] |= 0x80
+    cache[:, :, :16, 9] = cache[:, :, :16, 9].clamp(0x88, 0xF0)  # negative, not zero
+    ref = O8.attend(q, cache, table, lens, start, one_part=True)
+    q[0, 1, 9], q[rows - 1, 6, 9] = math.inf, -math.inf
+    out, lse = _attend(q, cache, table, lens, start, rows)
+    bad = torch.zeros(out.shape[:2], dtype=torch.bool)
+    bad[0, 1] = bad[rows - 1, 6] = True
+    assert out.cpu()[bad].isnan().all() and lse.cpu()[bad].isnan().all()
+    want = ref[0].clone()
+    want[bad] = math.nan
+    _check(out, None, (want, *ref[1:]), dt)

@@ -44,3 +44,26 @@ def test_queries_near_the_largest_number(rows, up):
     torch.cuda.synchronize()
     K.check_device_error(out.device)
     _check(out, lse, O.attend(q, cache, table, lens, start, scale, tiles=rows > 9), dt)
+
+
+@pytest.mark.parametrize("rows", [1, 7, 60])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_an_infinite_query_is_not_a_number(dt, rows):
+    """Whatever the keys' signs are in its channel: scores of -inf alone are no row without tokens."""
+    q, cache, table, lens, start = _one(rows, 100, dt)
+    codes, step, mid = O.unpack(cache, dt)
+    codes[0, ..., 9] = codes[0, ..., 9] % 8  # below the middle, and that is below zero
+    mid[0] = -mid[0].abs() - 0.125
+    cache = O.pack(codes, step, mid)
+    ref = O.attend(q, cache, table, lens, start, tiles=rows > 9)
+    q[0, 1, 9], q[rows - 1, 6, 9] = math.inf, -math.inf
+    out, lse = P.attention_kv4(q.cuda(), cache.cuda(), table.cuda(), lens.cuda(), start.cuda(), rows,
+                               return_lse=True)
+    torch.cuda.synchronize()
+    K.check_device_error(out.device)
+    bad = torch.zeros(out.shape[:2], dtype=torch.bool)
+    bad[0, 1] = bad[rows - 1, 6] = True
+    assert out.cpu()[bad].isnan().all() and lse.cpu()[bad].isnan().all()
+    want = ref[0].clone()
+    want[bad] = math.nan
+    _check(out, None, (want, *ref[1:]), dt)
