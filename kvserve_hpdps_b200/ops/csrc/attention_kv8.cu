@@ -47,6 +47,9 @@ constexpr int kOver = 256;          // what starting and ending an item costs, i
 constexpr int kLeast = 512, kFew = 256, kSpread = 148;
 // Largest weights are 2^kAbove when their row's units are set, and may come to 2^kMost.
 constexpr float kAbove = 7.f, kMost = 15.f;
+// Units whose scale is less than 2^-kFar of K's count in the sum of the weights alone: they weigh
+// 2^(kLazy - kFar) of K's unit at most, which fp16 rounds to nothing.
+constexpr float kFar = 60.f;
 
 struct Work {
   int units;       // a sequence's share of the line
@@ -322,12 +325,11 @@ KVS_DEV void team_role(const Attn4Launch& L, Share<kWarps / RG * kStep, 8 * NT *
 
     auto step = [&](auto tag, int t0, const uint8_t* st, uint32_t scales, uint32_t note) {
       constexpr bool MASKED = decltype(tag)::value;
-      float sc[2][NT][4], ev[2], fv[2], top[2][NT][2];
+      float sc[2][NT][4], ev[2], top[2][NT][2];
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const uint32_t two = scales >> (16 * hf) & 0xFFFFu;
         const float fk = __uint_as_float((two & 0xFFu) << 23);
-        fv[hf] = __uint_as_float(two >> 8 << 23);
         ev[hf] = static_cast<float>(static_cast<int>(two >> 8) - 127);
         float a[NT][4];
 #pragma unroll
@@ -417,14 +419,11 @@ KVS_DEV void team_role(const Attn4Launch& L, Share<kWarps / RG * kStep, 8 * NT *
           float w[4];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            // 2^(ev - K); the minimum is for rows that see none of these tokens
-            const float unit = fminf(fv[hf] * pow2(-static_cast<int>(K[nt][j])), 3e38f);
+            // 2^d in the exponent: it may pass fp32's largest number where p falls below the smallest
+            const float d = fmaxf(ev[hf] - K[nt][j], -kFar);
 #pragma unroll
-            for (int i = j; i < 4; i += 2) {
-              const float p = ex2(sc[hf][nt][i] - M[nt][j]);
-              l[nt][j] += p;
-              w[i] = p * unit;
-            }
+            for (int i = j; i < 4; i += 2) w[i] = ex2((sc[hf][nt][i] - M[nt][j]) + d);
+            l[nt][j] = fmaf(w[j] + w[j + 2], ex2(-d), l[nt][j]);
           }
           const uint32_t lo = half2_bits(w[0], w[1]), hi = half2_bits(w[2], w[3]);
           w0[nt] = transpose8(lo);

@@ -48,6 +48,22 @@ def test_small_values_under_scores_that_rise(rows, less):
     _check(*_attend(q, cache, table, lens, start, rows), ref, BF)
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_large_values_under_small_scores(rows):
+    """Values 2^130 times the others' under weights of 2^-122, which fp32 holds: the result is
+    theirs.  Tokens 128 to 159 are the second step of the warp that has taken tokens 0 to 31."""
+    q, cache, table, lens, start = _one(rows, 160)
+    q[:] = 1
+    cache[:, :, :16] = 0
+    cache[:, :, 32, 0] = 127
+    cache[:, :, 32, 1] = 17   # 2^-110
+    late = table[0, 8:10].long()
+    cache[late, :, :16] = 0xCF  # -7.5: a score of -84.9
+    cache[late, :, 32, 1] = 147
+    ref = O8.attend(q, cache, table, lens, start, causal=False)
+    _check(*_attend(q, cache, table, lens, start, rows, causal=False), ref, BF)
+
+
 @pytest.mark.parametrize("rows", [5, 40])
 @pytest.mark.parametrize("times", [300, 1000])
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
