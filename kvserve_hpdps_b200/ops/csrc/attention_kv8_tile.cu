@@ -13,7 +13,8 @@
 // V's codes become fp16 tiles, which hold every code exactly.  The scales stay out of the products: a
 // unit's key scale goes into the softmax's factor, its value scale b = 2^e into the weights,
 //   w = 2^(s - M + e - K),  l += 2^(K - e) w,  o = 2^K O / l,
-// M near the row's running maximum of s and K such that the largest w was 2^kAbove when it was set.
+// M a whole number near the row's running maximum of s, K such that the largest w was about 2^kAbove
+// when it was set.
 //
 // The other rounding to fewer bits than fp32's is that of the weights to fp16, 2^-11, as the matrix
 // instructions' A operand has to be of V's type; their sum is taken before that.  An fp16 output's
@@ -49,11 +50,13 @@ namespace {
 // the sum of 64 passes 2^20 without their units, too (times kSumBefore that is kMostSum).
 constexpr float kFar = 60.f;
 constexpr float kSumBefore = kMostSum * 0x1p-20f;
-// A score is a factor times 128 products of at most 2^9 and 2^9.  Where the factor lets it pass
-// 2^27, the product is rounded before the maximum is taken off: the fused multiply-add leaves the
-// maximum's own rounding over, up to 2^-25 of it, and weights are 2 to that from where they should
-// be (the same for all of a row's, so that 2^4 does no harm).
-constexpr float kHuge = 0x1p2f;
+// Equal scores have to weigh alike whatever their values' scales are.  The reference is a whole
+// number, so that it and a unit's exponent add up without a rounding below 2^24, and one fused
+// multiply-add takes a score against both.  A score is a factor times 128 products of at most
+// 448^2: where the factor lets it pass 2^22.7, every half is taken against its own maximum first
+// (the score rounded before, if that is above 2^23: what the maximum's rounding leaves over would
+// be an exponent of its own), and the units' exponents are added to the differences.
+constexpr float kHuge = 0x1p-2f;
 
 // An item's own cost in steps of 128 tokens: the share is what a CTA's pieces take, 18000 clocks each
 // and 4600 a step (2 x 2048 rows: 396 us with 2, 393 with 3 and 4, 396 with 6).
@@ -608,25 +611,25 @@ KVS_DEV void softmax_role(const Attn4Launch& L, int group, uint8_t* smem, uint32
         __syncwarp();
         if ((threadIdx.x & 31) == 0) mbar_arrive(&C->s_free[x]);
         const bool huge = fmaxf(fmaxf(up4[0], up4[1]), fmaxf(up4[2], up4[3])) > up_most;
-        if (t0 + kHalf > plain_to || gone != 0 || huge) {  // hidden scores become -inf, others are rounded
+        if (t0 + kHalf > plain_to || gone != 0) {  // hidden scores become -inf
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const uint32_t vis = visible(i, u, gone);
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               uint32_t& y = v[u >> 1][16 * (u & 1) + k];
-              y = vis >> k & 1u ? __float_as_uint(__fmul_rn(__uint_as_float(y), fs[u])) : 0xFF800000u;
+              y = vis >> k & 1u ? y : 0xFF800000u;
             }
-            fs[u] = 1.f;
           }
         }
         // Against the reference that there is, the scores only pass through once; a row whose
         // weights' sum has passed kMostSum (or 2^20 before the values' scales) makes the warp find the
-        // maximum, rescale and take the scores again (the first half always does).
+        // maximum, rescale and take the scores again (the first half always does, and one whose scores
+        // may be huge).
         uint32_t h[2][16];
         float sum;
         bool ready = false;
-        for (bool fresh = i == 0;; fresh = true) {
+        for (bool fresh = i == 0 || huge;; fresh = true) {
           if (fresh) {
             float part[4];
 #pragma unroll
@@ -638,7 +641,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, int group, uint8_t* smem, uint32
               part[u] *= fs[u];
             }
             const float m_new =
-                fmaxf(m, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+                fmaxf(m, ceilf(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]))));
             const float less = m - m_new;
             float most = part[0] - m_new + ev[0];
 #pragma unroll
@@ -666,7 +669,22 @@ KVS_DEV void softmax_role(const Attn4Launch& L, int group, uint8_t* smem, uint32
             }
             m = m_new;
             K = k_new;
+            if (huge) {
+              const bool rounded = fabsf(m) > 0x1p23f;
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                  uint32_t& y = v[u >> 1][16 * (u & 1) + k];
+                  const float s = __uint_as_float(y);
+                  y = __float_as_uint(rounded ? __fsub_rn(__fmul_rn(s, fs[u]), m)
+                                              : fmaf(s, fs[u], -m));
+                }
+                fs[u] = 1.f;
+              }
+            }
           }
+          const float off = huge ? 0.f : m;
           f32x2_t s2[4];
           float d[4];
 #pragma unroll
@@ -676,7 +694,7 @@ KVS_DEV void softmax_role(const Attn4Launch& L, int group, uint8_t* smem, uint32
           }
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const float ref = d[u] - m;
+            const float ref = d[u] - off;
             const f32x2_t fs2 = f2_pack(fs[u], fs[u]), ref2 = f2_pack(ref, ref);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {

@@ -64,6 +64,33 @@ def test_large_values_under_small_scores(rows):
     _check(*_attend(q, cache, table, lens, start, rows, causal=False), ref, BF)
 
 
+@pytest.mark.parametrize("rows", [1, 9, 40])
+@pytest.mark.parametrize("up", [0, 5, 13, 27, 53])
+def test_equal_scores_of_any_size_over_values_of_many_scales(rows, up):
+    """Equal keys (as codes of 1 and of 2 under half the scale), scores of 2^4 to 2^110: every token
+    weighs the same, whatever its values' scale (2^0, 2^-6, 2^-30, and zeros) and its score's size."""
+    n, hq, h = 400, 8, 2
+    q, cache, table, lens, start = _one(rows, n)
+    q = (2.0 ** up * (1 + q.double().abs())).to(BF)
+    odd = (torch.arange(25) % 2).to(torch.uint8)
+    value = torch.tensor([127, 121, 97, 17], dtype=torch.uint8)[torch.arange(25) * 7 // 5 % 4]
+    used = table[0, :25].long()
+    cache[used, :, :16] = (0x38 + 8 * odd)[:, None, None, None]
+    cache[used, :, 32, 0] = (127 + up - odd)[:, None]
+    cache[used, :, 32, 1] = value[:, None]
+    cache[used[value == 17], :, 16:32] = 0
+    out, _ = _attend(q, cache, table, lens, start, rows)
+    t = torch.arange(n)
+    x = O8.read(cache, table[0].long()[t // 16] * 16 + t % 16)[1]  # [n, h, 128]
+    for i in range(rows):
+        v = x[:n - rows + i + 1].repeat_interleave(hq // h, 1)
+        want, size = v.mean(0), v.abs().mean(0)
+        # weights to fp16 (those 2^-30 below go under: 2^-24 of the largest), fp32's sums, the output
+        tol = (2 ** -11 + 2 ** -17) * size + 2 ** -24 * v.abs().amax((0, 2))[:, None]
+        tol = tol + O8.half_step(BF) * (want.abs() + tol)
+        assert ((out[i].double().cpu() - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("rows", [5, 40])
 @pytest.mark.parametrize("times", [300, 1000])
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
