@@ -15,15 +15,17 @@ inline bool record_map(const Attn4Launch& L, unsigned rows, CUtensorMap* map) {
   const EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return false;
   const cuuint64_t record = 128ull * (2 * L.block_size + 1);
+  // A cache without blocks has no address; the encoder wants one and a block, which no id names.
+  const bool none = L.num_blocks == 0;
   const cuuint64_t dims[4] = {128, 2ull * L.block_size + 1, static_cast<cuuint64_t>(L.heads),
-                              static_cast<cuuint64_t>(L.num_blocks)};
+                              none ? 1 : static_cast<cuuint64_t>(L.num_blocks)};
   // a stride that nothing is multiplied by may be anything in torch
   const cuuint64_t strides[3] = {128,
                                  L.heads > 1 ? static_cast<cuuint64_t>(L.head_stride) : record,
                                  L.num_blocks > 1 ? static_cast<cuuint64_t>(L.block_stride) : record};
   const cuuint32_t box[4] = {128, rows, 1, 1}, step[4] = {1, 1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(L.cache), dims, strides, box,
-            step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, none ? L.out : const_cast<void*>(L.cache), dims,
+            strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 // Bytes that a phase waits for, beside its arrivals.

@@ -147,3 +147,22 @@ def test_an_infinite_query_is_not_a_number(dt, rows):
     want = ref[0].clone()
     want[bad] = math.nan
     _check(out, None, (want, *ref[1:]), dt)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_a_cache_without_blocks(rows):
+    """Sequences of no tokens are zeros; one that names a block records an error."""
+    cache = P.kv8_cache(0, 2)
+    table = torch.zeros((2, _wide(40, 2, 8, 2)), dtype=torch.int32)
+    assert _tiles(table, rows, 8, 2, 16) == (rows == 40)
+    q = torch.randn((2 * rows, 8, 128), generator=torch.Generator().manual_seed(1)).to(BF)
+    start = torch.tensor([0, rows, 2 * rows]).int()
+    for n in (0, 30):
+        out, lse = P.attention_kv8(q.cuda(), cache, table.cuda(), torch.tensor([0, n]).int().cuda(),
+                                   start.cuda(), rows, return_lse=True)
+        if n:
+            with pytest.raises(RuntimeError):
+                K.check_device_error(out.device)
+        else:
+            K.check_device_error(out.device)
+        assert not out.any() and (lse == -math.inf).all()
