@@ -121,7 +121,7 @@ KVS_DEV uint32_t phase_of(uint32_t step) {  // of its slot's barriers
 constexpr int kRestAt = 2 * kHalfTile;
 
 template <bool FP16, int NG>
-KVS_DEV void convert_role(const Attn4Launch& L, Walk<kOverTile> walk, int group, uint8_t* q_tile,
+KVS_DEV void convert_role(const Attn4Launch& L, Walk<kOverTile, false> walk, int group, uint8_t* q_tile,
                           uint8_t* k_tile, uint8_t* v_tile, Ctrl* C) {
   const int lane = threadIdx.x & 31, seg = (threadIdx.x >> 5) & 3, row = seg * 32 + lane;
   constexpr uint32_t kInf = FP16 ? 0x7C00u : 0x7F80u;
@@ -307,7 +307,7 @@ KVS_DEV void convert_role(const Attn4Launch& L, Walk<kOverTile> walk, int group,
 // their own.  A stage is free when both tiles' products with it are done; without a second tile
 // its warps only say so.
 template <bool FP16, bool QK>
-KVS_DEV void mma_role(const Attn4Launch& L, Walk<kOverTile> walk, int group, int x, uint32_t q_tile,
+KVS_DEV void mma_role(const Attn4Launch& L, Walk<kOverTile, false> walk, int group, int x, uint32_t q_tile,
                       uint32_t kv_tile, uint32_t tmem, Ctrl* C) {
   uint32_t step_no = 0, piece_no = 0, half_no = 0;
   Piece p;
@@ -383,7 +383,7 @@ KVS_DEV void mma_role(const Attn4Launch& L, Walk<kOverTile> walk, int group, int
 
 // ------------------------------------------------------------------ softmax
 template <bool FP16, int NG>
-KVS_DEV void softmax_role(const Attn4Launch& L, Walk<kOverTile> walk, int group, uint8_t* q_tile,
+KVS_DEV void softmax_role(const Attn4Launch& L, Walk<kOverTile, false> walk, int group, uint8_t* q_tile,
                           uint32_t tmem, const Parts& P, Ctrl* C) {
   const int x = threadIdx.x >> 7, row = threadIdx.x & 127;
   const uint32_t lanes = static_cast<uint32_t>((threadIdx.x >> 5) & 3) << 21;  // a warp's 32
@@ -780,7 +780,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn4_tile(const __grid_constan
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) total += C->scan[w];
   const long long least = static_cast<long long>(kLeastTile) * kTile * group;
-  Walk<kOverTile> walk;
+  Walk<kOverTile, false> walk;
   walk.U = total;
   walk.b = b;
   walk.used = static_cast<int>(min(static_cast<long long>(B), (total + least - 1) / least));

@@ -136,7 +136,7 @@ KVS_DEV bool take_piece(const Attn4Launch& L, Ctrl* C, Turn<kPieces>& at, Piece&
 
 // One warp walks through the CTA's share, ahead of all others, and asks the copy engine for codes.
 template <bool FP16>
-KVS_DEV void fetch_role(const Attn4Launch& L, const CUtensorMap* map, Walk<kOverTile> walk, int group,
+KVS_DEV void fetch_role(const Attn4Launch& L, const CUtensorMap* map, Walk<kOverTile, true> walk, int group,
                         uint32_t smem, Ctrl* C) {
   constexpr int RING = Room<FP16>::RING;
   const int lane = threadIdx.x & 31;
@@ -894,7 +894,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constan
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) total += C->scan[w];
   const long long least = static_cast<long long>(kLeastTile) * kTile * group;
-  Walk<kOverTile> walk;
+  Walk<kOverTile, true> walk;
   walk.U = total;
   walk.b = b;
   walk.used = static_cast<int>(min(static_cast<long long>(B), (total + least - 1) / least));

@@ -106,9 +106,12 @@ KVS_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: 
 // A tile's cost is linear in its number: with n rows' worth of queries and `len` tokens,
 // tile t's last row sees about len - n + (256 t + 255) / group + 1 of them (all without causal
 // limits).  In units of 1 / group tokens: cost(t) = first + more t, which sums up in closed form.
-// a / b of numbers that mostly have 32 bits (a 64-bit division is some 150 instructions).
+// a / b.  SHORT: of numbers that mostly have 32 bits, in a form of its own beside the long one's some
+// 150 instructions.  That pays where one warp walks (8 bits); where each role does, its code costs
+// more than it saves (4 bits, 2 x 2048 rows: 476 us without, 495 with it).
+template <bool SHORT>
 KVS_DEV long long div64(long long a, long long b) {
-  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  if (SHORT && ((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
   return a / b;
 }
 struct TileWork {
@@ -138,11 +141,11 @@ struct Piece {
 };
 
 // Walks the pieces of a CTA's share; every thread does the same.
-template <int OVER>
+template <int OVER, bool SHORT>
 struct Walk {
   long long U, pos, end, begin;
   int r, used, b;
-  KVS_DEV long long share(int i) const { return div64(U * i, used); }
+  KVS_DEV long long share(int i) const { return div64<SHORT>(U * i, used); }
   KVS_DEV bool next(const Attn4Launch& L, int group, Piece& p) {
     const long long unit = static_cast<long long>(kTile) * group;
     while (pos < end) {
@@ -154,7 +157,7 @@ struct Walk {
         continue;
       }
       long long off = pos - begin;
-      const int h = static_cast<int>(div64(off, w.head));
+      const int h = static_cast<int>(div64<SHORT>(off, w.head));
       off -= h * w.head;
       int lo = 0, hi = w.tiles - 1;  // the last tile that begins at or before off
       while (lo < hi) {
@@ -173,7 +176,7 @@ struct Walk {
       auto step_of = [&](long long x) {
         if (x >= item + cost) return all;
         if (x <= body) return 0;
-        const long long k = div64(x - body, unit);
+        const long long k = div64<SHORT>(x - body, unit);
         return static_cast<int>(k < all ? k : all);
       };
       const int u0 = step_of(pos), u1 = step_of(to);
@@ -191,7 +194,7 @@ struct Walk {
       p.whole = u0 == 0 && u1 == all;
       if (p.begins && !p.whole) {  // the last part is the CTA's whose share reaches the last step
         const long long x = min(item + cost, body + all * unit) - 1;
-        p.parts = static_cast<int>(div64((x + 1) * used + U - 1, U) - 1) - b + 1;
+        p.parts = static_cast<int>(div64<SHORT>((x + 1) * used + U - 1, U) - 1) - b + 1;
       }
       return true;
     }
