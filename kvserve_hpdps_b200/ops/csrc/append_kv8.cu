@@ -18,8 +18,9 @@
 // order at all that is quadratic: 16384 tokens of 8 heads take 45 us in order, 219 shuffled.
 //
 // What bounds it: for many tokens the instructions of rotating and encoding between the loads and the
-// stores (16379 tokens of 32+8 heads, 369 MB: 74 us, 76 % of the copy rate), for few the chain
-// slots, rows, codes (one token 3.5 us in a captured graph, 48 of as many sequences 3.8).
+// stores (16379 tokens of 32+8 heads, 378 MB: 74 us, 78 % of the copy rate), for few the chain
+// slots, rows, codes (in a captured graph of several states in turn: one token 2.9 us, 48 of as many
+// sequences 4.3).
 #include <type_traits>
 
 #include "append_kv.cuh"
@@ -92,8 +93,7 @@ struct Units {
 // 4 it + sub is token tok<it> at position pos<it>, or is not the call's (-1).
 template <bool FP16, int MODE>
 KVS_DEV void append_unit(const AppendLaunch& L, int tok0, int tok1, long long pos0, long long pos1,
-                                         bool begins, bool whole, int unit, int h, int value,
-                         uint32_t* s_top) {
+                         bool begins, bool whole, int unit, int h, int value, uint32_t* s_top) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & 7, sub = lane >> 3;
   const int tok[2] = {tok0, tok1};
   const long long pos[2] = {pos0, pos1};
@@ -109,7 +109,8 @@ KVS_DEV void append_unit(const AppendLaunch& L, int tok0, int tok1, long long po
   const uint32_t per = static_cast<uint32_t>(L.block_size) / kUnit8;
   const uint32_t blk = static_cast<uint32_t>(unit) / per;
   const int u = static_cast<int>(static_cast<uint32_t>(unit) - blk * per);
-  uint8_t* const rec = static_cast<uint8_t*>(L.cache) + static_cast<long long>(blk) * L.block_stride + h * L.head_stride;
+  uint8_t* const rec = static_cast<uint8_t*>(L.cache) +
+                       static_cast<long long>(blk) * L.block_stride + h * L.head_stride;
   uint8_t* const rows = rec + (value * L.block_size + u * kUnit8 + 8 * (warp & 1)) * 128ll;
   uint8_t* const byte = rec + 256ll * L.block_size + 2 * u + value;
   const int was = whole ? 0 : *byte;
@@ -120,8 +121,9 @@ KVS_DEV void append_unit(const AppendLaunch& L, int tok0, int tok1, long long po
   for (int it = 0; it < 2; ++it) {
     raw[it][0] = raw[it][1] = make_uint4(0u, 0u, 0u, 0u);
     if (tok[it] < 0) continue;
-    const uint16_t* src = value ? static_cast<const uint16_t*>(L.value) + tok[it] * L.val_ts + h * L.val_hs
-                                : static_cast<const uint16_t*>(L.key) + tok[it] * L.key_ts + h * L.key_hs;
+    const uint16_t* src =
+        value ? static_cast<const uint16_t*>(L.value) + tok[it] * L.val_ts + h * L.val_hs
+              : static_cast<const uint16_t*>(L.key) + tok[it] * L.key_ts + h * L.key_hs;
     raw[it][0] = *reinterpret_cast<const uint4*>(src + 8 * l);
     raw[it][1] = *reinterpret_cast<const uint4*>(src + 8 * l + 64);
     if (MODE == kPart && !value && L.pos != nullptr) {
@@ -424,8 +426,9 @@ int append(const AppendLaunch& L, cudaStream_t s) {
   const Spread S = spread_of(L.tokens, L.q_heads);
   const long long windows = (L.tokens + WINDOW - 1) / WINDOW;
   // All heads in one CTA when the windows fill the SMs: finding its units takes as long as a job.
-  // Measured, 32+8 heads, apart / in one CTA: one token a window, 64 tokens 4.1 / 6.2 us, 128 6.8 / 6.5,
-  // 256 13.3 / 8.5; 16 tokens a window, 2000 tokens 12.7 / 14.3, 3000 17.7 / 15.5, 4000 24.6 / 19.5.
+  // Measured, 32+8 heads, apart / in one CTA: one token a window, 64 tokens 4.1 / 6.2 us, 128 6.8 /
+  // 6.5, 256 13.3 / 8.5; 16 tokens a window, 2000 tokens 12.7 / 14.3, 3000 17.7 / 15.5, 4000 24.6 /
+  // 19.5.
   const int most = (2 * L.heads + kJobs - 1) / kJobs;
   const int parts = windows > 148 ? (most > 0) : most;
   const long long kv = windows * parts;
@@ -433,9 +436,10 @@ int append(const AppendLaunch& L, cudaStream_t s) {
   if (kv + q >= (1ll << 31) || L.num_slots / kUnit8 >= (1ll << 31)) return -2;
   const unsigned grid = static_cast<unsigned>(kv + q);
   const int kv_ctas = static_cast<int>(kv);
-  // Registers for two CTAs an SM, or for three whose windows are many: their loads cover one another's,
-  // and spilled registers cost less than that.  Measured, 32+8 heads, two / three: 700 tokens 7.5 / 9.2 us,
-  // 4096 20.1 / 26.3, 6000 30.7 / 32.1, 8192 41.3 / 41.0, 16379 83 / 74; rotated in part 16379 92 / 163.
+  // Registers for two CTAs an SM, or for three whose windows are many: their loads cover one
+  // another's, and spilled registers cost less than that.  Measured, 32+8 heads, two / three: 700
+  // tokens 7.5 / 9.2 us, 4096 20.1 / 26.3, 6000 30.7 / 32.1, 8192 41.3 / 41.0, 16379 83 / 74; rotated in
+  // part 16379 92 / 163.
   auto start = [&](auto each, auto ctas) {
     k_append_kv8<FP16, MODE, WINDOW, each.value, ctas.value>
         <<<grid, kThreads, 0, s>>>(L, S, kv_ctas, parts);

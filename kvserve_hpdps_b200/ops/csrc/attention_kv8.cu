@@ -26,9 +26,10 @@
 // an equal share; the parts of an item are joined by a second launch in a fixed order.
 //
 // What bounds it, in a captured graph: one chain of loads and the join for a few tokens (150: 7.4 us;
-// 49157, 28/4 heads: 24.6); HBM for many sequences (48 of up to 8192 tokens, 32/8 heads, 412 MB:
+// 49157, 28/4 heads: 24.4); HBM for many sequences (48 of up to 8192 tokens, 32/8 heads, 412 MB:
 // 79 us, 80 % of the copy rate; 24 over encoders, 16 heads: 30 us); the latency of a step with more
-// rows (16 x 5 tokens, 40/8 heads, 25 rows: fp16 39 us, bf16 37, of which the products are 11 and 7).
+// rows (16 x 5 and 4 tokens, 40/8 heads, 25 and 20 rows: fp16 39.6 us, bf16 37.5, of which the
+// products are 11 and 7).
 #include <type_traits>
 
 #include "attention_kv8.cuh"
@@ -756,12 +757,12 @@ Grid grid_of(const Attn4Launch* L) {
 
 // Whether a call goes to attention_kv8_tile.cu: many rows a kv head, and enough of them by what the
 // host knows (max_query_len, and the tokens that the table has room for).  Measured, us here / there
-// (bf16; fp16 is 10 to 16 % more here, 6 there): 32 sequences of 2000 tokens, 8 heads: 48 rows
-// 97 / 104, 64 rows 99 / 105 (fp16 114 / 112), 96 rows 138 / 106; 16 of 2000: 64 rows 58 / 61, 96 rows
-// 79 / 62; 8 of 8000, 4 heads: 56 rows 55 / 50, 84 rows 73 / 51; 64 of 1000, 4 heads: 84 rows 83 / 75.
+// (bf16; fp16 is 10 to 16 % more here, 8 there): 32 sequences of 2000 tokens, 8 heads: 48 rows
+// 99 / 101, 64 rows 101 / 102 (fp16 115 / 111), 96 rows 141 / 103; 16 of 2000: 64 rows 59 / 60, 96 rows
+// 80 / 61; 8 of 8000, 4 heads: 56 rows 55 / 51, 84 rows 74 / 51; 64 of 1000, 4 heads: 84 rows 84 / 75.
 // With little to do (Mi rows times tokens times heads): one of 1024 tokens, 4 heads: 448 rows (1.8 Mi)
-// 22 / 26; one of 4000, 8 heads: 128 rows (3.9 Mi) 33 / 29, 512 rows 55 / 38; one of 16000, 4 heads:
-// 112 rows (6.8 Mi) 39 / 32.
+// 22 / 26; one of 4000, 8 heads: 128 rows (3.9 Mi) 33 / 28, 512 rows 56 / 37; one of 16000, 4 heads:
+// 112 rows (6.8 Mi) 40 / 31.
 constexpr int kManyRows = 64;
 constexpr long long kMuchWork = 3ll << 20;
 bool many_rows(const Attn4Launch* L) {

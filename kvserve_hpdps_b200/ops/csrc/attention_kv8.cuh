@@ -44,8 +44,8 @@ KVS_DEV void load_rows(uint32_t dst, const CUtensorMap* map, int row, int head, 
       : "memory");
 }
 
-// Joins the parts of the items that several CTAs (or teams of one) share.  A part's weights are relative to its own
-// maximum; they are added up in order, so results do not depend on timing.
+// Joins the parts of the items that several CTAs (or teams of one) share.  A part's weights are
+// relative to its own maximum; they are added up in order, so results do not depend on timing.
 //
 // Few parts an item (many items): CTA b takes the item that begins with team b and goes on, if one
 // does, a warp a row.  Many parts (DEEP; few items, which the host knows): the CTAs of column i look for

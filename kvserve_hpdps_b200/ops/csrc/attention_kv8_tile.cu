@@ -33,9 +33,9 @@
 //
 // What bounds it: the softmax warps' chain, 2300 clocks for 64 tokens of both tiles, of which the
 // exponentials' rate (16 a clock and SM) is 1024 and the products take 1050 (fp16: 1320).
-// 2 x 2048 tokens over up to 8193, 28/4 heads (361 GFLOP), in a captured graph: bf16 386 us (935
-// TFLOP/s), fp16 402; 6 prompts of 389 tokens over up to 1501, 16 heads: 72 us, a third of it what
-// pieces cost beside their steps.  With K as fp16 tiles it was 633 us and 107.
+// 2048 tokens over 8193 and 1366 over 6144, 28/4 heads (317 GFLOP), in a captured graph: bf16 375 us
+// (846 TFLOP/s), fp16 398; 6 prompts of 389 and 260 tokens over up to 1501, 16 heads: 72 us (fp16 77), a
+// third of it what pieces cost beside their steps.  With K as fp16 tiles it was 633 us and 107.
 //
 // The work is dealt out as in attention_kv8.cu, here by the number of visible keys a tile has.
 #include "attention_kv8.cuh"
@@ -59,7 +59,8 @@ constexpr float kSumBefore = kMostSum * 0x1p-20f;
 constexpr float kHuge = 0x1p-2f;
 
 // An item's own cost in steps of 128 tokens: the share is what a CTA's pieces take, 18000 clocks each
-// and 4600 a step (2 x 2048 rows: 396 us with 2, 393 with 3 and 4, 396 with 6).
+// and 4600 a step (2048 and 1366 tokens: 379 us with 2, 374.6 with 3, 373 with 4, 374 with 6; 6 prompts
+// 72.6, 71.4, 71.6, 71.8).
 constexpr int kOverTile = 3;
 constexpr int kHalf = 64;                  // tokens
 constexpr int kCodes = kHalf * 128;        // bytes of a half's key or value codes
@@ -834,7 +835,8 @@ KVS_DEV void softmax_role(const Attn4Launch& L, int group, uint8_t* smem, uint32
 }
 
 template <bool FP16>
-__global__ void __launch_bounds__(kThreads, 1) k_attn8_tile(const __grid_constant__ Attn4Launch L, const __grid_constant__ CUtensorMap map) {
+__global__ void __launch_bounds__(kThreads, 1)
+    k_attn8_tile(const __grid_constant__ Attn4Launch L, const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));

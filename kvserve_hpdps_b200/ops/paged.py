@@ -218,6 +218,12 @@ def attention_kv8(query: torch.Tensor, cache: torch.Tensor, block_table: torch.T
     every query row sees all ``seq_lens[r]`` tokens of its sequence: cross attention to an
     encoder's states, whose keys and values :func:`append_kv` has put into the cache (without
     positions) and whose number has nothing to do with that of the query rows.
+
+    Both kernels take scores and sums in fp32.  That for many rows rounds weights to 11 bits in
+    both types, that for few rows in bf16 alone: an fp16 row's error is up to a third larger where
+    ``max_query_len`` and the room in the table choose the first.  Scales and scores may lie as far
+    apart as fp32 holds them.  A query row with an element that is not finite, and a token to see,
+    is NaN.
     """
     args = (query, cache, block_table, seq_lens, query_start, max_query_len, scale, out,
             return_lse, causal)
